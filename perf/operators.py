@@ -290,7 +290,7 @@ def _plain_sample(s, case):
     top = x.amax(1, keepdim=True)
     scaled = (x - top) / torch.where(t > 0, t, 1.0)
     e = torch.where(t > 0, torch.exp(scaled), (x == top).float())
-    mass = (e * 4294967296.0).long()  # whole numbers of 2^-32: their sums are the same in every order
+    mass = (e * 1099511627776.0).long()  # whole numbers of 2^-40: their sums are the same in every order
     order = torch.sort(x, dim=1, descending=True, stable=True).indices
     sorted_mass = mass.gather(1, order)
     rank = torch.arange(x.shape[1], device=DEV)[None]
@@ -382,7 +382,7 @@ def exact(case, seed):
             at += fresh
         return y
     probability = []
-    for r in range(case["rows"]):  # weights as they are, not in steps of 2^-32
+    for r in range(case["rows"]):  # weights as they are, not in steps of 2^-40
         x = s["logits"][r].double()
         t = float(s["temperature"][r])
         if t <= 0:
