@@ -288,6 +288,93 @@ int rq_moe_route_forward(rq_ctx* ctx, rq_moe* moe, const float* scores, int64_t 
                          int64_t x_k_stride, int64_t x_t_stride, int tokens, int include_shared, float* y, int64_t y_n_stride, int64_t y_t_stride,
                          void* stream);
 
+/* ---- a serving step around the projections: plan, rotation and cache, attention, the next token ------- */
+
+/* The four steps that a decode loop needs beside its projections, over a batch of requests that share one paged cache of keys
+ * and values. (The reference runs attention, rotation and its sampler inside its one persistent kernel and on the host, over
+ * one sequence with a contiguous cache: recipe.rs:20249-20309, :19444-19526; there is no paged cache in it.)
+ *
+ * A batch: request r has cached[r] positions in the cache and brings fresh[r] new tokens; the new tokens of all requests lie one
+ * after another, in request order, in every per-token array ("token t"). All of it is device memory, so that a recorded
+ * sequence serves batches of changing lengths.
+ *
+ * The cache: pages of page_size positions; element d of position `line` of page `page` of head h lies at
+ * page * page_stride + h * head_stride + line * line_stride + d, in elements, in k and in v. Any order of pages, heads and lines
+ * will do; a line's head_dim elements are contiguous, pointers are 16-byte aligned and strides multiples of eight.
+ * Row r of the page table (int32, table_stride apart, table_width entries) names the pages of request r's positions in order. */
+enum { RQ_KV_F16 = 0, RQ_KV_BF16 = 1 };
+typedef struct rq_kv_cache {
+    void* k;
+    void* v;
+    int32_t type;      /* RQ_KV_F16 or RQ_KV_BF16 */
+    int32_t heads;     /* key / value heads */
+    int32_t head_dim;  /* 64, 128 or 256 */
+    int32_t page_size; /* positions a page: a power of two, at most 4096 */
+    int64_t pages;     /* pages * page_size < 2^31 */
+    int64_t page_stride, head_stride, line_stride;
+} rq_kv_cache;
+
+/* The plan of a step, from the requests' lengths: gives the requests the pages they lack, in request order, from the front of
+ * free_pages[0 .. free_count), and writes
+ *   block_table: the new pages' entries, behind those of the pages that hold the cached positions (which stay as they are);
+ *   starts[0 .. requests]: each request's first token, and the number of tokens; lengths[r] = cached[r] + fresh[r];
+ *   per token t < max_tokens: slots[t] = page * page_size + line in the cache, positions[t] in its request, owners[t] = its request;
+ *     past the batch's tokens -1, 0 and -1;
+ *   status[0 .. 2]: tokens, pages taken, pages lacking.
+ * Where pages are lacking (the list is too short, or a request outgrows table_width), the entries are -1 (or not there) and so are
+ * the slots of their tokens: rq_rope_store passes over them, and nothing else of the batch changes. A negative length counts as
+ * zero. At most RQ_MAX_REQUESTS requests, fewer than 2^31 tokens and positions. Nothing is read and written by the same call but
+ * block_table, so a step may be planned again from the same lengths. */
+#define RQ_MAX_REQUESTS 4096
+int rq_batch_plan(rq_ctx* ctx, const int32_t* cached, const int32_t* fresh, int requests, int page_size, int32_t* block_table, int64_t table_stride, int table_width,
+                  const int32_t* free_pages, int free_count, int32_t* starts, int32_t* lengths, int32_t* slots, int32_t* positions, int32_t* owners, int max_tokens,
+                  int32_t* status, void* stream);
+
+/* The table that rq_rope_store reads: row p holds cos(a_i) for i < rotary / 2, then sin(a_i), with a_i = p * frequency_scale *
+ * base^(-2 i / rotary), computed in 64 bits and rounded once. (Any other table of that form serves as well.) */
+int rq_rope_table(rq_ctx* ctx, double base, double frequency_scale, int rotary, int64_t rows, float* table, void* stream);
+
+/* Queries and keys of `tokens` tokens, from the projections' outputs to what attention reads: an RMS norm over each head
+ * (x / sqrt(mean(x^2) + epsilon) * gain; gain null: no norm), then the rotation of its first `rotary` elements by the row
+ * positions[t] of the table (a position outside it is clamped into it),
+ *   (a, b) -> (a cos - b sin, a sin + b cos), pairs (a, b) = (x[i], x[i + rotary / 2]) for RQ_ROPE_HALVES, (x[2 i], x[2 i + 1]) for RQ_ROPE_PAIRS,
+ * queries to q_out (which may be q), keys and, as they are, values to the cache at slots[t] (a slot outside it is passed over),
+ * rounded to the cache's type once. Heads of a token lie head_dim apart; tokens *_t_stride apart, any alignment. rotary: a
+ * multiple of 16 up to head_dim, or 0 (no rotation, no table). */
+enum { RQ_ROPE_HALVES = 0, RQ_ROPE_PAIRS = 1 };
+int rq_rope_store(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, const float* k, int64_t k_t_stride, const float* v, int64_t v_t_stride, int tokens,
+                  const float* q_gain, const float* k_gain, float epsilon, const float* table, int64_t table_rows, int rotary, int style, const int32_t* positions,
+                  const int32_t* slots, float* q_out, int64_t q_out_t_stride, const rq_kv_cache* cache, void* stream);
+
+/* Attention of the batch's new tokens over the paged cache (their own keys and values stored before). Token t of request r, at
+ * position p = lengths[r] - (starts[r + 1] - t), sees the keys j <= p, with a window > 0 only those with j > p - window:
+ *   y[t][h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q[t][h] . k_j - max),  k_j, v_j of head h / (q_heads / heads).
+ * A row that sees no key gets zeros; keys that are masked, lie past lengths[r] or on a page outside the cache count for nothing,
+ * whatever they hold. Tokens from starts[requests] on are not written. q and y: heads head_dim apart, tokens *_t_stride apart, any
+ * alignment. max_fresh is the most new tokens that a request has, as far as the host knows: the choice of kernel rests on it,
+ * the results do not.
+ * Activations stay fp32: queries and weights meet the 16-bit keys and values as two (f16) or three (bf16) 16-bit parts, products
+ * are added in 32 bits. Queries times scale of magnitude above 65504 are not served over an f16 cache (inf / NaN). The same bits on every run.
+ * The context keeps a work area for rows whose keys are dealt out over several CTAs; the first call, or rq_attention_reserve ahead of a recording, allocates it. */
+int rq_attention_reserve(rq_ctx* ctx);
+int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, const rq_kv_cache* cache, const int32_t* block_table, int64_t table_stride,
+                 int table_width, const int32_t* starts, const int32_t* lengths, int requests, int tokens, int max_fresh, float scale, int window, float* y,
+                 int64_t y_t_stride, void* stream);
+
+/* The next token of `rows` rows of logits, each from one given random number uniform[r] in [0, 1). The weight of token i is the
+ * whole number w_i = floor(2^40 * exp((x_i - max x) / temperature)) (fp32 arithmetic), so that every sum of weights is exact and
+ * the result depends on no order of additions. Tokens are kept by rank, larger logits first and, among equal ones, lower indices first:
+ *   top_k:  the first top_k (<= 0: all);
+ *   top_p:  of those, the ones before which less than top_p of their mass lies, at least one (>= 1: all);
+ *   min_p:  of those, the ones whose weight is at least min_p of the largest.
+ * The token is the first, by index, at which the kept weights' running sum exceeds floor(uniform * their sum). token[r] receives
+ * it, probability[r] its weight over that sum (null: not wanted), kept[r] how many tokens of positive weight were kept (null: not wanted).
+ * temperature <= 0 takes the largest logit (the lowest index of equal ones); a null parameter array counts as 1, 0, 1, 0.
+ * NaN counts as -inf; a row without any value above -inf gets token -1, probability 0, kept 0. At most RQ_MAX_VOCABULARY tokens. */
+#define RQ_MAX_VOCABULARY 1048576
+int rq_sample(rq_ctx* ctx, const float* logits, int64_t row_stride, int rows, int64_t vocabulary, const float* temperature, const int32_t* top_k, const float* top_p,
+              const float* min_p, const float* uniform, int32_t* token, float* probability, int32_t* kept, void* stream);
+
 /* ---- recorded sequences: one boundary crossing per step ------------------------------------------ */
 
 /* The reference crosses its host / device boundary once per step: recipe_model_step is one launch that

@@ -24,6 +24,7 @@ from .capi import (  # noqa: F401
     Context,
     Exchange,
     Gguf,
+    KvCache,
     NcclComm,
     RqError,
     Weight,
@@ -35,5 +36,5 @@ from .capi import (  # noqa: F401
 
 __all__ = [
     "ACT_FLOAT", "ACT_INT8", "IQ4_NL", "IQ4_XS", "Q2_K", "Q3_K", "Q8_1", "Q8_K", "Q4_0", "Q4_1", "Q4_K", "Q5_0", "Q5_1", "Q5_K", "Q6_K", "Q8_0",
-    "Context", "Exchange", "Gguf", "NcclComm", "RqError", "Weight", "block_bytes", "block_values", "library_path", "load_library",
+    "Context", "Exchange", "Gguf", "KvCache", "NcclComm", "RqError", "Weight", "block_bytes", "block_values", "library_path", "load_library",
 ]

@@ -16,6 +16,8 @@ Q4_1, Q5_0, Q5_1, Q5_K, IQ4_NL = 3, 6, 7, 13, 20  # bound, decoded, dotted with 
 Q8_1, Q2_K, Q3_K, Q8_K, IQ4_XS = 9, 10, 11, 15, 23  # the same
 ACT_FLOAT, ACT_INT8 = 0, 1
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+KV_F16, KV_BF16 = 0, 1
+ROPE_STYLES = {"halves": 0, "pairs": 1}
 
 _PKG = Path(__file__).resolve().parent
 _LIB = None
@@ -87,6 +89,12 @@ def _declare(lib) -> None:
         "rq_moe_route_forward": (i32, [p, p, f32p, i64, i64, i32, i32, i32, f32p, f32p, i64, i64, f32p, i64, i64, i32, i32, f32p, i64, i64, p]),
         "rq_device_alloc": (i32, [p, i64, C.POINTER(p)]),
         "rq_device_free": (None, [p, p]),
+        "rq_batch_plan": (i32, [p, p, p, i32, i32, p, i64, i32, p, i32, p, p, p, p, p, i32, p, p]),
+        "rq_rope_table": (i32, [p, C.c_double, C.c_double, i32, i64, f32p, p]),
+        "rq_rope_store": (i32, [p, f32p, i64, i32, f32p, i64, f32p, i64, i32, f32p, f32p, C.c_float, f32p, i64, i32, i32, p, p, f32p, i64, p, p]),
+        "rq_attention_reserve": (i32, [p]),
+        "rq_attention": (i32, [p, f32p, i64, i32, p, p, i64, i32, p, p, i32, i32, i32, C.c_float, i32, f32p, i64, p]),
+        "rq_sample": (i32, [p, f32p, i64, i32, i64, f32p, p, f32p, f32p, f32p, p, f32p, p, p]),
         "rq_sequence_begin": (i32, [p, C.POINTER(p)]),
         "rq_sequence_end": (i32, [p, C.POINTER(p)]),
         "rq_sequence_run": (i32, [p, p]),
@@ -170,6 +178,22 @@ def _stream(stream) -> int:
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
+def _int32(a, size, who: str) -> None:
+    import torch
+
+    if a.dtype != torch.int32 or a.dim() != 1 or not a.is_cuda or not a.is_contiguous() or (size is not None and a.shape[0] != size):
+        raise ValueError(f"{who}: expected a contiguous CUDA int32 tensor" + ("" if size is None else f" of {size}"))
+
+
+def _plane(a, who: str) -> int:
+    """The values of a token of an fp32 plane [tokens, values] or [tokens, heads, head_dim] whose tokens are contiguous."""
+    import torch
+
+    if a.dtype != torch.float32 or not a.is_cuda or a.stride(-1) != 1 or (a.dim() == 3 and a.stride(1) != a.shape[2]) or a.dim() not in (2, 3):
+        raise ValueError(f"{who}: expected a CUDA fp32 plane [tokens, values] or [tokens, heads, head_dim] with contiguous tokens")
+    return a.shape[1] if a.dim() == 2 else a.shape[1] * a.shape[2]
+
+
 class Weight:
     """A stored weight resident in HBM (rq_weight)."""
 
@@ -202,6 +226,36 @@ class Weight:
             self.free()
         except Exception:
             pass
+
+
+class _KvCacheStruct(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int64),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("line_stride", C.c_int64)]
+
+
+class KvCache:
+    """A paged cache of keys and values (rq_kv_cache) over two CUDA tensors [pages, heads, page_size, head_dim], float16 or
+    bfloat16, of the same strides (any order of pages, heads and lines; a line's elements are contiguous)."""
+
+    def __init__(self, k, v):
+        import torch
+
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+            raise ValueError("KvCache: k and v must be [pages, heads, page_size, head_dim] of one shape, type and layout")
+        if k.dtype not in (torch.float16, torch.bfloat16) or not k.is_cuda or not v.is_cuda or k.stride(3) != 1:
+            raise ValueError("KvCache: k and v must be CUDA float16 or bfloat16 tensors with contiguous lines")
+        self.k, self.v = k, v
+        self.pages, self.heads, self.page_size, self.head_dim = k.shape
+        sp, sh, sl, _ = k.stride()
+        self._struct = _KvCacheStruct(k.data_ptr(), v.data_ptr(), KV_F16 if k.dtype == torch.float16 else KV_BF16, self.heads, self.head_dim, self.page_size, self.pages, sp, sh, sl)
+        self._ref = C.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, page_size: int, head_dim: int, dtype=None, device: int = 0) -> "KvCache":
+        import torch
+
+        k, v = (torch.empty((pages, heads, page_size, head_dim), dtype=dtype or torch.float16, device=f"cuda:{device}") for _ in range(2))
+        return cls(k, v)
 
 
 class MoeBank:
@@ -522,6 +576,120 @@ class Context:
                                              _ptr(bias), _ptr(weights), weights.stride(0), weights.stride(1), _ptr(x), x.stride(0),
                                              x.stride(1), tokens, int(include_shared), _ptr(y), y.stride(0), y.stride(1), _stream(stream)))
         return y, weights
+
+    # ---- a serving step around the projections ----
+    def batch_plan(self, cached, fresh, table, free_pages, page_size: int, max_tokens: int = 0, starts=None, lengths=None, slots=None, positions=None, owners=None, status=None,
+                   stream=None):
+        """cached, fresh: CUDA int32 [requests]; table: int32 [requests, width] page table, extended in place from free_pages (int32).
+        Returns starts [requests + 1], lengths, slots, positions, owners (of the slots given, or max_tokens) and status (tokens,
+        pages taken, pages lacking)."""
+        n = cached.shape[0]
+        if starts is None or lengths is None or slots is None or positions is None or owners is None or status is None:
+            import torch
+
+            def made(given, size):
+                return torch.empty(size, dtype=torch.int32, device=cached.device) if given is None else given
+
+            size = max_tokens or next((a.shape[0] for a in (slots, positions, owners) if a is not None), 0)
+            if size <= 0:
+                raise ValueError("batch_plan: pass max_tokens or one of the per-token arrays")
+            starts, lengths, status = made(starts, n + 1), made(lengths, n), made(status, 3)
+            slots, positions, owners = made(slots, size), made(positions, size), made(owners, size)
+        tokens = slots.shape[0]
+        for a, size in ((cached, n), (fresh, n), (starts, n + 1), (lengths, n), (slots, tokens), (positions, tokens), (owners, tokens), (status, 3), (free_pages, None)):
+            _int32(a, size, "batch_plan")
+        if table.dim() != 2 or table.shape[0] < n or table.stride(1) != 1 or table.dtype != cached.dtype:
+            raise ValueError("batch_plan: the page table must be int32 [requests, width] with contiguous rows")
+        status_code = self.lib.rq_batch_plan(self.handle, cached.data_ptr(), fresh.data_ptr(), n, page_size, table.data_ptr(), table.stride(0), table.shape[1], free_pages.data_ptr(),
+                                             free_pages.shape[0], starts.data_ptr(), lengths.data_ptr(), slots.data_ptr(), positions.data_ptr(), owners.data_ptr(), tokens,
+                                             status.data_ptr(), _stream(stream))
+        if status_code:
+            _check(status_code)
+        return starts, lengths, slots, positions, owners, status
+
+    def rope_table(self, rows: int, rotary: int, base: float = 10000.0, frequency_scale: float = 1.0, out=None, stream=None):
+        """[rows, rotary] fp32: cos of every angle of a position, then sin."""
+        import torch
+
+        if out is None:
+            out = torch.empty((rows, rotary), dtype=torch.float32, device=f"cuda:{self.device}")
+        _check(self.lib.rq_rope_table(self.handle, base, frequency_scale, rotary, rows, _ptr(out), _stream(stream)))
+        return out
+
+    def rope_store(self, q, k, v, positions, slots, table, cache: KvCache, q_gain=None, k_gain=None, epsilon: float = 1e-6, style: str = "halves", q_out=None, stream=None):
+        """q [tokens, q_heads * head_dim] (or [tokens, q_heads, head_dim]), k and v likewise with the cache's heads: fp32, heads
+        contiguous, any token stride. Norms (where gains are given) and rotates queries into q_out and keys into the cache, with
+        the values, at slots. table: rope_table's, or None."""
+        tokens = q.shape[0]
+        if q_out is None:
+            import torch
+
+            q_out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        d, width = cache.head_dim, cache.heads * cache.head_dim
+        qw = _plane(q, "rope_store")
+        if qw % d or _plane(q_out, "rope_store") != qw or _plane(k, "rope_store") != width or _plane(v, "rope_store") != width or not k.shape[0] == v.shape[0] == q_out.shape[0] == tokens:
+            raise ValueError("rope_store: q and q_out must hold whole heads, k and v the cache's heads, for the same tokens")
+        _int32(positions, None, "rope_store"), _int32(slots, None, "rope_store")
+        if positions.shape[0] < tokens or slots.shape[0] < tokens:
+            raise ValueError("rope_store: positions and slots must have an entry for every token")
+        for g in (q_gain, k_gain):
+            if g is not None and (g.shape != (d,) or g.stride(0) != 1):
+                raise ValueError("rope_store: a gain holds head_dim contiguous values")
+        rows, rotary = (0, 0) if table is None else table.shape
+        if table is not None and not table.is_contiguous():
+            raise ValueError("rope_store: the rotation table must be contiguous")
+        status = self.lib.rq_rope_store(self.handle, q.data_ptr(), q.stride(0), qw // d, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), tokens,
+                                        0 if q_gain is None else q_gain.data_ptr(), 0 if k_gain is None else k_gain.data_ptr(), epsilon,
+                                        0 if table is None else table.data_ptr(), rows, rotary, ROPE_STYLES[style], positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), q_out.stride(0),
+                                        cache._ref, _stream(stream))
+        if status:
+            _check(status)
+        return q_out
+
+    def attention_reserve(self) -> None:
+        """Allocates the work area of attention calls, so that none of them does (and they can be recorded)."""
+        _check(self.lib.rq_attention_reserve(self.handle))
+
+    def attention(self, q, cache: KvCache, table, starts, lengths, scale: float | None = None, window: int = 0, max_fresh: int = 0, y=None, stream=None):
+        """Causal attention of the batch's new tokens (q [tokens, q_heads, head_dim] or [tokens, q_heads * head_dim], fp32) over the paged
+        cache: request r's tokens are starts[r] .. starts[r + 1] at the end of its lengths[r] positions. max_fresh: the most new tokens
+        of a request as far as the host knows (0: that is not known). Returns y, of q's shape."""
+        tokens, n, d = q.shape[0], lengths.shape[0], cache.head_dim
+        if y is None:
+            import torch
+
+            y = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        qw = _plane(q, "attention")
+        if qw % d or _plane(y, "attention") != qw or y.shape[0] != tokens:
+            raise ValueError("attention: q and y must hold whole heads of the cache's head_dim for the same tokens")
+        _int32(starts, n + 1, "attention"), _int32(lengths, n, "attention")
+        if table.dim() != 2 or table.shape[0] < n or table.stride(1) != 1 or table.dtype != lengths.dtype:
+            raise ValueError("attention: the page table must be int32 [requests, width] with contiguous rows")
+        status = self.lib.rq_attention(self.handle, q.data_ptr(), q.stride(0), qw // d, cache._ref, table.data_ptr(), table.stride(0), table.shape[1], starts.data_ptr(), lengths.data_ptr(),
+                                       n, tokens, max_fresh, d**-0.5 if scale is None else scale, window, y.data_ptr(), y.stride(0), _stream(stream))
+        if status:
+            _check(status)
+        return y
+
+    def sample(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, token=None, probability=None, kept=None, stream=None):
+        """The next token of each row of logits (fp32 [rows, vocabulary]) from uniform [rows] in [0, 1); parameters are CUDA tensors [rows]
+        (top_k int32, the others fp32) or None. Returns token (int32 [rows]); probability and kept are filled where given."""
+        import torch
+
+        rows, vocabulary = logits.shape
+        if logits.dtype != torch.float32 or not logits.is_cuda or logits.stride(1) != 1:
+            raise ValueError("sample: logits must be CUDA fp32 [rows, vocabulary] with contiguous rows")
+        if token is None:
+            token = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        for a, dtype in ((uniform, torch.float32), (temperature, torch.float32), (top_p, torch.float32), (min_p, torch.float32), (probability, torch.float32), (top_k, torch.int32),
+                         (kept, torch.int32), (token, torch.int32)):
+            if a is not None and (a.dtype != dtype or a.shape != (rows,) or not a.is_contiguous() or not a.is_cuda):
+                raise ValueError("sample: per-row arrays must be contiguous CUDA tensors [rows], top_k, token and kept int32, the others fp32")
+        status = self.lib.rq_sample(self.handle, logits.data_ptr(), logits.stride(0), rows, vocabulary, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), uniform.data_ptr(),
+                                    token.data_ptr(), _ptr(probability), _ptr(kept), _stream(stream))
+        if status:
+            _check(status)
+        return token
 
     def activation_records(self, x, step: int, stream=None):
         """The 36-byte int8 records of x ([cols] or [tokens, cols]) as a uint8 CUDA tensor."""
