@@ -80,6 +80,7 @@ extern "C" void rq_destroy(rq_ctx* ctx) {
     if (!ctx) return;
     DeviceGuard guard(ctx->device);
     if (ctx->act_scratch) cudaFree(ctx->act_scratch);
+    if (ctx->attn_scratch) cudaFree(ctx->attn_scratch);
     if (ctx->error_flag) cudaFree(ctx->error_flag);
     if (ctx->pin_flag) cudaFreeHost(ctx->pin_flag);
     if (ctx->stage_x) cudaFree(ctx->stage_x);

@@ -1,0 +1,42 @@
+// What the kernels of rq_attention share: parameters, the 16-bit parts of fp32 numbers, and how a batch's keys are dealt out.
+#pragma once
+#include "rq_serve.cuh"
+
+namespace rqattn {
+
+struct AttentionParams {
+    const float* q;
+    float* y;
+    const uint16_t *k, *v;
+    const int32_t *block_table, *starts, *lengths;
+    float* partial;      // sums of rows whose keys several CTAs share
+    uint32_t* arrived;   // per CTA: how many have left their part of the rows that begin there; zero between calls
+    int64_t q_stride, y_stride, table_stride, page_stride, head_stride, line_stride, pages;
+    int tokens, requests, q_heads, kv_heads, table_width, page_shift, window;
+    float scale;
+    int wide;  // q and y allow 16-byte accesses
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+// Weights are 2^(s - max + kRaise): an f16 part below 2^-14 loses bits, raised by 2^12 that is a weight of 2^-26 of the row's largest
+constexpr float kRaise = 12.0f;
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+// two fp32 numbers as a pair of 16-bit ones (the first in the low half), and what the pair leaves of them
+template <int TYPE> __device__ __forceinline__ uint32_t pair_of(float a, float b) {
+    uint32_t w;
+    if (TYPE == RQ_KV_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    return w;
+}
+template <int TYPE> __device__ __forceinline__ uint32_t take_pair(float& a, float& b) {
+    const uint32_t w = pair_of<TYPE>(a, b);
+    a -= rqserve::to_float<TYPE>((uint16_t)w);
+    b -= rqserve::to_float<TYPE>((uint16_t)(w >> 16));
+    return w;
+}
+#endif
+
+}  // namespace rqattn

@@ -52,6 +52,7 @@ struct rq_ctx {
     // the stream of the last call that used the context's work areas (the activation scratch, a bank's plans), and the event
     // a call on another stream waits for before it touches them
     cudaStream_t work_stream; bool work_stream_set; cudaEvent_t work_event;
+    uint8_t* attn_scratch;  // rq_attention's work area (null until it is first needed)
     bool recording;  // between rq_sequence_begin and rq_sequence_end: the context's stream is capturing, nothing may allocate
 };
 

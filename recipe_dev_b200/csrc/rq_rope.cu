@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
             for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
             const float scale = 1.0f / sqrtf(sum / (float)D + p.epsilon);
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = x[i] * scale * __ldg(gain + first + i);
+            for (int i = 0; i < E; ++i) x[i] = x[i] * scale * __ldcg(gain + first + i);
         }
         if (p.rotary) {
             const int64_t position = max((int64_t)0, min((int64_t)p.positions[t], p.table_rows - 1));
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
                 if (first < p.rotary) {
 #pragma unroll
                     for (int i = 0; i < E; i += 2) {
-                        const float c = __ldg(row + (first + i) / 2), s = __ldg(row + half + (first + i) / 2), a = x[i], b = x[i + 1];
+                        const float c = __ldcg(row + (first + i) / 2), s = __ldcg(row + half + (first + i) / 2), a = x[i], b = x[i + 1];
                         x[i] = a * c - b * s;
                         x[i + 1] = a * s + b * c;
                     }
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
                 for (int i = 0; i < E; ++i) {
                     const float y = __shfl_sync(0xffffffffu, x[i], other & 31);
                     if (first < p.rotary) {
-                        const float c = __ldg(row + i0 + i), s = __ldg(row + half + i0 + i);
+                        const float c = __ldcg(row + i0 + i), s = __ldcg(row + half + i0 + i);
                         x[i] = low ? x[i] * c - y * s : y * s + x[i] * c;
                     }
                 }
