@@ -311,7 +311,7 @@ typedef struct rq_kv_cache {
     int32_t head_dim;  /* 64, 128 or 256 */
     int32_t page_size; /* positions a page: a power of two, at most 4096 */
     int64_t pages;     /* pages * page_size < 2^31 */
-    int64_t page_stride, head_stride, line_stride;
+    int64_t page_stride, head_stride, line_stride; /* page and line strides below 2^31 */
 } rq_kv_cache;
 
 /* The plan of a step, from the requests' lengths: gives the requests the pages they lack, in request order, from the front of

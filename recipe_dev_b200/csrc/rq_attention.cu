@@ -4,42 +4,68 @@
 //
 // rq_attention_rows_kernel, for up to sixteen rows (new tokens x the query heads that share a key head) at a time: a decode step. It is bound by the bytes of
 // the cache, read once, so everything else is arranged around loads:
-//   * a warp takes 32 keys at a time (16 of 256 elements) straight from global memory into the operand registers of mma.sync: which elements
-//     the tensor core takes together is free as long as both operands agree, so a thread loads sixteen bytes of a key (or of a value, for four
-//     keys, whose halves a byte permute pairs up) and nothing passes through shared memory. The keys of the next tile are under way while
-//     the values of this one are used.
+//   * a warp takes sixteen keys at a time through a ring of its own in shared memory, filled by 16-byte asynchronous copies a tile ahead: any
+//     page size, order and stride, and what no row sees arrives as zeros. Chunks of a line are permuted (chunk ^ line % 8) so that
+//     the matrix loads meet no bank twice. (Loads into registers instead, without shared memory, kept too little under way: 140 us for 131071 keys.)
 //   * fp32 activations: queries and weights are taken apart into 16-bit parts, hi + lo over f16 (22 bits), hi + mid + lo over
-//     bf16 (24 bits). The sixteen rows of an operand are eight rows' hi parts above their lo parts: one instruction does both.
+//     bf16 (24 bits). The sixteen rows of an operand are eight rows' hi parts above their lo parts: one mma.sync does both.
 //   * The tensor core adds by truncation, a bias that grows with the length of a chain: a sum stays in it for one tile and is then added, with
 //     round-to-nearest, to the row's fp32 sums, which are scaled by 2^(old max - new max) in the same multiply-add.
-//   * The keys of all requests and heads, in units of 128, are dealt out evenly: every CTA takes an equal range of units, wherever it begins and ends.
+//   * The keys of all requests and heads, in units of 64, are dealt out evenly: every CTA takes an equal range of units, wherever it begins and ends.
 //     Rows whose units fall to several CTAs are joined, in CTA order, by whichever of these is the last to leave its sums: the same bits on every run.
 #include "rq_attention.cuh"
+#include "rq_mma.cuh"
 
 using namespace rqserve;
 using namespace rqattn;
+using rqmma::smem_u32;
 
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kUnit = 128;  // keys
+constexpr int kTile = 16, kUnit = kWarps * kTile;  // keys a warp and a CTA take at a time
+constexpr int kStages = 2;  // of a warp's ring: one tile under way while the other is used
 
-template <int TYPE> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// c = (first ? 0 : c) + a b for sixteen rows, eight columns and sixteen products each
+template <int TYPE> __device__ __forceinline__ void mma(float (&c)[4], bool first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    const float c0 = first ? 0.0f : c[0], c1 = first ? 0.0f : c[1], c2 = first ? 0.0f : c[2], c3 = first ? 0.0f : c[3];
     if (TYPE == RQ_KV_F16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
     else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
+// acc = acc * f + d, two numbers an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ void add_scaled(float2 (&acc)[2], float f, const float (&d)[4]) {
+    acc[0] = fma2(acc[0], make_float2(f, f), make_float2(d[0], d[1]));
+    acc[1] = fma2(acc[1], make_float2(f, f), make_float2(d[2], d[3]));
+}
+// four matrices of eight lines x sixteen bytes, lane l giving line l % 8 of matrix l / 8
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_transposed(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// sixteen bytes, or zeros
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Whether a word's two 16-bit numbers are both finite
 template <int TYPE> __device__ __forceinline__ bool finite2(uint32_t w) {
     const uint32_t e = TYPE == RQ_KV_F16 ? 0x7c00u : 0x7f80u;
     return (w & e) != e && ((w >> 16) & e) != e;
 }
-
-__device__ __forceinline__ uint4 load16(const uint16_t* p) { return __ldcg((const uint4*)p); }
 
 // A request's rows and keys, as a CTA deals with them
 struct Request {
@@ -53,26 +79,26 @@ template <int ROWS> __device__ __forceinline__ Request request_of(const Attentio
     q.length = p.lengths[r];
     q.end = (int)min((int64_t)max(q.length, 0), (int64_t)p.table_width << p.page_shift);
     q.begin = p.window > 0 ? (int)max((int64_t)0, (int64_t)q.length - q.fresh - p.window + 1) : 0;
-    q.begin = min(q.begin, q.end) & ~31;  // tiles begin at whole multiples of 32 keys
+    q.begin = min(q.begin, q.end) & ~(kTile - 1);
     q.tiles = (q.fresh * (p.q_heads / p.kv_heads) + ROWS - 1) / ROWS;
     q.units = max((q.end - q.begin + kUnit - 1) / kUnit, 1);  // (a row that sees no key is written all the same)
     return q;
 }
 
 template <int D, int TYPE, int RT> struct Tiles {
-    uint4 q_hi[RT][D / 16][32];                          // operand registers of the queries: hi above lo (f16), hi above mid (bf16)
+    union {
+        uint16_t ring[kWarps][kStages][2][kTile][D];  // keys, values
+        float out[kWarps][8 * RT][D + 8];             // the warps' sums
+    };
+    uint4 q_hi[RT][D / 16][32];                           // operand registers of the queries: hi above lo (f16), hi above mid (bf16)
     uint2 q_lo[TYPE == RQ_KV_BF16 ? RT : 1][D / 16][32];  // the third parts
-    float out[kWarps][8 * RT][D + 4];                    // the warps' sums
 };
 
 template <int D, int TYPE, int RT>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) rq_attention_rows_kernel(AttentionParams p) {
-    constexpr int ROWS = 8 * RT, TK = D == 256 ? 16 : 32, NT = TK / 8, STEPS = D / 16, KC = D / 32, VC = D / 64, PARTS = TYPE == RQ_KV_F16 ? 2 : 3;
-    extern __shared__ __align__(16) unsigned char dynamic[];
+__global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionParams p) {
+    constexpr int ROWS = 8 * RT, STEPS = D / 16, PARTS = TYPE == RQ_KV_F16 ? 2 : 3, CHUNKS = D / 8, LINES = 32 / CHUNKS > 0 ? 32 / CHUNKS : 1;
+    extern __shared__ __align__(128) unsigned char dynamic[];
     Tiles<D, TYPE, RT>& sh = *(Tiles<D, TYPE, RT>*)dynamic;
-    auto& q_hi = sh.q_hi;
-    auto& q_lo = sh.q_lo;
-    auto& out = sh.out;
     int64_t* before = (int64_t*)(dynamic + sizeof(sh));  // units before each request
     __shared__ float warp_max[kWarps][ROWS], warp_sum[kWarps][ROWS];
     __shared__ int64_t sums[kWarps];
@@ -116,31 +142,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) rq_attention_rows_k
         const int key_first = rq.begin + (int)first_unit * kUnit, key_stop = min(rq.end, rq.begin + (int)(stop - item_begin) * kUnit);
         u = stop;
 
-        // queries: scaled, taken apart, in the order in which the tensor core takes a key's elements (see the loads below)
-        for (int i = tid; i < RT * STEPS * 32; i += kThreads) {
-            const int l = i & 31, step = (i >> 5) % STEPS, rt = i / (32 * STEPS), row = rt * 8 + (l >> 2);
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (row < rows) {
-                const int at = row0 + row;
-                const float* from = p.q + (int64_t)(p.starts[r] + at / group) * p.q_stride + (int64_t)(kv * group + at % group) * D + 8 * ((l & 3) + 4 * (step >> 1)) + 4 * (step & 1);
-                if (p.wide) { const float4 v = __ldcg((const float4*)from); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-                else { for (int e = 0; e < 4; ++e) x[e] = __ldcg(from + e); }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] *= p.scale * kLog2e;
-            uint4 a;
-            a.x = take_pair<TYPE>(x[0], x[1]);
-            a.z = take_pair<TYPE>(x[2], x[3]);
-            a.y = take_pair<TYPE>(x[0], x[1]);
-            a.w = take_pair<TYPE>(x[2], x[3]);
-            q_hi[rt][step][l] = a;
-            if (PARTS == 3) q_lo[rt % (PARTS == 3 ? RT : 1)][step][l] = make_uint2(pair_of<TYPE>(x[0], x[1]), pair_of<TYPE>(x[2], x[3]));
-        }
-        __syncthreads();
-
-        // the keys that this thread's rows see: [low, high)
+        // the keys that some row sees and that this thread's rows see: [low, high)
         int low[RT], high[RT];
-        const int position0 = rq.length - rq.fresh, seen_high = min(rq.end, position0 + (row0 + max(rows, 1) - 1) / group + 1);
+        const int position0 = rq.length - rq.fresh, seen_high = min(key_stop, position0 + (row0 + max(rows, 1) - 1) / group + 1);
         const int seen_low = p.window > 0 ? max(0, position0 + row0 / group - p.window + 1) : 0;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -150,102 +154,133 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) rq_attention_rows_k
         }
         const bool one_token = row0 / group == (row0 + max(rows, 1) - 1) / group;
 
-        float m[RT], sum[RT], acc[RT][VC][16];
+        const int32_t* table = p.block_table + r * p.table_stride;
+        const int line_mask = (1 << p.page_shift) - 1, lane_chunk = lane % CHUNKS, lane_line = lane / CHUNKS;
+        const char* k_lane = (const char*)(p.k + kv * p.head_stride + 8 * lane_chunk) + (int64_t)lane_line * p.line_bytes;
+        const int64_t k_to_v = (const char*)p.v - (const char*)p.k;
+        const uint32_t ring = smem_u32(&sh.ring[warp][0][0][0][0]);
+        // where a tile's keys lie: lanes l and l + 16 find key l's page, -1 for a key that no row sees
+        auto page_of = [&](int key0) -> int {
+            const int key = key0 + (lane & 15);
+            const int entry = key >= seen_low && key < seen_high ? __ldcg(table + (key >> p.page_shift)) : -1;
+            return entry < p.pages ? max(entry, -1) : -1;
+        };
+        // A warp copies LINES lines an instruction, this lane one chunk of one of them
+        const uint32_t stage_at = ring + lane_line * (D * 2);
+        auto fetch = [&](int key0, int page, uint32_t seen, int stage) {
+            const uint32_t to = stage_at + stage * (2 * kTile * D * 2);
+            if (p.page_shift >= 4) {  // the tile's keys, sixteen of a multiple of sixteen, share a page
+                const int first = __shfl_sync(0xffffffffu, page, seen ? __ffs(seen) - 1 : 0);
+                const char* from = k_lane + (uint64_t)(uint32_t)max(first, 0) * p.page_bytes + (uint64_t)(uint32_t)(key0 & line_mask) * p.line_bytes;
+#pragma unroll
+                for (int i = 0; i < kTile / LINES; ++i) {
+                    const uint32_t place = to + i * (LINES * D * 2) + ((lane_chunk ^ ((i * LINES + lane_line) & 7)) << 4);
+                    const bool there = seen >> (i * LINES + lane_line) & 1;
+                    copy16(place, from, there);
+                    copy16(place + kTile * D * 2, from + k_to_v, there);
+                    from += LINES * (uint64_t)p.line_bytes;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kTile / LINES; ++i) {
+                    const int line = i * LINES + lane_line, at = __shfl_sync(0xffffffffu, page, line);
+                    const char* from = k_lane + (int64_t)max(at, 0) * p.page_bytes + ((int64_t)((key0 + line) & line_mask) - lane_line) * p.line_bytes;
+                    const uint32_t place = to + i * (LINES * D * 2) + ((lane_chunk ^ (line & 7)) << 4);
+                    copy16(place, from, at >= 0);
+                    copy16(place + kTile * D * 2, from + k_to_v, at >= 0);
+                }
+            }
+        };
+        int key0 = key_first + warp * kTile, ahead = key0, stage = 0;
+        int page = page_of(ahead);
+        uint32_t seen = __ballot_sync(0xffffffffu, page >= 0) & 0xffff, seen_next = 0;  // the tile's keys that some row sees
+        if (ahead < key_stop) fetch(ahead, page, seen, 0);
+        copies_commit();
+        ahead += kUnit;
+        page = page_of(ahead);
+
+        // queries: scaled, taken apart, as the tensor core's operand registers
+        for (int i = tid; i < RT * STEPS * 32; i += kThreads) {
+            const int l = i & 31, step = (i >> 5) % STEPS, rt = i / (32 * STEPS), row = rt * 8 + (l >> 2);
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // elements 16 step + 2 (l % 4) + {0, 1, 8, 9}
+            if (row < rows) {
+                const int at = row0 + row;
+                const float* from = p.q + (int64_t)(p.starts[r] + at / group) * p.q_stride + (int64_t)(kv * group + at % group) * D + 16 * step + 2 * (l & 3);
+                if (p.wide) {
+                    const float2 v = __ldcg((const float2*)from), w = __ldcg((const float2*)(from + 8));
+                    x[0] = v.x; x[1] = v.y; x[2] = w.x; x[3] = w.y;
+                } else { x[0] = __ldcg(from); x[1] = __ldcg(from + 1); x[2] = __ldcg(from + 8); x[3] = __ldcg(from + 9); }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] *= p.scale * kLog2e;
+            uint4 a;
+            a.x = take_pair<TYPE>(x[0], x[1]);
+            a.z = take_pair<TYPE>(x[2], x[3]);
+            a.y = take_pair<TYPE>(x[0], x[1]);
+            a.w = take_pair<TYPE>(x[2], x[3]);
+            sh.q_hi[rt][step][l] = a;
+            if (PARTS == 3) sh.q_lo[PARTS == 3 ? rt : 0][step][l] = make_uint2(pair_of<TYPE>(x[0], x[1]), pair_of<TYPE>(x[2], x[3]));
+        }
+        __syncthreads();
+
+        float m[RT], sum[RT];
+        float2 acc[RT][D / 8][2];  // sums of the hi parts, and of the parts below them
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             m[rt] = -INFINITY;
             sum[rt] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < VC; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[rt][c][i] = 0.0f;
+            for (int n = 0; n < D / 8; ++n) acc[rt][n][0] = acc[rt][n][1] = make_float2(0.0f, 0.0f);
         }
-
-        // where a tile's keys lie: lane l finds key l's, -1 for a key that no row sees
-        auto entry_of = [&](int key0) -> int {
-            const int key = key0 + (lane & (TK - 1));
-            return key < key_stop ? __ldcg(p.block_table + r * p.table_stride + (key >> p.page_shift)) : -1;
-        };
-        auto place_of = [&](int key0, int entry) -> int64_t {
-            const int key = key0 + (lane & (TK - 1));
-            if (key < seen_low || key >= min(key_stop, seen_high) || entry < 0 || entry >= p.pages) return -1;
-            return entry * p.page_stride + (key & ((1 << p.page_shift) - 1)) * p.line_stride;
-        };
-        const uint16_t *k_head = p.k + kv * p.head_stride, *v_head = p.v + kv * p.head_stride;
-        uint4 kreg[NT][KC];
-        auto load_keys = [&](int64_t place) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int64_t at = __shfl_sync(0xffffffffu, place, 8 * i + g);
-#pragma unroll
-                for (int c = 0; c < KC; ++c) kreg[i][c] = at >= 0 ? load16(k_head + at + 8 * (t4 + 4 * c)) : make_uint4(0, 0, 0, 0);
-            }
-        };
-
-        int key0 = key_first + warp * TK;
-        int64_t place = -1;
-        int entry = -1;
-        if (key0 < key_stop) {
-            place = place_of(key0, entry_of(key0));
-            load_keys(place);
-            entry = entry_of(key0 + kWarps * TK);
-        }
-        for (; key0 < key_stop; key0 += kWarps * TK) {
-            const uint32_t valid = __ballot_sync(0xffffffffu, place >= 0);
-            // values, a chunk of 64 elements ahead of its use
-            uint4 vreg[2][TK / 4];
-            auto load_values = [&](int c) {
-#pragma unroll
-                for (int i = 0; i < TK / 4; ++i) {  // keys 16 s + 2 t4 + {0, 1, 8, 9}
-                    const int64_t at = __shfl_sync(0xffffffffu, place, 16 * (i >> 2) + 2 * t4 + (i & 1) + 8 * ((i >> 1) & 1));
-                    vreg[c & 1][i] = at >= 0 ? load16(v_head + at + 8 * (g + 8 * c)) : make_uint4(0, 0, 0, 0);
-                }
-            };
-            load_values(0);
-
-            // scores: of key 8 i + 2 t4 + {0, 1} and row g
-            float s[RT][NT][2];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float c[NT][4];
-#pragma unroll
-                for (int i = 0; i < NT; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
+        for (; key0 < key_stop; key0 += kUnit, stage ^= 1, seen = seen_next) {
+            const uint32_t keys = ring + stage * (2 * kTile * D * 2), values = keys + kTile * D * 2;
+            __syncwarp();  // the other stage has been read
+            seen_next = __ballot_sync(0xffffffffu, page >= 0) & 0xffff;
+            if (ahead < key_stop) fetch(ahead, page, seen_next, stage ^ 1);
+            copies_commit();
+            ahead += kUnit;
+            page = page_of(ahead);
+            copies_wait<1>();
+            __syncwarp();
+            // scores: of keys 8 i + 2 t4 + {0, 1} and row g
+            float s[RT][2][2];
+            {
+                float c[RT][2][4];
+                const int line = (lane & 7) + (lane & 16 ? 8 : 0), half = lane >> 3 & 1;
 #pragma unroll
                 for (int step = 0; step < STEPS; ++step) {
-                    const uint4 a = q_hi[rt][step][lane];
-                    uint2 lo = make_uint2(0, 0);
-                    if (PARTS == 3) lo = q_lo[rt % (PARTS == 3 ? RT : 1)][step][lane];
+                    uint32_t b[4];
+                    ldmatrix(b, keys + line * (D * 2) + (((2 * step + half) ^ (line & 7)) << 4));
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        const uint4 b = kreg[i][step >> 1];
-                        const uint32_t b0 = step & 1 ? b.z : b.x, b1 = step & 1 ? b.w : b.y;
-                        if (PARTS == 3) mma<TYPE>(c[i], 0, lo.x, 0, lo.y, b0, b1);  // with the small parts
-                        mma<TYPE>(c[i], a.x, a.y, a.z, a.w, b0, b1);
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const uint4 a = sh.q_hi[rt][step][lane];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            mma<TYPE>(c[rt][i], step == 0, a.x, a.y, a.z, a.w, b[2 * i], b[2 * i + 1]);
+                            if (PARTS == 3) {
+                                const uint2 lo = sh.q_lo[PARTS == 3 ? rt : 0][step][lane];
+                                mma<TYPE>(c[rt][i], false, 0, lo.x, 0, lo.y, b[2 * i], b[2 * i + 1]);  // into the rows of the small parts
+                            }
+                        }
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < NT; ++i) { s[rt][i][0] = c[i][0] + c[i][2]; s[rt][i][1] = c[i][1] + c[i][3]; }
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) { s[rt][i][0] = c[rt][i][0] + c[rt][i][2]; s[rt][i][1] = c[rt][i][1] + c[rt][i][3]; }
             }
-            // the next tile's keys, under way from here on
-            const int next = key0 + kWarps * TK;
-            const int64_t next_place = next < key_stop ? place_of(next, entry) : -1;
-            if (next < key_stop) {
-                load_keys(next_place);
-                entry = entry_of(next + kWarps * TK);
-            }
-
             // weights
-            uint32_t w_hi[RT][NT], w_mid[RT][NT], w_lo[RT][PARTS == 3 ? NT : 1];
+            uint32_t w_hi[RT][2], w_mid[RT][2], w_lo[RT][2];
             float old[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 float top = m[rt];
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int at = 8 * i + 2 * t4 + e, key = key0 + at;
-                        if (key < low[rt] || key >= high[rt] || !(valid >> at & 1)) s[rt][i][e] = -INFINITY;
+                        if (key < low[rt] || key >= high[rt] || !(seen >> at & 1)) s[rt][i][e] = -INFINITY;
                         top = fmaxf(top, s[rt][i][e]);
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -255,82 +290,76 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) rq_attention_rows_k
                 m[rt] = top;
                 float add = 0.0f;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
+                for (int i = 0; i < 2; ++i) {
                     float a = exp2_fast(s[rt][i][0] - base), b = exp2_fast(s[rt][i][1] - base);
                     add += a + b;
                     w_hi[rt][i] = take_pair<TYPE>(a, b);
                     w_mid[rt][i] = take_pair<TYPE>(a, b);
-                    if (PARTS == 3) w_lo[rt][i % (PARTS == 3 ? NT : 1)] = pair_of<TYPE>(a, b);
+                    w_lo[rt][i] = PARTS == 3 ? pair_of<TYPE>(a, b) : 0;
                 }
                 sum[rt] = fmaf(sum[rt], old[rt], add);
             }
-
             // A value that one row must not see may be infinite, and 0 * inf is no 0. Where a tile's rows do not see the same keys and a value
             // is not finite, the rows of each token meet the values by themselves, the unseen ones taken out.
-            int token = -1, tokens = 0;
-            const bool partial = !one_token && (key0 < seen_low + (rows - 1) / group + 1 || key0 + TK > position0 + row0 / group + 1);
-
+            const int value_line = (lane & 7) + (lane & 8), value_half = lane >> 4;
+            auto load_values = [&](int n2, uint32_t (&b)[4]) { ldmatrix_transposed(b, values + value_line * (D * 2) + (((2 * n2 + value_half) ^ (value_line & 7)) << 4)); };
+            const int first_token = row0 / group, tokens = (row0 + max(rows, 1) - 1) / group - first_token + 1;
+            bool apart = false;
+            if (!one_token && (key0 < seen_low + tokens || key0 + kTile > position0 + first_token + 1)) {
+                bool fine = true;
 #pragma unroll
-            for (int c = 0; c < VC; ++c) {
-                if (c + 1 < VC) load_values(c + 1);
-                uint4* v = vreg[c & 1];
-                if (partial) {
-                    bool fine = true;
-#pragma unroll
-                    for (int i = 0; i < TK / 4; ++i) fine = fine && finite2<TYPE>(v[i].x) && finite2<TYPE>(v[i].y) && finite2<TYPE>(v[i].z) && finite2<TYPE>(v[i].w);
-                    token = __all_sync(0xffffffffu, fine) ? -1 : row0 / group;
-                    tokens = token < 0 ? 0 : (row0 + rows - 1) / group - token;
+                for (int n2 = 0; n2 < D / 16; ++n2) {
+                    uint32_t b[4];
+                    load_values(n2, b);
+                    fine = fine && finite2<TYPE>(b[0]) && finite2<TYPE>(b[1]) && finite2<TYPE>(b[2]) && finite2<TYPE>(b[3]);
                 }
-                float scaled[RT];
+                apart = !__all_sync(0xffffffffu, fine);
+            }
+            if (!apart) {
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) scaled[rt] = old[rt];
-                for (int pass = 0; pass <= tokens; ++pass) {
-                    uint32_t shown = 0xffffffffu, row_on[RT];
+                for (int n2 = 0; n2 < D / 16; ++n2) {
+                    uint32_t b[4];
+                    load_values(n2, b);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) row_on[rt] = 0xffffffffu;
-                    if (token >= 0) {
-                        const int position = position0 + token + pass, from = p.window > 0 ? max(position - p.window + 1, 0) : 0;
-                        shown = 0;
+                    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                        for (int i = 0; i < TK; ++i) shown |= (key0 + i >= from && key0 + i <= position ? 1u : 0u) << i;
+                        for (int i = 0; i < 2; ++i) {
+                            float d[4];
+                            mma<TYPE>(d, true, w_hi[rt][0], w_mid[rt][0], w_hi[rt][1], w_mid[rt][1], b[2 * i], b[2 * i + 1]);
+                            if (PARTS == 3) mma<TYPE>(d, false, 0, w_lo[rt][0], 0, w_lo[rt][1], b[2 * i], b[2 * i + 1]);
+                            add_scaled(acc[rt][2 * n2 + i], old[rt], d);
+                        }
+                }
+            } else {
+                for (int token = first_token; token < first_token + tokens; ++token) {
+                    const int position = position0 + token, from = p.window > 0 ? position - p.window + 1 : 0;
+                    uint32_t shown[2];  // the words of keys 8 i + 2 t4 + {0, 1}
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) row_on[rt] = (row0 + rt * 8 + g) / group == token + pass ? 0xffffffffu : 0;
+                    for (int i = 0; i < 2; ++i) {
+                        const int key = key0 + 8 * i + 2 * t4;
+                        shown[i] = (key >= from && key <= position ? 0xffffu : 0) | (key + 1 >= from && key + 1 <= position ? 0xffff0000u : 0);
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float d[RT][4];
+                    for (int n2 = 0; n2 < D / 16; ++n2) {
+                        uint32_t b[4];
+                        load_values(n2, b);
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) d[rt][0] = d[rt][1] = d[rt][2] = d[rt][3] = 0.0f;
+                        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                        for (int step = 0; step < TK / 16; ++step) {
-                            uint32_t x[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint4 line = v[4 * step + i];
-                                x[i] = j / 2 == 0 ? line.x : (j / 2 == 1 ? line.y : (j / 2 == 2 ? line.z : line.w));
-                                if (token >= 0 && !(shown >> (16 * step + 2 * t4 + (i & 1) + 8 * (i >> 1)) & 1)) x[i] = 0;
+                            for (int i = 0; i < 2; ++i) {
+                                float d[4];
+                                const uint32_t b0 = b[2 * i] & shown[0], b1 = b[2 * i + 1] & shown[1];
+                                mma<TYPE>(d, true, w_hi[rt][0], w_mid[rt][0], w_hi[rt][1], w_mid[rt][1], b0, b1);
+                                if (PARTS == 3) mma<TYPE>(d, false, 0, w_lo[rt][0], 0, w_lo[rt][1], b0, b1);
+                                if ((row0 + rt * 8 + g) / group != token) continue;
+                                add_scaled(acc[rt][2 * n2 + i], old[rt], d);
                             }
-                            const uint32_t b0 = __byte_perm(x[0], x[1], j & 1 ? 0x7632 : 0x5410), b1 = __byte_perm(x[2], x[3], j & 1 ? 0x7632 : 0x5410);
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) {
-                                const uint32_t on = row_on[rt];
-                                if (PARTS == 3) mma<TYPE>(d[rt], 0, w_lo[rt][(2 * step) % (PARTS == 3 ? NT : 1)] & on, 0, w_lo[rt][(2 * step + 1) % (PARTS == 3 ? NT : 1)] & on, b0, b1);
-                                mma<TYPE>(d[rt], w_hi[rt][2 * step] & on, w_mid[rt][2 * step] & on, w_hi[rt][2 * step + 1] & on, w_mid[rt][2 * step + 1] & on, b0, b1);
-                            }
-                        }
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) {
-                            const bool on = row_on[rt] != 0;
-                            acc[rt][c][j] = fmaf(acc[rt][c][j], scaled[rt], on ? d[rt][0] + d[rt][2] : 0.0f);
-                            acc[rt][c][8 + j] = fmaf(acc[rt][c][8 + j], scaled[rt], on ? d[rt][1] + d[rt][3] : 0.0f);
-                        }
                     }
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) scaled[rt] = 1.0f;
                 }
             }
-            place = next_place;
         }
+        copies_wait<0>();
+        __syncthreads();  // the sums go where the ring was
 
         // ---- the four warps' sums, and other CTAs' ------------------------------------------------------
 #pragma unroll
@@ -339,10 +368,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) rq_attention_rows_k
             sum[rt] += __shfl_xor_sync(0xffffffffu, sum[rt], 2);
             if (t4 == 0) { warp_max[warp][rt * 8 + g] = m[rt]; warp_sum[warp][rt * 8 + g] = sum[rt]; }
 #pragma unroll
-            for (int c = 0; c < VC; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *(float4*)&out[warp][rt * 8 + g][64 * c + 16 * t4 + i] = make_float4(acc[rt][c][i], acc[rt][c][i + 1], acc[rt][c][i + 2], acc[rt][c][i + 3]);
+            for (int n = 0; n < D / 8; ++n) *(float2*)&sh.out[warp][rt * 8 + g][8 * n + 2 * t4] = make_float2(acc[rt][n][0].x + acc[rt][n][1].x, acc[rt][n][0].y + acc[rt][n][1].y);
         }
         __syncthreads();
         const int64_t first_cta = ((item_begin + 1) * ctas - 1) / total, last_cta = (item_end * ctas - 1) / total;
@@ -368,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) rq_attention_rows_k
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float f = exp2_fast(warp_max[w][row] - base);
-                const float4 o = *(const float4*)&out[w][row][e];
+                const float4 o = *(const float4*)&sh.out[w][row][e];
                 v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
                 weight = fmaf(warp_sum[w][row], f, weight);
             }
@@ -482,9 +508,8 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
     AttentionParams p = {};
     p.q = q; p.y = y; p.k = (const uint16_t*)cache->k; p.v = (const uint16_t*)cache->v; p.block_table = block_table; p.starts = starts; p.lengths = lengths;
     p.partial = (float*)ctx->attn_scratch; p.arrived = (uint32_t*)(ctx->attn_scratch + partial_bytes());
-    p.q_stride = q_t_stride; p.y_stride = y_t_stride; p.table_stride = table_stride; p.page_stride = cache->page_stride; p.head_stride = cache->head_stride;
-    p.line_stride = cache->line_stride; p.pages = cache->pages; p.tokens = tokens; p.requests = requests; p.q_heads = q_heads; p.kv_heads = cache->heads;
-    p.table_width = table_width; p.window = window; p.scale = scale;
+    p.q_stride = q_t_stride; p.y_stride = y_t_stride; p.table_stride = table_stride; p.head_stride = cache->head_stride; p.pages = cache->pages; p.tokens = tokens; p.requests = requests; p.q_heads = q_heads; p.kv_heads = cache->heads;
+    p.table_width = table_width; p.window = window; p.scale = scale; p.page_bytes = (uint32_t)(2 * cache->page_stride); p.line_bytes = (uint32_t)(2 * cache->line_stride);
     p.wide = (((uintptr_t)q | (uintptr_t)y) & 15) == 0 && (tokens == 1 || ((q_t_stride | y_t_stride) & 3) == 0);
     while (1 << p.page_shift < cache->page_size) ++p.page_shift;
     // rows that meet a key together: eight, or sixteen where a request may have more

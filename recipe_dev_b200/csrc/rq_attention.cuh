@@ -11,7 +11,8 @@ struct AttentionParams {
     const int32_t *block_table, *starts, *lengths;
     float* partial;      // sums of rows whose keys several CTAs share
     uint32_t* arrived;   // per CTA: how many have left their part of the rows that begin there; zero between calls
-    int64_t q_stride, y_stride, table_stride, page_stride, head_stride, line_stride, pages;
+    int64_t q_stride, y_stride, table_stride, head_stride, pages;
+    uint32_t page_bytes, line_bytes;
     int tokens, requests, q_heads, kv_heads, table_width, page_shift, window;
     float scale;
     int wide;  // q and y allow 16-byte accesses

@@ -112,6 +112,7 @@ int rqserve::check_cache(const char* who, const rq_kv_cache* c) {
     if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return rq_fail(RQ_ERR_INVALID, "%s: the cache's pointers must be 16-byte aligned", who);
     if (c->page_stride < 0 || c->head_stride < 0 || c->line_stride < 0 || (c->page_stride | c->head_stride | c->line_stride) & 7)
         return rq_fail(RQ_ERR_INVALID, "%s: the cache's strides must be non-negative multiples of 8 elements", who);
+    if (c->page_stride >= (int64_t)1 << 31 || c->line_stride >= (int64_t)1 << 31) return rq_fail(RQ_ERR_LIMIT, "%s: the cache's page and line strides must be below 2^31 elements", who);
     return RQ_OK;
 }
 
