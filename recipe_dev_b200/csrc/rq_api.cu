@@ -172,6 +172,15 @@ static const char* wait_code_text(int code) {
         case 22: return "matvec over a decode-only format: a row's bytes never arrived";
         case 21: return "wait self-test: the barrier nothing arrives on";
         case 31: return "exchange: a peer's arrival flag never came";
+        case 41: return "attention, softmax warps: a tile's sums were never finished";
+        case 42: return "attention, softmax warps: scores were never finished";
+        case 43: return "attention, softmax warps: the queries' place never came free";
+        case 44: return "attention, loading warps: a slot never came free";
+        case 45: return "attention, issuing warp: a tile of keys or values never arrived";
+        case 46: return "attention, issuing warp: the queries never arrived";
+        case 47: return "attention, issuing warp: weights never arrived";
+        case 48: return "attention, issuing warp: a tile's sums were never taken over";
+        case 49: return "attention, issuing warp: the products never completed";
         default: return "unknown wait";
     }
 }

@@ -437,18 +437,14 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
     }
 }
 
-// The work area: parts of rows for every CTA of the largest grid, and the counts of those that have left theirs
-constexpr int kMostCtas = 148 * 4;
-size_t partial_bytes() { return (size_t)kMostCtas * 2 * 16 * (256 + 2) * sizeof(float); }
-
 int ensure_work_area(rq_ctx* ctx) {
     if (ctx->attn_scratch) return RQ_OK;
     if (ctx->recording) return rq_fail(RQ_ERR_INVALID, "a recorded rq_attention needs its work area: call rq_attention_reserve before rq_sequence_begin");
-    const size_t bytes = partial_bytes() + kMostCtas * sizeof(uint32_t);
+    const size_t bytes = kPartialBytes + kRowCtas * sizeof(uint32_t);
     uint8_t* area = nullptr;
     cudaError_t e = cudaMalloc(&area, bytes);
     if (e != cudaSuccess) return rq_fail(RQ_ERR_ALLOC, "attention's work area of %zu bytes: %s", bytes, cudaGetErrorString(e));
-    e = cudaMemset(area + partial_bytes(), 0, kMostCtas * sizeof(uint32_t));
+    e = cudaMemset(area + kPartialBytes, 0, kRowCtas * sizeof(uint32_t));
     if (e == cudaSuccess) e = cudaDeviceSynchronize();  // streams that do not wait for the default one may use it next
     if (e != cudaSuccess) { cudaFree(area); return rq_fail(RQ_ERR_CUDA, "attention's work area: %s", cudaGetErrorString(e)); }
     ctx->attn_scratch = area;
@@ -467,7 +463,7 @@ int launch_rows(rq_ctx* ctx, const AttentionParams& p, cudaStream_t s) {
         resident = n < 1 ? 1 : (n > 4 ? 4 : n);
     }
     const int ctas = ctx->sm_count * resident;
-    return launch(kernel, dim3((unsigned)(ctas < kMostCtas ? ctas : kMostCtas)), kThreads, smem, s, p);
+    return launch(kernel, dim3((unsigned)(ctas < kRowCtas ? ctas : kRowCtas)), kThreads, smem, s, p);
 }
 
 template <int D>
@@ -507,13 +503,16 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
     if (rc) return rc;
     AttentionParams p = {};
     p.q = q; p.y = y; p.k = (const uint16_t*)cache->k; p.v = (const uint16_t*)cache->v; p.block_table = block_table; p.starts = starts; p.lengths = lengths;
-    p.partial = (float*)ctx->attn_scratch; p.arrived = (uint32_t*)(ctx->attn_scratch + partial_bytes());
+    p.partial = (float*)ctx->attn_scratch; p.arrived = (uint32_t*)(ctx->attn_scratch + kPartialBytes);
     p.q_stride = q_t_stride; p.y_stride = y_t_stride; p.table_stride = table_stride; p.head_stride = cache->head_stride; p.pages = cache->pages; p.tokens = tokens; p.requests = requests; p.q_heads = q_heads; p.kv_heads = cache->heads;
     p.table_width = table_width; p.window = window; p.scale = scale; p.page_bytes = (uint32_t)(2 * cache->page_stride); p.line_bytes = (uint32_t)(2 * cache->line_stride);
     p.wide = (((uintptr_t)q | (uintptr_t)y) & 15) == 0 && (tokens == 1 || ((q_t_stride | y_t_stride) & 3) == 0);
     while (1 << p.page_shift < cache->page_size) ++p.page_shift;
+    p.error_flag = ctx->error_flag; p.wait_ns = ctx->wait_limit_ns;
+    const int64_t rows = (int64_t)(max_fresh > 0 ? (max_fresh < tokens ? max_fresh : tokens) : tokens) * group;
+    if (rows > 32 && cache->head_dim <= 128) return launch_tensor(ctx, p, cache->head_dim, cache->type, rows <= 128, s);
     // rows that meet a key together: eight, or sixteen where a request may have more
-    const bool two = (int64_t)(max_fresh > 0 ? max_fresh : tokens) * group > 8;
+    const bool two = rows > 8;
     if (cache->head_dim == 64) return launch_rows<64>(ctx, p, cache->type, two, s);
     if (cache->head_dim == 128) return launch_rows<128>(ctx, p, cache->type, two, s);
     return launch_rows<256>(ctx, p, cache->type, two, s);
