@@ -172,6 +172,8 @@ static const char* wait_code_text(int code) {
         case 22: return "matvec over a decode-only format: a row's bytes never arrived";
         case 21: return "wait self-test: the barrier nothing arrives on";
         case 31: return "exchange: a peer's arrival flag never came";
+        case 40: return "attention: the next item never came";
+        case 50: return "attention, dealing warp: an item's place never came free";
         case 41: return "attention, softmax warps: a tile's sums were never finished";
         case 42: return "attention, softmax warps: scores were never finished";
         case 43: return "attention, softmax warps: the queries' place never came free";

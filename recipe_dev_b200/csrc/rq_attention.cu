@@ -506,7 +506,8 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
     p.partial = (float*)ctx->attn_scratch; p.arrived = (uint32_t*)(ctx->attn_scratch + kPartialBytes);
     p.q_stride = q_t_stride; p.y_stride = y_t_stride; p.table_stride = table_stride; p.head_stride = cache->head_stride; p.pages = cache->pages; p.tokens = tokens; p.requests = requests; p.q_heads = q_heads; p.kv_heads = cache->heads;
     p.table_width = table_width; p.window = window; p.scale = scale; p.page_bytes = (uint32_t)(2 * cache->page_stride); p.line_bytes = (uint32_t)(2 * cache->line_stride);
-    p.wide = (((uintptr_t)q | (uintptr_t)y) & 15) == 0 && (tokens == 1 || ((q_t_stride | y_t_stride) & 3) == 0);
+    auto aligned = [&](int bytes) { return (((uintptr_t)q | (uintptr_t)y) & (bytes - 1)) == 0 && (tokens == 1 || ((q_t_stride | y_t_stride) & (bytes / 4 - 1)) == 0); };
+    p.wide = (aligned(16) ? 1 : 0) | (aligned(32) ? 2 : 0);
     while (1 << p.page_shift < cache->page_size) ++p.page_shift;
     p.error_flag = ctx->error_flag; p.wait_ns = ctx->wait_limit_ns;
     const int64_t rows = (int64_t)(max_fresh > 0 ? (max_fresh < tokens ? max_fresh : tokens) : tokens) * group;

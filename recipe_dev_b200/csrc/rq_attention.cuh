@@ -15,7 +15,7 @@ struct AttentionParams {
     uint32_t page_bytes, line_bytes;
     int tokens, requests, q_heads, kv_heads, table_width, page_shift, window;
     float scale;
-    int wide;  // q and y allow 16-byte accesses
+    int wide;  // q and y allow accesses of 16 bytes (1), of 32 (2)
     int* error_flag;
     unsigned long long wait_ns;
 };
