@@ -173,16 +173,17 @@ static const char* wait_code_text(int code) {
         case 21: return "wait self-test: the barrier nothing arrives on";
         case 31: return "exchange: a peer's arrival flag never came";
         case 40: return "attention: the next item never came";
-        case 50: return "attention, dealing warp: an item's place never came free";
         case 41: return "attention, softmax warps: a tile's sums were never finished";
         case 42: return "attention, softmax warps: scores were never finished";
         case 43: return "attention, softmax warps: the queries' place never came free";
-        case 44: return "attention, loading warps: a slot never came free";
+        case 44: return "attention, loading warp: a slot never came free";
         case 45: return "attention, issuing warp: a tile of keys or values never arrived";
         case 46: return "attention, issuing warp: the queries never arrived";
         case 47: return "attention, issuing warp: weights never arrived";
         case 48: return "attention, issuing warp: a tile's sums were never taken over";
         case 49: return "attention, issuing warp: the products never completed";
+        case 50: return "attention, loading warp: an item's place never came free";
+        case 51: return "attention, mending warp: a tile of values never arrived";
         default: return "unknown wait";
     }
 }
@@ -275,19 +276,25 @@ static int alloc_weight(rq_ctx* ctx, int type, int64_t rows, int64_t cols, rq_we
     return RQ_OK;
 }
 
-int rq_make_tile_map(rq_weight* w) {
-    w->has_tile_map = 0;
-    if (!rq_type_has_fast_path(w->type)) return RQ_OK;
-    typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static EncodeTiled encode = nullptr;
+int rq_tensor_map_encoder(rq_encode_tiled* out) {
+    static rq_encode_tiled encode = nullptr;
     if (!encode) {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult found;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess || !fn)
             return rq_fail(RQ_ERR_CUDA, "the driver does not export cuTensorMapEncodeTiled");
-        encode = (EncodeTiled)fn;
+        encode = (rq_encode_tiled)fn;
     }
+    *out = encode;
+    return RQ_OK;
+}
+
+int rq_make_tile_map(rq_weight* w) {
+    w->has_tile_map = 0;
+    if (!rq_type_has_fast_path(w->type)) return RQ_OK;
+    rq_encode_tiled encode = nullptr;
+    const int found = rq_tensor_map_encoder(&encode);
+    if (found) return found;
     // bytes of one row of a tile: a superblock of the K-quants, 128 bytes (128 values, 256 values) of Q8_0 and Q4_0. Tiles of 128-byte
     // rows land swizzled, so that threads on adjacent rows read different banks; 144 and 208 bytes are odd counts of sixteen.
     const bool kquant = w->type == RQ_Q4_K || w->type == RQ_Q6_K;

@@ -511,7 +511,10 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
     while (1 << p.page_shift < cache->page_size) ++p.page_shift;
     p.error_flag = ctx->error_flag; p.wait_ns = ctx->wait_limit_ns;
     const int64_t rows = (int64_t)(max_fresh > 0 ? (max_fresh < tokens ? max_fresh : tokens) : tokens) * group;
-    if (rows > 32 && cache->head_dim <= 128) return launch_tensor(ctx, p, cache->head_dim, cache->type, rows <= 128, s);
+    if (rows > 32) {
+        rc = launch_tensor(ctx, p, *cache, rows <= 128, s);
+        if (rc != RQ_ERR_UNSUPPORTED) return rc;
+    }
     // rows that meet a key together: eight, or sixteen where a request may have more
     const bool two = rows > 8;
     if (cache->head_dim == 64) return launch_rows<64>(ctx, p, cache->type, two, s);

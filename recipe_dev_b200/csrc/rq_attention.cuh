@@ -26,8 +26,9 @@ constexpr int kTensorCtas = 148, kRowCtas = 148 * 4;
 constexpr size_t kTensorPartial = (size_t)kTensorCtas * 2 * 2 * 128 * (128 + 2), kRowPartial = (size_t)kRowCtas * 2 * 16 * (256 + 2);  // floats
 constexpr size_t kPartialBytes = sizeof(float) * (kTensorPartial > kRowPartial ? kTensorPartial : kRowPartial);
 
-// Rows by the hundred, head_dim 64 or 128 (rq_attention_tc.cu); one_tile: at most 128 rows a request and key head
-int launch_tensor(rq_ctx* ctx, const AttentionParams& p, int head_dim, int type, bool one_tile, cudaStream_t s);
+// Rows by the hundred (rq_attention_tc.cu); one_tile: at most 128 rows a request and key head. RQ_ERR_UNSUPPORTED (no error text) = a cache that it does not
+// serve: 256 elements a head, pages of fewer than eight positions, strides of zero.
+int launch_tensor(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool one_tile, cudaStream_t s);
 
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are 2^(s - max + kRaise): an f16 part below 2^-14 loses bits, raised by 2^12 that is a weight of 2^-26 of the row's largest

@@ -92,6 +92,10 @@ int rq_launch_export(const rq_weight* w, uint8_t* dev_blocks, cudaStream_t s);
 int rq_launch_dequant(const rq_weight* w, float* out, cudaStream_t s);
 int rq_launch_gemv_generic(rq_ctx* ctx, const rq_weight* w, const float* x, int64_t sk, int64_t st, int tokens, float* y, int64_t yn, int64_t yt, cudaStream_t s);
 int rq_launch_gather(const rq_weight* w, const int32_t* ids, int tokens, float* y, int64_t yn, int64_t yt, cudaStream_t s);
+// the driver's cuTensorMapEncodeTiled
+typedef CUresult (*rq_encode_tiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int rq_tensor_map_encoder(rq_encode_tiled* out);
 // fills w->tile_map for the four formats with kernels of their own (no-op for the others)
 int rq_make_tile_map(rq_weight* w);
 int rq_launch_requant_q8_0(const rq_weight* src, rq_weight* dst, cudaStream_t s);
