@@ -15,6 +15,8 @@
 // each: 2054 us for 1 x 262144 and 1863 us for 64 x 262144.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "rq_serve.cuh"
 
 using namespace rqserve;
@@ -22,7 +24,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kList = 1024, kMostCtas = 16;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kList = kThreads, kMostCtas = 16;
 constexpr int kShare = 16384;  // logits of a CTA in shared memory
 constexpr float kFade = 28.0f; // exp(-28) < 2^-40
 
@@ -40,6 +42,7 @@ typedef unsigned long long u64;
 // NaN as -inf, -0 as +0
 __device__ __forceinline__ float cleaned(float x) { return x != x ? -INFINITY : x + 0.0f; }
 __device__ __forceinline__ uint32_t ascending(float x) { const uint32_t u = __float_as_uint(x); return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u); }
+__device__ __forceinline__ float value_of(u64 key) { const uint32_t b = (uint32_t)(key >> 32); return __uint_as_float(b >> 31 ? b ^ 0x80000000u : ~b); }
 __device__ __forceinline__ u64 rank_key(float x, int index) { return (u64)ascending(x) << 32 | (uint32_t)~index; }
 // the weight over 2^40; equal to the largest logit: one, also where that is +inf
 __device__ __forceinline__ float weight(float x, float top, float temperature) {
@@ -49,22 +52,126 @@ __device__ __forceinline__ float weight(float x, float top, float temperature) {
 __device__ __forceinline__ u64 mass_of(float e) { return (u64)(e * 1099511627776.0f); }
 
 struct Shared {
-    u64 hist[kBins], merged[kBins];
+    // this CTA's sums, in words of 16, 13 and 12 bits of their terms: a 64-bit atomic addition in shared memory is a loop, and one that carries waits for an answer
+    uint32_t low[kBins], mid[kBins], high[kBins];
     u64 list[kList], list_mass[kList];
+    u64 merged[kBins], list_sum[kList];
     u64 warp_sum[kWarps], warp_count[kWarps];
     u64 sum, count;          // this CTA's kept weights and tokens
     u64 bound, before;       // the first CTA's answer; what lies before the part that was found
-    u64 total;
-    int part;
+    int part, sharing, best;
     uint32_t listed[16];     // the first CTA's lists, one after another
     float warp_top[kWarps], top;
     int chosen_warp;
     u64 chosen_want;
 };
 
+// Sum over the CTA; every thread gets it
+__device__ __forceinline__ u64 block_sum(u64 v, u64* warp_sums) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    __syncthreads();
+    if (lane == 0) warp_sums[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < kWarps ? warp_sums[lane] : 0;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+}
+
+// Sorts the first CTA's list by falling keys, the masses with them, and adds the masses up: list_sum[i] = those of keys above and at i. A bitonic network, a
+// thread an entry: steps within a warp by shuffles, between warps through shared memory. (Ranks by comparison with all others took 9 us for 330.)
+__device__ void sort_list(Shared& sh, int n) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int size = 32;
+    while (size < n) size <<= 1;
+    __syncthreads();
+    u64 key = tid < n ? sh.list[tid] : 0, mass = tid < n ? sh.list_mass[tid] : 0;
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            u64 other, other_mass;
+            if (j >= 32) {
+                __syncthreads();
+                sh.list[tid] = key;
+                sh.list_mass[tid] = mass;
+                __syncthreads();
+                other = sh.list[tid ^ j];
+                other_mass = sh.list_mass[tid ^ j];
+            } else {
+                other = __shfl_xor_sync(0xffffffffu, key, j);
+                other_mass = __shfl_xor_sync(0xffffffffu, mass, j);
+            }
+            const bool larger_here = ((tid & k) == 0) == ((tid & j) == 0);
+            if (key != other && (other > key) == larger_here) { key = other; mass = other_mass; }
+        }
+    u64 scan = mass;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) { const u64 o = __shfl_up_sync(0xffffffffu, scan, off); if (lane >= off) scan += o; }
+    __syncthreads();
+    if (lane == 31) sh.warp_sum[warp] = scan;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) scan += sh.warp_sum[w];
+    sh.list[tid] = key;
+    sh.list_mass[tid] = mass;
+    sh.list_sum[tid] = scan;
+    __syncthreads();
+}
+
+// Up to a thread's worth of candidates, every token of weight down to the last that top_k could keep among them: a thread has one and compares it with all
+__device__ void draw_from_list(const SampleParams& p, Shared& sh, int row, float top, float temperature, int top_k, float top_p, float min_p) {
+    const int tid = threadIdx.x, n = (int)sh.listed[0];
+    if (tid < n) sh.list_mass[tid] = mass_of(weight(value_of(sh.list[tid]), top, temperature));
+    sort_list(sh, n);
+    const u64 key = tid < n ? sh.list[tid] : 0, mass = tid < n ? sh.list_mass[tid] : 0, before = tid < n ? sh.list_sum[tid] - mass : 0;
+    const float x = value_of(key);
+    const double target = (double)top_p * (double)sh.list_sum[min(top_k, n) - 1];
+    const bool kept = tid < n && tid < top_k && (top_p >= 1.0f || (double)before < target || tid == 0) && (x == top || weight(x, top, temperature) >= min_p);
+    const u64 mine = kept ? mass : 0;
+    const u64 total = block_sum(mine, sh.warp_sum), tokens = block_sum(mine != 0, sh.warp_count);
+    // in the order of their indices: those are the complement of the keys' low halves
+    __syncthreads();
+    if (tid < n) { sh.list[tid] = (uint32_t)key; sh.list_mass[tid] = mine; }
+    sort_list(sh, n);
+    u64 want = (u64)(fmin(fmax((double)p.uniform[row], 0.0), 1.0) * (double)total);
+    if (want >= total) want = total - 1;
+    if (tid < n) {
+        const u64 w = sh.list_mass[tid], upto = sh.list_sum[tid];
+        if (upto > want && upto - w <= want) {
+            p.token[row] = (int32_t)~(uint32_t)sh.list[tid];
+            if (p.probability) p.probability[row] = (float)((double)w / (double)total);
+            if (p.kept) p.kept[row] = (int32_t)tokens;
+        }
+    }
+}
+
+// The weight's division by the temperature, one for a row, as a product with its reciprocal and a correction by the remainder (Markstein, 1990): rounded as
+// the quotient is, unless the divisor's fraction is all ones; far from where a step of it could overflow or lose bits.
+struct Weigher {
+    float top, temperature, reciprocal;
+    bool quick;
+    __device__ Weigher(float top_, float temperature_) : top(top_), temperature(temperature_), reciprocal(1.0f / temperature_) {
+        quick = top < INFINITY && temperature > 1e-15f && temperature < 1e15f && (__float_as_uint(temperature) & 0x7fffffu) != 0x7fffffu;
+    }
+    template <bool QUICK> __device__ __forceinline__ float share(float x) const {  // (of the largest logit itself: exp(0) = 1)
+        if (!QUICK) return weight(x, top, temperature);
+        const float n = x - top, q = n * reciprocal;
+        return expf(fmaf(fmaf(-q, temperature, n), reciprocal, q));
+    }
+    __device__ u64 operator()(float x) const { return mass_of(quick ? share<true>(x) : share<false>(x)); }
+};
+__device__ __forceinline__ u64 sum_of(const Shared& sh, int bin) { return ((u64)sh.high[bin] << 29) + ((u64)sh.mid[bin] << 16) + sh.low[bin]; }
+__device__ __forceinline__ void clear(Shared& sh) { *(uint2*)&sh.low[2 * threadIdx.x] = *(uint2*)&sh.mid[2 * threadIdx.x] = *(uint2*)&sh.high[2 * threadIdx.x] = make_uint2(0, 0); }
+__device__ __forceinline__ void add_to(Shared& sh, int bin, u64 v) {
+    const uint32_t lo = (uint32_t)v & 0xffff, mid = (uint32_t)(v >> 16) & 0x1fff, hi = (uint32_t)(v >> 29);
+    if (lo) atomicAdd(&sh.low[bin], lo);  // (at most 2^16 terms a CTA)
+    if (mid) atomicAdd(&sh.mid[bin], mid);
+    if (hi) atomicAdd(&sh.high[bin], hi);
+}
+
 // STAGED: the share lies in shared memory, cleaned; otherwise it is read again
 template <bool STAGED>
-__global__ void __launch_bounds__(kThreads) rq_sample_kernel(SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) {
     extern __shared__ __align__(16) float staged[];
     __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
@@ -72,36 +179,29 @@ __global__ void __launch_bounds__(kThreads) rq_sample_kernel(SampleParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = rank * p.share, count = max(min(p.vocabulary - first, p.share), 0);
     // a warp has neighbouring logits, so that sums in index order are sums of warps
-    const int warp_share = p.share / kWarps, begin = warp * warp_share, end = min(begin + warp_share, count);
+    const int warp_share = p.share / kWarps, begin = warp * warp_share, stop = begin + warp_share, end = min(stop, count);  // (a multiple of 128)
     launch_dependents();
-    for (int b = tid; b < kBins; b += kThreads) sh.hist[b] = 0;
+    for (int b = tid; b < kBins; b += kThreads) sh.low[b] = sh.mid[b] = sh.high[b] = 0;
     if (tid < 16) sh.listed[tid] = 0;
+    if (tid == 0) sh.best = p.vocabulary;
     Shared* const leader = cluster.map_shared_rank(&sh, 0);
     wait_for_previous();
     const float* x = p.logits + row * p.stride + first;
     const float temperature = p.temperature ? p.temperature[row] : 1.0f, top_p = p.top_p ? p.top_p[row] : 1.0f, min_p = p.min_p ? p.min_p[row] : 0.0f;
-    const int top_k = !(temperature > 0.0f) ? 1 : (p.top_k && p.top_k[row] > 0 ? p.top_k[row] : p.vocabulary);
+    const int top_k = (p.top_k && p.top_k[row] > 0 ? p.top_k[row] : p.vocabulary);
     auto at = [&](int i) { return STAGED ? staged[i] : cleaned(__ldcg(x + i)); };
 
     // ---- the largest logit ----------------------------------------------------------------------------
     float top = -INFINITY;
-    {
-        int i = begin + lane;
-        for (; i + 7 * 32 < end; i += 8 * 32) {
-            float v[8];
+    for (int i = begin + lane; i < stop; i += 128 * 2) {
+        float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = __ldcg(x + i + 32 * k);
+        for (int k = 0; k < 8; ++k) v[k] = i + 32 * k < end ? __ldcg(x + i + 32 * k) : -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                v[k] = cleaned(v[k]);
-                if (STAGED) staged[i + 32 * k] = v[k];
-                top = fmaxf(top, v[k]);
-            }
-        }
-        for (; i < end; i += 32) {
-            const float v = cleaned(__ldcg(x + i));
-            if (STAGED) staged[i] = v;
-            top = fmaxf(top, v);
+        for (int k = 0; k < 8; ++k) {
+            v[k] = cleaned(v[k]);
+            if (STAGED && i + 32 * k < stop) staged[i + 32 * k] = v[k];
+            top = fmaxf(top, v[k]);
         }
     }
 #pragma unroll
@@ -117,130 +217,272 @@ __global__ void __launch_bounds__(kThreads) rq_sample_kernel(SampleParams p) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
 
+    // Four logits of a thread at a time, side by side; -inf past the end
+    auto each_four = [&](auto&& use) {
+#pragma unroll 1
+        for (int i = begin + lane; i < stop; i += 128) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = STAGED || i + 32 * k < end ? at(i + 32 * k) : -INFINITY;
+            use(v, i);
+        }
+    };
+
     // ---- bounds ------------------------------------------------------------------------------------
-    const float limit = kFade * temperature, scale = (float)kBins / limit;
-    auto part_of = [&](float v) { const float d = top - v; return v == top ? 0 : (int)fminf(d * scale, (float)(kBins - 1)); };
-    auto fades = [&](float v) { return v != top && !(top - v <= limit); };
+    const Weigher weigh(top, temperature);
+    const float limit = fminf(kFade * temperature, 3e38f), scale = (float)kBins / limit;
+    auto floor_of = [](float place) { return (int)(__float_as_uint(__fadd_rd(fminf(place, (float)(kBins - 1)), 8388608.0f)) & 0x7fffffu); };  // 0 <= place, up to the last part
+    auto part_of = [&](float v) { return v == top ? 0 : floor_of((top - v) * scale); };
+    auto sub_of = [&](float v) { const float place = (top - v) * scale; return v == top ? 0 : floor_of((place - (float)floor_of(place)) * (float)kBins); };
+    // What lies so far below weighs nothing: by one comparison (the rounding of this value takes no logit's weight, for they are rounded alike)
+    const float fade = top < INFINITY ? fmaxf(top - limit, -3.4e38f) : top;
+    auto fades = [&](float v) { return v < fade; };
+    // A pass's loop for either way to divide (a branch around each would keep the steps of four logits from overlapping)
+    auto quickly = [&](auto&& pass) {
+        if (weigh.quick) pass(std::true_type());
+        else pass(std::false_type());
+    };
+    // Tokens whose key is at least a bound: (value, index), without putting the key together
+    struct Floor { float value; int index; };
+    auto floor_at = [&](u64 key, float least) -> Floor {
+        const float v = key ? value_of(key) : -INFINITY;
+        return v >= least ? Floor{v, (int)(~(uint32_t)key) - first} : Floor{least, 0x7fffffff};
+    };
+    auto above = [](const Floor& f, float v, int i) { return v > f.value || (v == f.value && i <= f.index); };
     int lists = 0;
+    bool few = false;
 
     // Adds up the CTAs' histograms and finds the last key's part: where the sum from the largest keys down (bins in the order given by `down`) reaches what is wanted.
     // `before`: the sum above the interval. False: it is not reached.
-    auto find = [&](bool by_mass, u64 want, double share_of_mass, bool first_round, bool down, u64& before, int& part) -> bool {
-        cluster.sync();  // all histograms are complete
-        const int mine = kBins / ctas;
-        for (int i = tid; i < mine; i += kThreads) {
-            const int b = rank * mine + i;
-            u64 sum = 0;
-            for (int c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(&sh, c)->hist[b];
-            for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&sh, c)->merged[b] = sum;
-        }
-        cluster.sync();
-        // two neighbouring parts a thread, from the largest keys down
-        const int a = 2 * tid, b0 = down ? kBins - 1 - a : a, b1 = down ? b0 - 1 : a + 1;
-        const u64 m0 = sh.merged[b0], m1 = sh.merged[b1];
-        sh.hist[a] = sh.hist[a + 1] = 0;
+    auto reached_by = [](bool by_mass, u64 want, double target) { return [=](u64 s) { return by_mass ? (double)s >= target : s >= want; }; };
+    // Which of the parts, two a thread in falling order of their keys, is the one in which the sum is reached, and the sum before it
+    auto reach_in = [&](u64 m0, u64 m1, int b0, int b1, auto&& reached, u64& before, int& part) -> bool {
         u64 scan = m0 + m1;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) { const u64 o = __shfl_up_sync(0xffffffffu, scan, off); if (lane >= off) scan += o; }
         if (lane == 31) sh.warp_sum[warp] = scan;
         if (tid == 0) sh.part = -1;
         __syncthreads();
-        u64 total = 0;
-        for (int w = 0; w < kWarps; ++w) { if (w < warp) scan += sh.warp_sum[w]; total += sh.warp_sum[w]; }
-        if (by_mass && first_round) {
-            share_of_mass = share_of_mass * (double)total;
-            if (!(share_of_mass > 0.0)) share_of_mass = 0.5;  // at least one token: any weight reaches a half
-            if (tid == 0) sh.total = __double_as_longlong(share_of_mass);
-        }
-        const u64 low = before + scan - m0 - m1, mid = low + m0, high = mid + m1;
-        auto reached = [&](u64 s) { return by_mass ? (double)s >= share_of_mass : s >= want; };
+        u64 others = lane < warp ? sh.warp_sum[lane % kWarps] : 0;
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) others += __shfl_xor_sync(0xffffffffu, others, off);
+        scan += before + __shfl_sync(0xffffffffu, others, 0);
+        const u64 low = scan - m0 - m1, mid = low + m0;
         if (m0 && reached(mid) && !reached(low)) { sh.part = b0; sh.before = low; }
-        if (m1 && reached(high) && !reached(mid)) { sh.part = b1; sh.before = mid; }
+        if (m1 && reached(scan) && !reached(mid)) { sh.part = b1; sh.before = mid; }
         __syncthreads();
         part = sh.part;
         if (part >= 0) before = sh.before;
+        __syncthreads();
         return part >= 0;
+    };
+    auto find = [&](bool by_mass, u64 want, double& share_of_mass, bool first_round, bool down, u64& before, int& part) -> bool {
+        cluster.sync();  // all histograms are complete
+        // this CTA's parts, a lane per source: two rounds whatever the cluster's size
+        const int source = tid & (ctas - 1);
+        const Shared* const from = cluster.map_shared_rank(&sh, source);
+        Shared* const to = cluster.map_shared_rank(&sh, source);
+        u64 sum[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sum[i] = sum_of(*from, (rank * kBins + i * kThreads + tid) / ctas);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            for (int off = ctas >> 1; off > 0; off >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], off);
+            to->merged[(rank * kBins + i * kThreads + tid) / ctas] = sum[i];
+        }
+        cluster.sync();
+        // two neighbouring parts a thread, from the largest keys down
+        const int a = 2 * tid, b0 = down ? kBins - 1 - a : a, b1 = down ? b0 - 1 : a + 1;
+        clear(sh);
+        if (by_mass && first_round) {
+            share_of_mass *= (double)block_sum(sh.merged[b0] + sh.merged[b1], sh.warp_count);
+            if (!(share_of_mass > 0.0)) share_of_mass = 0.5;  // at least one token: any weight reaches a half
+        }
+        return reach_in(sh.merged[b0], sh.merged[b1], b0, b1, reached_by(by_mass, want, share_of_mass), before, part);
     };
     // The last key, in falling order, up to which the counts reach `want` or the weights the share top_p of all, among keys of at least `floor`
     auto reach = [&](bool by_mass, u64 want, u64 floor) -> u64 {
-        const uint32_t floor_bits = (uint32_t)(floor >> 32);
-        for (int i = begin + lane; i < end; i += 32) {
-            const float v = at(i);
-            if (fades(v) || ascending(v) < floor_bits || (floor && rank_key(v, first + i) < floor)) continue;
-            const u64 add = by_mass ? mass_of(weight(v, top, temperature)) : 1;
-            if (add) atomicAdd(&sh.hist[part_of(v)], add);
+        const Floor from = floor_at(floor, fade);
+        if (!by_mass) {
+            each_four([&](const float (&v)[4], int i) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (above(from, v[k], i + 32 * k)) atomicAdd(&sh.low[part_of(v[k])], 1u);
+            });
+        } else {
+            quickly([&](auto quick) {
+                each_four([&](const float (&v)[4], int i) {
+                    u64 add[4];
+                    int bin[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        add[k] = above(from, v[k], i + 32 * k) ? mass_of(weigh.share<decltype(quick)::value>(v[k])) : 0;
+                        bin[k] = part_of(v[k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) add_to(sh, bin[k], add[k]);
+                });
+            });
         }
         u64 before = 0;
         int part;
         double target = top_p;
         if (!find(by_mass, want, target, true, false, before, part)) return floor;
-        if (by_mass) target = __longlong_as_double(sh.total);
+        if (!by_mass && before + sh.merged[part] <= kThreads) {  // so few that they are drawn from where they are listed
+            few = true;
+            const float high_place = part < kBins - 1 ? (float)(part + 1) : INFINITY;
+            each_four([&](const float (&v)[4], int i) {
+                bool any = false;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) any = any || (v[k] >= fade && !((top - v[k]) * scale >= high_place));
+                if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (!fades(v[k]) && part_of(v[k]) <= part) leader->list[atomicAdd(&leader->listed[0], 1u)] = rank_key(v[k], first + i + 32 * k);
+            });
+            cluster.sync();
+            return 0;
+        }
         // the tokens of that part, or of an interval of keys in it, to the first CTA
         u64 base = 0;
-        int shift = 64;
+        int shift = 64, sub_part = -1;
         while (true) {
             const int list = lists++ & 15;
-            auto inside = [&](float v, u64 key) { return part_of(v) == part && key >= floor && key >= base && (shift == 64 || !((key - base) >> shift)); };
-            for (int i = begin + lane; i < end; i += 32) {
-                const float v = at(i);
-                if (fades(v) || part_of(v) != part) continue;
-                const u64 key = rank_key(v, first + i);
-                if (!inside(v, key)) continue;
-                const u64 mass = by_mass ? mass_of(weight(v, top, temperature)) : 1;
-                if (!mass) continue;
-                const uint32_t place = atomicAdd(&leader->listed[list], 1u);
-                if (place < kList) { leader->list[place] = key; leader->list_mass[place] = mass; }
-            }
+            auto inside = [&](float v, u64 key) {
+                return part_of(v) == part && key >= floor && (sub_part < 0 || sub_of(v) == sub_part) && key >= base && (shift == 64 || !((key - base) >> shift));
+            };
+            const float low_place = part > 0 ? (float)part : -INFINITY, high_place = part < kBins - 1 ? (float)(part + 1) : INFINITY;
+            each_four([&](const float (&v)[4], int i) {
+                bool on[4], any = false;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float place = (top - v[k]) * scale;  // (exactly part_of's, before it is rounded down; none where both are infinite: the largest)
+                    on[k] = !(place < low_place) && !(place >= high_place) && v[k] >= fade;
+                    any = any || on[k];
+                }
+                if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (!on[k]) continue;
+                    const u64 key = rank_key(v[k], first + i + 32 * k);
+                    if (!inside(v[k], key)) continue;
+                    const u64 mass = by_mass ? weigh(v[k]) : 1;
+                    if (!mass) continue;
+                    const uint32_t entry = atomicAdd(&leader->listed[list], 1u);
+                    if (entry < kList) { leader->list[entry] = key; leader->list_mass[entry] = mass; }
+                }
+            });
             cluster.sync();
             const uint32_t n = leader->listed[list];
             if (n <= kList) {
                 if (rank == 0) {
-                    for (uint32_t i = tid; i < n; i += kThreads) {
-                        const u64 key = sh.list[i], mass = sh.list_mass[i];
-                        u64 above = before;
-#pragma unroll 4
-                        for (uint32_t j = 0; j < n; ++j) above += sh.list[j] > key ? sh.list_mass[j] : 0;
-                        const bool reached = by_mass ? (double)(above + mass) >= target && !((double)above >= target) : above + mass >= want && above < want;
-                        if (reached) sh.bound = key;
+                    // the list by a 1024th of the part (or ten bits of the key), then the few that share one by comparison with each other
+                    const int next = max(shift - 10, 0);
+                    const bool mine = tid < (int)n;
+                    const u64 key = mine ? sh.list[tid] : 0, mass = mine ? sh.list_mass[tid] : 0;
+                    const int bin = sub_part < 0 ? kBins - 1 - sub_of(value_of(key)) : (int)((key - base) >> next);  // rising with the key
+                    if (mine) add_to(sh, bin, mass);
+                    __syncthreads();
+                    int sub;
+                    u64 above_it = before;
+                    if (tid == 0) sh.sharing = 0;
+                    const u64 a = sum_of(sh, kBins - 1 - 2 * tid), b = sum_of(sh, kBins - 2 - 2 * tid);
+                    reach_in(a, b, kBins - 1 - 2 * tid, kBins - 2 - 2 * tid, reached_by(by_mass, want, target), above_it, sub);
+                    if (mine && bin == sub) {
+                        const int place = atomicAdd(&sh.sharing, 1);
+                        sh.merged[place] = key;
+                        sh.list_sum[place] = mass;
                     }
+                    __syncthreads();
+                    const int sharing = sh.sharing;
+                    if (tid < sharing) {
+                        const u64 key = sh.merged[tid], mass = sh.list_sum[tid];
+                        for (int j = 0; j < sharing; ++j) above_it += sh.merged[j] > key ? sh.list_sum[j] : 0;
+                        const auto reached = reached_by(by_mass, want, target);
+                        if (reached(above_it + mass) && !reached(above_it)) sh.bound = key;
+                    }
+                    __syncthreads();
+                    clear(sh);
                 }
                 cluster.sync();
                 if (tid == 0 && rank == 0) sh.listed[(list + 8) & 15] = 0;  // (eight lists on: nobody looks at that one any more)
                 return leader->bound;
             }
-            // more than fit: ten bits of the key further
+            // more than fit: a 1024th of the part, then ten bits of the key after ten
+            const bool by_key = sub_part >= 0;
             const int next = max(shift - 10, 0);
             for (int i = begin + lane; i < end; i += 32) {
                 const float v = at(i);
                 if (fades(v)) continue;
                 const u64 key = rank_key(v, first + i);
                 if (!inside(v, key)) continue;
-                const u64 mass = by_mass ? mass_of(weight(v, top, temperature)) : 1;
-                if (mass) atomicAdd(&sh.hist[(int)((key - base) >> next)], mass);
+                const u64 mass = by_mass ? weigh(v) : 1;
+                if (mass) add_to(sh, by_key ? (int)((key - base) >> next) : sub_of(v), mass);
             }
             int sub = 0;
-            find(by_mass, want, target, false, true, before, sub);
+            find(by_mass, want, target, false, by_key, before, sub);
             if (tid == 0 && rank == 0) sh.listed[(list + 8) & 15] = 0;
+            if (!by_key) { sub_part = max(sub, 0); continue; }
             base += (u64)max(sub, 0) << next;
             shift = next;
         }
     };
     const bool nothing = top == -INFINITY;
     u64 bound = 0;
+    if (!(temperature > 0.0f) && !nothing) {  // the largest logit, the first of equal ones
+        int least = p.vocabulary;
+        each_four([&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (v[k] == top) least = min(least, first + i + 32 * k);
+        });
+        least = __reduce_min_sync(0xffffffffu, least);
+        if (lane == 0) sh.warp_count[warp] = (u64)least;
+        __syncthreads();
+        if (warp == 0) {
+            least = __reduce_min_sync(0xffffffffu, lane < kWarps ? (int)sh.warp_count[lane] : p.vocabulary);
+            if (lane == 0) atomicMin(&leader->best, least);
+        }
+        cluster.sync();
+        if (rank == 0 && tid == 0) {
+            p.token[row] = sh.best;
+            if (p.probability) p.probability[row] = 1.0f;
+            if (p.kept) p.kept[row] = 1;
+        }
+        return;
+    }
     if (!nothing && top_k < p.vocabulary) bound = reach(false, (u64)top_k, 0);
+    if (few) {
+        if (rank == 0) draw_from_list(p, sh, row, top, temperature, top_k, top_p, min_p);
+        return;  // (nobody reads another CTA's memory any more)
+    }
     if (!nothing && top_p < 1.0f) bound = reach(true, 0, bound);
 
     // ---- the draw -----------------------------------------------------------------------------------
-    const uint32_t bound_bits = (uint32_t)(bound >> 32);
-    auto kept_mass = [&](int i) -> u64 {
-        const float v = at(i);
-        if (ascending(v) < bound_bits || fades(v) || rank_key(v, first + i) < bound) return 0;
-        const float e = weight(v, top, temperature);
-        return e >= min_p || v == top ? mass_of(e) : 0;
+    // (min_p as a value too, a little low: what lies below it is not looked at, what lies above is asked itself)
+    const bool by_min = min_p > 0.0f;
+    const float least = by_min && min_p < 1.0f && weigh.quick ? fmaxf(fade, top + temperature * (logf(min_p) * 1.001f - 0.001f)) : fade;
+    const Floor from = floor_at(bound, least);
+    auto masses = [&](auto quick, const float (&v)[4], const bool (&on)[4], u64 (&w)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float e = weigh.share<decltype(quick)::value>(v[k]);
+            w[k] = on[k] && (!by_min || e >= min_p || v[k] == top) ? mass_of(e) : 0;
+        }
     };
-    u64 sum = 0, tokens = 0;
+    u64 sum = 0;
+    uint32_t tokens = 0;
     if (!nothing)
-        for (int i = begin + lane; i < end; i += 32) { const u64 w = kept_mass(i); sum += w; tokens += w != 0; }
+        quickly([&](auto quick) { each_four([&](const float (&v)[4], int i) {
+            bool on[4], any = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { on[k] = above(from, v[k], i + 32 * k); any = any || on[k]; }
+            if (!__any_sync(0xffffffffu, any)) return;
+            u64 w[4];
+            masses(quick, v, on, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { sum += w[k]; tokens += w[k] != 0; }
+        }); });
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) { sum += __shfl_xor_sync(0xffffffffu, sum, off); tokens += __shfl_xor_sync(0xffffffffu, tokens, off); }
     if (lane == 0) { sh.warp_sum[warp] = sum; sh.warp_count[warp] = tokens; }
@@ -253,11 +495,18 @@ __global__ void __launch_bounds__(kThreads) rq_sample_kernel(SampleParams p) {
     }
     cluster.sync();
     u64 total = 0, ahead = 0, all = 0;
-    for (int c = 0; c < ctas; ++c) {
-        const Shared* other = cluster.map_shared_rank(&sh, c);
-        if (c < rank) ahead += other->sum;
-        total += other->sum;
-        all += other->count;
+    {
+        const Shared* other = cluster.map_shared_rank(&sh, lane & (ctas - 1));
+        const u64 s = lane < ctas ? other->sum : 0, n = lane < ctas ? other->count : 0;
+        total = s;
+        all = n;
+        ahead = lane < rank ? s : 0;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            total += __shfl_xor_sync(0xffffffffu, total, off);
+            all += __shfl_xor_sync(0xffffffffu, all, off);
+            ahead += __shfl_xor_sync(0xffffffffu, ahead, off);
+        }
     }
     if (nothing) {
         if (rank == 0 && tid == 0) { p.token[row] = -1; if (p.probability) p.probability[row] = 0.0f; if (p.kept) p.kept[row] = 0; }
@@ -265,24 +514,45 @@ __global__ void __launch_bounds__(kThreads) rq_sample_kernel(SampleParams p) {
         const double u = fmin(fmax((double)p.uniform[row], 0.0), 1.0);
         u64 want = (u64)(u * (double)total);
         if (want >= total) want = total - 1;
-        for (int w = 0; w < warp; ++w) ahead += sh.warp_sum[w];
-        if (ahead <= want && want < ahead + sh.warp_sum[warp]) {
-            u64 run = ahead;
-            for (int i0 = begin; i0 < end; i0 += 32) {
-                const u64 w = i0 + lane < end ? kept_mass(i0 + lane) : 0;
-                u64 scan = w;
+        if (ahead <= want && want < ahead + sh.sum) {
+            // this CTA's: the warp's share that it is in, neighbours a thread, and the one thread's neighbours one by one
+            int in = 0;
+            for (; in < kWarps - 1 && ahead + sh.warp_sum[in] <= want; ++in) ahead += sh.warp_sum[in];
+            const int each = (warp_share + kThreads - 1) / kThreads, from_here = in * warp_share + tid * each, upto = min(min(from_here + each, (in + 1) * warp_share), count);
+            u64 w = 0;
+            quickly([&](auto quick) {
+                for (int i = from_here; i < upto; i += 4) {
+                    float v[4];
+                    bool on[4];
+                    u64 mass[4];
 #pragma unroll
-                for (int off = 1; off < 32; off <<= 1) { const u64 o = __shfl_up_sync(0xffffffffu, scan, off); if (lane >= off) scan += o; }
-                const uint32_t past = __ballot_sync(0xffffffffu, run + scan > want);
-                if (past) {
-                    if (lane == __ffs(past) - 1) {
-                        p.token[row] = first + i0 + lane;
-                        if (p.probability) p.probability[row] = (float)((double)w / (double)total);
-                        if (p.kept) p.kept[row] = (int32_t)all;
+                    for (int k = 0; k < 4; ++k) {
+                        v[k] = i + k < upto ? at(i + k) : -INFINITY;
+                        on[k] = above(from, v[k], i + k);
                     }
-                    break;
+                    masses(quick, v, on, mass);
+                    w += mass[0] + mass[1] + mass[2] + mass[3];
                 }
-                run += __shfl_sync(0xffffffffu, scan, 31);
+            });
+            u64 scan = w;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) { const u64 o = __shfl_up_sync(0xffffffffu, scan, off); if (lane >= off) scan += o; }
+            if (lane == 31) sh.list_sum[warp] = scan;
+            __syncthreads();
+            for (int k = 0; k < warp; ++k) ahead += sh.list_sum[k];
+            if (ahead + scan > want && ahead + scan - w <= want) {
+                u64 run = ahead + scan - w;
+                for (int i = from_here; i < upto; ++i) {
+                    const float v = at(i);
+                    const u64 m = above(from, v, i) && (!by_min || weight(v, top, temperature) >= min_p || v == top) ? weigh(v) : 0;
+                    run += m;
+                    if (run > want) {
+                        p.token[row] = first + i;
+                        if (p.probability) p.probability[row] = (float)((double)m / (double)total);
+                        if (p.kept) p.kept[row] = (int32_t)all;
+                        break;
+                    }
+                }
             }
         }
     }
@@ -324,10 +594,13 @@ extern "C" int rq_sample(rq_ctx* ctx, const float* logits, int64_t row_stride, i
     if (vocabulary > RQ_MAX_VOCABULARY) return rq_fail(RQ_ERR_LIMIT, "rq_sample: %lld tokens; at most %d", (long long)vocabulary, RQ_MAX_VOCABULARY);
     if (rows > (1 << 26)) return rq_fail(RQ_ERR_LIMIT, "rq_sample: %d rows; at most 2^26", rows);
     DeviceGuard guard(ctx->device);
-    // CTAs a row: as few as hold it, and more while the GPU has room and a share would still be some thousand logits
+    // CTAs a row. While the rows' shares all fit the GPU at once in shared memory (clusters of sixteen, two CTAs an SM: fourteen), as many as hold a row, and more
+    // while a share would still be some thousand logits. Beyond, as few as let all rows run at once, and logits are read again from L2.
     int ctas = 1;
     while (ctas < kMostCtas && (vocabulary > (int64_t)ctas * kShare || ((int64_t)rows * ctas * 2 <= ctx->sm_count && vocabulary > (int64_t)ctas * 4096))) ctas *= 2;
-    const int64_t unit = kThreads;  // a share is so many logits a warp, a whole number of 32
+    if ((int64_t)rows * ctas > 14 * 16)
+        while (ctas > 1 && (int64_t)rows * ctas > 2 * ctx->sm_count && (vocabulary + ctas / 2 - 1) / (ctas / 2) <= 65536) ctas /= 2;
+    const int64_t unit = 4 * kThreads;  // a warp's share is a whole number of 128
     SampleParams p = {logits, temperature, top_p, min_p, uniform, top_k, token, kept, probability, row_stride, (int)vocabulary, 0};
     p.share = (int)(((vocabulary + ctas - 1) / ctas + unit - 1) / unit * unit);
     if (p.share <= kShare) return launch_sample<true>(p, rows, ctas, (cudaStream_t)stream);
