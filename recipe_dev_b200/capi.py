@@ -178,20 +178,29 @@ def _stream(stream) -> int:
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _int32(a, size, who: str) -> None:
-    import torch
+_I32 = _F32 = None  # torch's types, once a context exists (an import statement in a short call costs as much as its checks)
 
-    if a.dtype != torch.int32 or a.dim() != 1 or not a.is_cuda or not a.is_contiguous() or (size is not None and a.shape[0] != size):
+
+def _int32(a, size, who: str) -> None:
+    if a.dtype is not _I32 or not a.is_cuda or (a.stride() != (1,) and not (a.dim() == 1 and a.is_contiguous())) or (size is not None and a.shape[0] != size):
         raise ValueError(f"{who}: expected a contiguous CUDA int32 tensor" + ("" if size is None else f" of {size}"))
 
 
-def _plane(a, who: str) -> int:
-    """The values of a token of an fp32 plane [tokens, values] or [tokens, heads, head_dim] whose tokens are contiguous."""
-    import torch
-
-    if a.dtype != torch.float32 or not a.is_cuda or a.stride(-1) != 1 or (a.dim() == 3 and a.stride(1) != a.shape[2]) or a.dim() not in (2, 3):
+def _plane(a, who: str) -> tuple[int, int]:
+    """The values of a token and the token stride of an fp32 plane [tokens, values] or [tokens, heads, head_dim] whose tokens are contiguous."""
+    shape, stride = a.shape, a.stride()
+    n = len(shape)
+    if a.dtype is not _F32 or not a.is_cuda or n not in (2, 3) or stride[-1] != 1 or (n == 3 and stride[1] != shape[2]):
         raise ValueError(f"{who}: expected a CUDA fp32 plane [tokens, values] or [tokens, heads, head_dim] with contiguous tokens")
-    return a.shape[1] if a.dim() == 2 else a.shape[1] * a.shape[2]
+    return (shape[1] if n == 2 else shape[1] * shape[2]), stride[0]
+
+
+def _table(table, requests: int, who: str) -> tuple[int, int]:
+    """The stride and the width of a page table's rows."""
+    shape, stride = table.shape, table.stride()
+    if len(shape) != 2 or table.dtype is not _I32 or not table.is_cuda or stride[1] != 1 or shape[0] < requests:
+        raise ValueError(f"{who}: the page table must be CUDA int32 [requests, width] with contiguous rows")
+    return stride[0], shape[1]
 
 
 class Weight:
@@ -294,11 +303,20 @@ class Context:
     """One device context (rq_ctx)."""
 
     def __init__(self, device: int = 0):
+        global _I32, _F32
+        import torch
+
+        _I32, _F32 = torch.int32, torch.float32
         self.lib = load_library()
         handle = C.c_void_p()
         _check(self.lib.rq_init(device, C.byref(handle)))
         self.handle = handle.value
         self.device = device
+        self._current_stream = torch._C._cuda_getCurrentRawStream
+
+    def _on(self, stream) -> int:
+        """The stream's handle; the device's current stream for None."""
+        return self._current_stream(self.device) if stream is None else _stream(stream)
 
     def close(self) -> None:
         if getattr(self, "handle", 0):
@@ -596,15 +614,13 @@ class Context:
             starts, lengths, status = made(starts, n + 1), made(lengths, n), made(status, 3)
             slots, positions, owners = made(slots, size), made(positions, size), made(owners, size)
         tokens = slots.shape[0]
-        for a, size in ((cached, n), (fresh, n), (starts, n + 1), (lengths, n), (slots, tokens), (positions, tokens), (owners, tokens), (status, 3), (free_pages, None)):
-            _int32(a, size, "batch_plan")
-        if table.dim() != 2 or table.shape[0] < n or table.stride(1) != 1 or table.dtype != cached.dtype:
-            raise ValueError("batch_plan: the page table must be int32 [requests, width] with contiguous rows")
-        status_code = self.lib.rq_batch_plan(self.handle, cached.data_ptr(), fresh.data_ptr(), n, page_size, table.data_ptr(), table.stride(0), table.shape[1], free_pages.data_ptr(),
-                                             free_pages.shape[0], starts.data_ptr(), lengths.data_ptr(), slots.data_ptr(), positions.data_ptr(), owners.data_ptr(), tokens,
-                                             status.data_ptr(), _stream(stream))
-        if status_code:
-            _check(status_code)
+        _int32(cached, n, "batch_plan"), _int32(fresh, n, "batch_plan"), _int32(starts, n + 1, "batch_plan"), _int32(lengths, n, "batch_plan"), _int32(status, 3, "batch_plan")
+        _int32(slots, tokens, "batch_plan"), _int32(positions, tokens, "batch_plan"), _int32(owners, tokens, "batch_plan"), _int32(free_pages, None, "batch_plan")
+        stride, width = _table(table, n, "batch_plan")
+        rc = self.lib.rq_batch_plan(self.handle, cached.data_ptr(), fresh.data_ptr(), n, page_size, table.data_ptr(), stride, width, free_pages.data_ptr(), free_pages.shape[0], starts.data_ptr(),
+                                    lengths.data_ptr(), slots.data_ptr(), positions.data_ptr(), owners.data_ptr(), tokens, status.data_ptr(), self._on(stream))
+        if rc:
+            _check(rc)
         return starts, lengths, slots, positions, owners, status
 
     def rope_table(self, rows: int, rotary: int, base: float = 10000.0, frequency_scale: float = 1.0, out=None, stream=None):
@@ -626,24 +642,26 @@ class Context:
 
             q_out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
         d, width = cache.head_dim, cache.heads * cache.head_dim
-        qw = _plane(q, "rope_store")
-        if qw % d or _plane(q_out, "rope_store") != qw or _plane(k, "rope_store") != width or _plane(v, "rope_store") != width or not k.shape[0] == v.shape[0] == q_out.shape[0] == tokens:
+        (qw, q_stride), (ow, out_stride), (kw, k_stride), (vw, v_stride) = _plane(q, "rope_store"), _plane(q_out, "rope_store"), _plane(k, "rope_store"), _plane(v, "rope_store")
+        if qw % d or ow != qw or kw != width or vw != width or not k.shape[0] == v.shape[0] == q_out.shape[0] == tokens:
             raise ValueError("rope_store: q and q_out must hold whole heads, k and v the cache's heads, for the same tokens")
         _int32(positions, None, "rope_store"), _int32(slots, None, "rope_store")
         if positions.shape[0] < tokens or slots.shape[0] < tokens:
             raise ValueError("rope_store: positions and slots must have an entry for every token")
+        gains = []
         for g in (q_gain, k_gain):
-            if g is not None and (g.shape != (d,) or g.stride(0) != 1):
-                raise ValueError("rope_store: a gain holds head_dim contiguous values")
-        rows, rotary = (0, 0) if table is None else table.shape
-        if table is not None and not table.is_contiguous():
-            raise ValueError("rope_store: the rotation table must be contiguous")
-        status = self.lib.rq_rope_store(self.handle, q.data_ptr(), q.stride(0), qw // d, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), tokens,
-                                        0 if q_gain is None else q_gain.data_ptr(), 0 if k_gain is None else k_gain.data_ptr(), epsilon,
-                                        0 if table is None else table.data_ptr(), rows, rotary, ROPE_STYLES[style], positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), q_out.stride(0),
-                                        cache._ref, _stream(stream))
-        if status:
-            _check(status)
+            if g is not None and (g.dtype is not _F32 or not g.is_cuda or g.shape != (d,) or not g.is_contiguous()):
+                raise ValueError("rope_store: a gain holds head_dim contiguous fp32 values")
+            gains.append(0 if g is None else g.data_ptr())
+        rows = rotary = at = 0
+        if table is not None:
+            if table.dim() != 2 or table.dtype is not _F32 or not table.is_cuda or not table.is_contiguous():
+                raise ValueError("rope_store: the rotation table must be contiguous CUDA fp32 [rows, rotary]")
+            (rows, rotary), at = table.shape, table.data_ptr()
+        rc = self.lib.rq_rope_store(self.handle, q.data_ptr(), q_stride, qw // d, k.data_ptr(), k_stride, v.data_ptr(), v_stride, tokens, gains[0], gains[1], epsilon, at, rows, rotary,
+                                    ROPE_STYLES[style], positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), out_stride, cache._ref, self._on(stream))
+        if rc:
+            _check(rc)
         return q_out
 
     def attention_reserve(self) -> None:
@@ -659,36 +677,39 @@ class Context:
             import torch
 
             y = torch.empty(q.shape, dtype=torch.float32, device=q.device)
-        qw = _plane(q, "attention")
-        if qw % d or _plane(y, "attention") != qw or y.shape[0] != tokens:
+        (qw, q_stride), (yw, y_stride) = _plane(q, "attention"), _plane(y, "attention")
+        if qw % d or yw != qw or y.shape[0] != tokens:
             raise ValueError("attention: q and y must hold whole heads of the cache's head_dim for the same tokens")
         _int32(starts, n + 1, "attention"), _int32(lengths, n, "attention")
-        if table.dim() != 2 or table.shape[0] < n or table.stride(1) != 1 or table.dtype != lengths.dtype:
-            raise ValueError("attention: the page table must be int32 [requests, width] with contiguous rows")
-        status = self.lib.rq_attention(self.handle, q.data_ptr(), q.stride(0), qw // d, cache._ref, table.data_ptr(), table.stride(0), table.shape[1], starts.data_ptr(), lengths.data_ptr(),
-                                       n, tokens, max_fresh, d**-0.5 if scale is None else scale, window, y.data_ptr(), y.stride(0), _stream(stream))
-        if status:
-            _check(status)
+        stride, width = _table(table, n, "attention")
+        rc = self.lib.rq_attention(self.handle, q.data_ptr(), q_stride, qw // d, cache._ref, table.data_ptr(), stride, width, starts.data_ptr(), lengths.data_ptr(), n, tokens, max_fresh,
+                                   d**-0.5 if scale is None else scale, window, y.data_ptr(), y_stride, self._on(stream))
+        if rc:
+            _check(rc)
         return y
 
     def sample(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, token=None, probability=None, kept=None, stream=None):
         """The next token of each row of logits (fp32 [rows, vocabulary]) from uniform [rows] in [0, 1); parameters are CUDA tensors [rows]
         (top_k int32, the others fp32) or None. Returns token (int32 [rows]); probability and kept are filled where given."""
-        import torch
-
         rows, vocabulary = logits.shape
-        if logits.dtype != torch.float32 or not logits.is_cuda or logits.stride(1) != 1:
+        stride = logits.stride()
+        if logits.dtype is not _F32 or not logits.is_cuda or stride[1] != 1:
             raise ValueError("sample: logits must be CUDA fp32 [rows, vocabulary] with contiguous rows")
         if token is None:
+            import torch
+
             token = torch.empty(rows, dtype=torch.int32, device=logits.device)
-        for a, dtype in ((uniform, torch.float32), (temperature, torch.float32), (top_p, torch.float32), (min_p, torch.float32), (probability, torch.float32), (top_k, torch.int32),
-                         (kept, torch.int32), (token, torch.int32)):
-            if a is not None and (a.dtype != dtype or a.shape != (rows,) or not a.is_contiguous() or not a.is_cuda):
+        at = []
+        for a, dtype in ((temperature, _F32), (top_k, _I32), (top_p, _F32), (min_p, _F32), (uniform, _F32), (token, _I32), (probability, _F32), (kept, _I32)):
+            if a is None:
+                at.append(0)
+                continue
+            if a.dtype is not dtype or not a.is_cuda or a.shape != (rows,) or not a.is_contiguous():
                 raise ValueError("sample: per-row arrays must be contiguous CUDA tensors [rows], top_k, token and kept int32, the others fp32")
-        status = self.lib.rq_sample(self.handle, logits.data_ptr(), logits.stride(0), rows, vocabulary, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), uniform.data_ptr(),
-                                    token.data_ptr(), _ptr(probability), _ptr(kept), _stream(stream))
-        if status:
-            _check(status)
+            at.append(a.data_ptr())
+        rc = self.lib.rq_sample(self.handle, logits.data_ptr(), stride[0], rows, vocabulary, *at, self._on(stream))
+        if rc:
+            _check(rc)
         return token
 
     def activation_records(self, x, step: int, stream=None):
