@@ -181,9 +181,11 @@ def _stream(stream) -> int:
 _I32 = _F32 = None  # torch's types, once a context exists (an import statement in a short call costs as much as its checks)
 
 
-def _int32(a, size, who: str) -> None:
-    if a.dtype is not _I32 or not a.is_cuda or (a.stride() != (1,) and not (a.dim() == 1 and a.is_contiguous())) or (size is not None and a.shape[0] != size):
+def _int32(a, size, who: str) -> int:
+    """The address of a contiguous CUDA int32 tensor (of `size` values, where that is given)."""
+    if a.dtype is not _I32 or not a.is_cuda or not a.is_contiguous() or (size is not None and a.numel() != size):
         raise ValueError(f"{who}: expected a contiguous CUDA int32 tensor" + ("" if size is None else f" of {size}"))
+    return a.data_ptr()
 
 
 def _plane(a, who: str) -> tuple[int, int]:
@@ -614,11 +616,11 @@ class Context:
             starts, lengths, status = made(starts, n + 1), made(lengths, n), made(status, 3)
             slots, positions, owners = made(slots, size), made(positions, size), made(owners, size)
         tokens = slots.shape[0]
-        _int32(cached, n, "batch_plan"), _int32(fresh, n, "batch_plan"), _int32(starts, n + 1, "batch_plan"), _int32(lengths, n, "batch_plan"), _int32(status, 3, "batch_plan")
-        _int32(slots, tokens, "batch_plan"), _int32(positions, tokens, "batch_plan"), _int32(owners, tokens, "batch_plan"), _int32(free_pages, None, "batch_plan")
-        stride, width = _table(table, n, "batch_plan")
-        rc = self.lib.rq_batch_plan(self.handle, cached.data_ptr(), fresh.data_ptr(), n, page_size, table.data_ptr(), stride, width, free_pages.data_ptr(), free_pages.shape[0], starts.data_ptr(),
-                                    lengths.data_ptr(), slots.data_ptr(), positions.data_ptr(), owners.data_ptr(), tokens, status.data_ptr(), self._on(stream))
+        who = "batch_plan"
+        stride, width = _table(table, n, who)
+        rc = self.lib.rq_batch_plan(self.handle, _int32(cached, n, who), _int32(fresh, n, who), n, page_size, table.data_ptr(), stride, width, _int32(free_pages, None, who), free_pages.numel(),
+                                    _int32(starts, n + 1, who), _int32(lengths, n, who), _int32(slots, tokens, who), _int32(positions, tokens, who), _int32(owners, tokens, who), tokens,
+                                    _int32(status, 3, who), self._on(stream))
         if rc:
             _check(rc)
         return starts, lengths, slots, positions, owners, status
@@ -645,8 +647,8 @@ class Context:
         (qw, q_stride), (ow, out_stride), (kw, k_stride), (vw, v_stride) = _plane(q, "rope_store"), _plane(q_out, "rope_store"), _plane(k, "rope_store"), _plane(v, "rope_store")
         if qw % d or ow != qw or kw != width or vw != width or not k.shape[0] == v.shape[0] == q_out.shape[0] == tokens:
             raise ValueError("rope_store: q and q_out must hold whole heads, k and v the cache's heads, for the same tokens")
-        _int32(positions, None, "rope_store"), _int32(slots, None, "rope_store")
-        if positions.shape[0] < tokens or slots.shape[0] < tokens:
+        positions_at, slots_at = _int32(positions, None, "rope_store"), _int32(slots, None, "rope_store")
+        if positions.numel() < tokens or slots.numel() < tokens:
             raise ValueError("rope_store: positions and slots must have an entry for every token")
         gains = []
         for g in (q_gain, k_gain):
@@ -659,7 +661,7 @@ class Context:
                 raise ValueError("rope_store: the rotation table must be contiguous CUDA fp32 [rows, rotary]")
             (rows, rotary), at = table.shape, table.data_ptr()
         rc = self.lib.rq_rope_store(self.handle, q.data_ptr(), q_stride, qw // d, k.data_ptr(), k_stride, v.data_ptr(), v_stride, tokens, gains[0], gains[1], epsilon, at, rows, rotary,
-                                    ROPE_STYLES[style], positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), out_stride, cache._ref, self._on(stream))
+                                    ROPE_STYLES[style], positions_at, slots_at, q_out.data_ptr(), out_stride, cache._ref, self._on(stream))
         if rc:
             _check(rc)
         return q_out
@@ -680,9 +682,9 @@ class Context:
         (qw, q_stride), (yw, y_stride) = _plane(q, "attention"), _plane(y, "attention")
         if qw % d or yw != qw or y.shape[0] != tokens:
             raise ValueError("attention: q and y must hold whole heads of the cache's head_dim for the same tokens")
-        _int32(starts, n + 1, "attention"), _int32(lengths, n, "attention")
+        starts_at, lengths_at = _int32(starts, n + 1, "attention"), _int32(lengths, n, "attention")
         stride, width = _table(table, n, "attention")
-        rc = self.lib.rq_attention(self.handle, q.data_ptr(), q_stride, qw // d, cache._ref, table.data_ptr(), stride, width, starts.data_ptr(), lengths.data_ptr(), n, tokens, max_fresh,
+        rc = self.lib.rq_attention(self.handle, q.data_ptr(), q_stride, qw // d, cache._ref, table.data_ptr(), stride, width, starts_at, lengths_at, n, tokens, max_fresh,
                                    d**-0.5 if scale is None else scale, window, y.data_ptr(), y_stride, self._on(stream))
         if rc:
             _check(rc)

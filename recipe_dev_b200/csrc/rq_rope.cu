@@ -2,16 +2,18 @@
 //
 //   x' = x / sqrt(mean(x^2) + epsilon) * gain;  (a, b) -> (a cos - b sin, a sin + b cos) over the pairs of the first `rotary` elements
 //
-// Bound by bytes for a prompt (everything is read once and written once) and by latency for a few tokens: a warp takes one head of one token, its
-// lanes hold head_dim / 32 neighbouring elements each, so that a head is one contiguous access, the sum of squares five shuffles
-// and the other element of a pair half a head apart one more. Everything is held in fp32 and a key or value is rounded once.
+// Bound by bytes for a prompt (everything is read once and written once) and by the launch for a few tokens: a warp takes four heads of one token, all of them on
+// their way at once and with one reading of the token's row of the table; its lanes hold head_dim / 32 neighbouring elements of each, so that a head is one
+// contiguous access, the sum of squares five shuffles and the other element of a pair half a head apart one more. Everything is held in fp32 and a key or value is
+// rounded once, to the cache's type. (In place: a warp has read what it writes.) 2039 tokens of 32 + 2 x 8 heads of 128: 23.8 us, 3.9 TB/s; with two heads a warp
+// 24.4, eight 27.7, one 30.3; CTAs of eight warps 24.9. 64 tokens 10.4 us, one 9.6, which is what a call from Python takes.
 #include "rq_serve.cuh"
 
 using namespace rqserve;
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4, kHeads = 4;
 
 struct RopeParams {
     const float *q, *k, *v, *q_gain, *k_gain, *table;
@@ -23,15 +25,21 @@ struct RopeParams {
     float epsilon;
 };
 
-// E neighbouring fp32 numbers, in 16-byte (E = 2: 8-byte) accesses where the caller's planes allow them
-template <int E, bool WIDE> __device__ __forceinline__ void load(const float* p, float (&x)[E]) {
-    if (WIDE && E == 2) { const float2 a = __ldcg((const float2*)p); x[0] = a.x; x[1] = a.y; }
-    else if (WIDE) {
+// N neighbouring fp32 numbers, in 16-byte (two: 8-byte) accesses where the caller's planes allow them; KEEP: through the L1 cache, for what other warps read too
+// (through L2 alone, the few lines of the gains are asked for by every warp: 102 us in place of 25 for 2039 tokens)
+template <int N, bool WIDE, bool KEEP = false> __device__ __forceinline__ void load(const float* p, float (&x)[N]) {
+    if (WIDE && N >= 4) {
 #pragma unroll
-        for (int i = 0; i < E; i += 4) { const float4 a = __ldcg((const float4*)(p + i)); x[i] = a.x; x[i + 1] = a.y; x[i + 2] = a.z; x[i + 3] = a.w; }
+        for (int i = 0; i < N; i += 4) {
+            const float4 a = KEEP ? *(const float4*)(p + i) : __ldcg((const float4*)(p + i));
+            x[i] = a.x; x[(i + 1) % N] = a.y; x[(i + 2) % N] = a.z; x[(i + 3) % N] = a.w;
+        }
+    } else if (WIDE && N == 2) {
+        const float2 a = KEEP ? *(const float2*)p : __ldcg((const float2*)p);
+        x[0] = a.x; x[1 % N] = a.y;
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = __ldcg(p + i);
+        for (int i = 0; i < N; ++i) x[i] = KEEP ? p[i] : __ldcg(p + i);
     }
 }
 template <int E, bool WIDE> __device__ __forceinline__ void store(float* p, const float (&x)[E]) {
@@ -49,68 +57,92 @@ template <int D, int TYPE, bool WIDE>
 __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
     constexpr int E = D / 32;
     launch_dependents();
-    const int heads = p.q_heads + 2 * p.kv_heads, lane = threadIdx.x & 31, first = lane * E;
-    const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int heads = p.q_heads + 2 * p.kv_heads, groups = (heads + kHeads - 1) / kHeads, lane = threadIdx.x & 31, first = lane * E, half = p.rotary / 2;
+    const uint32_t item = blockIdx.x * kWarps + (threadIdx.x >> 5), t = item / (uint32_t)groups;
+    const int head0 = (int)(item % (uint32_t)groups) * kHeads;
     wait_for_previous();
-    if (item >= (int64_t)p.tokens * heads) return;
-    const int t = (int)(item / heads), head = (int)(item % heads);
-    const int kind = head < p.q_heads ? 0 : (head < p.q_heads + p.kv_heads ? 1 : 2), h = kind == 0 ? head : (head - p.q_heads) % p.kv_heads;
-    const int slot = kind == 0 ? 0 : p.slots[t];
-    const int64_t page = slot >> p.page_shift;
-    if (slot < 0 || (kind != 0 && page >= p.pages)) return;  // passed over: a padding token, or one whose page is lacking
-    float x[E];
-    load<E, WIDE>((kind == 0 ? p.q + t * p.q_stride : (kind == 1 ? p.k + t * p.k_stride : p.v + t * p.v_stride)) + (int64_t)h * D + first, x);
-    if (kind < 2) {
-        const float* gain = kind == 0 ? p.q_gain : p.k_gain;
-        if (gain) {
-            float sum = 0.0f;
+    if (t >= (uint32_t)p.tokens) return;
+    // every head's elements on their way at once, with the token's place and position
+    float x[kHeads][E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) sum = fmaf(x[i], x[i], sum);
+    for (int i = 0; i < kHeads; ++i) {
+        const int head = head0 + i;
+        if (head >= heads) break;
+        const bool is_q = head < p.q_heads, is_k = head < p.q_heads + p.kv_heads;
+        const float* from = is_q ? p.q + t * p.q_stride + (int64_t)head * D
+                                 : (is_k ? p.k + t * p.k_stride + (int64_t)(head - p.q_heads) * D : p.v + t * p.v_stride + (int64_t)(head - p.q_heads - p.kv_heads) * D);
+        load<E, WIDE>(from + first, x[i]);
+    }
+    const int slot = __ldcg(p.slots + t);
+    const bool turns = first < p.rotary && head0 < p.q_heads + p.kv_heads, low = first < half;
+    float c[E], s[E];
+    if (turns) {
+        const int64_t position = max((int64_t)0, min((int64_t)__ldcg(p.positions + t), p.table_rows - 1));
+        const float* row = p.table + position * p.rotary;
+        if (p.style == RQ_ROPE_PAIRS) {
+            float cs[E / 2], ss[E / 2];
+            load<E / 2, WIDE, true>(row + first / 2, cs);
+            load<E / 2, WIDE, true>(row + half + first / 2, ss);
 #pragma unroll
-            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            const float scale = 1.0f / sqrtf(sum / (float)D + p.epsilon);
-#pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = x[i] * scale * __ldcg(gain + first + i);
+            for (int i = 0; i < E; i += 2) { c[i] = cs[i / 2]; s[i] = ss[i / 2]; }
+        } else {
+            const int at = low ? first : first - half;
+            load<E, WIDE, true>(row + at, c);
+            load<E, WIDE, true>(row + half + at, s);
         }
-        if (p.rotary) {
-            const int64_t position = max((int64_t)0, min((int64_t)p.positions[t], p.table_rows - 1));
-            const float* row = p.table + position * p.rotary;
-            const int half = p.rotary / 2;
-            if (p.style == RQ_ROPE_PAIRS) {
-                if (first < p.rotary) {
+    }
+    const int64_t page = slot >> p.page_shift;
+    const bool stored = slot >= 0 && page < p.pages;  // else passed over: a padding token, or one whose page is lacking
+    const int64_t line = page * p.page_stride + (slot & ((1 << p.page_shift) - 1)) * p.line_stride + first;
+#pragma unroll
+    for (int n = 0; n < kHeads; ++n) {
+        const int head = head0 + n;
+        if (head >= heads) break;
+        const bool is_q = head < p.q_heads, is_k = !is_q && head < p.q_heads + p.kv_heads;
+        if (is_q || is_k) {
+            const float* gain = is_q ? p.q_gain : p.k_gain;
+            if (gain) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < E; ++i) sum = fmaf(x[n][i], x[n][i], sum);
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                const float scale = 1.0f / sqrtf(sum / (float)D + p.epsilon);
+                float g[E];
+                load<E, WIDE, true>(gain + first, g);
+#pragma unroll
+                for (int i = 0; i < E; ++i) x[n][i] = x[n][i] * scale * g[i];
+            }
+            if (p.rotary && p.style == RQ_ROPE_PAIRS) {
+                if (turns) {
 #pragma unroll
                     for (int i = 0; i < E; i += 2) {
-                        const float c = __ldcg(row + (first + i) / 2), s = __ldcg(row + half + (first + i) / 2), a = x[i], b = x[i + 1];
-                        x[i] = a * c - b * s;
-                        x[i + 1] = a * s + b * c;
+                        const float a = x[n][i], b = x[n][i + 1];
+                        x[n][i] = a * c[i] - b * s[i];
+                        x[n][i + 1] = a * s[i] + b * c[i];
                     }
                 }
-            } else {
+            } else if (p.rotary) {
                 // half is a whole number of lanes: the lane that holds the other elements of this lane's pairs
-                const bool low = first < half;
-                const int other = low ? lane + half / E : lane - half / E;
-                const int i0 = low ? first : first - half;
+                const int other = (low ? lane + half / E : lane - half / E) & 31;
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const float y = __shfl_sync(0xffffffffu, x[i], other & 31);
-                    if (first < p.rotary) {
-                        const float c = __ldcg(row + i0 + i), s = __ldcg(row + half + i0 + i);
-                        x[i] = low ? x[i] * c - y * s : y * s + x[i] * c;
-                    }
+                    const float y = __shfl_sync(0xffffffffu, x[n][i], other);
+                    if (turns) x[n][i] = low ? x[n][i] * c[i] - y * s[i] : y * s[i] + x[n][i] * c[i];
                 }
             }
         }
-    }
-    if (kind == 0) {
-        store<E, WIDE>(p.q_out + t * p.out_stride + (int64_t)h * D + first, x);
-    } else {
-        uint16_t* to = (kind == 1 ? p.k_cache : p.v_cache) + page * p.page_stride + h * p.head_stride + (slot & ((1 << p.page_shift) - 1)) * p.line_stride + first;
-        uint32_t w[E / 2];
+        if (is_q) {
+            store<E, WIDE>(p.q_out + t * p.out_stride + (int64_t)head * D + first, x[n]);
+        } else if (stored) {
+            uint16_t* to = (is_k ? p.k_cache + (head - p.q_heads) * p.head_stride : p.v_cache + (head - p.q_heads - p.kv_heads) * p.head_stride) + line;
+            uint32_t w[E / 2];
 #pragma unroll
-        for (int i = 0; i < E; i += 2) w[i / 2] = from_float<TYPE>(x[i]) | (uint32_t)from_float<TYPE>(x[i + 1]) << 16;
-        if (E == 2) *(uint32_t*)to = w[0];
-        else if (E == 4) *(uint2*)to = make_uint2(w[0], w[1 % (E / 2)]);
-        else *(uint4*)to = make_uint4(w[0], w[1 % (E / 2)], w[2 % (E / 2)], w[3 % (E / 2)]);
+            for (int i = 0; i < E; i += 2) w[i / 2] = from_float<TYPE>(x[n][i]) | (uint32_t)from_float<TYPE>(x[n][i + 1]) << 16;
+            if (E == 2) *(uint32_t*)to = w[0];
+            else if (E == 4) *(uint2*)to = make_uint2(w[0], w[1 % (E / 2)]);
+            else *(uint4*)to = make_uint4(w[0], w[1 % (E / 2)], w[2 % (E / 2)], w[3 % (E / 2)]);
+        }
     }
 }
 
@@ -129,7 +161,7 @@ __global__ void __launch_bounds__(256) rq_rope_table_kernel(double base, double 
 
 template <int D>
 int launch_rope(const RopeParams& p, int type, bool wide, cudaStream_t s) {
-    const int64_t items = (int64_t)p.tokens * (p.q_heads + 2 * p.kv_heads);
+    const int64_t items = (int64_t)p.tokens * ((p.q_heads + 2 * p.kv_heads + kHeads - 1) / kHeads);
     const dim3 grid((unsigned)((items + kWarps - 1) / kWarps));
     auto kernel = type == RQ_KV_F16 ? (wide ? rq_rope_kernel<D, RQ_KV_F16, true> : rq_rope_kernel<D, RQ_KV_F16, false>)
                                     : (wide ? rq_rope_kernel<D, RQ_KV_BF16, true> : rq_rope_kernel<D, RQ_KV_BF16, false>);
@@ -170,7 +202,7 @@ extern "C" int rq_rope_store(rq_ctx* ctx, const float* q, int64_t q_t_stride, in
     p.page_stride = cache->page_stride; p.head_stride = cache->head_stride; p.line_stride = cache->line_stride; p.pages = cache->pages;
     p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = cache->heads; p.rotary = rotary; p.style = style; p.epsilon = epsilon;
     while (1 << p.page_shift < cache->page_size) ++p.page_shift;
-    const bool wide = (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out) & 15) == 0 && (tokens == 1 || ((q_t_stride | k_t_stride | v_t_stride | q_out_t_stride) & 3) == 0);
+    const bool wide = (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain | (uintptr_t)table) & 15) == 0 && (tokens == 1 || ((q_t_stride | k_t_stride | v_t_stride | q_out_t_stride) & 3) == 0);
     if (d == 64) return launch_rope<64>(p, cache->type, wide, (cudaStream_t)stream);
     if (d == 128) return launch_rope<128>(p, cache->type, wide, (cudaStream_t)stream);
     return launch_rope<256>(p, cache->type, wide, (cudaStream_t)stream);
