@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
     if (tid == 0) before[0] = 0;
     for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
         int64_t units = 0;
-        if (r0 + tid < p.requests) { const Request q = request_of<ROWS>(p, r0 + tid); units = q.units * q.tiles * p.kv_heads; }
+        if (r0 + tid < p.requests) { const Request q = request_of<ROWS>(p, r0 + tid); units = (int64_t)q.fresh * group > p.few ? 0 : q.units * q.tiles * p.kv_heads; }
         int64_t scan = units;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) { const int64_t o = __shfl_up_sync(0xffffffffu, scan, off); if (lane >= off) scan += o; }
@@ -471,6 +471,11 @@ int launch_rows(rq_ctx* ctx, const AttentionParams& p, int type, bool two, cudaS
     if (type == RQ_KV_F16) return two ? launch_rows<D, RQ_KV_F16, 2>(ctx, p, s) : launch_rows<D, RQ_KV_F16, 1>(ctx, p, s);
     return two ? launch_rows<D, RQ_KV_BF16, 2>(ctx, p, s) : launch_rows<D, RQ_KV_BF16, 1>(ctx, p, s);
 }
+int launch_rows_of(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s) {
+    if (cache.head_dim == 64) return launch_rows<64>(ctx, p, cache.type, two, s);
+    if (cache.head_dim == 128) return launch_rows<128>(ctx, p, cache.type, two, s);
+    return launch_rows<256>(ctx, p, cache.type, two, s);
+}
 
 }  // namespace
 
@@ -511,13 +516,19 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
     while (1 << p.page_shift < cache->page_size) ++p.page_shift;
     p.error_flag = ctx->error_flag; p.wait_ns = ctx->wait_limit_ns;
     const int64_t rows = (int64_t)(max_fresh > 0 ? (max_fresh < tokens ? max_fresh : tokens) : tokens) * group;
+    // The rows kernel reads a request's keys once for every sixteen rows (from L2, from the second time on), the tensor-core kernel makes scores of 128 whatever
+    // there is. 8192 cached keys, 32 + 2 x 8 heads of 128, f16, rows kernel | tensor cores: 16 requests of 16 rows 106 | 183 us, 32 rows 182 | 184, 48 rows 264 | 185,
+    // 128 rows 695 | 179; one request of 32 rows 36 | 44, 48 rows 41 | 45, 128 rows 62 | 45. bf16: 16 requests of 32 rows 277 | 317, 48 rows 404 | 319.
     if (rows > 32) {
+        // Where a request may be a decode step among prompts, the rows kernel takes those and the tensor-core kernel the rest: 63 decode steps over 4096 keys and
+        // a chunk of 512 are 269 us in two launches, 494 by the tensor cores alone, 556 by the rows kernel alone; 7 over 300 keys and a prompt of 100: 32, 41, 23.
+        const int few = requests > 1 && tokens < requests * (rows / group) ? (group <= 8 ? 8 : 32) : 0;
+        p.few = group <= few ? few : 0;
         rc = launch_tensor(ctx, p, *cache, rows <= 128, s);
-        if (rc != RQ_ERR_UNSUPPORTED) return rc;
+        if (rc != RQ_ERR_UNSUPPORTED && (rc != RQ_OK || !p.few)) return rc;
+        if (rc == RQ_OK) return launch_rows_of(ctx, p, *cache, group > 8, s);
     }
+    p.few = 0x7fffffff;
     // rows that meet a key together: eight, or sixteen where a request may have more
-    const bool two = rows > 8;
-    if (cache->head_dim == 64) return launch_rows<64>(ctx, p, cache->type, two, s);
-    if (cache->head_dim == 128) return launch_rows<128>(ctx, p, cache->type, two, s);
-    return launch_rows<256>(ctx, p, cache->type, two, s);
+    return launch_rows_of(ctx, p, *cache, rows > 8, s);
 }

@@ -14,6 +14,7 @@ struct AttentionParams {
     int64_t q_stride, y_stride, table_stride, head_stride, pages;
     uint32_t page_bytes, line_bytes;
     int tokens, requests, q_heads, kv_heads, table_width, page_shift, window;
+    int few;  // requests of at most so many rows a key head are the rows kernel's, the others the tensor-core kernel's
     float scale;
     int wide;  // q and y allow accesses of 16 bytes (1), of 32 (2)
     int* error_flag;

@@ -59,7 +59,8 @@ struct Block {
     int units;
 };
 template <typename F> __device__ __forceinline__ int blocks_of(const AttentionParams& p, int r, int group) {
-    return (max(p.starts[r + 1] - p.starts[r], 0) * group + F::BLOCK - 1) / F::BLOCK;
+    const int rows = max(p.starts[r + 1] - p.starts[r], 0) * group;
+    return rows > p.few ? (rows + F::BLOCK - 1) / F::BLOCK : 0;
 }
 template <typename F> __device__ __forceinline__ Block block_of(const AttentionParams& p, int r, int b, int group) {
     Block k;

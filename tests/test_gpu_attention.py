@@ -244,6 +244,45 @@ def test_many_requests(rq_ctx):
     compare(run(rq_ctx, b), b)
 
 
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (7, 1, 64), (20, 1, 128), (40, 1, 64), (4, 2, 256)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("cached,fresh", [([40, 700, 0, 5, 300], [1, 1, 150, 0, 1]), ([0, 130, 0], [3, 90, 1]), ([900, 0, 31], [1, 33, 0])])
+def test_decode_steps_among_prompts(rq_ctx, hq, hk, d, dtype, cached, fresh):
+    b = batch(cached, fresh, hq, hk, d, 16, dtype)
+    compare(run(rq_ctx, b), b)
+    assert (run(rq_ctx, b) == run(rq_ctx, b)).all()
+
+
+@pytest.mark.parametrize("fresh", [[1, 1], [1, 80]])
+def test_recorded_and_replayed_over_longer_requests(fresh):
+    """The lengths are read when a recorded call runs, not when it is recorded; the work area has to be there before."""
+    import torch
+
+    import recipe_dev_b200 as rq
+
+    ctx = rq.Context(0)  # one that has no work area yet
+    long = batch([700, 333], fresh, 8, 2, 128, 16)
+    starts = torch.tensor(long["starts"], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([30 + fresh[0], 20 + fresh[1]], dtype=torch.int32, device="cuda")
+    y = torch.zeros_like(long["q"])
+    stream = ctx.sequence_begin()
+    with pytest.raises(rq.RqError, match="rq_attention_reserve"):
+        ctx.attention(long["q"], long["cache"], long["table"], starts, lengths, max_fresh=max(fresh), y=y, stream=stream)
+    ctx.sequence_end().free()
+    ctx.attention_reserve()
+    stream = ctx.sequence_begin()
+    ctx.attention(long["q"], long["cache"], long["table"], starts, lengths, max_fresh=max(fresh), y=y, stream=stream)
+    sequence = ctx.sequence_end()
+    for now in ([30 + fresh[0], 20 + fresh[1]], long["lengths"]):
+        lengths.copy_(torch.tensor(now, dtype=torch.int32))
+        sequence.run()
+        torch.cuda.synchronize()
+        compare(y.reshape(-1, 8, 128), dict(long, lengths=now))
+    sequence.free()
+    ctx.check()
+    ctx.close()
+
+
 def test_two_streams_share_the_work_area(rq_ctx):
     import torch
 
