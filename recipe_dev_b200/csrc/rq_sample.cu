@@ -4,15 +4,18 @@
 // which one the random number meets depend on no order of additions (and of atomics). Tokens are ranked by a 64-bit key, the logit's bits made
 // ascending above the complement of the index; the kept tokens are those whose key is at least a bound.
 //
-// A row is dealt out over a cluster of up to sixteen CTAs, each with its share in shared memory, read once from HBM. A bound is found from a histogram, over 1024 parts of the
-// logits' distance from the largest (the weights fade within 28 T of it), of counts (top_k) or of weights (top_p): the CTAs'
-// histograms are added up through distributed shared memory, every CTA finds the part in which the sum is reached, the tokens of that part, some
-// hundreds, are sent to the first CTA, and there each finds its rank and the weights before it by comparison with all others. Where
-// a part holds more than fit (equal logits), it is taken apart by ten bits of the key at a time until they do.
+// A row is dealt out over a cluster of up to sixteen CTAs, each with its share in shared memory, read once from HBM (or, of many long rows, again from L2). A bound is
+// found from a histogram, over 1024 parts of the logits' distance from the largest, of counts (top_k) or of weights (top_p, over no more than the distance that
+// the bound can have): the CTAs' histograms are added up through distributed shared memory, every CTA finds the part in which the sum is reached, the tokens of
+// that part, some hundreds, are sent to the first CTA, which finds the one by a histogram of its own and comparison of the few that share a place in it. Where a
+// part holds more than fit (equal logits), it is taken apart by its 1024ths and then ten bits of the key at a time until they do. Where top_k leaves at most 512,
+// these are sent to the first CTA, sorted, and everything else happens there. The draw is by sums in index order: of CTAs, of warps, of threads.
 //
-// For one row it is bound by the chain of some ten cluster barriers with a pass over the share between them; for many rows by instructions: an
-// exponential, a division and an atomic addition in shared memory a token. One thread block a row, with seven rounds over ten bits of the key
-// each: 2054 us for 1 x 262144 and 1863 us for 64 x 262144.
+// For one row it is bound by the chain of some ten cluster barriers with a pass over the share between them: 1 x 262144 with top_k = 64 and top_p = 0.95 20 us,
+// with top_p alone 30, greedy 6. For many rows by instructions, some hundred a logit in four passes (an exponential in two of them, an addition in shared memory
+// of two or three words): 64 x 262144 with top_p = 0.9 112 us, with min_p = 0.02 too 94, top_k = 64 52, no filter 47, greedy 22. With one CTA a row and seven
+// rounds over ten bits of the key each it was 2054 us for one row and 1863 for 64; with parts over all 28 T, lists of 512 and weights made whole numbers by
+// conversion 118 for the 64, at T = 1.2 191 (now 116).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -24,7 +27,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kList = kThreads, kMostCtas = 16;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kList = 2 * kThreads, kMostCtas = 16;
 constexpr int kShare = 16384;  // logits of a CTA in shared memory
 constexpr float kFade = 28.0f; // exp(-28) < 2^-40
 
@@ -50,6 +53,12 @@ __device__ __forceinline__ float weight(float x, float top, float temperature) {
     return temperature > 0.0f ? expf((x - top) / temperature) : 0.0f;
 }
 __device__ __forceinline__ u64 mass_of(float e) { return (u64)(e * 1099511627776.0f); }
+// floor(x), 0 <= x < 2^22, as the low bits of x + 2^23 rounded down; x = a * b. What is left of the product is exact.
+__device__ __forceinline__ uint32_t take_whole(float a, float b, float& left) {
+    const float t = __fmaf_rd(a, b, 8388608.0f);
+    left = fmaf(a, b, 8388608.0f - t);
+    return __float_as_uint(t) - 0x4b000000u;
+}
 
 struct Shared {
     // this CTA's sums, in words of 16, 13 and 12 bits of their terms: a 64-bit atomic addition in shared memory is a loop, and one that carries waits for an answer
@@ -62,8 +71,6 @@ struct Shared {
     int part, sharing, best;
     uint32_t listed[16];     // the first CTA's lists, one after another
     float warp_top[kWarps], top;
-    int chosen_warp;
-    u64 chosen_want;
 };
 
 // Sum over the CTA; every thread gets it
@@ -162,12 +169,20 @@ struct Weigher {
 };
 __device__ __forceinline__ u64 sum_of(const Shared& sh, int bin) { return ((u64)sh.high[bin] << 29) + ((u64)sh.mid[bin] << 16) + sh.low[bin]; }
 __device__ __forceinline__ void clear(Shared& sh) { *(uint2*)&sh.low[2 * threadIdx.x] = *(uint2*)&sh.mid[2 * threadIdx.x] = *(uint2*)&sh.high[2 * threadIdx.x] = make_uint2(0, 0); }
-__device__ __forceinline__ void add_to(Shared& sh, int bin, u64 v) {
-    const uint32_t lo = (uint32_t)v & 0xffff, mid = (uint32_t)(v >> 16) & 0x1fff, hi = (uint32_t)(v >> 29);
+__device__ __forceinline__ void add_words(Shared& sh, int bin, uint32_t hi, uint32_t mid, uint32_t lo) {
     if (lo) atomicAdd(&sh.low[bin], lo);  // (at most 2^16 terms a CTA)
     if (mid) atomicAdd(&sh.mid[bin], mid);
     if (hi) atomicAdd(&sh.high[bin], hi);
 }
+// the same without a branch a word (three words of a part lie a plane apart), where `here`
+__device__ __forceinline__ void add_words_if(bool here, uint32_t part_low, uint32_t hi, uint32_t mid, uint32_t lo) {
+    asm volatile(
+        "{\n.reg .pred h, p, q, r;\nsetp.ne.u32 h, %4, 0;\nsetp.ne.and.u32 p, %1, 0, h;\nsetp.ne.and.u32 q, %2, 0, h;\nsetp.ne.and.u32 r, %3, 0, h;\n"
+        "@p red.shared.add.u32 [%0], %1;\n@q red.shared.add.u32 [%0 + %5], %2;\n@r red.shared.add.u32 [%0 + %6], %3;\n}" ::"r"(part_low), "r"(lo), "r"(mid), "r"(hi),
+        "r"((uint32_t)here), "n"(4 * kBins), "n"(8 * kBins)
+        : "memory");
+}
+__device__ __forceinline__ void add_to(Shared& sh, int bin, u64 v) { add_words(sh, bin, (uint32_t)(v >> 29), (uint32_t)(v >> 16) & 0x1fff, (uint32_t)v & 0xffff); }
 
 // STAGED: the share lies in shared memory, cleaned; otherwise it is read again
 template <bool STAGED>
@@ -193,15 +208,30 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
 
     // ---- the largest logit ----------------------------------------------------------------------------
     float top = -INFINITY;
-    for (int i = begin + lane; i < stop; i += 128 * 2) {
-        float v[8];
+    const bool wide = ((uintptr_t)x & 15) == 0;
+    // four neighbours of the row; -inf past the end
+    auto read = [&](int i, float (&v)[4]) {
+        if (wide && i + 4 <= end) {
+            const float4 a = __ldcg((const float4*)(x + i));
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = i + 32 * k < end ? __ldcg(x + i + 32 * k) : -INFINITY;
+            for (int k = 0; k < 4; ++k) v[k] = i + k < end ? __ldcg(x + i + k) : -INFINITY;
+        }
+    };
+    constexpr int kAtOnce = 4;
+    for (int i = begin + 4 * lane; i < stop; i += 128 * kAtOnce) {
+        float v[kAtOnce][4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            v[k] = cleaned(v[k]);
-            if (STAGED && i + 32 * k < stop) staged[i + 32 * k] = v[k];
-            top = fmaxf(top, v[k]);
+        for (int n = 0; n < kAtOnce; ++n) read(i + 128 * n, v[n]);
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[n][k] = cleaned(v[n][k]);
+                top = fmaxf(top, v[n][k]);
+            }
+            if (STAGED && i + 128 * n < stop) *(float4*)(staged + i + 128 * n) = make_float4(v[n][0], v[n][1], v[n][2], v[n][3]);
         }
     }
 #pragma unroll
@@ -217,20 +247,32 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
 
-    // Four logits of a thread at a time, side by side; -inf past the end
-    auto each_four = [&](auto&& use) {
+    // Four neighbouring logits of a thread at a time, -inf past the end. CLEAN: NaN as -inf and -0 as +0, which keys are made of; comparisons and
+    // weights need neither.
+    auto each_four = [&](auto clean, auto&& use) {
+        float next[4];
+        if (!STAGED) read(begin + 4 * lane, next);
 #pragma unroll 1
-        for (int i = begin + lane; i < stop; i += 128) {
+        for (int i = begin + 4 * lane; i < stop; i += 128) {
             float v[4];
+            if (STAGED) {
+                const float4 a = *(const float4*)(staged + i);
+                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = STAGED || i + 32 * k < end ? at(i + 32 * k) : -INFINITY;
+                for (int k = 0; k < 4; ++k) v[k] = decltype(clean)::value ? cleaned(next[k]) : next[k];
+                read(i + 128, next);  // (on their way while these are looked at)
+            }
             use(v, i);
         }
     };
+    const std::true_type for_keys;
+    const std::false_type for_sums;
 
     // ---- bounds ------------------------------------------------------------------------------------
     const Weigher weigh(top, temperature);
-    const float limit = fminf(kFade * temperature, 3e38f), scale = (float)kBins / limit;
+    const float limit = fminf(kFade * temperature, 3e38f);
+    float scale = (float)kBins / limit;
     auto floor_of = [](float place) { return (int)(__float_as_uint(__fadd_rd(fminf(place, (float)(kBins - 1)), 8388608.0f)) & 0x7fffffu); };  // 0 <= place, up to the last part
     auto part_of = [&](float v) { return v == top ? 0 : floor_of((top - v) * scale); };
     auto sub_of = [&](float v) { const float place = (top - v) * scale; return v == top ? 0 : floor_of((place - (float)floor_of(place)) * (float)kBins); };
@@ -304,25 +346,46 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
     auto reach = [&](bool by_mass, u64 want, u64 floor) -> u64 {
         const Floor from = floor_at(floor, fade);
         if (!by_mass) {
-            each_four([&](const float (&v)[4], int i) {
+            each_four(for_sums, [&](const float (&v)[4], int i) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (above(from, v[k], i + 32 * k)) atomicAdd(&sh.low[part_of(v[k])], 1u);
+                    if (above(from, v[k], i + k)) atomicAdd(&sh.low[part_of(v[k])], 1u);
             });
         } else {
-            quickly([&](auto quick) {
-                each_four([&](const float (&v)[4], int i) {
-                    u64 add[4];
+            // Logits further off than T ln(V / (1 - top_p)) weigh less than 1 - top_p together, for the largest alone weighs 1: the parts are
+            // finer by as much, and what lies in the last one is added up in registers. (One part more or less does no harm: what is found is looked up.)
+            scale = (float)kBins / fminf(fminf(logf((float)p.vocabulary / (1.0f - top_p)) + 1.0f, kFade) * temperature, 3e38f);
+            uint32_t far_hi = 0, far_mid = 0, far_low = 0;
+            const uint32_t parts_at = (uint32_t)__cvta_generic_to_shared(sh.low);
+            static_assert(offsetof(Shared, mid) == offsetof(Shared, low) + 4 * kBins && offsetof(Shared, high) == offsetof(Shared, mid) + 4 * kBins, "planes");
+            auto add_up = [&](auto quick, auto ties) {
+                each_four(for_sums, [&](const float (&v)[4], int i) {
+                    uint32_t hi[4], mid[4], low[4];
                     int bin[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        add[k] = above(from, v[k], i + 32 * k) ? mass_of(weigh.share<decltype(quick)::value>(v[k])) : 0;
-                        bin[k] = part_of(v[k]);
+                        const bool on = decltype(ties)::value ? above(from, v[k], i + k) : v[k] >= from.value;
+                        float left = on ? weigh.share<decltype(quick)::value>(v[k]) : 0.0f;
+                        hi[k] = take_whole(left, 2048.0f, left);
+                        mid[k] = take_whole(left, 8192.0f, left);
+                        low[k] = take_whole(left, 65536.0f, left);
+                        bin[k] = decltype(quick)::value ? floor_of((v[k] - top) * -scale) : part_of(v[k]);  // (the same: 0 for the largest, which is finite)
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) add_to(sh, bin[k], add[k]);
+                    for (int k = 0; k < 4; ++k) {
+                        const bool far = bin[k] == kBins - 1;
+                        far_hi += far ? hi[k] : 0;
+                        far_mid += far ? mid[k] : 0;
+                        far_low += far ? low[k] : 0;
+                        add_words_if(!far, parts_at + 4 * bin[k], hi[k], mid[k], low[k]);
+                    }
                 });
-            });
+            };
+            if (!weigh.quick) add_up(std::false_type(), std::true_type());
+            else if (from.index == 0x7fffffff) add_up(std::true_type(), std::false_type());  // no token of that value is left out
+            else add_up(std::true_type(), std::true_type());
+            far_hi = __reduce_add_sync(0xffffffffu, far_hi); far_mid = __reduce_add_sync(0xffffffffu, far_mid); far_low = __reduce_add_sync(0xffffffffu, far_low);
+            if (lane == 0) add_words(sh, kBins - 1, far_hi, far_mid, far_low);
         }
         u64 before = 0;
         int part;
@@ -331,14 +394,14 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
         if (!by_mass && before + sh.merged[part] <= kThreads) {  // so few that they are drawn from where they are listed
             few = true;
             const float high_place = part < kBins - 1 ? (float)(part + 1) : INFINITY;
-            each_four([&](const float (&v)[4], int i) {
+            each_four(for_keys, [&](const float (&v)[4], int i) {
                 bool any = false;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) any = any || (v[k] >= fade && !((top - v[k]) * scale >= high_place));
                 if (!__any_sync(0xffffffffu, any)) return;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (!fades(v[k]) && part_of(v[k]) <= part) leader->list[atomicAdd(&leader->listed[0], 1u)] = rank_key(v[k], first + i + 32 * k);
+                    if (!fades(v[k]) && part_of(v[k]) <= part) leader->list[atomicAdd(&leader->listed[0], 1u)] = rank_key(v[k], first + i + k);
             });
             cluster.sync();
             return 0;
@@ -351,20 +414,22 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
             auto inside = [&](float v, u64 key) {
                 return part_of(v) == part && key >= floor && (sub_part < 0 || sub_of(v) == sub_part) && key >= base && (shift == 64 || !((key - base) >> shift));
             };
-            const float low_place = part > 0 ? (float)part : -INFINITY, high_place = part < kBins - 1 ? (float)(part + 1) : INFINITY;
-            each_four([&](const float (&v)[4], int i) {
+            // the part's values and a little more; those between are asked for their part
+            const float most = part > 0 ? top - ((float)part - 0.5f) / scale : top, least = part < kBins - 1 ? fmaxf(fade, top - ((float)part + 1.5f) / scale) : fade;
+            each_four(for_sums, [&](const float (&raw)[4], int i) {
                 bool on[4], any = false;
+                float v[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float place = (top - v[k]) * scale;  // (exactly part_of's, before it is rounded down; none where both are infinite: the largest)
-                    on[k] = !(place < low_place) && !(place >= high_place) && v[k] >= fade;
+                    on[k] = raw[k] >= least && raw[k] <= most;
                     any = any || on[k];
+                    v[k] = raw[k] + 0.0f;
                 }
                 if (!__any_sync(0xffffffffu, any)) return;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     if (!on[k]) continue;
-                    const u64 key = rank_key(v[k], first + i + 32 * k);
+                    const u64 key = rank_key(v[k], first + i + k);
                     if (!inside(v[k], key)) continue;
                     const u64 mass = by_mass ? weigh(v[k]) : 1;
                     if (!mass) continue;
@@ -378,25 +443,25 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
                 if (rank == 0) {
                     // the list by a 1024th of the part (or ten bits of the key), then the few that share one by comparison with each other
                     const int next = max(shift - 10, 0);
-                    const bool mine = tid < (int)n;
-                    const u64 key = mine ? sh.list[tid] : 0, mass = mine ? sh.list_mass[tid] : 0;
-                    const int bin = sub_part < 0 ? kBins - 1 - sub_of(value_of(key)) : (int)((key - base) >> next);  // rising with the key
-                    if (mine) add_to(sh, bin, mass);
+                    auto bin_of = [&](u64 key) { return sub_part < 0 ? kBins - 1 - sub_of(value_of(key)) : (int)((key - base) >> next); };  // rising with the key
+                    for (int e = tid; e < (int)n; e += kThreads) add_to(sh, bin_of(sh.list[e]), sh.list_mass[e]);
                     __syncthreads();
                     int sub;
-                    u64 above_it = before;
+                    u64 above_all = before;
                     if (tid == 0) sh.sharing = 0;
                     const u64 a = sum_of(sh, kBins - 1 - 2 * tid), b = sum_of(sh, kBins - 2 - 2 * tid);
-                    reach_in(a, b, kBins - 1 - 2 * tid, kBins - 2 - 2 * tid, reached_by(by_mass, want, target), above_it, sub);
-                    if (mine && bin == sub) {
+                    reach_in(a, b, kBins - 1 - 2 * tid, kBins - 2 - 2 * tid, reached_by(by_mass, want, target), above_all, sub);
+                    for (int e = tid; e < (int)n; e += kThreads) {
+                        if (bin_of(sh.list[e]) != sub) continue;
                         const int place = atomicAdd(&sh.sharing, 1);
-                        sh.merged[place] = key;
-                        sh.list_sum[place] = mass;
+                        sh.merged[place] = sh.list[e];
+                        sh.list_sum[place] = sh.list_mass[e];
                     }
                     __syncthreads();
                     const int sharing = sh.sharing;
-                    if (tid < sharing) {
-                        const u64 key = sh.merged[tid], mass = sh.list_sum[tid];
+                    for (int e = tid; e < sharing; e += kThreads) {
+                        const u64 key = sh.merged[e], mass = sh.list_sum[e];
+                        u64 above_it = above_all;
                         for (int j = 0; j < sharing; ++j) above_it += sh.merged[j] > key ? sh.list_sum[j] : 0;
                         const auto reached = reached_by(by_mass, want, target);
                         if (reached(above_it + mass) && !reached(above_it)) sh.bound = key;
@@ -431,10 +496,10 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
     u64 bound = 0;
     if (!(temperature > 0.0f) && !nothing) {  // the largest logit, the first of equal ones
         int least = p.vocabulary;
-        each_four([&](const float (&v)[4], int i) {
+        each_four(for_sums, [&](const float (&v)[4], int i) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (v[k] == top) least = min(least, first + i + 32 * k);
+                if (v[k] == top) least = min(least, first + i + k);
         });
         least = __reduce_min_sync(0xffffffffu, least);
         if (lane == 0) sh.warp_count[warp] = (u64)least;
@@ -463,26 +528,30 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
     const bool by_min = min_p > 0.0f;
     const float least = by_min && min_p < 1.0f && weigh.quick ? fmaxf(fade, top + temperature * (logf(min_p) * 1.001f - 0.001f)) : fade;
     const Floor from = floor_at(bound, least);
-    auto masses = [&](auto quick, const float (&v)[4], const bool (&on)[4], u64 (&w)[4]) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float e = weigh.share<decltype(quick)::value>(v[k]);
-            w[k] = on[k] && (!by_min || e >= min_p || v[k] == top) ? mass_of(e) : 0;
-        }
+    const float enough = by_min ? fmaxf(min_p, 0x1p-40f) : 0x1p-40f;  // (of less than 2^-40 nothing is left as a whole number)
+    auto weight_of = [&](auto quick, float v, bool on) {
+        const float e = weigh.share<decltype(quick)::value>(v);
+        return on && (e >= enough || v == top) ? e : 0.0f;
     };
     u64 sum = 0;
     uint32_t tokens = 0;
-    if (!nothing)
-        quickly([&](auto quick) { each_four([&](const float (&v)[4], int i) {
+    if (!nothing) {
+        uint32_t high = 0, low = 0;  // words of 20 bits of the weights of at most 2^7 logits
+        quickly([&](auto quick) { each_four(for_sums, [&](const float (&v)[4], int i) {
             bool on[4], any = false;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { on[k] = above(from, v[k], i + 32 * k); any = any || on[k]; }
+            for (int k = 0; k < 4; ++k) { on[k] = above(from, v[k], i + k); any = any || on[k]; }
             if (!__any_sync(0xffffffffu, any)) return;
-            u64 w[4];
-            masses(quick, v, on, w);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { sum += w[k]; tokens += w[k] != 0; }
+            for (int k = 0; k < 4; ++k) {
+                float e = weight_of(quick, v[k], on[k]);
+                tokens += e > 0.0f;
+                high += take_whole(e, 1048576.0f, e);
+                low += take_whole(e, 1048576.0f, e);
+            }
         }); });
+        sum = ((u64)high << 20) + low;
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) { sum += __shfl_xor_sync(0xffffffffu, sum, off); tokens += __shfl_xor_sync(0xffffffffu, tokens, off); }
     if (lane == 0) { sh.warp_sum[warp] = sum; sh.warp_count[warp] = tokens; }
@@ -522,16 +591,11 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
             u64 w = 0;
             quickly([&](auto quick) {
                 for (int i = from_here; i < upto; i += 4) {
-                    float v[4];
-                    bool on[4];
-                    u64 mass[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        v[k] = i + k < upto ? at(i + k) : -INFINITY;
-                        on[k] = above(from, v[k], i + k);
+                        const float v = i + k < upto ? at(i + k) : -INFINITY;
+                        w += mass_of(weight_of(quick, v, above(from, v, i + k)));
                     }
-                    masses(quick, v, on, mass);
-                    w += mass[0] + mass[1] + mass[2] + mass[3];
                 }
             });
             u64 scan = w;
@@ -544,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
                 u64 run = ahead + scan - w;
                 for (int i = from_here; i < upto; ++i) {
                     const float v = at(i);
-                    const u64 m = above(from, v, i) && (!by_min || weight(v, top, temperature) >= min_p || v == top) ? weigh(v) : 0;
+                    const u64 m = mass_of(weigh.quick ? weight_of(std::true_type(), v, above(from, v, i)) : weight_of(std::false_type(), v, above(from, v, i)));
                     run += m;
                     if (run > want) {
                         p.token[row] = first + i;
@@ -594,10 +658,12 @@ extern "C" int rq_sample(rq_ctx* ctx, const float* logits, int64_t row_stride, i
     if (vocabulary > RQ_MAX_VOCABULARY) return rq_fail(RQ_ERR_LIMIT, "rq_sample: %lld tokens; at most %d", (long long)vocabulary, RQ_MAX_VOCABULARY);
     if (rows > (1 << 26)) return rq_fail(RQ_ERR_LIMIT, "rq_sample: %d rows; at most 2^26", rows);
     DeviceGuard guard(ctx->device);
-    // CTAs a row. While the rows' shares all fit the GPU at once in shared memory (clusters of sixteen, two CTAs an SM: fourteen), as many as hold a row, and more
-    // while a share would still be some thousand logits. Beyond, as few as let all rows run at once, and logits are read again from L2.
+    // CTAs a row: as many as hold it in shared memory, and more while the GPU holds them all at once (two an SM; of clusters of sixteen fourteen) and a share is some
+    // thousand logits. Where they do not all fit, as few as let all rows run at once, and logits are read again from L2.
+    // T = 0.9, top_p = 0.95: 64 x 32000 by two CTAs a row 34 us, by four 25; 24 x 64000 by four 36, by eight 28. Shares of two thousand: 4 x 32000 by sixteen 24, by
+    // eight 16.
     int ctas = 1;
-    while (ctas < kMostCtas && (vocabulary > (int64_t)ctas * kShare || ((int64_t)rows * ctas * 2 <= ctx->sm_count && vocabulary > (int64_t)ctas * 4096))) ctas *= 2;
+    while (ctas < kMostCtas && (vocabulary > (int64_t)ctas * kShare || ((int64_t)rows * ctas * 2 <= (ctas == 8 ? 14 * 16 : 2 * ctx->sm_count) && vocabulary > (int64_t)ctas * 4096))) ctas *= 2;
     if ((int64_t)rows * ctas > 14 * 16)
         while (ctas > 1 && (int64_t)rows * ctas > 2 * ctx->sm_count && (vocabulary + ctas / 2 - 1) / (ctas / 2) <= 65536) ctas /= 2;
     const int64_t unit = 4 * kThreads;  // a warp's share is a whole number of 128
