@@ -79,6 +79,11 @@ template <typename F> __device__ __forceinline__ Block block_of(const AttentionP
     return k;
 }
 
+// Taking a block up (its queries, the first scores, the sums at the end: 21 us) costs as much as some units (3.9 us): so many lead each block's own in the dealing.
+// Without it the CTAs that got a prompt's first blocks, short ones, were the last to end. 32 + 2 x 8 heads of 128, f16, without | with: prompts of 1021 to 3001 tokens
+// 612 | 334 us, one of 12001 2781 | 1930, eight of 512 137 | 119; 32 of 128, all blocks of one unit, 67 | 74.
+constexpr int kLead = 4;
+
 // One block's part of a CTA's range of units, as the roles need it; take = 0: there are no more
 struct Item {
     int take;                                    // units
@@ -184,7 +189,7 @@ template <int D, int TYPE, bool KEYS> __device__ __forceinline__ void load_queri
 }
 
 template <int D, int TYPE, bool KEYS>
-__global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(AttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+__global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using F = Form<D, TYPE, KEYS>;
     constexpr int PARTS = F::PARTS, KT = F::KT, STAGES = F::STAGES;
     extern __shared__ __align__(1024) unsigned char dynamic[];
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(AttentionP
             const int r = r0 + tid;
             int64_t units = 0;
             if (r < p.requests)
-                for (int b = blocks_of<F>(p, r, group) - 1; b >= 0; --b) units += block_of<F>(p, r, b, group).units;
+                for (int b = blocks_of<F>(p, r, group) - 1; b >= 0; --b) units += kLead + block_of<F>(p, r, b, group).units;
             units *= p.kv_heads;
             int64_t scan = units;
 #pragma unroll
@@ -249,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(AttentionP
             int units = 1;
             if (total)
                 while (true) {
-                    units = block_of<F>(p, r, b, group).units;
+                    units = kLead + block_of<F>(p, r, b, group).units;
                     if (left < (int64_t)units * p.kv_heads) break;
                     left -= (int64_t)units * p.kv_heads;
                     ++b;
@@ -725,13 +730,15 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(AttentionP
             Item i = {};
             if (u < end && !dead) {
                 const Block k = block_of<F>(p, r, b, group);
-                i.take = (int)min((int64_t)(k.units - offset), end - u);
-                i.first_key = k.begin + offset * F::UNIT;
+                const int64_t item_begin = u - offset, item_end = item_begin + kLead + k.units;
+                const int first_unit = max(offset - kLead, 0);
+                u = min(item_end, end);
+                i.take = max((int)(u - item_begin) - kLead - first_unit, 0);  // (none where a range ends in a block's lead: the next CTA has it all)
+                i.first_key = k.begin + first_unit * F::UNIT;
                 i.low = k.low; i.high = k.high; i.end = k.end; i.start = k.start; i.row0 = k.row0; i.rows = k.rows; i.position0 = k.position0; i.kv = kv; i.r = r;
-                const int64_t item_begin = u - offset, item_end = item_begin + k.units;
-                i.first_cta = (int)(((item_begin + 1) * ctas - 1) / total);
-                i.last_cta = (int)((item_end * ctas - 1) / total);
-                u += i.take;
+                const bool all = offset <= kLead && u == item_end;  // nobody else's
+                i.first_cta = all ? blockIdx.x : (int)(((item_begin + kLead + 1) * ctas - 1) / total);
+                i.last_cta = all ? blockIdx.x : (int)((item_end * ctas - 1) / total);
                 offset = 0;
                 if (++kv == p.kv_heads) {
                     kv = 0;
@@ -755,7 +762,6 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(AttentionP
         Item following = deal();
         while (following.take) {
             const Item i = following;
-            following = deal();  // ahead of its use: its queries are fetched while this one's tiles are
             const int tiles = i.take * (KEYS ? 2 : 1);
             const int32_t* table = p.block_table + (int64_t)i.r * p.table_stride;
             auto page_of = [&](int tile) -> int {  // of this lane's copy; one past the last for none: such a copy reads zeros
@@ -794,6 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(AttentionP
                 }
                 __syncwarp();
                 at.next();
+                if (n == 1) following = deal();  // ahead of its use: its queries are fetched while this one's tiles are
             }
         }
         // every copy has landed before the CTA ends: the last use of each slot was waited for by the issuing warp, unless a wait ran out
