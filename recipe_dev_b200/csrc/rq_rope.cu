@@ -4,9 +4,10 @@
 //
 // Bound by bytes for a prompt (everything is read once and written once) and by the launch for a few tokens: a warp takes four heads of one token, all of them on
 // their way at once and with one reading of the token's row of the table; its lanes hold head_dim / 32 neighbouring elements of each, so that a head is one
-// contiguous access, the sum of squares five shuffles and the other element of a pair half a head apart one more. Everything is held in fp32 and a key or value is
-// rounded once, to the cache's type. (In place: a warp has read what it writes.) 2039 tokens of 32 + 2 x 8 heads of 128: 23.8 us, 3.9 TB/s; with two heads a warp
-// 24.4, eight 27.7, one 30.3; CTAs of eight warps 24.9. 64 tokens 10.4 us, one 9.6, which is what a call from Python takes.
+// contiguous access and the other element of a pair half a head apart one shuffle; the four sums of squares are added up together. Everything is held in fp32 and a
+// key or value is rounded once, to the cache's type. (In place: a warp has read what it writes.) 2039 tokens of 32 + 2 x 8 heads of 128: 22.0 us, 4.2 TB/s; with five
+// shuffles and a square root a head 23.8, and of that form with two heads a warp 24.4, eight 27.7, CTAs of eight warps 24.9; one head a warp 30.3. 64 tokens 10.1 us, one
+// 9.4, which is what a call from Python takes.
 #include "rq_serve.cuh"
 
 using namespace rqserve;
@@ -66,8 +67,7 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
     float x[kHeads][E];
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
-        const int head = head0 + i;
-        if (head >= heads) break;
+        const int head = min(head0 + i, heads - 1);  // (one past the last is loaded for nothing)
         const bool is_q = head < p.q_heads, is_k = head < p.q_heads + p.kv_heads;
         const float* from = is_q ? p.q + t * p.q_stride + (int64_t)head * D
                                  : (is_k ? p.k + t * p.k_stride + (int64_t)(head - p.q_heads) * D : p.v + t * p.v_stride + (int64_t)(head - p.q_heads - p.kv_heads) * D);
@@ -91,6 +91,26 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
             load<E, WIDE, true>(row + half + at, s);
         }
     }
+    // The heads' sums of squares, added up together: each exchange leaves a lane half as many heads to go on with, and at the end one of the four, by bits 4 and 3 of
+    // the lane, whose scale it makes for all
+    float scale = 0.0f;
+    if (p.q_gain || p.k_gain) {
+        static_assert(kHeads == 4, "two exchanges of heads");
+        float sum[kHeads];
+#pragma unroll
+        for (int n = 0; n < kHeads; ++n) {
+            sum[n] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) sum[n] = fmaf(x[n][i], x[n][i], sum[n]);
+        }
+        const bool second = lane & 16, odd = lane & 8;
+        const float a0 = (second ? sum[2] : sum[0]) + __shfl_xor_sync(0xffffffffu, second ? sum[0] : sum[2], 16);
+        const float a1 = (second ? sum[3] : sum[1]) + __shfl_xor_sync(0xffffffffu, second ? sum[1] : sum[3], 16);
+        float all = (odd ? a1 : a0) + __shfl_xor_sync(0xffffffffu, odd ? a0 : a1, 8);
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+        scale = 1.0f / sqrtf(all / (float)D + p.epsilon);
+    }
     const int64_t page = slot >> p.page_shift;
     const bool stored = slot >= 0 && page < p.pages;  // else passed over: a padding token, or one whose page is lacking
     const int64_t line = page * p.page_stride + (slot & ((1 << p.page_shift) - 1)) * p.line_stride + first;
@@ -102,16 +122,11 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
         if (is_q || is_k) {
             const float* gain = is_q ? p.q_gain : p.k_gain;
             if (gain) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < E; ++i) sum = fmaf(x[n][i], x[n][i], sum);
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                const float scale = 1.0f / sqrtf(sum / (float)D + p.epsilon);
+                const float own = __shfl_sync(0xffffffffu, scale, (n >> 1) * 16 + (n & 1) * 8);
                 float g[E];
                 load<E, WIDE, true>(gain + first, g);
 #pragma unroll
-                for (int i = 0; i < E; ++i) x[n][i] = x[n][i] * scale * g[i];
+                for (int i = 0; i < E; ++i) x[n][i] = x[n][i] * own * g[i];
             }
             if (p.rotary && p.style == RQ_ROPE_PAIRS) {
                 if (turns) {

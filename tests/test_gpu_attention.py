@@ -253,6 +253,12 @@ def test_decode_steps_among_prompts(rq_ctx, hq, hk, d, dtype, cached, fresh):
     assert (run(rq_ctx, b) == run(rq_ctx, b)).all()
 
 
+def test_nothing_but_decode_steps_when_the_host_does_not_know(rq_ctx):
+    b = batch([40, 700, 0, 5, 300, 64, 63, 1, 999], [1] * 9, 8, 2, 128, 16)
+    compare(run(rq_ctx, b, max_fresh=0), b)
+    compare(run(rq_ctx, b, max_fresh=500), b)
+
+
 @pytest.mark.parametrize("fresh", [[1, 1], [1, 80]])
 def test_recorded_and_replayed_over_longer_requests(fresh):
     """The lengths are read when a recorded call runs, not when it is recorded; the work area has to be there before."""
