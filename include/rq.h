@@ -350,7 +350,7 @@ int rq_rope_store(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, 
  * position p = lengths[r] - (starts[r + 1] - t), sees the keys j <= p, with a window > 0 only those with j > p - window:
  *   y[t][h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q[t][h] . k_j - max),  k_j, v_j of head h / (q_heads / heads).
  * A row that sees no key gets zeros; keys that are masked, lie past lengths[r] or on a page outside the cache count for nothing,
- * whatever they hold. Tokens from starts[requests] on are not written. q and y: heads head_dim apart, tokens *_t_stride apart, any
+ * whatever they hold. Tokens from starts[requests] on are not written; tokens of the batch from `tokens` on are passed over. q and y: heads head_dim apart, tokens *_t_stride apart, any
  * alignment. max_fresh is the most new tokens that a request has, as far as the host knows: the choice of kernel rests on it,
  * the results do not.
  * Activations stay fp32: queries and weights meet the 16-bit keys and values as two (f16) or three (bf16) 16-bit parts, products

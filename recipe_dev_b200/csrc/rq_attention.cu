@@ -70,18 +70,20 @@ template <int TYPE> __device__ __forceinline__ bool finite2(uint32_t w) {
 
 // A request's rows and keys, as a CTA deals with them
 struct Request {
-    int fresh, length, begin, end, tiles;  // keys [begin, end) are seen by some row; row tiles
+    int fresh, here, length, begin, end, tiles;  // new tokens, those with queries; keys [begin, end) are seen by some row; row tiles
     int64_t units;                         // of one row tile and head
 };
 template <int ROWS> __device__ __forceinline__ Request request_of(const AttentionParams& p, int r) {
     Request q;
     const int start = p.starts[r];
-    q.fresh = max(p.starts[r + 1] - start, 0);
+    const int next = p.starts[r + 1];
+    q.fresh = max(next - start, 0);
+    q.here = tokens_here(p, start, next);
     q.length = p.lengths[r];
     q.end = (int)min((int64_t)max(q.length, 0), (int64_t)p.table_width << p.page_shift);
     q.begin = p.window > 0 ? (int)max((int64_t)0, (int64_t)q.length - q.fresh - p.window + 1) : 0;
     q.begin = min(q.begin, q.end) & ~(kTile - 1);
-    q.tiles = (q.fresh * (p.q_heads / p.kv_heads) + ROWS - 1) / ROWS;
+    q.tiles = (q.here * (p.q_heads / p.kv_heads) + ROWS - 1) / ROWS;
     q.units = max((q.end - q.begin + kUnit - 1) / kUnit, 1);  // (a row that sees no key is written all the same)
     return q;
 }
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
     if (tid == 0) before[0] = 0;
     for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
         int64_t units = 0;
-        if (r0 + tid < p.requests) { const Request q = request_of<ROWS>(p, r0 + tid); units = (int64_t)q.fresh * group > p.few ? 0 : q.units * q.tiles * p.kv_heads; }
+        if (r0 + tid < p.requests) { const Request q = request_of<ROWS>(p, r0 + tid); units = (int64_t)q.here * group > p.few ? 0 : q.units * q.tiles * p.kv_heads; }
         int64_t scan = units;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) { const int64_t o = __shfl_up_sync(0xffffffffu, scan, off); if (lane >= off) scan += o; }
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
         for (int hi = p.requests - 1; r < hi;) { const int mid = (r + hi + 1) >> 1; if (before[mid] <= u) r = mid; else hi = mid - 1; }
         const Request rq = request_of<ROWS>(p, r);
         const int64_t in_request = u - before[r], item = in_request / rq.units, first_unit = in_request % rq.units;
-        const int kv = (int)(item % p.kv_heads), row0 = (int)(item / p.kv_heads) * ROWS, rows = min(ROWS, rq.fresh * group - row0);
+        const int kv = (int)(item % p.kv_heads), row0 = (int)(item / p.kv_heads) * ROWS, rows = min(ROWS, rq.here * group - row0);
         const int64_t item_begin = u - first_unit, item_end = item_begin + rq.units, stop = min(item_end, my_end);
         const int key_first = rq.begin + (int)first_unit * kUnit, key_stop = min(rq.end, rq.begin + (int)(stop - item_begin) * kUnit);
         u = stop;

@@ -36,6 +36,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 12.0f;
 
 #ifdef __CUDACC__
+// How many of a request's new tokens the call has queries for: a batch may be longer than the call
+__device__ __forceinline__ int tokens_here(const AttentionParams& p, int start, int next) { return start < 0 ? 0 : max(min(next, p.tokens) - start, 0); }
+
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // two fp32 numbers as a pair of 16-bit ones (the first in the low half), and what the pair leaves of them

@@ -48,7 +48,7 @@ template <int D, int TYPE, bool KEYS_> struct Form {
     static constexpr int PARTS = TYPE == RQ_KV_F16 ? 2 : 3;
     static constexpr int KT = TYPE == RQ_KV_F16 || D == 64 ? 128 : 64;  // keys a tile (bf16, 128 elements: 2 KT + 2 D + KT columns are what tensor memory holds with 64)
     static constexpr int TILE_BYTES = KT * D * 2, Q_PART = 128 * D * 2, Q_BYTES = (KEYS ? 1 : 2) * PARTS * Q_PART;
-    static constexpr int STAGES_FIT = (227 * 1024 - 3072 - Q_BYTES) / TILE_BYTES, STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
+    static constexpr int STAGES_FIT = ((227 - 3) * 1024 - Q_BYTES) / TILE_BYTES, STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
     static constexpr int BLOCK = KEYS ? 128 : 256;                // rows
     static constexpr int UNIT = KEYS ? 2 * KT : KT;               // keys
     static constexpr int T_COL = 2 * KT, LO_COL = T_COL + 2 * D;  // tensor memory: scores (then weights), tile sums, bf16's third parts
@@ -58,22 +58,22 @@ template <int D, int TYPE, bool KEYS_> struct Form {
 
 // A block of rows of one request and key head, and the keys that some row of it sees
 struct Block {
-    int start, fresh, row0, rows, position0, begin, low, high, end;  // keys [low, high), from the tile at begin; end: the request's keys
+    int start, row0, rows, position0, begin, low, high, end;  // keys [low, high), from the tile at begin; end: the request's keys
     int units;
 };
 template <typename F> __device__ __forceinline__ int blocks_of(const AttentionParams& p, int r, int group) {
-    const int rows = max(p.starts[r + 1] - p.starts[r], 0) * group;
+    const int rows = tokens_here(p, p.starts[r], p.starts[r + 1]) * group;
     return rows > p.few ? (rows + F::BLOCK - 1) / F::BLOCK : 0;
 }
 template <typename F> __device__ __forceinline__ Block block_of(const AttentionParams& p, int r, int b, int group) {
     Block k;
     k.start = p.starts[r];
-    k.fresh = max(p.starts[r + 1] - k.start, 0);
+    const int next = p.starts[r + 1];
     const int length = p.lengths[r];
     k.end = (int)min((int64_t)max(length, 0), (int64_t)p.table_width << p.page_shift);
-    k.position0 = length - k.fresh;
+    k.position0 = length - max(next - k.start, 0);
     k.row0 = b * F::BLOCK;
-    k.rows = min(F::BLOCK, k.fresh * group - k.row0);
+    k.rows = min(F::BLOCK, tokens_here(p, k.start, next) * group - k.row0);
     const int first = k.row0 / group, last = (k.row0 + k.rows - 1) / group;
     k.high = max(0, min(k.end, k.position0 + last + 1));
     k.low = p.window > 0 ? min(k.high, max(0, k.position0 + first - p.window + 1)) : 0;

@@ -157,6 +157,21 @@ def test_tokens_past_the_batch_are_not_written(rq_ctx):
         compare(got, b)
 
 
+@pytest.mark.parametrize("fresh,given", [([1, 1, 1], 2), ([3, 40], 30), ([3, 40], 2), ([90, 100], 120), ([4, 5], 4)])
+def test_a_batch_longer_than_the_call(rq_ctx, fresh, given):
+    """The plan may count more tokens than the arrays that the call is given have room for: those are passed over, the others are what they are."""
+    import torch
+
+    b = batch([20] * len(fresh), fresh, 4, 2, 128, 16)
+    whole = torch.full(b["q"].shape, 9.0, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    rq_ctx.attention(b["q"][:given], b["cache"], b["table"], torch.tensor(b["starts"], **i32), torch.tensor(b["lengths"], **i32), max_fresh=max(fresh), y=whole[:given])
+    rq_ctx.check()
+    assert (whole[given:] == 9.0).all()
+    want, bound = ref.attention(b["q"].reshape(-1, 4, 128), b["cache"].k, b["cache"].v, b["table"], b["starts"], b["lengths"], 128**-0.5)
+    assert ((whole.reshape(-1, 4, 128).double() - want).abs() <= bound)[:given].all()
+
+
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf"), -65504.0, 65504.0])
 @pytest.mark.parametrize("fresh", [1, 2, 40, 200])
 def test_whatever_masked_places_hold(rq_ctx, value, fresh):
