@@ -84,12 +84,13 @@ def test_every_step_against_64_bits(model):
     model.ctx.check()
 
 
+@pytest.mark.parametrize("requests", [3, 11])
 @pytest.mark.parametrize("filters", [dict(), dict(temperature=0.9, top_k=50, top_p=0.9, seed=3)])
-def test_replayed_steps_give_the_direct_steps_tokens(model, filters):
+def test_replayed_steps_give_the_direct_steps_tokens(model, filters, requests):
     def run(record):
         from recipe_dev_b200 import serve
 
-        served = serve.Batch(model, [[5, 6, 7], [8, 9, 10], [11, 12, 13]], new=20, record=record, **filters)
+        served = serve.Batch(model, [[5 + r, 6, 7] for r in range(requests)], new=20, record=record, **filters)
         out = served.run()
         assert (served.sequence is not None) == record
         served.free_sequence()
