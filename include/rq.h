@@ -365,8 +365,8 @@ int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, c
  * whole number w_i = floor(2^40 * exp((x_i - max x) / temperature)) (fp32 arithmetic), so that every sum of weights is exact and
  * the result depends on no order of additions. Tokens are kept by rank, larger logits first and, among equal ones, lower indices first:
  *   top_k:  the first top_k (<= 0: all);
- *   top_p:  of those, the ones before which less than top_p of their mass lies, at least one (>= 1: all);
- *   min_p:  of those, the ones whose weight is at least min_p of the largest.
+ *   top_p:  of those, the ones before which less than top_p of their mass lies, at least one (>= 1 or NaN: all; <= 0: the first);
+ *   min_p:  of those, the ones whose weight is at least min_p of the largest (<= 0 or NaN: all; >= 1: those that weigh as much as it).
  * The token is the first, by index, at which the kept weights' running sum exceeds floor(uniform * their sum). token[r] receives
  * it, probability[r] its weight over that sum (null: not wanted), kept[r] how many tokens of positive weight were kept (null: not wanted).
  * temperature <= 0 takes the largest logit (the lowest index of equal ones); a null parameter array counts as 1, 0, 1, 0.

@@ -202,7 +202,9 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
     Shared* const leader = cluster.map_shared_rank(&sh, 0);
     wait_for_previous();
     const float* x = p.logits + row * p.stride + first;
-    const float temperature = p.temperature ? p.temperature[row] : 1.0f, top_p = p.top_p ? p.top_p[row] : 1.0f, min_p = p.min_p ? p.min_p[row] : 0.0f;
+    const float temperature = p.temperature ? p.temperature[row] : 1.0f, given_p = p.top_p ? p.top_p[row] : 1.0f, given_min = p.min_p ? p.min_p[row] : 0.0f;
+    // into their ranges, NaN to the end that keeps all (the parts of a histogram are made for these: logf(V / (1 - top_p)) is not below 0)
+    const float top_p = given_p < 1.0f ? fmaxf(given_p, 0.0f) : 1.0f, min_p = given_min > 0.0f ? fminf(given_min, 1.0f) : 0.0f;
     const int top_k = (p.top_k && p.top_k[row] > 0 ? p.top_k[row] : p.vocabulary);
     auto at = [&](int i) { return STAGED ? staged[i] : cleaned(__ldcg(x + i)); };
 
@@ -273,7 +275,8 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
     const Weigher weigh(top, temperature);
     const float limit = fminf(kFade * temperature, 3e38f);
     float scale = (float)kBins / limit;
-    auto floor_of = [](float place) { return (int)(__float_as_uint(__fadd_rd(fminf(place, (float)(kBins - 1)), 8388608.0f)) & 0x7fffffu); };  // 0 <= place, up to the last part
+    // 0 <= place (and NaN, which comes out as the last part): distances from the largest logit times a scale that is positive, since all of what it is made of is
+    auto floor_of = [](float place) { return (int)(__float_as_uint(__fadd_rd(fminf(place, (float)(kBins - 1)), 8388608.0f)) & 0x7fffffu); };
     auto part_of = [&](float v) { return v == top ? 0 : floor_of((top - v) * scale); };
     auto sub_of = [&](float v) { const float place = (top - v) * scale; return v == top ? 0 : floor_of((place - (float)floor_of(place)) * (float)kBins); };
     // What lies so far below weighs nothing: by one comparison (the rounding of this value takes no logit's weight, for they are rounded alike)
