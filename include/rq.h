@@ -322,7 +322,7 @@ typedef struct rq_kv_cache {
  *     past the batch's tokens -1, 0 and -1;
  *   status[0 .. 2]: tokens, pages taken, pages lacking.
  * Where pages are lacking (the list is too short, or a request outgrows table_width), the entries are -1 (or not there) and so are
- * the slots of their tokens: rq_rope_store passes over them, and nothing else of the batch changes. A negative length counts as
+ * the slots of their tokens (as of those on a page whose positions would be 2^31 or more): rq_rope_store passes over them, and nothing else of the batch changes. A negative length counts as
  * zero. At most RQ_MAX_REQUESTS requests, fewer than 2^31 tokens and positions. Nothing is read and written by the same call but
  * block_table, so a step may be planned again from the same lengths. */
 #define RQ_MAX_REQUESTS 4096

@@ -91,7 +91,9 @@ __global__ void __launch_bounds__(kThreads) rq_batch_plan_kernel(PlanParams p) {
                 const int i = before[owner] + column - held;  // a new page: from the list, its entry may not be written yet
                 entry = column < held ? p.block_table[(int64_t)owner * p.table_stride + column] : (i < p.free_count ? p.free_pages[i] : -1);
             }
-            if (entry >= 0) slot = (entry << p.page_shift) + (position & (page - 1));
+            // (an entry that names no page of any cache must not come out as a position of another one's)
+            const int64_t place = ((int64_t)entry << p.page_shift) + (position & (page - 1));
+            if (entry >= 0 && place <= 0x7fffffff) slot = (int)place;
         }
         p.slots[t] = slot;
         p.positions[t] = position;
