@@ -133,6 +133,7 @@ extern "C" int rq_batch_plan(rq_ctx* ctx, const int32_t* cached, const int32_t* 
     const int64_t ctas = ((int64_t)max_tokens + kThreads - 1) / kThreads;
     const unsigned grid = (unsigned)(ctas < ctx->sm_count ? ctas : ctx->sm_count);
     const size_t smem = sizeof(int32_t) * (3 * (size_t)requests + 2);
-    if (smem > 48 * 1024) RQ_CUDA(cudaFuncSetAttribute(rq_batch_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // (48 KB without asking are for it and the kernel's static shared memory together)
+    if (smem > 47 * 1024) RQ_CUDA(cudaFuncSetAttribute(rq_batch_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     return launch(rq_batch_plan_kernel, dim3(grid), kThreads, smem, (cudaStream_t)stream, p);
 }

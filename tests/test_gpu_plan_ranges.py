@@ -38,3 +38,25 @@ def test_the_last_slots_that_there_are(rq_ctx):
 def test_a_free_list_that_names_no_page(rq_ctx):
     got = planned(rq_ctx, [0, 0], [17, 1], [[-7, -7], [-7, -7]], [2**30, 4, -3], 16, 18)
     assert got[0] == [[2**30, 4], [-3, -7]] and got[3] == [-1] * 16 + [64, -1]
+
+
+@pytest.mark.parametrize("requests", [4010, 4085, 4089, 4090, 4092, 4094, 4095, 4096])
+def test_nearly_as_many_requests_as_there_can_be(requests):
+    """Their lengths are just below and above what shared memory holds without being asked for; in a process of its own, where nobody has asked before."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    program = f"""
+import torch
+import recipe_dev_b200 as rq
+n = {requests}
+i32 = dict(dtype=torch.int32, device="cuda")
+ctx = rq.Context(0)
+free = torch.arange(n, **i32).flip(0).contiguous()
+got = ctx.batch_plan(torch.zeros(n, **i32), torch.ones(n, **i32), torch.full((n, 1), -1, **i32), free, 16, max_tokens=n)
+ctx.check()
+assert got[2].tolist() == (16 * free).tolist() and got[5].tolist() == [n, n, 0]
+"""
+    run = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
+    assert run.returncode == 0, run.stderr[-2000:]
