@@ -323,7 +323,7 @@ typedef struct rq_kv_cache {
  *   status[0 .. 2]: tokens, pages taken, pages lacking.
  * Where pages are lacking (the list is too short, or a request outgrows table_width), the entries are -1 (or not there) and so are
  * the slots of their tokens (as of those on a page whose positions would be 2^31 or more): rq_rope_store passes over them, and nothing else of the batch changes. A negative length counts as
- * zero. At most RQ_MAX_REQUESTS requests, fewer than 2^31 tokens and positions. Nothing is read and written by the same call but
+ * zero. At most RQ_MAX_REQUESTS requests. Where a batch's tokens or a request's positions pass 2^31 - 1, their counts end there, and positions beyond have no slot. Nothing is read and written by the same call but
  * block_table, so a step may be planned again from the same lengths. */
 #define RQ_MAX_REQUESTS 4096
 int rq_batch_plan(rq_ctx* ctx, const int32_t* cached, const int32_t* fresh, int requests, int page_size, int32_t* block_table, int64_t table_stride, int table_width,

@@ -19,12 +19,14 @@ struct PlanParams {
     int requests, table_width, free_count, max_tokens, page_shift;
 };
 
+constexpr int64_t kMost = 0x7fffffff;
+
 // Inclusive sum over the CTA's threads of two numbers at once
-__device__ __forceinline__ int2 block_sums(int2 v, int2* warp_sums) {
+__device__ __forceinline__ longlong2 block_sums(longlong2 v, longlong2* warp_sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, v.x, off), b = __shfl_up_sync(0xffffffffu, v.y, off);
+        const int64_t a = __shfl_up_sync(0xffffffffu, v.x, off), b = __shfl_up_sync(0xffffffffu, v.y, off);
         if (lane >= off) { v.x += a; v.y += b; }
     }
     if (lane == 31) warp_sums[warp] = v;
@@ -36,14 +38,16 @@ __device__ __forceinline__ int2 block_sums(int2 v, int2* warp_sums) {
 
 __global__ void __launch_bounds__(kThreads) rq_batch_plan_kernel(PlanParams p) {
     extern __shared__ int32_t table[];  // starts [requests + 1] | pages before [requests + 1] | cached [requests]
-    __shared__ int2 warp_sums[kThreads / 32];
-    __shared__ int lacking;
+    __shared__ longlong2 warp_sums[kThreads / 32];
+    __shared__ unsigned long long lacking;
     launch_dependents();
     int32_t *starts = table, *before = table + p.requests + 1, *cached = before + p.requests + 1;
     const int page = 1 << p.page_shift, tid = threadIdx.x;
+    // (of up to 2^31 - 1 positions: an unsigned sum does not wrap)
+    auto pages_of = [&](int positions) { return (int)(((uint32_t)positions + (uint32_t)(page - 1)) >> p.page_shift); };
     wait_for_previous();
-    int2 carry = make_int2(0, 0);
-    int too_wide = 0;
+    longlong2 carry = make_longlong2(0, 0);  // sums in 64 bits, kept up to 2^31 - 1: whatever the lengths are, starts ascend and every index below lies inside its array
+    int64_t too_wide = 0;
     if (tid == 0) { starts[0] = 0; before[0] = 0; lacking = 0; }
     for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
         const int r = r0 + tid;
@@ -51,49 +55,57 @@ __global__ void __launch_bounds__(kThreads) rq_batch_plan_kernel(PlanParams p) {
         if (r < p.requests) {
             have = max(p.cached[r], 0);
             more = max(p.fresh[r], 0);
-            const int held = (have + page - 1) >> p.page_shift, all = (have + more + page - 1) >> p.page_shift;
-            need = max(min(all, p.table_width) - held, 0);
+            const int64_t all = ((int64_t)have + more + page - 1) >> p.page_shift;
+            const int held = pages_of(have);
+            need = max((int)min(all, (int64_t)p.table_width) - held, 0);
             too_wide += all - held - need;
             cached[r] = have;
-            if (blockIdx.x == 0) p.lengths[r] = have + more;
+            if (blockIdx.x == 0) p.lengths[r] = (int)min((int64_t)have + more, kMost);
         }
-        int2 sum = block_sums(make_int2(more, need), warp_sums);
-        sum.x += carry.x;
-        sum.y += carry.y;
+        longlong2 sum = block_sums(make_longlong2(more, need), warp_sums);
+        sum.x = min(sum.x + carry.x, (long long)kMost);
+        sum.y = min(sum.y + carry.y, (long long)kMost);
         if (r < p.requests) {
-            starts[r + 1] = sum.x;
-            before[r + 1] = sum.y;
-            if (blockIdx.x == 0) p.starts[r + 1] = sum.x;
+            starts[r + 1] = (int)sum.x;
+            before[r + 1] = (int)sum.y;
+            if (blockIdx.x == 0) p.starts[r + 1] = (int)sum.x;
         }
         __syncthreads();
         const int last = min(r0 + kThreads, p.requests);
-        carry = make_int2(starts[last], before[last]);
+        carry = make_longlong2(starts[last], before[last]);
     }
-    const int tokens = carry.x, pages = carry.y;
+    const int tokens = (int)carry.x, pages = (int)carry.y;
     if (blockIdx.x == 0) {
-        if (too_wide) atomicAdd(&lacking, too_wide);  // whole numbers: any order gives the same
+        if (too_wide) atomicAdd(&lacking, (unsigned long long)too_wide);  // whole numbers: any order gives the same
         __syncthreads();
-        if (tid == 0) { p.starts[0] = 0; p.status[0] = tokens; p.status[1] = min(pages, p.free_count); p.status[2] = max(pages - p.free_count, 0) + lacking; }
+        if (tid == 0) {
+            p.starts[0] = 0;
+            p.status[0] = tokens;
+            p.status[1] = min(pages, p.free_count);
+            p.status[2] = (int)min((int64_t)max(pages - p.free_count, 0) + (int64_t)lacking, kMost);
+        }
     }
-    for (int i = blockIdx.x * kThreads + tid; i < pages; i += gridDim.x * kThreads) {
-        const int r = owner_of(before, p.requests, i);
-        const int column = ((cached[r] + page - 1) >> p.page_shift) + i - before[r];
+    const int64_t first = (int64_t)blockIdx.x * kThreads + tid, step = (int64_t)gridDim.x * kThreads;
+    for (int64_t n = first; n < pages; n += step) {
+        const int i = (int)n, r = owner_of(before, p.requests, i);
+        const int column = pages_of(cached[r]) + i - before[r];
         p.block_table[(int64_t)r * p.table_stride + column] = i < p.free_count ? p.free_pages[i] : -1;
     }
-    for (int t = blockIdx.x * kThreads + tid; t < p.max_tokens; t += gridDim.x * kThreads) {
+    for (int64_t t = first; t < p.max_tokens; t += step) {
         int slot = -1, position = 0, owner = -1;
         if (t < tokens) {
-            owner = owner_of(starts, p.requests, t);
-            position = cached[owner] + t - starts[owner];
-            const int column = position >> p.page_shift, held = (cached[owner] + page - 1) >> p.page_shift;
+            owner = owner_of(starts, p.requests, (int)t);
+            const int64_t at = (int64_t)cached[owner] + t - starts[owner];
+            position = (int)min(at, kMost);
+            const int column = position >> p.page_shift, held = pages_of(cached[owner]);
             int entry = -1;
-            if (column < p.table_width) {
-                const int i = before[owner] + column - held;  // a new page: from the list, its entry may not be written yet
+            if (at <= kMost && column < p.table_width) {
+                const int64_t i = (int64_t)before[owner] + column - held;  // a new page: from the list, its entry may not be written yet
                 entry = column < held ? p.block_table[(int64_t)owner * p.table_stride + column] : (i < p.free_count ? p.free_pages[i] : -1);
             }
             // (an entry that names no page of any cache must not come out as a position of another one's)
             const int64_t place = ((int64_t)entry << p.page_shift) + (position & (page - 1));
-            if (entry >= 0 && place <= 0x7fffffff) slot = (int)place;
+            if (entry >= 0 && place <= kMost) slot = (int)place;
         }
         p.slots[t] = slot;
         p.positions[t] = position;
