@@ -456,16 +456,18 @@ int ensure_work_area(rq_ctx* ctx) {
 
 template <int D, int TYPE, int RT>
 int launch_rows(rq_ctx* ctx, const AttentionParams& p, cudaStream_t s) {
-    static int resident = 0;  // CTAs an SM holds
     auto kernel = rq_attention_rows_kernel<D, TYPE, RT>;
     const size_t smem = sizeof(Tiles<D, TYPE, RT>) + sizeof(int64_t) * ((size_t)p.requests + 1);
-    if (!resident) {
+    static int resident[64] = {};  // by device: CTAs an SM holds; 0 before the opt-in to large shared memory
+    const int dev = ctx->device;
+    int n = dev < 64 ? resident[dev] : 0;
+    if (!n) {
         RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(Tiles<D, TYPE, RT>) + sizeof(int64_t) * (RQ_MAX_REQUESTS + 1))));
-        int n = 0;
         RQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, smem));
-        resident = n < 1 ? 1 : (n > 4 ? 4 : n);
+        n = n < 1 ? 1 : (n > 4 ? 4 : n);
+        if (dev < 64) resident[dev] = n;
     }
-    const int ctas = ctx->sm_count * resident;
+    const int ctas = ctx->sm_count * n;
     return launch(kernel, dim3((unsigned)(ctas < kRowCtas ? ctas : kRowCtas)), kThreads, smem, s, p);
 }
 

@@ -823,10 +823,10 @@ int launch_form(rq_ctx* ctx, const AttentionParams& p, const CUtensorMap& k, con
     auto kernel = rq_attention_tc_kernel<D, TYPE, KEYS>;
     constexpr size_t smem = F::Q_BYTES + F::STAGES * F::TILE_BYTES + sizeof(Shared<F>);
     static_assert(smem <= 227 * 1024, "shared memory");
-    static bool allowed = false;
-    if (!allowed) {
+    static bool configured[64] = {};  // by device: the opt-in to large shared memory
+    if (ctx->device >= 64 || !configured[ctx->device]) {
         RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        allowed = true;
+        if (ctx->device < 64) configured[ctx->device] = true;
     }
     const int ctas = ctx->sm_count < kTensorCtas ? ctx->sm_count : kTensorCtas;
     return launch(kernel, dim3((unsigned)ctas), kThreads, smem, s, p, k, v);

@@ -627,13 +627,13 @@ __global__ void __launch_bounds__(kThreads, 2) rq_sample_kernel(SampleParams p) 
 }
 
 template <bool STAGED>
-int launch_sample(const SampleParams& p, int rows, int ctas, cudaStream_t s) {
-    static bool allowed = false;
+int launch_sample(rq_ctx* ctx, const SampleParams& p, int rows, int ctas, cudaStream_t s) {
     auto kernel = rq_sample_kernel<STAGED>;
-    if (!allowed) {
+    static bool configured[64] = {};  // by device: the opt-ins to clusters of sixteen and to large shared memory
+    if (ctx->device >= 64 || !configured[ctx->device]) {
         RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         if (STAGED) RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShare * (int)sizeof(float)));
-        allowed = true;
+        if (ctx->device < 64) configured[ctx->device] = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * ctas));
@@ -672,6 +672,6 @@ extern "C" int rq_sample(rq_ctx* ctx, const float* logits, int64_t row_stride, i
     const int64_t unit = 4 * kThreads;  // a warp's share is a whole number of 128
     SampleParams p = {logits, temperature, top_p, min_p, uniform, top_k, token, kept, probability, row_stride, (int)vocabulary, 0};
     p.share = (int)(((vocabulary + ctas - 1) / ctas + unit - 1) / unit * unit);
-    if (p.share <= kShare) return launch_sample<true>(p, rows, ctas, (cudaStream_t)stream);
-    return launch_sample<false>(p, rows, ctas, (cudaStream_t)stream);
+    if (p.share <= kShare) return launch_sample<true>(ctx, p, rows, ctas, (cudaStream_t)stream);
+    return launch_sample<false>(ctx, p, rows, ctas, (cudaStream_t)stream);
 }
