@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 16, kUnit = kWarps * kTile;  // keys a warp and a CTA take at a time
+constexpr int kRequestStep = 128;
 constexpr int kStages = 2;  // of a warp's ring: one tile under way while the other is used
 
 // c = (first ? 0 : c) + a b for sixteen rows, eight columns and sixteen products each
@@ -457,18 +458,20 @@ int ensure_work_area(rq_ctx* ctx) {
 template <int D, int TYPE, int RT>
 int launch_rows(rq_ctx* ctx, const AttentionParams& p, cudaStream_t s) {
     auto kernel = rq_attention_rows_kernel<D, TYPE, RT>;
-    const size_t smem = sizeof(Tiles<D, TYPE, RT>) + sizeof(int64_t) * ((size_t)p.requests + 1);
-    static int resident[64] = {};  // by device: CTAs an SM holds; 0 before the opt-in to large shared memory
-    const int dev = ctx->device;
-    int n = dev < 64 ? resident[dev] : 0;
+    // The grid decides where rows are cut, and with it the last bits: it follows from the call alone. Shared memory holds eight bytes a request, by steps of 128 of them.
+    const int step = (p.requests + kRequestStep - 1) / kRequestStep, dev = ctx->device;
+    auto bytes = [](int steps) { return sizeof(Tiles<D, TYPE, RT>) + sizeof(int64_t) * ((size_t)steps * kRequestStep + 1); };
+    constexpr int kSteps = RQ_MAX_REQUESTS / kRequestStep;
+    static uint8_t resident[64][kSteps + 1] = {};  // by device: CTAs an SM holds; 0: not known yet
+    int n = dev < 64 ? resident[dev][step] : 0;
     if (!n) {
-        RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(Tiles<D, TYPE, RT>) + sizeof(int64_t) * (RQ_MAX_REQUESTS + 1))));
-        RQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, smem));
+        RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(kSteps)));
+        RQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, bytes(step)));
         n = n < 1 ? 1 : (n > 4 ? 4 : n);
-        if (dev < 64) resident[dev] = n;
+        if (dev < 64) resident[dev][step] = (uint8_t)n;
     }
     const int ctas = ctx->sm_count * n;
-    return launch(kernel, dim3((unsigned)(ctas < kRowCtas ? ctas : kRowCtas)), kThreads, smem, s, p);
+    return launch(kernel, dim3((unsigned)(ctas < kRowCtas ? ctas : kRowCtas)), kThreads, bytes(step), s, p);
 }
 
 // two: sixteen rows at a time. Not for 256 elements a head, whose sums of sixteen rows do not fit a thread's registers: 16 requests of eight tokens over 8192 keys, 8 + 2 x 4
