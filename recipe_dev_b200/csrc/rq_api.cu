@@ -184,6 +184,7 @@ static const char* wait_code_text(int code) {
         case 49: return "attention, issuing warp: the products never completed";
         case 50: return "attention, loading warp: an item's place never came free";
         case 51: return "attention, mending warp: a tile of values never arrived";
+        case 52: return "attention, softmax warps: the other pipe's sums never came";
         default: return "unknown wait";
     }
 }

@@ -444,11 +444,11 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
 int ensure_work_area(rq_ctx* ctx) {
     if (ctx->attn_scratch) return RQ_OK;
     if (ctx->recording) return rq_fail(RQ_ERR_INVALID, "a recorded rq_attention needs its work area: call rq_attention_reserve before rq_sequence_begin");
-    const size_t bytes = kPartialBytes + kRowCtas * sizeof(uint32_t);
+    const size_t bytes = kPartialBytes + kCounts * sizeof(uint32_t);
     uint8_t* area = nullptr;
     cudaError_t e = cudaMalloc(&area, bytes);
     if (e != cudaSuccess) return rq_fail(RQ_ERR_ALLOC, "attention's work area of %zu bytes: %s", bytes, cudaGetErrorString(e));
-    e = cudaMemset(area + kPartialBytes, 0, kRowCtas * sizeof(uint32_t));
+    e = cudaMemset(area + kPartialBytes, 0, kCounts * sizeof(uint32_t));
     if (e == cudaSuccess) e = cudaDeviceSynchronize();  // streams that do not wait for the default one may use it next
     if (e != cudaSuccess) { cudaFree(area); return rq_fail(RQ_ERR_CUDA, "attention's work area: %s", cudaGetErrorString(e)); }
     ctx->attn_scratch = area;

@@ -10,7 +10,7 @@ struct AttentionParams {
     const uint16_t *k, *v;
     const int32_t *block_table, *starts, *lengths;
     float* partial;      // sums of rows whose keys several CTAs share
-    uint32_t* arrived;   // per CTA: how many have left their part of the rows that begin there; zero between calls
+    uint32_t* arrived;   // per CTA (the tensor-core kernel: and warp of rows): how many have left their part of the rows that begin there; zero between calls
     int64_t q_stride, y_stride, table_stride, head_stride, pages;
     uint32_t page_bytes, line_bytes;
     int tokens, requests, q_heads, kv_heads, table_width, page_shift, window;
@@ -25,6 +25,7 @@ struct AttentionParams {
 // maxima and sums of weights), then the counts.
 constexpr int kTensorCtas = 148, kRowCtas = 148 * 4;
 constexpr size_t kTensorPartial = (size_t)kTensorCtas * 2 * 2 * 128 * (128 + 2), kRowPartial = (size_t)kRowCtas * 2 * 16 * (256 + 2);  // floats
+constexpr size_t kCounts = kTensorCtas * 2 * 4 > kRowCtas ? kTensorCtas * 2 * 4 : kRowCtas;
 constexpr size_t kPartialBytes = sizeof(float) * (kTensorPartial > kRowPartial ? kTensorPartial : kRowPartial);
 
 // Rows by the hundred (rq_attention_tc.cu); one_tile: at most 128 rows a request and key head. RQ_ERR_UNSUPPORTED (no error text) = a cache that it does not

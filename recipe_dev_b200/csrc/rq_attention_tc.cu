@@ -136,17 +136,15 @@ __device__ __forceinline__ void store32(float* p, const float* x, float f) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_to_tensor_core() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-template <int THREADS> __device__ __forceinline__ void named_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
-
 
 template <typename F> struct Shared {
-    uint64_t full[F::STAGES], empty[F::STAGES], item_full[kItems], item_empty[kItems], q_full[2], s_full[2], p_full[2][2], t_full[2], t_empty[2], q_empty, landed[F::STAGES], ended;
+    uint64_t full[F::STAGES], empty[F::STAGES], item_full[kItems], item_empty[kItems], q_full[2], s_full[2], p_full[2][2], t_full[2], t_empty[2], q_empty, landed[F::STAGES], joined[4], ended;
     int64_t warp_sums[kThreads / 32], range[2];
     int where[4];
     Item items[kItems];
     uint32_t pages_there[kWords];  // a tile's pages that the cache has, a bit each; all ones: all of them
     uint32_t odd[kWords];          // whether something was taken out of a tile's values
-    uint32_t arrival[2], tmem_slot;
+    uint32_t tmem_slot;
     float joint[2][F::KEYS ? 128 : 1];  // keys form: the second pipe's maximum and sum of each row
 };
 
@@ -214,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
             mbar_init(&sh.t_full[i], 1);
             mbar_init(&sh.t_empty[i], 4);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(&sh.joined[i], 1);
         mbar_init(&sh.q_empty, 1);
         mbar_init(&sh.ended, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -479,9 +478,10 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     sh.joint[0][row] = m;
                     sh.joint[1][row] = sum;
                     fence_before();
-                    named_sync<64>(3 + quarter);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.joined[quarter]);
                 } else {
-                    named_sync<64>(3 + quarter);
+                    if (!mbar_wait_warp(&sh.joined[quarter], items_done & 1, p.wait_ns, dead)) atomicExch(p.error_flag, 52);
                     fence_after();
                     const float other = sh.joint[0][row], top = fmaxf(m, other), base = top == -INFINITY ? 0.0f : top;
                     const float fa = exp2_fast(m - base), fb = exp2_fast(other - base);
@@ -527,12 +527,14 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     for (int i = 0; i < D; i += 4) __stcg((float4*)(to + mine + i * 128), make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
                     __stcg(to + 128 * D + row, m);
                     __stcg(to + 128 * (D + 1) + row, sum);
+                    // (a warp's rows are joined by themselves: it waits for no other warp of its CTA)
+                    uint32_t* const count = p.arrived + (first_cta * 2 + pipe) * 4 + quarter;
                     __threadfence();
-                    named_sync<128>(1 + pipe);
-                    if (row == 0) sh.arrival[pipe] = atomicAdd(&p.arrived[first_cta * 2 + pipe], 1);
-                    named_sync<128>(1 + pipe);
-                    if (sh.arrival[pipe] == (uint32_t)(last_cta - first_cta)) {
-                        if (row == 0) p.arrived[first_cta * 2 + pipe] = 0;
+                    __syncwarp();
+                    uint32_t before = 0;
+                    if (lane == 0) before = atomicAdd(count, 1);
+                    if (__shfl_sync(0xffffffffu, before, 0) == (uint32_t)(last_cta - first_cta)) {
+                        if (lane == 0) *count = 0;
                         __threadfence();
                         m = -INFINITY;
                         for (int c = first_cta; c <= last_cta; ++c) m = fmaxf(m, __ldcg(part(c) + 128 * D + row));
