@@ -621,8 +621,9 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
             }
             ++sums[pipe];
         };
+        // (once a wait has run out nothing is handed on: who waits for it gives up as well, and no barrier sees an arrival that it does not expect)
         auto release = [&](uint64_t* bar) {
-            if (elect_one()) mma_commit(bar);
+            if (elect_one() && !dead) mma_commit(bar);
             __syncwarp();
         };
         while (const Item* it = next_item()) {
@@ -665,8 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
             ++item_count;
         }
         // nothing may be in flight when tensor memory is freed
-        release(&sh.ended);
         dead = false;
+        release(&sh.ended);
         if (!arrived(&sh.ended, 0)) atomicExch(p.error_flag, 49);
     } else if (warp == kFetcher) {
         // ------------------------------------------------------------ the items' queries, into L2 ahead of their use
@@ -693,6 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                 const int key0 = it->first_key + tile_of(n, tiles) * KT, slot = at.slot;
                 if (is_edge(*it, key0)) {
                     if (!mbar_wait_warp(&sh.landed[slot], phases >> slot & 1, p.wait_ns, dead)) atomicExch(p.error_flag, 51);
+                    if (dead) break;  // (the tile may be on its way: it is not touched, and not handed on)
                     phases ^= 1u << slot;
                     const int first = min(max(it->low - key0, 0), KT), last = min(max(it->high - key0, 0), KT);
                     constexpr uint32_t kExponent = TYPE == RQ_KV_F16 ? 0x7c007c00u : 0x7f807f80u, kCarry = 0x80008000u - kExponent;
@@ -753,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     }
                 }
             }
-            if (lane == 0) {
+            if (lane == 0 && !dead) {
                 sh.items[item_at.slot] = i;
                 mbar_arrive(&sh.item_full[item_at.slot]);
             }
@@ -764,8 +766,9 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
         const int box = lane & (boxes - 1), column = lane / boxes;                               // this lane's copy
         Ring at(STAGES);
         uint32_t key_tiles = 0, value_tiles = 0;
+        uint32_t landings = 0;  // a bit a slot: the parity of its next copies that go to the mending warp
         Item following = deal();
-        while (following.take) {
+        while (following.take && !dead) {
             const Item i = following;
             const int tiles = i.take * (KEYS ? 2 : 1);
             const int32_t* table = p.block_table + (int64_t)i.r * p.table_stride;
@@ -782,6 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                 const int now = page;
                 if (n + 1 < 2 * tiles) page = page_of(tile_of(n + 1, tiles));
                 if (!mbar_wait_warp(&sh.empty[slot], at.phase ^ 1, p.wait_ns, dead)) atomicExch(p.error_flag, 44);
+                if (dead) break;  // (a slot that never came free is not armed again)
                 if (!values) {
                     const uint32_t ok = __ballot_sync(0xffffffffu, now < p.pages || lane >= boxes), all = boxes == 32 ? 0xffffffffu : (1u << boxes) - 1;
                     // (keys past the last one that some row sees have no page here: they are masked by their position)
@@ -796,7 +800,11 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     if (lane == 0) sh.odd[value_tiles % kWords] = 0;
                     ++value_tiles;
                 }
-                uint64_t* bar = values && is_edge(i, key0) ? &sh.landed[slot] : &sh.full[slot];  // (to the mending warp first, which hands it on)
+                uint64_t* bar = &sh.full[slot];
+                if (values && is_edge(i, key0)) {  // (to the mending warp first, which hands it on)
+                    bar = &sh.landed[slot];
+                    landings ^= 1u << slot;
+                }
                 if (lane == 0) mbar_expect_tx(bar, F::TILE_BYTES);
                 __syncwarp();
                 if (column < D / 64) {
@@ -808,10 +816,14 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                 if (n == 1) following = deal();  // ahead of its use: its queries are fetched while this one's tiles are
             }
         }
-        // every copy has landed before the CTA ends: the last use of each slot was waited for by the issuing warp, unless a wait ran out
-        if (dead) {
+        // Every copy has landed before the CTA ends, whoever gave up: the last ones to the mending warp, and the last ones of each slot (a barrier that nothing was
+        // counted by looks as if it had; where the mending warp gave up, a slot's own wait runs out)
+#pragma unroll 1
+        for (int n = 0; n < 2 * STAGES; ++n) {
+            const int slot = n >> 1;
             bool late = false;
-            for (int s = 0; s < STAGES; ++s) { mbar_wait_warp(&sh.full[at.slot], at.phase ^ 1, p.wait_ns, late); at.next(); }
+            if (n & 1) mbar_wait_warp(&sh.landed[slot], (landings >> slot & 1) ^ 1, p.wait_ns, late);
+            else mbar_wait_warp(&sh.full[slot], slot < at.slot ? at.phase : at.phase ^ 1, p.wait_ns, late);
         }
     }
     fence_before();

@@ -28,3 +28,54 @@ def test_the_work_area_has_a_count_for_every_warp_of_rows():
     assert counts == "kTensorCtas * 2 * 4 > kRowCtas ? kTensorCtas * 2 * 4 : kRowCtas" and rows <= ctas * 2 * 4
     host = (CSRC / "rq_attention.cu").read_text()
     assert host.count("kCounts * sizeof(uint32_t)") == 2 and "kRowCtas * sizeof" not in host
+
+
+def test_a_role_that_gave_up_hands_nothing_on():
+    """Armed or arrived at once more, a barrier whose copies are in flight would count what it does not expect; a tile on its way is not mended."""
+    kernel = source().split("rq_attention_tc_kernel(")[1]
+    issuing, rest = kernel.split("if (warp == kIssuer) {\n        \n")[1].split("} else if (warp == kFetcher)")
+    mending, loading = rest.split("} else if (warp == kMender)")[1].split("} else if (warp == kLoader)")
+    # the issuing warp: products and commits
+    for body in re.findall(r"if \(elect_one\(\)([^)]*)\)", issuing):
+        assert body == " && !dead"
+    assert issuing.count("elect_one()") == issuing.count("elect_one() && !dead") == 3
+    last = issuing[issuing.index("dead = false;") :]
+    assert last.index("release(&sh.ended);") < last.index("arrived(&sh.ended, 0)") and issuing.count("sh.ended") == 2
+    # the mending warp
+    waited = mending.index("&sh.landed[slot]")
+    assert waited < mending.index("if (dead) break;") < mending.index("uint4* v") < mending.index("mbar_arrive(&sh.full[slot])")
+    # the loading warp: neither slots nor items
+    tiles = loading[loading.index("&sh.empty[slot]") :]
+    assert tiles.index("if (dead) break;") < tiles.index("mbar_expect_tx(") < tiles.index("tma_load_4d(")
+    assert "while (following.take && !dead)" in loading
+    assert re.search(r"if \(lane == 0 && !dead\) \{\s*sh\.items\[item_at\.slot\] = i;\s*mbar_arrive\(&sh\.item_full", loading)
+
+
+def test_every_copy_has_landed_before_the_cta_ends():
+    """The loading warp waits for each slot's last copies at the barriers that they are counted by, whether it gave up or another role did."""
+    loading = source().split("} else if (warp == kLoader)")[1].split("tcgen05.dealloc")[0]
+    copies, last = loading.split("for (int n = 0; n < 2 * STAGES; ++n)")
+    assert copies.count("tma_load_4d(") == 1 and re.search(r"bar = &sh\.landed\[slot\];\s*landings \^= 1u << slot;", copies)
+    assert "const int slot = n >> 1;" in last and last.count("late);") == 2 and last.count("bool late = false;") == 1
+    assert "mbar_wait_warp(&sh.landed[slot], (landings >> slot & 1) ^ 1," in last and "mbar_wait_warp(&sh.full[slot], slot < at.slot ? at.phase : at.phase ^ 1," in last
+    assert not re.search(r"\bif \(dead\)", last) and last.index("mbar_wait_warp(") < last.index("__syncthreads();")
+
+
+def test_the_parities_that_the_last_waits_look_at():
+    """A wait of parity q is over when the phase before the one that runs has that parity: it must be the phase of the slot's last fill, and of its last landing, for
+    every length and mixture."""
+    import random
+
+    rng = random.Random(2)
+    for stages in (3, 4, 5, 8):
+        for fills in range(5 * stages):
+            full, landed = [0] * stages, [0] * stages  # completed phases: by the copies themselves, or by the mending warp behind them
+            landings = at = phase = 0
+            for edge in (rng.random() < 0.4 for _ in range(fills)):
+                full[at] += 1
+                landed[at] += edge
+                landings ^= edge << at
+                at, phase = (at + 1, phase) if at + 1 < stages else (0, phase ^ 1)
+            for slot in range(stages):  # (none: the phase before the first one has parity 1)
+                assert (landings >> slot & 1) ^ 1 == (landed[slot] - 1) & 1
+                assert (phase if slot < at else phase ^ 1) == (full[slot] - 1) & 1
