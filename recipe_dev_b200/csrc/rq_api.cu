@@ -196,7 +196,11 @@ extern "C" int rq_check(rq_ctx* ctx) {
     int flag = 0;
     RQ_CUDA(cudaMemcpy(&flag, ctx->error_flag, sizeof(int), cudaMemcpyDeviceToHost));
     if (flag) {
-        cudaMemset(ctx->error_flag, 0, sizeof(int));
+        // (what a kernel that gave up left half counted, too: the next call's joins begin from zero)
+        const int rc = rq_attention_forget(ctx);
+        if (rc) return rc;
+        RQ_CUDA(cudaMemset(ctx->error_flag, 0, sizeof(int)));
+        RQ_CUDA(cudaDeviceSynchronize());  // streams that do not wait for the default one may run next
         return rq_fail(RQ_ERR_WAIT, "a kernel gave up a bounded wait (code %d: %s); its outputs are not valid", flag, wait_code_text(flag));
     }
     return RQ_OK;

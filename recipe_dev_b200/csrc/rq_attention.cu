@@ -490,6 +490,11 @@ int launch_rows_of(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cac
 
 }  // namespace
 
+int rq_attention_forget(rq_ctx* ctx) {
+    if (ctx->attn_scratch) RQ_CUDA(cudaMemset(ctx->attn_scratch + kPartialBytes, 0, kCounts * sizeof(uint32_t)));
+    return RQ_OK;
+}
+
 extern "C" int rq_attention_reserve(rq_ctx* ctx) {
     if (!ctx) return rq_fail(RQ_ERR_INVALID, "rq_attention_reserve: null context");
     DeviceGuard guard(ctx->device);

@@ -92,6 +92,8 @@ int rq_launch_export(const rq_weight* w, uint8_t* dev_blocks, cudaStream_t s);
 int rq_launch_dequant(const rq_weight* w, float* out, cudaStream_t s);
 int rq_launch_gemv_generic(rq_ctx* ctx, const rq_weight* w, const float* x, int64_t sk, int64_t st, int tokens, float* y, int64_t yn, int64_t yt, cudaStream_t s);
 int rq_launch_gather(const rq_weight* w, const int32_t* ids, int tokens, float* y, int64_t yn, int64_t yt, cudaStream_t s);
+// sets the counts in rq_attention's work area to zero, where there is one (on the default stream, nothing else running)
+int rq_attention_forget(rq_ctx* ctx);
 // the driver's cuTensorMapEncodeTiled
 typedef CUresult (*rq_encode_tiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                     CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

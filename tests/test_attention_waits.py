@@ -27,7 +27,7 @@ def test_the_work_area_has_a_count_for_every_warp_of_rows():
     counts = re.search(r"constexpr size_t kCounts = (.*);", shared)[1]
     assert counts == "kTensorCtas * 2 * 4 > kRowCtas ? kTensorCtas * 2 * 4 : kRowCtas" and rows <= ctas * 2 * 4
     host = (CSRC / "rq_attention.cu").read_text()
-    assert host.count("kCounts * sizeof(uint32_t)") == 2 and "kRowCtas * sizeof" not in host
+    assert host.count("kCounts * sizeof(uint32_t)") == 3 and "kRowCtas * sizeof" not in host
 
 
 def test_a_role_that_gave_up_hands_nothing_on():
@@ -79,3 +79,12 @@ def test_the_parities_that_the_last_waits_look_at():
             for slot in range(stages):  # (none: the phase before the first one has parity 1)
                 assert (landings >> slot & 1) ^ 1 == (landed[slot] - 1) & 1
                 assert (phase if slot < at else phase ^ 1) == (full[slot] - 1) & 1
+
+
+def test_a_check_that_reports_a_wait_clears_what_was_counted():
+    """A CTA that gave up leaves the counts of parts short: the next call would join rows before all of their parts are there."""
+    api = (CSRC / "rq_api.cu").read_text().split('extern "C" int rq_check(')[1].split("\n}")[0]
+    reported = api.split("if (flag) {")[1]
+    assert reported.index("rq_attention_forget(ctx)") < reported.index("cudaMemset(ctx->error_flag, 0") < reported.index("cudaDeviceSynchronize()") < reported.index("RQ_ERR_WAIT")
+    forget = (CSRC / "rq_attention.cu").read_text().split("int rq_attention_forget(rq_ctx* ctx) {")[1].split("\n}")[0]
+    assert "if (ctx->attn_scratch) RQ_CUDA(cudaMemset(ctx->attn_scratch + kPartialBytes, 0, kCounts * sizeof(uint32_t)));" in forget

@@ -49,3 +49,32 @@ def test_a_call_gives_the_same_bits_whatever_came_first():
     want = after("1")
     assert after("4096") == want
     assert after("700,1,64") == want
+
+
+@pytest.mark.parametrize("fresh", [1, 40])
+def test_calls_after_a_reported_wait(fresh):
+    """A check that reports a wait that ran out clears the context's counts of parts; rows dealt out over many CTAs are the same before and after."""
+    import torch
+
+    import recipe_dev_b200 as rq
+
+    ctx = rq.Context(0)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = rq.KvCache(*((torch.randn((300, 2, 64, 128), generator=gen, device="cuda").half()) for _ in range(2)))
+    q = torch.randn((fresh, 8, 128), generator=gen, device="cuda")
+
+    def call():
+        return ctx.attention(q, cache, torch.arange(300, **i32)[None], torch.tensor([0, fresh], **i32), torch.tensor([19_000], **i32), max_fresh=fresh)
+
+    want = call()
+    ctx.check()
+    ctx.set_wait_limit(2_000_000)
+    ctx.wait_selftest()
+    with pytest.raises(rq.RqError, match="self-test"):
+        ctx.check()
+    ctx.set_wait_limit(2_000_000_000)
+    for _ in range(3):
+        assert torch.equal(call(), want)
+    ctx.check()
+    ctx.close()
