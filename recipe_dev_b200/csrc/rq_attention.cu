@@ -10,7 +10,10 @@
 //   * fp32 activations: queries and weights are taken apart into 16-bit parts, hi + lo over f16 (22 bits), hi + mid + lo over
 //     bf16 (24 bits). The sixteen rows of an operand are eight rows' hi parts above their lo parts: one mma.sync does both.
 //   * The tensor core adds by truncation, a bias that grows with the length of a chain: a sum stays in it for one tile and is then added, with
-//     round-to-nearest, to the row's fp32 sums, which are scaled by 2^(old max - new max) in the same multiply-add.
+//     round-to-nearest, to the row's fp32 sums, which are scaled by 2^(old base - new base) in the same multiply-add. A row's base is what its weights are made
+//     against, its maximum less 12 as rounded: kept itself, the factor is exactly one where the base stays. (Of the maximum, and the 12 added and taken off
+//     again, it was one rounding off on every tile, the same one: 64 requests of 32768 keys, flat heads of 128 elements, 4.2e-5 of a
+//     head's outputs in place of 5e-7.)
 //   * The keys of all requests and heads, in units of 64, are dealt out evenly: every CTA takes an equal range of units, wherever it begins and ends.
 //     Rows whose units fall to several CTAs are joined, in CTA order, by whichever of these is the last to leave its sums: the same bits on every run.
 // One token over 131071 keys, 32 + 2 x 8 heads of 128, f16: 96.7 us, 0.85 of the measured copy's bandwidth; 64 requests of up to 8191 keys, bf16: 190 us, 0.87.
@@ -104,7 +107,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
     extern __shared__ __align__(128) unsigned char dynamic[];
     Tiles<D, TYPE, RT>& sh = *(Tiles<D, TYPE, RT>*)dynamic;
     int64_t* before = (int64_t*)(dynamic + sizeof(sh));  // units before each request
-    __shared__ float warp_max[kWarps][ROWS], warp_sum[kWarps][ROWS];
+    __shared__ float warp_base[kWarps][ROWS], warp_sum[kWarps][ROWS];
     __shared__ int64_t sums[kWarps];
     __shared__ uint32_t last_arrival;
     launch_dependents();
@@ -227,11 +230,11 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
         }
         __syncthreads();
 
-        float m[RT], sum[RT];
+        float base[RT], sum[RT];  // base: -inf while the row has seen no key
         float2 acc[RT][D / 8][2];  // sums of the hi parts, and of the parts below them
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            m[rt] = -INFINITY;
+            base[rt] = -INFINITY;
             sum[rt] = 0.0f;
 #pragma unroll
             for (int n = 0; n < D / 8; ++n) acc[rt][n][0] = acc[rt][n][1] = make_float2(0.0f, 0.0f);
@@ -278,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
             float old[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                float top = m[rt];
+                float top = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -289,13 +292,14 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float base = (top == -INFINITY ? 0.0f : top) - kRaise;
-                old[rt] = exp2_fast(m[rt] - (base + kRaise));
-                m[rt] = top;
+                top = fmaxf(base[rt], top - kRaise);
+                const float from = top == -INFINITY ? 0.0f : top;
+                old[rt] = exp2_fast(base[rt] - from);
+                base[rt] = top;
                 float add = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float a = exp2_fast(s[rt][i][0] - base), b = exp2_fast(s[rt][i][1] - base);
+                    float a = exp2_fast(s[rt][i][0] - from), b = exp2_fast(s[rt][i][1] - from);
                     add += a + b;
                     w_hi[rt][i] = take_pair<TYPE>(a, b);
                     w_mid[rt][i] = take_pair<TYPE>(a, b);
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
         for (int rt = 0; rt < RT; ++rt) {
             sum[rt] += __shfl_xor_sync(0xffffffffu, sum[rt], 1);
             sum[rt] += __shfl_xor_sync(0xffffffffu, sum[rt], 2);
-            if (t4 == 0) { warp_max[warp][rt * 8 + g] = m[rt]; warp_sum[warp][rt * 8 + g] = sum[rt]; }
+            if (t4 == 0) { warp_base[warp][rt * 8 + g] = base[rt]; warp_sum[warp][rt * 8 + g] = sum[rt]; }
 #pragma unroll
             for (int n = 0; n < D / 8; ++n) *(float2*)&sh.out[warp][rt * 8 + g][8 * n + 2 * t4] = make_float2(acc[rt][n][0].x + acc[rt][n][1].x, acc[rt][n][0].y + acc[rt][n][1].y);
         }
@@ -389,15 +393,15 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
         for (int i = tid; i < ROWS * (D / 4); i += kThreads) {
             const int row = i / (D / 4), e = 4 * (i % (D / 4));
             if (row >= rows) break;
-            float top = warp_max[0][row];
+            float top = warp_base[0][row];
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, warp_max[w][row]);
-            const float base = top == -INFINITY ? 0.0f : top;
+            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, warp_base[w][row]);
+            const float to = top == -INFINITY ? 0.0f : top;
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float weight = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float f = exp2_fast(warp_max[w][row] - base);
+                const float f = exp2_fast(warp_base[w][row] - to);
                 const float4 o = *(const float4*)&sh.out[w][row][e];
                 v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
                 weight = fmaf(warp_sum[w][row], f, weight);
@@ -424,11 +428,11 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
                     float weight = 0.0f, top = -INFINITY;
 #pragma unroll 8
                     for (int64_t c = first_cta; c <= last_cta; ++c) top = fmaxf(top, __ldcg(p.partial + (c * 2 + (c == first_cta)) * stride + ROWS * D + row));
-                    const float base = top == -INFINITY ? 0.0f : top;
+                    const float to = top == -INFINITY ? 0.0f : top;
 #pragma unroll 8
                     for (int64_t c = first_cta; c <= last_cta; ++c) {
                         const float* from = p.partial + (c * 2 + (c == first_cta)) * stride;
-                        const float f = exp2_fast(__ldcg(from + ROWS * D + row) - base);
+                        const float f = exp2_fast(__ldcg(from + ROWS * D + row) - to);
                         const float4 o = __ldcg((const float4*)(from + row * D + e));
                         v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
                         weight = fmaf(__ldcg(from + ROWS * D + ROWS + row), f, weight);

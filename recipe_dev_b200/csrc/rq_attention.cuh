@@ -22,7 +22,7 @@ struct AttentionParams {
 };
 
 // What the work area holds: sums of rows for each CTA's first and last item (the tensor-core kernel: two tiles of 128 rows of 128 elements and their
-// maxima and sums of weights), then the counts.
+// bases and sums of weights), then the counts.
 constexpr int kTensorCtas = 148, kRowCtas = 148 * 4;
 constexpr size_t kTensorPartial = (size_t)kTensorCtas * 2 * 2 * 128 * (128 + 2), kRowPartial = (size_t)kRowCtas * 2 * 16 * (256 + 2);  // floats
 constexpr size_t kCounts = kTensorCtas * 2 * 4 > kRowCtas ? kTensorCtas * 2 * 4 : kRowCtas;

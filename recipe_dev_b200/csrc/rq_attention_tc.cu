@@ -6,8 +6,9 @@
 //   rows form (f16): the pipes are two tiles of 128 rows, which share every tile of 128 keys;
 //   keys form (few rows; bf16, whose third parts leave no room for a second row tile): one row tile, the pipes take alternate tiles of keys and
 //     are joined at the end, through tensor memory.
-// Per tile of keys: S = Q K^T (tcgen05.mma, Q and K in shared memory), weights P = 2^(S - max) from and to tensor memory, T = P V (P in tensor memory,
-// V in shared memory as it lies in the cache, keys times elements), sums O = O 2^(old max - max) + T in fp32 registers.
+// Per tile of keys: S = Q K^T (tcgen05.mma, Q and K in shared memory), weights P = 2^(S - base) from and to tensor memory, T = P V (P in tensor memory,
+// V in shared memory as it lies in the cache, keys times elements), sums O = O 2^(old base - base) + T in fp32 registers, base = max - 12 as rounded
+// (kept itself, so that the factor is exactly one where the base stays).
 //   * fp32 activations: Q and P are taken apart into 16-bit parts (hi + lo over f16, 22 bits; hi + mid + lo over bf16), each part a
 //     product of its own into the same accumulator, the smallest first. Products double (treble) against 16-bit activations; with one part the
 //     results would be off by 2^-11 (2^-8) where the framework's fp32 activations are good for 1e-6.
@@ -145,7 +146,7 @@ template <typename F> struct Shared {
     uint32_t pages_there[kWords];  // a tile's pages that the cache has, a bit each; all ones: all of them
     uint32_t odd[kWords];          // whether something was taken out of a tile's values
     uint32_t tmem_slot;
-    float joint[2][F::KEYS ? 128 : 1];  // keys form: the second pipe's maximum and sum of each row
+    float joint[2][F::KEYS ? 128 : 1];  // keys form: the second pipe's base and sum of each row
 };
 
 __device__ __forceinline__ bool finite16(uint32_t v, int type) { const uint32_t e = type == RQ_KV_F16 ? 0x7c00u : 0x7f80u; return (v & e) != e; }
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                 high = in_block < it->rows ? min(position + 1, it->end) : 0;
                 low = p.window > 0 ? max(position - p.window + 1, 0) : 0;
             }
-            float m = -INFINITY, sum = 0.0f, old = 1.0f;
+            float base = -INFINITY, sum = 0.0f, old = 1.0f;  // base: -inf while the row has seen no key
 #pragma unroll
             for (int i = 0; i < D; ++i) o[i] = 0.0f;
             // The values of a tile that are not finite, to the sums of the rows that see them
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                 // The loops over columns are loops: laid out in a line, with the masks, they were longer than the instruction caches are.
                 auto tile = [&](auto masked) {
                     constexpr bool kMasked = decltype(masked)::value;
-                    float top = m, top2 = -INFINITY;
+                    float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll 1
                     for (int c = 0; c < KT / 32; ++c) {
                         uint32_t s[32];
@@ -408,11 +409,11 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                             top2 = fmaxf(fmaxf(top2, __uint_as_float(s[i + 2])), __uint_as_float(s[i + 3]));
                         }
                     }
-                    top = fmaxf(top, top2);
-                    const float base = (top == -INFINITY ? 0.0f : top) - kRaise;
-                    f = exp2_fast(m - (base + kRaise));
-                    m = top;
-                    const Pair down = pair_of(-base, -base), minus = pair_of(-1.0f, -1.0f);
+                    top = fmaxf(base, fmaxf(top, top2) - kRaise);
+                    const float from = top == -INFINITY ? 0.0f : top;
+                    f = exp2_fast(base - from);
+                    base = top;
+                    const Pair down = pair_of(-from, -from), minus = pair_of(-1.0f, -1.0f);
                     Pair add[2] = {pair_of(0.0f, 0.0f), pair_of(0.0f, 0.0f)};
 #pragma unroll 1
                     for (int c = 0; c < KT / 32; ++c) {
@@ -475,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                         tmem_st16(sums_at + 16 * c, t);
                     }
                     tmem_st_wait();
-                    sh.joint[0][row] = m;
+                    sh.joint[0][row] = base;
                     sh.joint[1][row] = sum;
                     fence_before();
                     __syncwarp();
@@ -483,10 +484,10 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                 } else {
                     if (!mbar_wait_warp(&sh.joined[quarter], items_done & 1, p.wait_ns, dead)) atomicExch(p.error_flag, 52);
                     fence_after();
-                    const float other = sh.joint[0][row], top = fmaxf(m, other), base = top == -INFINITY ? 0.0f : top;
-                    const float fa = exp2_fast(m - base), fb = exp2_fast(other - base);
+                    const float other = sh.joint[0][row], top = fmaxf(base, other), to = top == -INFINITY ? 0.0f : top;
+                    const float fa = exp2_fast(base - to), fb = exp2_fast(other - to);
                     sum = sum * fa + sh.joint[1][row] * fb;
-                    m = top;
+                    base = top;
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
                         uint32_t t[32];
@@ -518,14 +519,14 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                 if (first_cta == last_cta) {
                     put();
                 } else {
-                    // [CTA][first or last of its items][pipe]: sums four elements a row, maxima, sums of weights
+                    // [CTA][first or last of its items][pipe]: sums four elements a row, bases, sums of weights
                     constexpr int64_t PART = 128 * (D + 2);
                     auto part = [&](int cta) { return p.partial + (((int64_t)cta * 2 + (cta == first_cta)) * 2 + pipe) * PART; };
                     const int mine = row * 4;
                     float* to = part((int)blockIdx.x);
 #pragma unroll
                     for (int i = 0; i < D; i += 4) __stcg((float4*)(to + mine + i * 128), make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
-                    __stcg(to + 128 * D + row, m);
+                    __stcg(to + 128 * D + row, base);
                     __stcg(to + 128 * (D + 1) + row, sum);
                     // (a warp's rows are joined by themselves: it waits for no other warp of its CTA)
                     uint32_t* const count = p.arrived + (first_cta * 2 + pipe) * 4 + quarter;
@@ -536,15 +537,15 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     if (__shfl_sync(0xffffffffu, before, 0) == (uint32_t)(last_cta - first_cta)) {
                         if (lane == 0) *count = 0;
                         __threadfence();
-                        m = -INFINITY;
-                        for (int c = first_cta; c <= last_cta; ++c) m = fmaxf(m, __ldcg(part(c) + 128 * D + row));
-                        const float base = m == -INFINITY ? 0.0f : m;
+                        base = -INFINITY;
+                        for (int c = first_cta; c <= last_cta; ++c) base = fmaxf(base, __ldcg(part(c) + 128 * D + row));
+                        const float at_all = base == -INFINITY ? 0.0f : base;
                         sum = 0.0f;
 #pragma unroll
                         for (int i = 0; i < D; ++i) o[i] = 0.0f;
                         for (int c = first_cta; c <= last_cta; ++c) {
                             const float* from = part(c);
-                            const float f = exp2_fast(__ldcg(from + 128 * D + row) - base);
+                            const float f = exp2_fast(__ldcg(from + 128 * D + row) - at_all);
                             sum = fmaf(__ldcg(from + 128 * (D + 1) + row), f, sum);
 #pragma unroll
                             for (int i = 0; i < D; i += 4) {
