@@ -351,10 +351,11 @@ int rq_rope_store(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, 
  *   y[t][h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q[t][h] . k_j - max),  k_j, v_j of head h / (q_heads / heads).
  * A row that sees no key gets zeros; keys that are masked, lie past lengths[r] or on a page outside the cache count for nothing,
  * whatever they hold. Tokens from starts[requests] on are not written; tokens of the batch from `tokens` on are passed over. q and y: heads head_dim apart, tokens *_t_stride apart, any
- * alignment. max_fresh is the most new tokens that a request has, as far as the host knows: the choice of kernel rests on it,
- * the results do not.
+ * alignment. max_fresh is the most new tokens that a request has, as far as the host knows: the choice of kernel, and with
+ * it the last bits, rests on it; every kernel serves every batch.
  * Activations stay fp32: queries and weights meet the 16-bit keys and values as two (f16) or three (bf16) 16-bit parts, products
- * are added in 32 bits. Queries times scale of magnitude above 65504 are not served over an f16 cache (inf / NaN). The same bits on every run.
+ * are added in 32 bits. Queries and keys may be of any size as long as scale times their products stays within fp32; a row of queries that is not finite, or that sees
+ * keys or values that are not, gets outputs that are not. The same bits on every run of the same call.
  * The context keeps a work area for rows whose keys are dealt out over several CTAs; the first call, or rq_attention_reserve ahead of a recording, allocates it. */
 int rq_attention_reserve(rq_ctx* ctx);
 int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, const rq_kv_cache* cache, const int32_t* block_table, int64_t table_stride,

@@ -185,6 +185,7 @@ static const char* wait_code_text(int code) {
         case 50: return "attention, loading warp: an item's place never came free";
         case 51: return "attention, mending warp: a tile of values never arrived";
         case 52: return "attention, softmax warps: the other pipe's sums never came";
+        case 53: return "attention, softmax warps: a row's factor never came";
         default: return "unknown wait";
     }
 }

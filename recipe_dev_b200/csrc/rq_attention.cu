@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
     Tiles<D, TYPE, RT>& sh = *(Tiles<D, TYPE, RT>*)dynamic;
     int64_t* before = (int64_t*)(dynamic + sizeof(sh));  // units before each request
     __shared__ float warp_base[kWarps][ROWS], warp_sum[kWarps][ROWS];
+    __shared__ uint32_t row_largest[kWarps][ROWS];
     __shared__ int64_t sums[kWarps];
     __shared__ uint32_t last_arrival;
     launch_dependents();
@@ -206,27 +207,66 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
         ahead += kUnit;
         page = page_of(ahead);
 
-        // queries: scaled, taken apart, as the tensor core's operand registers
-        for (int i = tid; i < RT * STEPS * 32; i += kThreads) {
-            const int l = i & 31, step = (i >> 5) % STEPS, rt = i / (32 * STEPS), row = rt * 8 + (l >> 2);
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // elements 16 step + 2 (l % 4) + {0, 1, 8, 9}
-            if (row < rows) {
-                const int at = row0 + row;
-                const float* from = p.q + (int64_t)(p.starts[r] + at / group) * p.q_stride + (int64_t)(kv * group + at % group) * D + 16 * step + 2 * (l & 3);
-                if (p.wide) {
-                    const float2 v = __ldcg((const float2*)from), w = __ldcg((const float2*)(from + 8));
-                    x[0] = v.x; x[1] = v.y; x[2] = w.x; x[3] = w.y;
-                } else { x[0] = __ldcg(from); x[1] = __ldcg(from + 1); x[2] = __ldcg(from + 8); x[3] = __ldcg(from + 9); }
+        // queries: brought to one size (f16) and taken apart, as the tensor core's operand registers; a warp has every fourth step of all rows
+        float factor[RT];  // of the scores of row g
+        {
+            constexpr int MINE = RT * STEPS / kWarps;
+            float x[MINE][4];  // elements 16 step + 2 t4 + {0, 1, 8, 9}
+            uint32_t largest[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) largest[rt] = 0;
+#pragma unroll
+            for (int n = 0; n < MINE; ++n) {
+                const int rt = n * kWarps / STEPS, step = n * kWarps % STEPS + warp, row = rt * 8 + g;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[n][e] = 0.0f;
+                if (row < rows) {
+                    const int at = row0 + row;
+                    const float* from = p.q + (int64_t)(p.starts[r] + at / group) * p.q_stride + (int64_t)(kv * group + at % group) * D + 16 * step + 2 * t4;
+                    if (p.wide) {
+                        const float2 v = __ldcg((const float2*)from), w = __ldcg((const float2*)(from + 8));
+                        x[n][0] = v.x; x[n][1] = v.y; x[n][2] = w.x; x[n][3] = w.y;
+                    } else { x[n][0] = __ldcg(from); x[n][1] = __ldcg(from + 1); x[n][2] = __ldcg(from + 8); x[n][3] = __ldcg(from + 9); }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) largest[rt] = max(largest[rt], __float_as_uint(x[n][e]) & 0x7fffffffu);
+            }
+            if (PARTS == 2) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    largest[rt] = max(largest[rt], __shfl_xor_sync(0xffffffffu, largest[rt], 1));
+                    largest[rt] = max(largest[rt], __shfl_xor_sync(0xffffffffu, largest[rt], 2));
+                    if (t4 == 0) row_largest[warp][rt * 8 + g] = largest[rt];
+                }
+                __syncthreads();
+            }
+            float raised[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                raised[rt] = 1.0f;
+                factor[rt] = factor_of(p.scale, 0);
+                if (PARTS == 2) {
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) largest[rt] = max(largest[rt], row_largest[w][rt * 8 + g]);
+                    const int raise = raise_of(largest[rt]);
+                    raised[rt] = power_of_two(raise);
+                    factor[rt] = factor_of(p.scale, raise);
+                }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] *= p.scale * kLog2e;
-            uint4 a;
-            a.x = take_pair<TYPE>(x[0], x[1]);
-            a.z = take_pair<TYPE>(x[2], x[3]);
-            a.y = take_pair<TYPE>(x[0], x[1]);
-            a.w = take_pair<TYPE>(x[2], x[3]);
-            sh.q_hi[rt][step][l] = a;
-            if (PARTS == 3) sh.q_lo[PARTS == 3 ? rt : 0][step][l] = make_uint2(pair_of<TYPE>(x[0], x[1]), pair_of<TYPE>(x[2], x[3]));
+            for (int n = 0; n < MINE; ++n) {
+                const int rt = n * kWarps / STEPS, step = n * kWarps % STEPS + warp;
+                if (PARTS == 2)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][e] *= raised[rt];
+                uint4 a;
+                a.x = take_pair<TYPE>(x[n][0], x[n][1]);
+                a.z = take_pair<TYPE>(x[n][2], x[n][3]);
+                a.y = take_pair<TYPE>(x[n][0], x[n][1]);
+                a.w = take_pair<TYPE>(x[n][2], x[n][3]);
+                sh.q_hi[rt][step][lane] = a;
+                if (PARTS == 3) sh.q_lo[PARTS == 3 ? rt : 0][step][lane] = make_uint2(pair_of<TYPE>(x[n][0], x[n][1]), pair_of<TYPE>(x[n][2], x[n][3]));
+            }
         }
         __syncthreads();
 
@@ -292,14 +332,14 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                top = fmaxf(base[rt], top - kRaise);
+                top = fmaxf(base[rt], fmaf(top, factor[rt], -kRaise));
                 const float from = top == -INFINITY ? 0.0f : top;
                 old[rt] = exp2_fast(base[rt] - from);
                 base[rt] = top;
                 float add = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float a = exp2_fast(s[rt][i][0] - from), b = exp2_fast(s[rt][i][1] - from);
+                    float a = exp2_fast(fmaf(s[rt][i][0], factor[rt], -from)), b = exp2_fast(fmaf(s[rt][i][1], factor[rt], -from));
                     add += a + b;
                     w_hi[rt][i] = take_pair<TYPE>(a, b);
                     w_mid[rt][i] = take_pair<TYPE>(a, b);

@@ -55,6 +55,15 @@ template <int TYPE> __device__ __forceinline__ uint32_t take_pair(float& a, floa
     b -= rqserve::to_float<TYPE>((uint16_t)(w >> 16));
     return w;
 }
+
+// Queries over an f16 cache: a row is multiplied by a power of two that brings its largest element to 2 or more (at best to 2^14 .. 2^15), so that its parts keep their 22
+// bits whatever the row's size (an f16 number below 2^-14 loses bits, one above 65504 is none), and the scores' factor makes up for it. `largest`: the bits
+// of that element without its sign; rows of zeros and below 2^-112 stay below, those that are not finite are none afterwards either.
+__device__ __forceinline__ int raise_of(uint32_t largest) { return min(141 - (int)(largest >> 23), 126); }  // from -114
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+constexpr int kUsualRaise = 7;  // right for rows whose largest element is 2^-6 .. 2^9
+// What scores are multiplied by to be exponents of two: positive and finite, so that masked scores stay -inf and scores of zero stay zero
+__device__ __forceinline__ float factor_of(float scale, int raise) { return fminf(fmaxf(scale * power_of_two(-raise) * kLog2e, 1.2e-38f), 3e38f); }
 #endif
 
 }  // namespace rqattn
