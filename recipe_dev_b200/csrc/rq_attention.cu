@@ -11,7 +11,7 @@
 //     bf16 (24 bits). The sixteen rows of an operand are eight rows' hi parts above their lo parts: one mma.sync does both.
 //   * The tensor core adds by truncation, a bias that grows with the length of a chain: a sum stays in it for one tile and is then added, with
 //     round-to-nearest, to the row's fp32 sums, which are scaled by 2^(old base - new base) in the same multiply-add. A row's base is what its weights are made
-//     against, its maximum less 12 as rounded: kept itself, the factor is exactly one where the base stays. (Of the maximum, and the 12 added and taken off
+//     against, its maximum less 12 (bf16: 0) as rounded: kept itself, the factor is exactly one where the base stays. (Of the maximum, and the 12 added and taken off
 //     again, it was one rounding off on every tile, the same one: 64 requests of 32768 keys, flat heads of 128 elements, 4.2e-5 of a
 //     head's outputs in place of 5e-7.)
 //   * The keys of all requests and heads, in units of 64, are dealt out evenly: every CTA takes an equal range of units, wherever it begins and ends.
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                top = fmaxf(base[rt], fmaf(top, factor[rt], -kRaise));
+                top = fmaxf(base[rt], fmaf(top, factor[rt], -kRaise<TYPE>));
                 const float from = top == -INFINITY ? 0.0f : top;
                 old[rt] = exp2_fast(base[rt] - from);
                 base[rt] = top;

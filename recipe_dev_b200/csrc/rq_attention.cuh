@@ -33,8 +33,9 @@ constexpr size_t kPartialBytes = sizeof(float) * (kTensorPartial > kRowPartial ?
 int launch_tensor(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool one_tile, cudaStream_t s);
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights are 2^(s - max + kRaise): an f16 part below 2^-14 loses bits, raised by 2^12 that is a weight of 2^-26 of the row's largest
-constexpr float kRaise = 12.0f;
+// Weights are 2^(s - max + kRaise): an f16 part below 2^-14 loses bits, raised by 2^12 that is a weight of 2^-26 of the row's largest. bf16 has fp32's exponents: its
+// parts need none of it, and values near the end of its range leave sums no room for it.
+template <int TYPE> constexpr float kRaise = TYPE == RQ_KV_F16 ? 12.0f : 0.0f;
 
 #ifdef __CUDACC__
 // How many of a request's new tokens the call has queries for: a batch may be longer than the call

@@ -7,7 +7,7 @@
 //   keys form (few rows; bf16, whose third parts leave no room for a second row tile): one row tile, the pipes take alternate tiles of keys and
 //     are joined at the end, through tensor memory.
 // Per tile of keys: S = Q K^T (tcgen05.mma, Q and K in shared memory), weights P = 2^(S - base) from and to tensor memory, T = P V (P in tensor memory,
-// V in shared memory as it lies in the cache, keys times elements), sums O = O 2^(old base - base) + T in fp32 registers, base = max - 12 as rounded
+// V in shared memory as it lies in the cache, keys times elements), sums O = O 2^(old base - base) + T in fp32 registers, base = max - 12 (bf16: 0) as rounded
 // (kept itself, so that the factor is exactly one where the base stays).
 //   * fp32 activations: Q and P are taken apart into 16-bit parts (hi + lo over f16, 22 bits; hi + mid + lo over bf16), each part a
 //     product of its own into the same accumulator, the smallest first. Products double (treble) against 16-bit activations; with one part the
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                             top2 = fmaxf(fmaxf(top2, __uint_as_float(s[i + 2])), __uint_as_float(s[i + 3]));
                         }
                     }
-                    top = fmaxf(base, fmaf(fmaxf(top, top2), factor, -kRaise));
+                    top = fmaxf(base, fmaf(fmaxf(top, top2), factor, -kRaise<TYPE>));
                     const float from = top == -INFINITY ? 0.0f : top;
                     f = exp2_fast(base - from);
                     base = top;
