@@ -178,7 +178,14 @@ def _stream(stream) -> int:
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-_I32 = _F32 = None  # torch's types, once a context exists (an import statement in a short call costs as much as its checks)
+_I32 = _F32 = _current_stream = None  # torch's, once a serving call needs them (an import statement in a short call costs as much as its checks)
+
+
+def _with_torch() -> None:
+    global _I32, _F32, _current_stream
+    import torch
+
+    _I32, _F32, _current_stream = torch.int32, torch.float32, torch._C._cuda_getCurrentRawStream
 
 
 def _int32(a, size, who: str) -> int:
@@ -305,20 +312,15 @@ class Context:
     """One device context (rq_ctx)."""
 
     def __init__(self, device: int = 0):
-        global _I32, _F32
-        import torch
-
-        _I32, _F32 = torch.int32, torch.float32
         self.lib = load_library()
         handle = C.c_void_p()
         _check(self.lib.rq_init(device, C.byref(handle)))
         self.handle = handle.value
         self.device = device
-        self._current_stream = torch._C._cuda_getCurrentRawStream
 
     def _on(self, stream) -> int:
         """The stream's handle; the device's current stream for None."""
-        return self._current_stream(self.device) if stream is None else _stream(stream)
+        return _current_stream(self.device) if stream is None else _stream(stream)
 
     def close(self) -> None:
         if getattr(self, "handle", 0):
@@ -603,6 +605,8 @@ class Context:
         """cached, fresh: CUDA int32 [requests]; table: int32 [requests, width] page table, extended in place from free_pages (int32).
         Returns starts [requests + 1], lengths, slots, positions, owners (of the slots given, or max_tokens) and status (tokens,
         pages taken, pages lacking)."""
+        if _F32 is None:
+            _with_torch()
         n = cached.shape[0]
         if starts is None or lengths is None or slots is None or positions is None or owners is None or status is None:
             import torch
@@ -638,6 +642,8 @@ class Context:
         """q [tokens, q_heads * head_dim] (or [tokens, q_heads, head_dim]), k and v likewise with the cache's heads: fp32, heads
         contiguous, any token stride. Norms (where gains are given) and rotates queries into q_out and keys into the cache, with
         the values, at slots. table: rope_table's, or None."""
+        if _F32 is None:
+            _with_torch()
         tokens = q.shape[0]
         if q_out is None:
             import torch
@@ -674,6 +680,8 @@ class Context:
         """Causal attention of the batch's new tokens (q [tokens, q_heads, head_dim] or [tokens, q_heads * head_dim], fp32) over the paged
         cache: request r's tokens are starts[r] .. starts[r + 1] at the end of its lengths[r] positions. max_fresh: the most new tokens
         of a request as far as the host knows (0: that is not known). Returns y, of q's shape."""
+        if _F32 is None:
+            _with_torch()
         tokens, n, d = q.shape[0], lengths.shape[0], cache.head_dim
         if y is None:
             import torch
@@ -693,6 +701,8 @@ class Context:
     def sample(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, token=None, probability=None, kept=None, stream=None):
         """The next token of each row of logits (fp32 [rows, vocabulary]) from uniform [rows] in [0, 1); parameters are CUDA tensors [rows]
         (top_k int32, the others fp32) or None. Returns token (int32 [rows]); probability and kept are filled where given."""
+        if _F32 is None:
+            _with_torch()
         rows, vocabulary = logits.shape
         stride = logits.stride()
         if logits.dtype is not _F32 or not logits.is_cuda or stride[1] != 1:
