@@ -635,7 +635,11 @@ class Context:
 
         if out is None:
             out = torch.empty((rows, rotary), dtype=torch.float32, device=f"cuda:{self.device}")
-        _check(self.lib.rq_rope_table(self.handle, base, frequency_scale, rotary, rows, _ptr(out), _stream(stream)))
+        elif out.dtype is not torch.float32 or not out.is_cuda or out.shape != (rows, rotary) or not out.is_contiguous():
+            raise ValueError("rope_table: out must be contiguous CUDA fp32 [rows, rotary]")
+        if _F32 is None:
+            _with_torch()
+        _check(self.lib.rq_rope_table(self.handle, base, frequency_scale, rotary, rows, _ptr(out), self._on(stream)))
         return out
 
     def rope_store(self, q, k, v, positions, slots, table, cache: KvCache, q_gain=None, k_gain=None, epsilon: float = 1e-6, style: str = "halves", q_out=None, stream=None):
