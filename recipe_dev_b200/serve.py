@@ -41,7 +41,7 @@ class Decoder:
         self.layers = [dict(qkv=[weight(capi.Q4_K, n, hidden) for n in (q, kv, kv)], o=weight(capi.Q4_K, hidden, q), gate=weight(capi.Q4_K, ffn, hidden), up=weight(capi.Q4_K, ffn, hidden),
                             down=weight(capi.Q4_K, hidden, ffn), gains=[gain(hidden), gain(hidden), gain(head_dim), gain(head_dim)],
                             cache=capi.KvCache.empty(pages, kv_heads, page_size, head_dim, dtype, ctx.device)) for _ in range(layers)]
-        self.rotation = ctx.rope_table(positions, head_dim)
+        self.positions, self.rotation = positions, ctx.rope_table(positions, head_dim)
         ctx.reserve(max(vocabulary, ffn), max(hidden, ffn, q), RECORDED)
         ctx.attention_reserve()
 
@@ -93,11 +93,17 @@ class Decoder:
 
 
 class Batch:
-    """Requests that are served together: their lengths, pages and tokens."""
+    """Requests that are served together: their lengths, pages and tokens. The model's cache is theirs: one batch at a time."""
 
     def __init__(self, model: Decoder, prompts, new: int, chunk: int = 512, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, seed: int = 0, record: bool = True):
         import torch
 
+        if not prompts or not all(prompts) or new < 1 or chunk < 1:
+            raise ValueError("Batch: every request needs a prompt, a new token and chunks of at least one")
+        if max(len(p) for p in prompts) + new - 1 > model.positions:  # (the last token is not fed back)
+            raise ValueError(f"Batch: the longest request passes the model's {model.positions} positions")
+        if not all(0 <= t < model.vocabulary for p in prompts for t in p):
+            raise ValueError(f"Batch: a prompt's tokens are 0 .. {model.vocabulary - 1}")
         self.model, self.prompts, self.new, self.chunk, self.record = model, prompts, new, chunk, record
         n, ints = len(prompts), dict(dtype=torch.int32, device=model.device)
         pages = model.layers[0]["cache"].pages
