@@ -75,7 +75,7 @@ enum { RQ_SCORE_SOFTMAX = 0, RQ_SCORE_SIGMOID = 1 };
 int rq_init(int device, rq_ctx** out);
 void rq_destroy(rq_ctx* ctx);
 /* Synchronises the device and reports whether any kernel of this context gave up one of its
- * bounded waits since the last check (the device code never traps and never spins unbounded;
+ * bounded waits since the last check, and makes the context ready for the next call (the device code never traps and never spins unbounded;
  * the reference's hand PTX waits return a status the same way, barrier.ptx:1653-1748). */
 int rq_check(rq_ctx* ctx);
 /* How long a kernel of this context waits on a barrier (a copy that has not landed, a ring slot, a peer's
@@ -355,7 +355,7 @@ int rq_rope_store(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, 
  * it the last bits, rests on it; every kernel serves every batch.
  * Activations stay fp32: queries and weights meet the 16-bit keys and values as two (f16) or three (bf16) 16-bit parts, products
  * are added in 32 bits. Queries and keys may be of any size as long as scale times their products stays within fp32; a row of queries that is not finite, or that sees
- * keys or values that are not, gets outputs that are not. The same bits on every run of the same call.
+ * keys or values that are not, has no defined outputs (the other rows are as ever). The same bits on every run of the same call.
  * The context keeps a work area for rows whose keys are dealt out over several CTAs; the first call, or rq_attention_reserve ahead of a recording, allocates it. */
 int rq_attention_reserve(rq_ctx* ctx);
 int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, const rq_kv_cache* cache, const int32_t* block_table, int64_t table_stride,

@@ -7,8 +7,8 @@
 //   * a warp takes sixteen keys at a time through a ring of its own in shared memory, filled by 16-byte asynchronous copies a tile ahead: any
 //     page size, order and stride, and what no row sees arrives as zeros. Chunks of a line are permuted (chunk ^ line % 8) so that
 //     the matrix loads meet no bank twice. (Loads into registers instead, without shared memory, kept too little under way: 140 us for 131071 keys.)
-//   * fp32 activations: queries and weights are taken apart into 16-bit parts, hi + lo over f16 (22 bits), hi + mid + lo over
-//     bf16 (24 bits). The sixteen rows of an operand are eight rows' hi parts above their lo parts: one mma.sync does both.
+//   * fp32 activations: queries and weights are taken apart into 16-bit parts, hi + lo over f16 (22 bits, a row of queries brought to f16's range by a power of two
+//     first), hi + mid + lo over bf16 (24 bits). The sixteen rows of an operand are eight rows' hi parts above their lo parts: one mma.sync does both.
 //   * The tensor core adds by truncation, a bias that grows with the length of a chain: a sum stays in it for one tile and is then added, with
 //     round-to-nearest, to the row's fp32 sums, which are scaled by 2^(old base - new base) in the same multiply-add. A row's base is what its weights are made
 //     against, its maximum less 12 (bf16: 0) as rounded: kept itself, the factor is exactly one where the base stays. (Of the maximum, and the 12 added and taken off
@@ -16,7 +16,7 @@
 //     head's outputs in place of 5e-7.)
 //   * The keys of all requests and heads, in units of 64, are dealt out evenly: every CTA takes an equal range of units, wherever it begins and ends.
 //     Rows whose units fall to several CTAs are joined, in CTA order, by whichever of these is the last to leave its sums: the same bits on every run.
-// One token over 131071 keys, 32 + 2 x 8 heads of 128, f16: 96.7 us, 0.85 of the measured copy's bandwidth; 64 requests of up to 8191 keys, bf16: 190 us, 0.87.
+// One token over 131071 keys, 32 + 2 x 8 heads of 128, f16: 94.5 us, 0.87 of the measured copy's bandwidth; 64 requests of up to 8191 keys, bf16: 176 us, 0.93.
 #include "rq_attention.cuh"
 #include "rq_mma.cuh"
 
@@ -28,7 +28,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 16, kUnit = kWarps * kTile;  // keys a warp and a CTA take at a time
-constexpr int kRequestStep = 128;
+constexpr int kRequestStep = 128;  // requests' places in shared memory are taken by so many
 constexpr int kStages = 2;  // of a warp's ring: one tile under way while the other is used
 
 // c = (first ? 0 : c) + a b for sixteen rows, eight columns and sixteen products each
@@ -519,7 +519,7 @@ int launch_rows(rq_ctx* ctx, const AttentionParams& p, cudaStream_t s) {
 }
 
 // two: sixteen rows at a time. Not for 256 elements a head, whose sums of sixteen rows do not fit a thread's registers: 16 requests of eight tokens over 8192 keys, 8 + 2 x 4
-// heads, f16, 242 us by sixteen rows and 179 by eight; 509 tokens over 7680, 16 + 2 x 4 heads, 1486 and 1008.
+// heads, f16, 240 us by sixteen rows and 178 by eight; 509 tokens over 7680, 16 + 2 x 4 heads, 1460 and 998.
 template <int D>
 int launch_rows(rq_ctx* ctx, const AttentionParams& p, int type, bool two, cudaStream_t s) {
     constexpr int MOST = D < 256 ? 2 : 1;
@@ -577,11 +577,11 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
     p.error_flag = ctx->error_flag; p.wait_ns = ctx->wait_limit_ns;
     const int64_t rows = (int64_t)(max_fresh > 0 ? (max_fresh < tokens ? max_fresh : tokens) : tokens) * group;
     // The rows kernel reads a request's keys once for every sixteen rows (from L2, from the second time on), the tensor-core kernel makes scores of 128 whatever
-    // there is. 8192 cached keys, 32 + 2 x 8 heads of 128, f16, rows kernel | tensor cores: 16 requests of 16 rows 106 | 183 us, 32 rows 182 | 184, 48 rows 264 | 185,
-    // 128 rows 695 | 179; one request of 32 rows 36 | 44, 48 rows 41 | 45, 128 rows 62 | 45. bf16: 16 requests of 32 rows 277 | 317, 48 rows 404 | 319.
+    // there is. 8192 cached keys, 32 + 2 x 8 heads of 128, f16, rows kernel | tensor cores: 16 requests of 16 rows 102 | 217 us, 32 rows 180 | 219, 48 rows 259 | 219,
+    // 128 rows 656 | 209; one request of 32 rows 35 | 44, 48 rows 39 | 44, 128 rows 71 | 45. bf16: 16 requests of 32 rows 265 | 371, 48 rows 407 | 373.
     if (rows > 32) {
         // Where a request may be a decode step among prompts, the rows kernel takes those and the tensor-core kernel the rest: 63 decode steps over 4096 keys and
-        // a chunk of 512 are 269 us in two launches, 494 by the tensor cores alone, 556 by the rows kernel alone; 7 over 300 keys and a prompt of 100: 32, 41, 23.
+        // a chunk of 512 are 267 us in two launches, 509 by the tensor cores alone, 531 by the rows kernel alone; 7 over 300 keys and a prompt of 100: 33, 27, 22.
         const int few = requests > 1 && tokens < requests * (rows / group) ? (group <= 8 ? 8 : 32) : 0;
         p.few = group <= few ? few : 0;
         rc = launch_tensor(ctx, p, *cache, rows <= 128, s);

@@ -9,8 +9,8 @@
 // Per tile of keys: S = Q K^T (tcgen05.mma, Q and K in shared memory), weights P = 2^(S - base) from and to tensor memory, T = P V (P in tensor memory,
 // V in shared memory as it lies in the cache, keys times elements), sums O = O 2^(old base - base) + T in fp32 registers, base = max - 12 (bf16: 0) as rounded
 // (kept itself, so that the factor is exactly one where the base stays).
-//   * fp32 activations: Q and P are taken apart into 16-bit parts (hi + lo over f16, 22 bits; hi + mid + lo over bf16), each part a
-//     product of its own into the same accumulator, the smallest first. Products double (treble) against 16-bit activations; with one part the
+//   * fp32 activations: Q and P are taken apart into 16-bit parts (hi + lo over f16, 22 bits, Q brought to f16's range by a power of two a row; hi + mid + lo over
+//     bf16), each part a product of its own into the same accumulator, the smallest first. Products double (treble) against 16-bit activations; with one part the
 //     results would be off by 2^-11 (2^-8) where the framework's fp32 activations are good for 1e-6.
 //   * The tensor core adds by truncation: T is one tile's sum only, and O is added up with round-to-nearest.
 //   * P takes the place of its S in tensor memory, 32 keys' hi and lo parts over the 32 scores they came from.
@@ -21,13 +21,14 @@
 // rows whose keys fall to several CTAs are joined in CTA order by the last of these (the same bits on every run). Keys and values come by TMA, a
 // page (at most a tile) of 64 elements a copy, into a ring of stages; an entry of the page table that names no page becomes a coordinate outside, which reads zeros.
 //
-// A value that a row does not see may be infinite, and 0 * inf is no 0: where a tile is not seen by all rows, the loading warp takes what is not
+// A value that a row does not see may be infinite, and 0 * inf is no 0: where a tile is not seen by all rows, the mending warp takes what is not
 // finite out of it, and the softmax threads add it to the sums of the rows that do see it.
 //
-// Every wait is bounded; a wait that runs out records a code in the context's error word and the warp waits no more.
+// Every wait between the roles is bounded; a wait that runs out records a code in the context's error word, and the warp waits no more and hands nothing on, so that
+// the others' waits run out too and all meet at the end. The loading warp leaves when every copy has landed.
 //
-// 509 tokens over 7680 keys, 32 + 2 x 8 heads of 128, f16: 139 us, 66 GFLOP of them useful (0.29 of the measured peak, 0.58 with both parts), products under way
-// 56 % of the time; prompts of 1021 to 3001 tokens 383 us, 150 GFLOP.
+// 509 tokens over 7680 keys, 32 + 2 x 8 heads of 128, f16: 137 us, 66 GFLOP of them useful (0.29 of the measured peak, 0.59 with both parts), products under way
+// 56 % of the time; four prompts of 1021 to 3001 tokens 378 us, 150 GFLOP (both called among other cases; over the same two batches again and again 123 and 350).
 #include <type_traits>
 
 #include "rq_attention.cuh"
@@ -84,8 +85,9 @@ template <typename F> __device__ __forceinline__ Block block_of(const AttentionP
 }
 
 // Taking a block up (its queries, the first scores, the sums at the end: 21 us) costs as much as some units (3.9 us): so many lead each block's own in the dealing.
-// Without it the CTAs that got a prompt's first blocks, short ones, were the last to end. 32 + 2 x 8 heads of 128, f16, without | with: prompts of 1021 to 3001 tokens
-// 612 | 334 us, one of 12001 2781 | 1930, eight of 512 137 | 119; 32 of 128, all blocks of one unit, 67 | 74.
+// Without it the CTAs that got a prompt's first blocks, short ones, were the last to end. 32 + 2 x 8 heads of 128, f16, without | with, over the same batches again and
+// again: four prompts of 1021 to 3001 tokens 620 | 350 us, one of 12001 2816 | 1883, eight of 512 138 | 120, two of 3001 with windows of 1000 425 | 244, 509 tokens over 7680 125 |
+// 123; 32 of 128, all blocks of one unit, 67 | 68; 16 requests of 48 rows over 8192 keys 205 | 219.
 constexpr int kLead = 4;
 
 // One block's part of a CTA's range of units, as the roles need it; take = 0: there are no more
@@ -202,7 +204,7 @@ template <int D, int TYPE, bool KEYS> __device__ __noinline__ int rescale_querie
 // accesses on their way at a time. (A thread that reads a row of its own meets 32 lines an instruction.) Returns the factor of the scores of the lane's row.
 // Over f16 all rows are multiplied by the same power of two first, and the parts themselves say whether that was the right one for each: a row's largest element has
 // to be 2 or more, and finite, as an f16 number. Where it is not, the warp's rows are taken once more. (Every row by its own largest element at once made a block's
-// take-up 1.7 us longer: 32 prompts of 128 tokens 71 us in place of 65.)
+// take-up 1.7 us longer: 32 prompts of 128 tokens 71 us in place of 68. Queries a thousandth of the usual size: 88 us, and the four prompts 402 in place of 356.)
 template <int D, int TYPE, bool KEYS> __device__ __forceinline__ float load_queries(const AttentionParams& p, const Item& it, uint8_t* to, int block_row, int first, int group) {
     using F = Form<D, TYPE, KEYS>;
     constexpr int SHARE = 128 / D, ROWS = KEYS ? 16 : 32, BATCH = ROWS / SHARE < 8 ? ROWS / SHARE : 8;  // rows an access; rows a warp; accesses at a time
