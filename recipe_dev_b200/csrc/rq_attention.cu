@@ -16,7 +16,7 @@
 //     head's outputs in place of 5e-7.)
 //   * The keys of all requests and heads, in units of 64, are dealt out evenly: every CTA takes an equal range of units, wherever it begins and ends.
 //     Rows whose units fall to several CTAs are joined, in CTA order, by whichever of these is the last to leave its sums: the same bits on every run.
-// One token over 131071 keys, 32 + 2 x 8 heads of 128, f16: 94.5 us, 0.87 of the measured copy's bandwidth; 64 requests of up to 8191 keys, bf16: 176 us, 0.93.
+// One token over 131071 keys, 32 + 2 x 8 heads of 128, f16: 94.5 us, 0.87 of the measured copy's bandwidth (another GPU 96.5); 64 requests of up to 8191 keys, bf16: 176 us, 0.93 (184).
 #include "rq_attention.cuh"
 #include "rq_mma.cuh"
 
