@@ -185,6 +185,16 @@ int rq_rmsnorm(rq_ctx* ctx, const float* x, int64_t x_k_stride, int64_t x_t_stri
 int rq_add(rq_ctx* ctx, const float* a, const float* b, int64_t n, float* y, void* stream);
 int rq_softcap(rq_ctx* ctx, const float* x, int64_t n, double cap, float* y, void* stream);
 
+/* From one block of a layer to the next in one launch, `tokens` positions of n values each: the norm behind the block, its gate and scale, the residual sum, and
+ * the norm in front of the next block,
+ *   x' = x + residual_scale * gate * norm(delta; delta_gain),  y = norm(x'; gain),  norm(v; g) = v / sqrt(mean(v^2) + epsilon) * g.
+ * delta_gain null: delta as it is; gate null: one; gain null: the norm without a gain. A gate's value for element k of token t lies at gate[k * gate_k_stride +
+ * t * gate_t_stride], gate_k_stride 0 or 1, gate_t_stride not negative: a gate a channel, a token, or an element. Elements of a token are contiguous, tokens
+ * *_t_stride apart, any alignment. x_out may be x, and y may be delta; otherwise outputs overlap nothing. A token's result does not depend on the others of the call. */
+int rq_residual_norm(rq_ctx* ctx, const float* x, int64_t x_t_stride, const float* delta, int64_t delta_t_stride, int64_t n, int tokens, const float* delta_gain,
+                     const float* gate, int64_t gate_k_stride, int64_t gate_t_stride, float residual_scale, const float* gain, float epsilon, float* x_out,
+                     int64_t x_out_t_stride, float* y, int64_t y_t_stride, void* stream);
+
 /* The batched product (prefill, multi-sequence decode): the same contraction as rq_matvec for many
  * tokens, on the tensor cores (tcgen05.mma, fp32 accumulation in tensor memory) for Q4_K / Q6_K / Q8_0 /
  * Q4_0 weights: exact-integer weight operands, activations as fp16 hi + lo pairs, for RQ_ACT_FLOAT and for
@@ -300,18 +310,25 @@ int rq_moe_route_forward(rq_ctx* ctx, rq_moe* moe, const float* scores, int64_t 
  *
  * The cache: pages of page_size positions; element d of position `line` of page `page` of head h lies at
  * page * page_stride + h * head_stride + line * line_stride + d, in elements, in k and in v. Any order of pages, heads and lines
- * will do; a line's head_dim elements are contiguous, pointers are 16-byte aligned and strides multiples of eight.
+ * will do; a line's head_dim elements are contiguous, pointers are 16-byte aligned and strides multiples of eight (RQ_KV_INT8: of sixteen).
+ * RQ_KV_INT8: an element is an 8-bit code of -127 .. 127 and stands for code * scale; a position's head has a scale of its own, an fp32 number at
+ * page * scale_page_stride + head * scale_head_stride + line * scale_line_stride of k_scale and of v_scale. (One scale for several positions
+ * would have to be raised, and the codes that lie there rounded again, when a larger key joins them: what a cache holds would depend on how a prompt was cut.)
  * Row r of the page table (int32, table_stride apart, table_width entries) names the pages of request r's positions in order. */
-enum { RQ_KV_F16 = 0, RQ_KV_BF16 = 1 };
+enum { RQ_KV_F16 = 0, RQ_KV_BF16 = 1, RQ_KV_INT8 = 2 };
 typedef struct rq_kv_cache {
     void* k;
     void* v;
-    int32_t type;      /* RQ_KV_F16 or RQ_KV_BF16 */
+    int32_t type;      /* RQ_KV_F16, RQ_KV_BF16 or RQ_KV_INT8 */
     int32_t heads;     /* key / value heads */
     int32_t head_dim;  /* 64, 128 or 256 */
     int32_t page_size; /* positions a page: a power of two, at most 4096 */
     int64_t pages;     /* pages * page_size < 2^31 */
     int64_t page_stride, head_stride, line_stride; /* page and line strides below 2^31 */
+    /* RQ_KV_INT8 alone; not looked at for the other types */
+    float* k_scale;
+    float* v_scale;
+    int64_t scale_page_stride, scale_head_stride, scale_line_stride; /* not negative, page and line strides below 2^31; any alignment */
 } rq_kv_cache;
 
 /* The plan of a step, from the requests' lengths: gives the requests the pages they lack, in request order, from the front of
@@ -339,7 +356,8 @@ int rq_rope_table(rq_ctx* ctx, double base, double frequency_scale, int rotary, 
  * positions[t] of the table (a position outside it is clamped into it),
  *   (a, b) -> (a cos - b sin, a sin + b cos), pairs (a, b) = (x[i], x[i + rotary / 2]) for RQ_ROPE_HALVES, (x[2 i], x[2 i + 1]) for RQ_ROPE_PAIRS,
  * queries to q_out (which may be q), keys and, as they are, values to the cache at slots[t] (a slot outside it is passed over),
- * rounded to the cache's type once. Heads of a token lie head_dim apart; tokens *_t_stride apart, any alignment. rotary: a
+ * rounded to the cache's type once. RQ_KV_INT8: a head's scale is its largest magnitude over 127 (fp32), its codes are x / scale rounded to the nearest whole
+ * number, ties to even; a head of zeros (or one whose scale would be less than 2^-126) has scale 0 and codes 0, one with an infinity or a NaN has that as its scale. Heads of a token lie head_dim apart; tokens *_t_stride apart, any alignment. rotary: a
  * multiple of 16 up to head_dim, or 0 (no rotation, no table). */
 enum { RQ_ROPE_HALVES = 0, RQ_ROPE_PAIRS = 1 };
 int rq_rope_store(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, const float* k, int64_t k_t_stride, const float* v, int64_t v_t_stride, int tokens,
@@ -354,7 +372,7 @@ int rq_rope_store(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, 
  * alignment. max_fresh is the most new tokens that a request has, as far as the host knows: the choice of kernel, and with
  * it the last bits, rests on it; every kernel serves every batch.
  * Activations stay fp32: queries and weights meet the 16-bit keys and values as two (f16) or three (bf16) 16-bit parts, products
- * are added in 32 bits. Queries and keys may be of any size as long as scale times their products stays within fp32; a row of queries that is not finite, or that sees
+ * are added in 32 bits. (RQ_KV_INT8: codes are f16 numbers, scales are applied in fp32; values up to 2^90 in size.) Queries and keys may be of any size as long as scale times their products stays within fp32; a row of queries that is not finite, or that sees
  * keys or values that are not, has no defined outputs (the other rows are as ever). The same bits on every run of the same call.
  * The context keeps a work area for rows whose keys are dealt out over several CTAs; the first call, or rq_attention_reserve ahead of a recording, allocates it. */
 int rq_attention_reserve(rq_ctx* ctx);
@@ -375,6 +393,18 @@ int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, c
 #define RQ_MAX_VOCABULARY 1048576
 int rq_sample(rq_ctx* ctx, const float* logits, int64_t row_stride, int rows, int64_t vocabulary, const float* temperature, const int32_t* top_k, const float* top_p,
               const float* min_p, const float* uniform, int32_t* token, float* probability, int32_t* kept, void* stream);
+
+/* Log probabilities of `rows` rows of logits, x_i being a row's logits and log p_i = x_i - log(sum_j exp(x_j)):
+ *   logprob[r] = log p of the token token[r]; rank[r] = how many tokens have a larger logit, or an equal one and a lower index (0: the likeliest);
+ *   entropy[r] = -sum_i p_i log p_i;
+ *   top_token[r][n], top_logprob[r][n], n < top: the likeliest tokens in that order, with their log probabilities.
+ * token null: logprob and rank are not written; a null output is not wanted (top = 0: no alternatives). A token outside the vocabulary (a padding row's)
+ * gets logprob 0 and rank -1. NaN counts as -inf; tokens at -inf are no alternatives: where fewer than `top` are left the rest is -1 and -inf. A row without any value
+ * above -inf has logprob -inf, rank -1, entropy 0; one with +inf has no defined outputs. fp32 arithmetic, sums in a fixed order. At most RQ_MAX_VOCABULARY
+ * tokens and RQ_MAX_ALTERNATIVES alternatives. */
+#define RQ_MAX_ALTERNATIVES 64
+int rq_logprobs(rq_ctx* ctx, const float* logits, int64_t row_stride, int rows, int64_t vocabulary, const int32_t* token, float* logprob, float* entropy, int32_t* rank,
+                int top, int32_t* top_token, float* top_logprob, void* stream);
 
 /* ---- recorded sequences: one boundary crossing per step ------------------------------------------ */
 

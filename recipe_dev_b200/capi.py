@@ -16,7 +16,8 @@ Q4_1, Q5_0, Q5_1, Q5_K, IQ4_NL = 3, 6, 7, 13, 20  # bound, decoded, dotted with 
 Q8_1, Q2_K, Q3_K, Q8_K, IQ4_XS = 9, 10, 11, 15, 23  # the same
 ACT_FLOAT, ACT_INT8 = 0, 1
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
-KV_F16, KV_BF16 = 0, 1
+KV_F16, KV_BF16, KV_INT8 = 0, 1, 2
+MAX_ALTERNATIVES = 64  # of a row of log probabilities
 ROPE_STYLES = {"halves": 0, "pairs": 1}
 
 _PKG = Path(__file__).resolve().parent
@@ -95,6 +96,8 @@ def _declare(lib) -> None:
         "rq_attention_reserve": (i32, [p]),
         "rq_attention": (i32, [p, f32p, i64, i32, p, p, i64, i32, p, p, i32, i32, i32, C.c_float, i32, f32p, i64, p]),
         "rq_sample": (i32, [p, f32p, i64, i32, i64, f32p, p, f32p, f32p, f32p, p, f32p, p, p]),
+        "rq_logprobs": (i32, [p, f32p, i64, i32, i64, p, f32p, f32p, p, i32, p, f32p, p]),
+        "rq_residual_norm": (i32, [p, f32p, i64, f32p, i64, i64, i32, f32p, f32p, i64, i64, C.c_float, f32p, C.c_float, f32p, i64, f32p, i64, p]),
         "rq_sequence_begin": (i32, [p, C.POINTER(p)]),
         "rq_sequence_end": (i32, [p, C.POINTER(p)]),
         "rq_sequence_run": (i32, [p, p]),
@@ -248,24 +251,36 @@ class Weight:
 
 class _KvCacheStruct(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int64),
-                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("line_stride", C.c_int64)]
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("line_stride", C.c_int64), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("scale_page_stride", C.c_int64), ("scale_head_stride", C.c_int64), ("scale_line_stride", C.c_int64)]
 
 
 class KvCache:
-    """A paged cache of keys and values (rq_kv_cache) over two CUDA tensors [pages, heads, page_size, head_dim], float16 or
-    bfloat16, of the same strides (any order of pages, heads and lines; a line's elements are contiguous)."""
+    """A paged cache of keys and values (rq_kv_cache) over two CUDA tensors [pages, heads, page_size, head_dim], float16, bfloat16 or int8, of the same strides (any order of
+    pages, heads and lines; a line's elements are contiguous). int8: codes of -127 .. 127, with a scale for each position's head in two float32 tensors
+    [pages, heads, page_size] of the same strides; an element stands for code * scale."""
 
-    def __init__(self, k, v):
+    def __init__(self, k, v, k_scale=None, v_scale=None):
         import torch
 
+        kinds = {torch.float16: KV_F16, torch.bfloat16: KV_BF16, torch.int8: KV_INT8}
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
             raise ValueError("KvCache: k and v must be [pages, heads, page_size, head_dim] of one shape, type and layout")
-        if k.dtype not in (torch.float16, torch.bfloat16) or not k.is_cuda or not v.is_cuda or k.stride(3) != 1:
-            raise ValueError("KvCache: k and v must be CUDA float16 or bfloat16 tensors with contiguous lines")
-        self.k, self.v = k, v
+        if k.dtype not in kinds or not k.is_cuda or not v.is_cuda or k.stride(3) != 1:
+            raise ValueError("KvCache: k and v must be CUDA float16, bfloat16 or int8 tensors with contiguous lines")
+        scales = ()
+        if k.dtype == torch.int8:
+            if k_scale is None or v_scale is None:
+                raise ValueError("KvCache: an int8 cache needs k_scale and v_scale")
+            if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or not k_scale.is_cuda or not v_scale.is_cuda or k_scale.shape != k.shape[:3] or v_scale.shape != k.shape[:3] or k_scale.stride() != v_scale.stride():
+                raise ValueError("KvCache: k_scale and v_scale must be CUDA float32 tensors [pages, heads, page_size] of one layout")
+            scales = (k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride())
+        elif k_scale is not None or v_scale is not None:
+            raise ValueError("KvCache: only an int8 cache has scales")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page_size, self.head_dim = k.shape
         sp, sh, sl, _ = k.stride()
-        self._struct = _KvCacheStruct(k.data_ptr(), v.data_ptr(), KV_F16 if k.dtype == torch.float16 else KV_BF16, self.heads, self.head_dim, self.page_size, self.pages, sp, sh, sl)
+        self._struct = _KvCacheStruct(k.data_ptr(), v.data_ptr(), kinds[k.dtype], self.heads, self.head_dim, self.page_size, self.pages, sp, sh, sl, *scales)
         self._ref = C.addressof(self._struct)
 
     @classmethod
@@ -273,7 +288,9 @@ class KvCache:
         import torch
 
         k, v = (torch.empty((pages, heads, page_size, head_dim), dtype=dtype or torch.float16, device=f"cuda:{device}") for _ in range(2))
-        return cls(k, v)
+        if dtype is not torch.int8:
+            return cls(k, v)
+        return cls(k, v, *(torch.empty((pages, heads, page_size), dtype=torch.float32, device=f"cuda:{device}") for _ in range(2)))
 
 
 class MoeBank:
@@ -645,7 +662,7 @@ class Context:
     def rope_store(self, q, k, v, positions, slots, table, cache: KvCache, q_gain=None, k_gain=None, epsilon: float = 1e-6, style: str = "halves", q_out=None, stream=None):
         """q [tokens, q_heads * head_dim] (or [tokens, q_heads, head_dim]), k and v likewise with the cache's heads: fp32, heads
         contiguous, any token stride. Norms (where gains are given) and rotates queries into q_out and keys into the cache, with
-        the values, at slots. table: rope_table's, or None."""
+        the values, at slots (an int8 cache: as codes, with their heads' scales). table: rope_table's, or None."""
         if _F32 is None:
             _with_torch()
         tokens = q.shape[0]
@@ -727,6 +744,78 @@ class Context:
         if rc:
             _check(rc)
         return token
+
+    def logprobs(self, logits, token=None, logprob=None, entropy=None, rank=None, top_token=None, top_logprob=None, stream=None):
+        """Log probabilities of a token (int32 [rows]) of each row of logits (fp32 [rows, vocabulary]). Returns logprob (fp32 [rows]; None without token); where given, entropy
+        (fp32 [rows]), rank (int32 [rows]: how many tokens are likelier) and the likeliest tokens, top_token (int32 [rows, n]) with top_logprob (fp32 [rows, n]), n up to
+        MAX_ALTERNATIVES, are filled. A token outside the vocabulary has logprob 0 and rank -1."""
+        if _F32 is None:
+            _with_torch()
+        rows, vocabulary = logits.shape
+        stride = logits.stride()
+        if logits.dtype is not _F32 or logits.get_device() != self.device or stride[1] != 1:
+            raise ValueError("logprobs: logits must be CUDA fp32 [rows, vocabulary] with contiguous rows, on the context's device")
+        if token is None:
+            if logprob is not None or rank is not None:
+                raise ValueError("logprobs: logprob and rank are those of given tokens")
+        elif logprob is None:
+            import torch
+
+            logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        top, at = 0, []
+        for a, dtype in ((top_token, _I32), (top_logprob, _F32)):
+            if a is not None:
+                if a.dim() != 2 or a.shape[0] != rows or (top and a.shape[1] != top) or a.shape[1] == 0:
+                    raise ValueError("logprobs: top_token and top_logprob must be [rows, n] of one n")
+                top = a.shape[1]
+        for a, dtype, shape in ((token, _I32, (rows,)), (logprob, _F32, (rows,)), (entropy, _F32, (rows,)), (rank, _I32, (rows,)), (top_token, _I32, (rows, top)), (top_logprob, _F32, (rows, top))):
+            if a is None:
+                at.append(0)
+                continue
+            if a.dtype is not dtype or a.get_device() != self.device or a.shape != shape or not a.is_contiguous():
+                raise ValueError("logprobs: per-row arrays must be contiguous CUDA tensors on the context's device; token, rank and top_token int32, the others fp32")
+            at.append(a.data_ptr())
+        rc = self.lib.rq_logprobs(self.handle, logits.data_ptr(), stride[0], rows, vocabulary, *at[:4], top, *at[4:], self._on(stream))
+        if rc:
+            _check(rc)
+        return logprob
+
+    def residual_norm(self, x, delta, gain=None, delta_gain=None, gate=None, residual_scale: float = 1.0, epsilon: float = 1e-6, x_out=None, y=None, stream=None):
+        """From one block to the next: x_out = x + residual_scale * gate * norm(delta; delta_gain) (in place where x_out is None), returns y = norm(x_out; gain).
+        Planes are fp32 [tokens, n] with contiguous tokens; without delta_gain delta is taken as it is, without gain the norm has none; gate: [n], [tokens, 1] or [tokens, n]."""
+        if _F32 is None:
+            _with_torch()
+        if x_out is None:
+            x_out = x
+        if y is None:
+            import torch
+
+            y = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+        tokens, n = x.shape
+        planes = []
+        for a in (x, delta, x_out, y):
+            if a.dtype is not _F32 or a.get_device() != self.device or a.shape != x.shape or a.stride(1) != 1:
+                raise ValueError("residual_norm: x, delta, x_out and y must be CUDA fp32 planes [tokens, n] with contiguous tokens, on the context's device")
+            planes.append((a.data_ptr(), a.stride(0)))
+        gains = []
+        for g in (delta_gain, gain):
+            if g is not None and (g.dtype is not _F32 or g.get_device() != self.device or g.shape != (n,) or not g.is_contiguous()):
+                raise ValueError("residual_norm: a gain holds n contiguous fp32 values")
+            gains.append(0 if g is None else g.data_ptr())
+        at = by_element = by_token = 0
+        if gate is not None:
+            shape, stride = gate.shape, gate.stride()
+            if gate.dtype is not _F32 or gate.get_device() != self.device or shape not in ((n,), (tokens, 1), (tokens, n)):
+                raise ValueError("residual_norm: a gate is CUDA fp32 [n], [tokens, 1] or [tokens, n]")
+            at, by_element, by_token = gate.data_ptr(), int(shape[-1] == n and n > 1), stride[0] if len(shape) == 2 else 0
+            if by_element and stride[-1] != 1:
+                raise ValueError("residual_norm: a gate's values of a token must be contiguous")
+        (x_at, x_stride), (d_at, d_stride), (o_at, o_stride), (y_at, y_stride) = planes
+        rc = self.lib.rq_residual_norm(self.handle, x_at, x_stride, d_at, d_stride, n, tokens, gains[0], at, by_element, by_token, residual_scale, gains[1], epsilon, o_at, o_stride,
+                                       y_at, y_stride, self._on(stream))
+        if rc:
+            _check(rc)
+        return y
 
     def activation_records(self, x, step: int, stream=None):
         """The 36-byte int8 records of x ([cols] or [tokens, cols]) as a uint8 CUDA tensor."""

@@ -17,8 +17,7 @@
 //   * The keys of all requests and heads, in units of 64, are dealt out evenly: every CTA takes an equal range of units, wherever it begins and ends.
 //     Rows whose units fall to several CTAs are joined, in CTA order, by whichever of these is the last to leave its sums: the same bits on every run.
 // One token over 131071 keys, 32 + 2 x 8 heads of 128, f16: 94.5 us, 0.87 of the measured copy's bandwidth (another GPU 96.5); 64 requests of up to 8191 keys, bf16: 176 us, 0.93 (184).
-#include "rq_attention.cuh"
-#include "rq_mma.cuh"
+#include "rq_attention_rows.cuh"
 
 using namespace rqserve;
 using namespace rqattn;
@@ -26,9 +25,7 @@ using rqmma::smem_u32;
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 16, kUnit = kWarps * kTile;  // keys a warp and a CTA take at a time
-constexpr int kRequestStep = 128;  // requests' places in shared memory are taken by so many
 constexpr int kStages = 2;  // of a warp's ring: one tile under way while the other is used
 
 // c = (first ? 0 : c) + a b for sixteen rows, eight columns and sixteen products each
@@ -41,55 +38,15 @@ template <int TYPE> __device__ __forceinline__ void mma(float (&c)[4], bool firs
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
             : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-// acc = acc * f + d, two numbers an instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
+// acc = acc * f + d
 __device__ __forceinline__ void add_scaled(float2 (&acc)[2], float f, const float (&d)[4]) {
     acc[0] = fma2(acc[0], make_float2(f, f), make_float2(d[0], d[1]));
     acc[1] = fma2(acc[1], make_float2(f, f), make_float2(d[2], d[3]));
 }
-// four matrices of eight lines x sixteen bytes, lane l giving line l % 8 of matrix l / 8
-__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_transposed(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-// sixteen bytes, or zeros
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Whether a word's two 16-bit numbers are both finite
 template <int TYPE> __device__ __forceinline__ bool finite2(uint32_t w) {
     const uint32_t e = TYPE == RQ_KV_F16 ? 0x7c00u : 0x7f80u;
     return (w & e) != e && ((w >> 16) & e) != e;
-}
-
-// A request's rows and keys, as a CTA deals with them
-struct Request {
-    int fresh, here, length, begin, end, tiles;  // new tokens, those with queries; keys [begin, end) are seen by some row; row tiles
-    int64_t units;                         // of one row tile and head
-};
-template <int ROWS> __device__ __forceinline__ Request request_of(const AttentionParams& p, int r) {
-    Request q;
-    const int start = p.starts[r];
-    const int next = p.starts[r + 1];
-    q.fresh = max(next - start, 0);
-    q.here = tokens_here(p, start, next);
-    q.length = p.lengths[r];
-    q.end = (int)min((int64_t)max(q.length, 0), (int64_t)p.table_width << p.page_shift);
-    q.begin = p.window > 0 ? (int)max((int64_t)0, (int64_t)q.length - q.fresh - p.window + 1) : 0;
-    q.begin = min(q.begin, q.end) & ~(kTile - 1);
-    q.tiles = (q.here * (p.q_heads / p.kv_heads) + ROWS - 1) / ROWS;
-    q.units = max((q.end - q.begin + kUnit - 1) / kUnit, 1);  // (a row that sees no key is written all the same)
-    return q;
 }
 
 template <int D, int TYPE, int RT> struct Tiles {
@@ -116,37 +73,18 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
     const int group = p.q_heads / p.kv_heads;
     wait_for_previous();
 
-    // ---- where this CTA's units lie -----------------------------------------------------------------
-    int64_t total = 0;
-    if (tid == 0) before[0] = 0;
-    for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
-        int64_t units = 0;
-        if (r0 + tid < p.requests) { const Request q = request_of<ROWS>(p, r0 + tid); units = (int64_t)q.here * group > p.few ? 0 : q.units * q.tiles * p.kv_heads; }
-        int64_t scan = units;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) { const int64_t o = __shfl_up_sync(0xffffffffu, scan, off); if (lane >= off) scan += o; }
-        __syncthreads();
-        if (lane == 31) sums[warp] = scan;
-        __syncthreads();
-        scan += total;
-        for (int w = 0; w < kWarps; ++w) { if (w < warp) scan += sums[w]; total += sums[w]; }
-        if (r0 + tid < p.requests) before[r0 + tid + 1] = scan;
-    }
-    __syncthreads();
-    if (total == 0) return;
-    const int64_t ctas = min((int64_t)gridDim.x, total);
-    if (blockIdx.x >= ctas) return;
-    const int64_t my_end = (blockIdx.x + 1) * total / ctas;
-    int64_t u = blockIdx.x * total / ctas;
+    const Deal deal = deal_units<ROWS, kTile>(p, before, sums);
+    if (blockIdx.x >= deal.ctas) return;
+    int64_t u = deal.begin;
 
-    while (u < my_end) {
+    while (u < deal.end) {
         // the rows that unit u belongs to
         int r = 0;
         for (int hi = p.requests - 1; r < hi;) { const int mid = (r + hi + 1) >> 1; if (before[mid] <= u) r = mid; else hi = mid - 1; }
-        const Request rq = request_of<ROWS>(p, r);
+        const Request rq = request_of<ROWS, kTile>(p, r);
         const int64_t in_request = u - before[r], item = in_request / rq.units, first_unit = in_request % rq.units;
         const int kv = (int)(item % p.kv_heads), row0 = (int)(item / p.kv_heads) * ROWS, rows = min(ROWS, rq.here * group - row0);
-        const int64_t item_begin = u - first_unit, item_end = item_begin + rq.units, stop = min(item_end, my_end);
+        const int64_t item_begin = u - first_unit, item_end = item_begin + rq.units, stop = min(item_end, deal.end);
         const int key_first = rq.begin + (int)first_unit * kUnit, key_stop = min(rq.end, rq.begin + (int)(stop - item_begin) * kUnit);
         u = stop;
 
@@ -419,68 +357,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionPa
             for (int n = 0; n < D / 8; ++n) *(float2*)&sh.out[warp][rt * 8 + g][8 * n + 2 * t4] = make_float2(acc[rt][n][0].x + acc[rt][n][1].x, acc[rt][n][0].y + acc[rt][n][1].y);
         }
         __syncthreads();
-        const int64_t first_cta = ((item_begin + 1) * ctas - 1) / total, last_cta = (item_end * ctas - 1) / total;
-        const bool whole = first_cta == last_cta;
-        const int64_t stride = ROWS * (D + 2);
-        float* mine = p.partial + ((int64_t)blockIdx.x * 2 + (blockIdx.x == first_cta)) * stride;
-        auto row_of = [&](int row) { const int at = row0 + row; return p.y + (int64_t)(p.starts[r] + at / group) * p.y_stride + (int64_t)(kv * group + at % group) * D; };
-        auto put = [&](float* y, int e, float4 v, float total_weight) {
-            const float inverse = total_weight == 0.0f ? 0.0f : 1.0f / total_weight;
-            v.x *= inverse; v.y *= inverse; v.z *= inverse; v.w *= inverse;
-            if (p.wide) *(float4*)(y + e) = v;
-            else { y[e] = v.x; y[e + 1] = v.y; y[e + 2] = v.z; y[e + 3] = v.w; }
-        };
-        for (int i = tid; i < ROWS * (D / 4); i += kThreads) {
-            const int row = i / (D / 4), e = 4 * (i % (D / 4));
-            if (row >= rows) break;
-            float top = warp_base[0][row];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, warp_base[w][row]);
-            const float to = top == -INFINITY ? 0.0f : top;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float weight = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float f = exp2_fast(warp_base[w][row] - to);
-                const float4 o = *(const float4*)&sh.out[w][row][e];
-                v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
-                weight = fmaf(warp_sum[w][row], f, weight);
-            }
-            if (whole) {
-                put(row_of(row), e, v, weight);
-            } else {
-                __stcg((float4*)(mine + row * D + e), v);
-                if (e == 0) { __stcg(mine + ROWS * D + row, top); __stcg(mine + ROWS * D + ROWS + row, weight); }
-            }
-        }
-        if (!whole) {
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) last_arrival = atomicAdd(&p.arrived[first_cta], 1);
-            __syncthreads();
-            if (last_arrival == (uint32_t)(last_cta - first_cta)) {
-                if (tid == 0) p.arrived[first_cta] = 0;
-                __threadfence();
-                for (int i = tid; i < ROWS * (D / 4); i += kThreads) {
-                    const int row = i / (D / 4), e = 4 * (i % (D / 4));
-                    if (row >= rows) break;
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    float weight = 0.0f, top = -INFINITY;
-#pragma unroll 8
-                    for (int64_t c = first_cta; c <= last_cta; ++c) top = fmaxf(top, __ldcg(p.partial + (c * 2 + (c == first_cta)) * stride + ROWS * D + row));
-                    const float to = top == -INFINITY ? 0.0f : top;
-#pragma unroll 8
-                    for (int64_t c = first_cta; c <= last_cta; ++c) {
-                        const float* from = p.partial + (c * 2 + (c == first_cta)) * stride;
-                        const float f = exp2_fast(__ldcg(from + ROWS * D + row) - to);
-                        const float4 o = __ldcg((const float4*)(from + row * D + e));
-                        v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
-                        weight = fmaf(__ldcg(from + ROWS * D + ROWS + row), f, weight);
-                    }
-                    put(row_of(row), e, v, weight);
-                }
-            }
-        }
+        join_rows<D, ROWS>(p, &sh.out[0][0][0], warp_base, warp_sum, item_begin, item_end, deal, p.starts[r], row0, rows, kv, last_arrival);
         __syncthreads();  // the shared sums are free again
     }
 }
@@ -527,6 +404,7 @@ int launch_rows(rq_ctx* ctx, const AttentionParams& p, int type, bool two, cudaS
     return two ? launch_rows<D, RQ_KV_BF16, MOST>(ctx, p, s) : launch_rows<D, RQ_KV_BF16, 1>(ctx, p, s);
 }
 int launch_rows_of(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s) {
+    if (cache.type == RQ_KV_INT8) return launch_rows_int8(ctx, p, cache, two, s);
     if (cache.head_dim == 64) return launch_rows<64>(ctx, p, cache.type, two, s);
     if (cache.head_dim == 128) return launch_rows<128>(ctx, p, cache.type, two, s);
     return launch_rows<256>(ctx, p, cache.type, two, s);
@@ -575,6 +453,11 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
     p.wide = (aligned(16) ? 1 : 0) | (aligned(32) ? 2 : 0);
     while (1 << p.page_shift < cache->page_size) ++p.page_shift;
     p.error_flag = ctx->error_flag; p.wait_ns = ctx->wait_limit_ns;
+    if (cache->type == RQ_KV_INT8) {
+        p.page_bytes = (uint32_t)cache->page_stride; p.line_bytes = (uint32_t)cache->line_stride;
+        p.k_scale = cache->k_scale; p.v_scale = cache->v_scale;
+        p.scale_page = cache->scale_page_stride; p.scale_head = cache->scale_head_stride; p.scale_line = cache->scale_line_stride;
+    }
     const int64_t rows = (int64_t)(max_fresh > 0 ? (max_fresh < tokens ? max_fresh : tokens) : tokens) * group;
     // The rows kernel reads a request's keys once for every sixteen rows (from L2, from the second time on), the tensor-core kernel makes scores of 128 whatever
     // there is. 8192 cached keys, 32 + 2 x 8 heads of 128, f16, rows kernel | tensor cores: 16 requests of 16 rows 102 | 217 us, 32 rows 180 | 219, 48 rows 259 | 219,

@@ -19,6 +19,8 @@ struct AttentionParams {
     int wide;  // q and y allow accesses of 16 bytes (1), of 32 (2)
     int* error_flag;
     unsigned long long wait_ns;
+    const float *k_scale, *v_scale;  // a cache of codes: of each position's head
+    int64_t scale_page, scale_head, scale_line;
 };
 
 // What the work area holds: sums of rows for each CTA's first and last item (the tensor-core kernel: two tiles of 128 rows of 128 elements and their
@@ -32,6 +34,9 @@ constexpr size_t kPartialBytes = sizeof(float) * (kTensorPartial > kRowPartial ?
 // serve: 256 elements a head, pages of fewer than eight positions, strides of zero.
 int launch_tensor(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool one_tile, cudaStream_t s);
 
+// Rows by the few over a cache of codes (rq_attention_int8.cu); two: sixteen rows at a time
+int launch_rows_int8(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s);
+
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are 2^(s - max + kRaise): an f16 part below 2^-14 loses bits, raised by 2^12 that is a weight of 2^-26 of the row's largest. bf16 has fp32's exponents: its
 // parts need none of it, and values near the end of its range leave sums no room for it.
@@ -42,6 +47,23 @@ template <int TYPE> constexpr float kRaise = TYPE == RQ_KV_F16 ? 12.0f : 0.0f;
 __device__ __forceinline__ int tokens_here(const AttentionParams& p, int start, int next) { return start < 0 ? 0 : max(min(next, p.tokens) - start, 0); }
 
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+// Codes of a cache as f16 numbers, exactly: with the sign bit turned over a code is c + 128, as the low byte under 0x64 that is 1024 + c + 128. FIRST, SECOND: which bytes
+// of the word.
+__device__ __forceinline__ uint32_t turn_codes(uint32_t word) { return word ^ 0x80808080u; }
+template <int FIRST, int SECOND> __device__ __forceinline__ uint32_t widen_codes(uint32_t turned) {
+    const uint32_t w = __byte_perm(turned, 0x64646464u, FIRST | 4 << 4 | SECOND << 8 | 4 << 12);
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0x64806480u));
+    return r;
+}
+
+// A value's scale takes part in the row's base (the largest of score + log2 of the scale), by its exponent, so that weights times scales stay within f16's range whatever the
+// scales are; one that is no number takes no part
+__device__ __forceinline__ float exponent_of(float scale) {
+    const int e = (int)(__float_as_uint(scale) >> 23 & 0xff);
+    return __uint_as_float(0x4b000000u | (uint32_t)(e == 255 ? 127 : min(max(e, 127 - 80), 127 + 90))) - (8388608.0f + 127.0f);
+}
 
 // two fp32 numbers as a pair of 16-bit ones (the first in the low half), and what the pair leaves of them
 template <int TYPE> __device__ __forceinline__ uint32_t pair_of(float a, float b) {

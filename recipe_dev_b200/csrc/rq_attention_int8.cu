@@ -1,0 +1,357 @@
+// Attention of a few rows at a time (decode steps) over a cache of 8-bit codes with a scale for each position's head:
+//
+//   y = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q . k_j - m),  k_j = sk_j ck_j,  v_j = sv_j cv_j
+//
+// The form of rq_attention.cu's kernel: a warp takes its keys through a ring of its own in shared memory, queries and weights are taken apart into hi + lo f16 parts, one
+// mma.sync does both, sums are added up in fp32. What differs, since a tile is half the bytes and the codes are no operands yet:
+//   * Codes become f16 numbers on their way from shared memory into operand registers, exactly (a byte permute and a subtraction a pair). Scores are multiplied by sk, weights
+//     by sv before they are taken apart, both in fp32: nothing is rounded that the 16-bit caches' kernel would not round.
+//   * The elements of a product's sixteen may be any, if the queries' are the same: a thread's operands of four steps are sixteen neighbouring codes of a key, one 16-byte load.
+//     For the values a transposing matrix load moves pairs of neighbouring elements: the even ones make one column of the product, the odd ones the next.
+//   * A warp's tile is 32 keys (16 for heads of 256): the same bytes on their way as there, and half the work on sums for each key.
+//   * A row's base is the largest score plus its value's scale's exponent, less 12: hi parts of weight * sv lie below 2^13 whatever the scales are.
+#include "rq_attention_rows.cuh"
+
+using namespace rqserve;
+using namespace rqattn;
+using rqmma::smem_u32;
+
+namespace {
+
+// c = (first ? 0 : c) + a b for sixteen rows, eight columns and sixteen products each
+__device__ __forceinline__ void mma(float (&c)[4], bool first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    const float c0 = first ? 0.0f : c[0], c1 = first ? 0.0f : c[1], c2 = first ? 0.0f : c[2], c3 = first ? 0.0f : c[3];
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+// four bytes, or zeros
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+
+template <int D> struct Form {
+    static constexpr int TILE = D == 256 ? 16 : 32, STAGES = 2;  // keys a warp takes at a time; tiles of its ring
+    static constexpr int CHUNKS = D / 16, LINES = 32 / CHUNKS;   // 16-byte pieces of a line; lines that a warp copies an instruction
+    static constexpr int STAGE = 2 * TILE * D;                   // bytes: keys, values
+};
+// Where a line's pieces lie, so that neither eight lines' same piece (matrix loads) nor four pieces each of two lines meet a bank twice
+template <int D> __device__ __forceinline__ int placed(int line, int chunk) { return chunk ^ (D == 64 ? line >> 1 & 3 : (line & 1) << 2 | (line >> 1 & 3)); }
+
+template <int D, int RT> struct Tiles {
+    union {
+        struct {
+            uint8_t codes[kWarps][Form<D>::STAGES][2][Form<D>::TILE][D];
+            float scales[kWarps][Form<D>::STAGES][2][Form<D>::TILE];
+        };
+        float out[kWarps][8 * RT][D + 8];  // the warps' sums
+    };
+    uint4 q[RT][D / 16][32];  // operand registers of the queries: hi above lo
+};
+
+template <int D, int RT>
+__global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionParams p) {
+    using F = Form<D>;
+    constexpr int ROWS = 8 * RT, STEPS = D / 16, TILE = F::TILE, UNIT = kWarps * TILE, NT = TILE / 8, LINES = F::LINES;
+    constexpr uint32_t ALL = TILE == 32 ? 0xffffffffu : 0xffffu;
+    extern __shared__ __align__(128) unsigned char dynamic[];
+    Tiles<D, RT>& sh = *(Tiles<D, RT>*)dynamic;
+    int64_t* before = (int64_t*)(dynamic + sizeof(sh));  // units before each request
+    __shared__ float warp_base[kWarps][ROWS], warp_sum[kWarps][ROWS];
+    __shared__ uint32_t row_largest[kWarps][ROWS];
+    __shared__ int64_t sums[kWarps];
+    __shared__ uint32_t last_arrival;
+    launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int group = p.q_heads / p.kv_heads;
+    wait_for_previous();
+
+    const Deal deal = deal_units<ROWS, TILE>(p, before, sums);
+    if (blockIdx.x >= deal.ctas) return;
+    int64_t u = deal.begin;
+
+    while (u < deal.end) {
+        // the rows that unit u belongs to
+        int r = 0;
+        for (int hi = p.requests - 1; r < hi;) { const int mid = (r + hi + 1) >> 1; if (before[mid] <= u) r = mid; else hi = mid - 1; }
+        const Request rq = request_of<ROWS, TILE>(p, r);
+        const int64_t in_request = u - before[r], item = in_request / rq.units, first_unit = in_request % rq.units;
+        const int kv = (int)(item % p.kv_heads), row0 = (int)(item / p.kv_heads) * ROWS, rows = min(ROWS, rq.here * group - row0);
+        const int64_t item_begin = u - first_unit, item_end = item_begin + rq.units, stop = min(item_end, deal.end);
+        const int key_first = rq.begin + (int)first_unit * UNIT, key_stop = min(rq.end, rq.begin + (int)(stop - item_begin) * UNIT);
+        u = stop;
+
+        // the keys that some row sees and that this thread's rows see: [low, high)
+        int low[RT], high[RT];
+        const int position0 = rq.length - rq.fresh, seen_high = min(key_stop, position0 + (row0 + max(rows, 1) - 1) / group + 1);
+        const int seen_low = p.window > 0 ? max(0, position0 + row0 / group - p.window + 1) : 0;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int position = position0 + (row0 + rt * 8 + g) / group;
+            high[rt] = rt * 8 + g < rows ? min(position + 1, rq.end) : 0;
+            low[rt] = p.window > 0 ? max(position - p.window + 1, 0) : 0;
+        }
+
+        const int32_t* table = p.block_table + r * p.table_stride;
+        const int line_mask = (1 << p.page_shift) - 1, lane_chunk = lane % F::CHUNKS, lane_line = lane / F::CHUNKS, lane_key = lane & (TILE - 1);
+        const char* k_lane = (const char*)p.k + kv * p.head_stride + 16 * lane_chunk;
+        const int64_t k_to_v = (const char*)p.v - (const char*)p.k;
+        const float *k_scale = p.k_scale + kv * p.scale_head, *v_scale = p.v_scale + kv * p.scale_head;
+        const uint32_t ring = smem_u32(&sh.codes[warp][0][0][0][0]), scales_at = smem_u32(&sh.scales[warp][0][0][lane_key]);
+        // where a tile's keys lie: lane l finds key l's page, -1 for a key that no row sees
+        auto page_of = [&](int key0) -> int {
+            const int key = key0 + lane_key;
+            const int entry = key >= seen_low && key < seen_high ? __ldcg(table + (key >> p.page_shift)) : -1;
+            return entry < p.pages ? max(entry, -1) : -1;
+        };
+        // A warp copies LINES lines an instruction, this lane one piece of one of them
+        auto fetch = [&](int key0, int page, uint32_t seen, int stage) {
+            const uint32_t to = ring + stage * F::STAGE + lane_line * D;
+#pragma unroll
+            for (int half = 0; half < TILE / 16; ++half) {
+                if (p.page_shift >= 4) {  // sixteen keys of a multiple of sixteen share a page
+                    const uint32_t here = seen >> (16 * half) & 0xffffu;
+                    const int first = __shfl_sync(0xffffffffu, page, 16 * half + (here ? __ffs(here) - 1 : 0));
+                    const char* from = k_lane + (uint64_t)(uint32_t)max(first, 0) * p.page_bytes + (uint64_t)(uint32_t)(((key0 + 16 * half) & line_mask) + lane_line) * p.line_bytes;
+#pragma unroll
+                    for (int i = 0; i < 16 / LINES; ++i) {
+                        const int line = 16 * half + i * LINES;
+                        const uint32_t place = to + line * D + (placed<D>(line + lane_line, lane_chunk) << 4);
+                        const bool there = seen >> (line + lane_line) & 1;
+                        copy16(place, from, there);
+                        copy16(place + TILE * D, from + k_to_v, there);
+                        from += LINES * (uint64_t)p.line_bytes;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16 / LINES; ++i) {
+                        const int line = 16 * half + i * LINES + lane_line, at = __shfl_sync(0xffffffffu, page, line);
+                        const char* from = k_lane + (uint64_t)(uint32_t)max(at, 0) * p.page_bytes + (uint64_t)(uint32_t)((key0 + line) & line_mask) * p.line_bytes;
+                        const uint32_t place = to + (line - lane_line) * D + (placed<D>(line, lane_chunk) << 4);
+                        copy16(place, from, at >= 0);
+                        copy16(place + TILE * D, from + k_to_v, at >= 0);
+                    }
+                }
+            }
+            // a lane its key's scales (sixteen keys: one half of the lanes the keys', the other the values')
+            const int64_t scale_at = (int64_t)max(page, 0) * p.scale_page + (int64_t)((key0 + lane_key) & line_mask) * p.scale_line;
+            const uint32_t scale_to = scales_at + stage * (2 * TILE * 4);
+            if (TILE == 32 || lane < 16) copy4(scale_to, k_scale + scale_at, page >= 0);
+            if (TILE == 32 || lane >= 16) copy4(scale_to + TILE * 4, v_scale + scale_at, page >= 0);
+        };
+        int key0 = key_first + warp * TILE, ahead = key0, stage = 0;
+        int page = page_of(ahead);
+        uint32_t seen = __ballot_sync(0xffffffffu, page >= 0) & ALL, seen_next = 0;  // the tile's keys that some row sees
+        if (ahead < key_stop) fetch(ahead, page, seen, 0);
+        copies_commit();
+        ahead += UNIT;
+        page = page_of(ahead);
+
+        // queries: brought to one size and taken apart, as the tensor core's operand registers (a thread's of step 4 j + i: elements 64 j + 16 t4 + 4 i + 0 .. 3); a warp
+        // has every fourth step of all rows
+        float factor[RT];  // of the scores of row g
+        {
+            constexpr int MINE = RT * STEPS / kWarps;
+            float4 x[MINE];
+            uint32_t largest[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) largest[rt] = 0;
+#pragma unroll
+            for (int n = 0; n < MINE; ++n) {
+                const int rt = n * kWarps / STEPS, step = n * kWarps % STEPS + warp, row = rt * 8 + g;
+                x[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (row < rows) {
+                    const int at = row0 + row;
+                    const float* from = p.q + (int64_t)(p.starts[r] + at / group) * p.q_stride + (int64_t)(kv * group + at % group) * D + 64 * (step >> 2) + 16 * t4 + 4 * (step & 3);
+                    if (p.wide) x[n] = __ldcg((const float4*)from);
+                    else x[n] = make_float4(__ldcg(from), __ldcg(from + 1), __ldcg(from + 2), __ldcg(from + 3));
+                }
+                largest[rt] = max(max(largest[rt], __float_as_uint(x[n].x) & 0x7fffffffu), __float_as_uint(x[n].y) & 0x7fffffffu);
+                largest[rt] = max(max(largest[rt], __float_as_uint(x[n].z) & 0x7fffffffu), __float_as_uint(x[n].w) & 0x7fffffffu);
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                largest[rt] = max(largest[rt], __shfl_xor_sync(0xffffffffu, largest[rt], 1));
+                largest[rt] = max(largest[rt], __shfl_xor_sync(0xffffffffu, largest[rt], 2));
+                if (t4 == 0) row_largest[warp][rt * 8 + g] = largest[rt];
+            }
+            __syncthreads();
+            float raised[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) largest[rt] = max(largest[rt], row_largest[w][rt * 8 + g]);
+                const int raise = raise_of(largest[rt]);
+                raised[rt] = power_of_two(raise);
+                factor[rt] = factor_of(p.scale, raise);
+            }
+#pragma unroll
+            for (int n = 0; n < MINE; ++n) {
+                const int rt = n * kWarps / STEPS, step = n * kWarps % STEPS + warp;
+                x[n].x *= raised[rt]; x[n].y *= raised[rt]; x[n].z *= raised[rt]; x[n].w *= raised[rt];
+                uint4 a;
+                a.x = take_pair<RQ_KV_F16>(x[n].x, x[n].y);
+                a.z = take_pair<RQ_KV_F16>(x[n].z, x[n].w);
+                a.y = rqattn::pair_of<RQ_KV_F16>(x[n].x, x[n].y);
+                a.w = rqattn::pair_of<RQ_KV_F16>(x[n].z, x[n].w);
+                sh.q[rt][step][lane] = a;
+            }
+        }
+        __syncthreads();
+
+        float base[RT], sum[RT];  // base: -inf while the row has seen no key
+        float2 acc[RT][D / 8];    // elements 16 c + 4 t4 + {0, 2} (2 c), + {1, 3} (2 c + 1)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            base[rt] = -INFINITY;
+            sum[rt] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) acc[rt][n] = make_float2(0.0f, 0.0f);
+        }
+        for (; key0 < key_stop; key0 += UNIT, stage = stage + 1 == F::STAGES ? 0 : stage + 1, seen = seen_next) {
+            const uint32_t keys = ring + stage * F::STAGE, values = keys + TILE * D;
+            __syncwarp();  // the other stage has been read
+            seen_next = __ballot_sync(0xffffffffu, page >= 0) & ALL;
+            if (ahead < key_stop) fetch(ahead, page, seen_next, stage ^ 1);
+            copies_commit();
+            ahead += UNIT;
+            page = page_of(ahead);
+            copies_wait<1>();
+            __syncwarp();
+            // scores: of keys 8 i + 2 t4 + {0, 1} and row g
+            float c[RT][NT][4];
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+                uint4 w[NT];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const uint32_t from = keys + (8 * i + g) * D + (placed<D>(8 * i + g, 4 * j + t4) << 4);
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w) : "r"(from) : "memory");
+                }
+#pragma unroll
+                for (int step = 0; step < 4; ++step) {
+                    uint4 a[RT];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) a[rt] = sh.q[rt][4 * j + step][lane];
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        const uint32_t word = turn_codes(step == 0 ? w[i].x : step == 1 ? w[i].y : step == 2 ? w[i].z : w[i].w);
+                        const uint32_t b0 = widen_codes<0, 1>(word), b1 = widen_codes<2, 3>(word);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) mma(c[rt][i], j == 0 && step == 0, a[rt].x, a[rt].y, a[rt].z, a[rt].w, b0, b1);
+                    }
+                }
+            }
+            // weights
+            uint32_t w_hi[RT][NT], w_lo[RT][NT];
+            float old[RT];
+            {
+                float2 ks[NT], vs[NT];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) { ks[i] = *(const float2*)&sh.scales[warp][stage][0][8 * i + 2 * t4]; vs[i] = *(const float2*)&sh.scales[warp][stage][1][8 * i + 2 * t4]; }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    float s[NT][2], top = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < NT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int at = 8 * i + 2 * t4 + e, key = key0 + at;
+                            s[i][e] = (c[rt][i][e] + c[rt][i][2 + e]) * (e ? ks[i].y : ks[i].x);
+                            if (key < low[rt] || key >= high[rt] || !(seen >> at & 1)) s[i][e] = -INFINITY;
+                            top = fmaxf(top, fmaf(s[i][e], factor[rt], exponent_of(e ? vs[i].y : vs[i].x)));
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    top = fmaxf(base[rt], top - kRaise<RQ_KV_F16>);
+                    const float from = top == -INFINITY ? 0.0f : top;
+                    old[rt] = exp2_fast(base[rt] - from);
+                    base[rt] = top;
+                    float add = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        const float a = exp2_fast(fmaf(s[i][0], factor[rt], -from)), b = exp2_fast(fmaf(s[i][1], factor[rt], -from));
+                        add += a + b;
+                        // (a scale that the row must not see may be infinite, and 0 * inf is no 0)
+                        float x = s[i][0] == -INFINITY ? 0.0f : a * vs[i].x, y = s[i][1] == -INFINITY ? 0.0f : b * vs[i].y;
+                        w_hi[rt][i] = take_pair<RQ_KV_F16>(x, y);
+                        w_lo[rt][i] = rqattn::pair_of<RQ_KV_F16>(x, y);
+                    }
+                    sum[rt] = fmaf(sum[rt], old[rt], add);
+                }
+            }
+            const int value_line = lane & 15, value_half = lane >> 4;
+#pragma unroll
+            for (int n2 = 0; n2 < D / 32; ++n2) {
+                uint32_t b[TILE / 16][4];
+#pragma unroll
+                for (int half = 0; half < TILE / 16; ++half) {
+                    const int line = 16 * half + value_line;
+                    ldmatrix_transposed(b[half], values + line * D + (placed<D>(line, 2 * n2 + value_half) << 4));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) b[half][i] = turn_codes(b[half][i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // sixteen elements, even ones, odd ones
+                    uint32_t b0[TILE / 16], b1[TILE / 16];
+#pragma unroll
+                    for (int half = 0; half < TILE / 16; ++half) {
+                        const uint32_t x = b[half][i & 2], y = b[half][(i & 2) + 1];
+                        b0[half] = i & 1 ? widen_codes<1, 3>(x) : widen_codes<0, 2>(x);
+                        b1[half] = i & 1 ? widen_codes<1, 3>(y) : widen_codes<0, 2>(y);
+                    }
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        float d[4];
+#pragma unroll
+                        for (int half = 0; half < TILE / 16; ++half)
+                            mma(d, half == 0, w_hi[rt][2 * half], w_lo[rt][2 * half], w_hi[rt][2 * half + 1], w_lo[rt][2 * half + 1], b0[half], b1[half]);
+                        acc[rt][4 * n2 + i] = fma2(acc[rt][4 * n2 + i], make_float2(old[rt], old[rt]), make_float2(d[0] + d[2], d[1] + d[3]));
+                    }
+                }
+            }
+        }
+        copies_wait<0>();
+        __syncthreads();  // the sums go where the ring was
+
+        // ---- the four warps' sums, and other CTAs' ------------------------------------------------------
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            sum[rt] += __shfl_xor_sync(0xffffffffu, sum[rt], 1);
+            sum[rt] += __shfl_xor_sync(0xffffffffu, sum[rt], 2);
+            if (t4 == 0) { warp_base[warp][rt * 8 + g] = base[rt]; warp_sum[warp][rt * 8 + g] = sum[rt]; }
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+                *(float4*)&sh.out[warp][rt * 8 + g][16 * n + 4 * t4] = make_float4(acc[rt][2 * n].x, acc[rt][2 * n + 1].x, acc[rt][2 * n].y, acc[rt][2 * n + 1].y);
+        }
+        __syncthreads();
+        join_rows<D, ROWS>(p, &sh.out[0][0][0], warp_base, warp_sum, item_begin, item_end, deal, p.starts[r], row0, rows, kv, last_arrival);
+        __syncthreads();  // the shared sums are free again
+    }
+}
+
+template <int D, int RT>
+int launch_rows(rq_ctx* ctx, const AttentionParams& p, cudaStream_t s) {
+    auto kernel = rq_attention_int8_kernel<D, RT>;
+    // The grid decides where rows are cut, and with it the last bits: it follows from the call alone. Shared memory holds eight bytes a request, by steps of 128 of them.
+    const int step = (p.requests + kRequestStep - 1) / kRequestStep, dev = ctx->device;
+    auto bytes = [](int steps) { return sizeof(Tiles<D, RT>) + sizeof(int64_t) * ((size_t)steps * kRequestStep + 1); };
+    constexpr int kSteps = RQ_MAX_REQUESTS / kRequestStep;
+    static uint8_t resident[64][kSteps + 1] = {};  // by device: CTAs an SM holds; 0: not known yet
+    int n = dev < 64 ? resident[dev][step] : 0;
+    if (!n) {
+        RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(kSteps)));
+        RQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, bytes(step)));
+        n = n < 1 ? 1 : (n > 4 ? 4 : n);
+        if (dev < 64) resident[dev][step] = (uint8_t)n;
+    }
+    const int ctas = ctx->sm_count * n;
+    return launch(kernel, dim3((unsigned)(ctas < kRowCtas ? ctas : kRowCtas)), kThreads, bytes(step), s, p);
+}
+
+}  // namespace
+
+int rqattn::launch_rows_int8(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s) {
+    if (cache.head_dim == 64) return two ? launch_rows<64, 2>(ctx, p, s) : launch_rows<64, 1>(ctx, p, s);
+    if (cache.head_dim == 128) return two ? launch_rows<128, 2>(ctx, p, s) : launch_rows<128, 1>(ctx, p, s);
+    return launch_rows<256, 1>(ctx, p, s);
+}

@@ -949,6 +949,7 @@ int make_map(CUtensorMap* map, const void* base, const rq_kv_cache& c, int lines
 }  // namespace
 
 int rqattn::launch_tensor(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& c, bool one_tile, cudaStream_t s) {
+    if (c.type == RQ_KV_INT8) return RQ_ERR_UNSUPPORTED;
     // pages of whole groups of eight lines (the swizzle's), and strides that a tensor map can hold
     if (c.head_dim > 128 || c.page_size < 8 || c.line_stride <= 0 || (c.heads > 1 && c.head_stride <= 0) || (c.pages > 1 && c.page_stride <= 0) || c.head_stride >= (int64_t)1 << 38) return RQ_ERR_UNSUPPORTED;
     const int tile = c.type == RQ_KV_F16 || c.head_dim == 64 ? 128 : 64, lines = c.page_size < tile ? c.page_size : tile;

@@ -20,7 +20,9 @@ struct RopeParams {
     const float *q, *k, *v, *q_gain, *k_gain, *table;
     float* q_out;
     const int32_t *positions, *slots;
-    uint16_t *k_cache, *v_cache;
+    void *k_cache, *v_cache;
+    float *k_scale, *v_scale;
+    int64_t scale_page, scale_head, scale_line;
     int64_t q_stride, k_stride, v_stride, out_stride, table_rows, page_stride, head_stride, line_stride, pages;
     int tokens, q_heads, kv_heads, rotary, style, page_shift;
     float epsilon;
@@ -149,14 +151,46 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
         }
         if (is_q) {
             store<E, WIDE>(p.q_out + t * p.out_stride + (int64_t)head * D + first, x[n]);
-        } else if (stored) {
-            uint16_t* to = (is_k ? p.k_cache + (head - p.q_heads) * p.head_stride : p.v_cache + (head - p.q_heads - p.kv_heads) * p.head_stride) + line;
+        } else if (TYPE != RQ_KV_INT8 && stored) {
+            uint16_t* to = (is_k ? (uint16_t*)p.k_cache + (head - p.q_heads) * p.head_stride : (uint16_t*)p.v_cache + (head - p.q_heads - p.kv_heads) * p.head_stride) + line;
             uint32_t w[E / 2];
 #pragma unroll
             for (int i = 0; i < E; i += 2) w[i / 2] = from_float<TYPE>(x[n][i]) | (uint32_t)from_float<TYPE>(x[n][i + 1]) << 16;
             if (E == 2) *(uint32_t*)to = w[0];
             else if (E == 4) *(uint2*)to = make_uint2(w[0], w[1 % (E / 2)]);
             else *(uint4*)to = make_uint4(w[0], w[1 % (E / 2)], w[2 % (E / 2)], w[3 % (E / 2)]);
+        }
+    }
+    if (TYPE == RQ_KV_INT8 && stored) {
+        // A head's largest magnitude (as bits without the sign: infinities and NaN lie above the numbers), its scale, and its codes: x / scale + 1.5 * 2^23 rounded once,
+        // to a whole number, whose low byte is the code
+        const int64_t place = page * p.scale_page + (slot & ((1 << p.page_shift) - 1)) * p.scale_line;
+#pragma unroll
+        for (int n = 0; n < kHeads; ++n) {
+            const int at = head0 + n - p.q_heads;  // among the keys' heads and then the values'
+            if (at < 0 || at >= 2 * p.kv_heads) continue;
+            uint32_t largest = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) largest = max(largest, __float_as_uint(x[n][i]) & 0x7fffffffu);
+            largest = __reduce_max_sync(0xffffffffu, largest);
+            float of_head = __uint_as_float(largest) / 127.0f;
+            if (of_head < 1.17549435e-38f) of_head = 0.0f;
+            const float inverse = of_head == 0.0f ? 0.0f : 1.0f / of_head;
+            uint32_t codes[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) codes[i] = __float_as_uint(fmaf(x[n][i], inverse, 12582912.0f));
+            const int kv = at < p.kv_heads ? at : at - p.kv_heads;
+            int8_t* to = (int8_t*)(at < p.kv_heads ? p.k_cache : p.v_cache) + kv * p.head_stride + line;
+            uint32_t w[E / 4 > 0 ? E / 4 : 1];
+            w[0] = __byte_perm(codes[0], codes[1], 0x0040);
+            if (E >= 4) {
+#pragma unroll
+                for (int i = 0; i < E / 4; ++i) w[i] = __byte_perm(__byte_perm(codes[4 * i % E], codes[(4 * i + 1) % E], 0x0040), __byte_perm(codes[(4 * i + 2) % E], codes[(4 * i + 3) % E], 0x0040), 0x5410);
+            }
+            if (E == 2) *(uint16_t*)to = (uint16_t)w[0];
+            else if (E == 4) *(uint32_t*)to = w[0];
+            else *(uint2*)to = make_uint2(w[0], w[1 % (E / 4 > 0 ? E / 4 : 1)]);
+            if (lane == 0) (at < p.kv_heads ? p.k_scale : p.v_scale)[place + kv * p.scale_head] = of_head;
         }
     }
 }
@@ -178,8 +212,9 @@ template <int D>
 int launch_rope(const RopeParams& p, int type, bool wide, cudaStream_t s) {
     const int64_t items = (int64_t)p.tokens * ((p.q_heads + 2 * p.kv_heads + kHeads - 1) / kHeads);
     const dim3 grid((unsigned)((items + kWarps - 1) / kWarps));
-    auto kernel = type == RQ_KV_F16 ? (wide ? rq_rope_kernel<D, RQ_KV_F16, true> : rq_rope_kernel<D, RQ_KV_F16, false>)
-                                    : (wide ? rq_rope_kernel<D, RQ_KV_BF16, true> : rq_rope_kernel<D, RQ_KV_BF16, false>);
+    auto kernel = type == RQ_KV_F16    ? (wide ? rq_rope_kernel<D, RQ_KV_F16, true> : rq_rope_kernel<D, RQ_KV_F16, false>)
+                  : type == RQ_KV_BF16 ? (wide ? rq_rope_kernel<D, RQ_KV_BF16, true> : rq_rope_kernel<D, RQ_KV_BF16, false>)
+                                       : (wide ? rq_rope_kernel<D, RQ_KV_INT8, true> : rq_rope_kernel<D, RQ_KV_INT8, false>);
     return launch(kernel, grid, kWarps * 32, 0, s, p);
 }
 
@@ -212,7 +247,11 @@ extern "C" int rq_rope_store(rq_ctx* ctx, const float* q, int64_t q_t_stride, in
     DeviceGuard guard(ctx->device);
     RopeParams p = {};
     p.q = q; p.k = k; p.v = v; p.q_gain = q_gain; p.k_gain = k_gain; p.table = table; p.q_out = q_out; p.positions = positions; p.slots = slots;
-    p.k_cache = (uint16_t*)cache->k; p.v_cache = (uint16_t*)cache->v;
+    p.k_cache = cache->k; p.v_cache = cache->v;
+    if (cache->type == RQ_KV_INT8) {
+        p.k_scale = cache->k_scale; p.v_scale = cache->v_scale;
+        p.scale_page = cache->scale_page_stride; p.scale_head = cache->scale_head_stride; p.scale_line = cache->scale_line_stride;
+    }
     p.q_stride = q_t_stride; p.k_stride = k_t_stride; p.v_stride = v_t_stride; p.out_stride = q_out_t_stride; p.table_rows = table_rows;
     p.page_stride = cache->page_stride; p.head_stride = cache->head_stride; p.line_stride = cache->line_stride; p.pages = cache->pages;
     p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = cache->heads; p.rotary = rotary; p.style = style; p.epsilon = epsilon;

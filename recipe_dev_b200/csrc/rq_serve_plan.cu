@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) rq_batch_plan_kernel(PlanParams p) {
 
 int rqserve::check_cache(const char* who, const rq_kv_cache* c) {
     if (!c || !c->k || !c->v) return rq_fail(RQ_ERR_INVALID, "%s: null cache", who);
-    if (c->type != RQ_KV_F16 && c->type != RQ_KV_BF16) return rq_fail(RQ_ERR_INVALID, "%s: cache type %d is neither F16(0) nor BF16(1)", who, c->type);
+    if (c->type != RQ_KV_F16 && c->type != RQ_KV_BF16 && c->type != RQ_KV_INT8) return rq_fail(RQ_ERR_INVALID, "%s: cache type %d is none of F16(0), BF16(1) and INT8(2)", who, c->type);
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return rq_fail(RQ_ERR_UNSUPPORTED, "%s: head_dim=%d is not 64, 128 or 256", who, c->head_dim);
     if (c->heads <= 0 || c->pages <= 0) return rq_fail(RQ_ERR_INVALID, "%s: the cache's heads and pages must be positive", who);
     if (c->page_size <= 0 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
@@ -126,6 +126,12 @@ int rqserve::check_cache(const char* who, const rq_kv_cache* c) {
     if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return rq_fail(RQ_ERR_INVALID, "%s: the cache's pointers must be 16-byte aligned", who);
     if (c->page_stride < 0 || c->head_stride < 0 || c->line_stride < 0 || (c->page_stride | c->head_stride | c->line_stride) & 7)
         return rq_fail(RQ_ERR_INVALID, "%s: the cache's strides must be non-negative multiples of 8 elements", who);
+    if (c->type == RQ_KV_INT8) {
+        if (!c->k_scale || !c->v_scale || (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3)) return rq_fail(RQ_ERR_INVALID, "%s: an INT8 cache needs 4-byte aligned k_scale and v_scale", who);
+        if ((c->page_stride | c->head_stride | c->line_stride) & 15) return rq_fail(RQ_ERR_INVALID, "%s: an INT8 cache's strides must be multiples of 16 elements", who);
+        if (c->scale_page_stride < 0 || c->scale_head_stride < 0 || c->scale_line_stride < 0 || c->scale_page_stride >= (int64_t)1 << 31 || c->scale_line_stride >= (int64_t)1 << 31)
+            return rq_fail(RQ_ERR_LIMIT, "%s: the scales' strides must not be negative, those of pages and lines below 2^31", who);
+    }
     if (c->page_stride >= (int64_t)1 << 31 || c->line_stride >= (int64_t)1 << 31) return rq_fail(RQ_ERR_LIMIT, "%s: the cache's page and line strides must be below 2^31 elements", who);
     return RQ_OK;
 }
