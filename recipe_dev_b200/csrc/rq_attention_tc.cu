@@ -43,18 +43,25 @@ namespace {
 
 constexpr int kSoftmaxWarps = 8, kIssuer = 8, kLoader = 9, kFetcher = 10, kMender = 11, kThreads = 12 * 32;
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;                              // 2 * 224 + 56 = 3 * 168, what the block is launched with
+constexpr int kCodesShift = 4;  // a copy of codes brings at most sixteen lines
+constexpr int kUneven = 1 << 20, kEven = 12;  // exponents of a tile's scales of values: further apart than kEven, or of one that is no number
 constexpr int kItems = 4, kWords = 16;  // rings in shared memory: items, words on tiles of keys
 
-template <int D, int TYPE, bool KEYS_> struct Form {
-    static constexpr bool KEYS = KEYS_;
+// CODES: the cache holds 8-bit codes, TYPE is what they become
+template <int D, int TYPE, bool KEYS_, bool CODES_> struct Form {
+    static constexpr bool KEYS = KEYS_, CODES = CODES_;
     static constexpr int PARTS = TYPE == RQ_KV_F16 ? 2 : 3;
     static constexpr int KT = TYPE == RQ_KV_F16 || D == 64 ? 128 : 64;  // keys a tile (bf16, 128 elements: 2 KT + 2 D + KT columns are what tensor memory holds with 64)
     static constexpr int TILE_BYTES = KT * D * 2, Q_PART = 128 * D * 2, Q_BYTES = (KEYS ? 1 : 2) * PARTS * Q_PART;
-    static constexpr int STAGES_FIT = ((227 - 3) * 1024 - Q_BYTES) / TILE_BYTES, STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
+    static constexpr int STAGES_FIT = ((227 - 3) * 1024 - Q_BYTES) / TILE_BYTES, STAGES = CODES ? (D == 64 ? 6 : (KEYS ? 4 : 3)) : (STAGES_FIT > 8 ? 8 : STAGES_FIT);
+    // Codes: tiles whose scales are held. A tile's are written once its keys have landed, where the slot's tile before has been used: of three slots that is the values two
+    // tiles back, of six at most the ones five back.
+    static constexpr int SCALE_TILES = !CODES ? 1 : (STAGES == 3 ? 2 : 8);
+    static constexpr int LANDED_BYTES = CODES ? TILE_BYTES / 2 : TILE_BYTES;
     static constexpr int BLOCK = KEYS ? 128 : 256;                // rows
     static constexpr int UNIT = KEYS ? 2 * KT : KT;               // keys
     static constexpr int T_COL = 2 * KT, LO_COL = T_COL + 2 * D;  // tensor memory: scores (then weights), tile sums, bf16's third parts
-    static_assert(STAGES >= (KEYS ? 4 : 3), "ring");
+    static_assert(STAGES >= (KEYS ? 4 : 3) && STAGES <= STAGES_FIT, "ring");
     static_assert(LO_COL + (PARTS == 3 ? KT : 0) <= 512, "tensor memory");
 };
 
@@ -150,6 +157,8 @@ template <typename F> struct Shared {
     uint32_t tmem_slot;
     float factors[2][F::KEYS && F::PARTS == 2 ? 128 : 1];  // keys form over f16: of the rows' scores, the items in turn
     float joint[2][F::KEYS ? 128 : 1];  // keys form: the second pipe's base and sum of each row
+    alignas(16) float scales[F::SCALE_TILES][2][F::CODES ? F::KT : 1];  // codes: of a tile's keys, of its values
+    int level[F::SCALE_TILES];                                            // codes: the largest exponent of its values' scales, or kUneven
 };
 
 __device__ __forceinline__ bool finite16(uint32_t v, int type) { const uint32_t e = type == RQ_KV_F16 ? 0x7c00u : 0x7f80u; return (v & e) != e; }
@@ -164,7 +173,7 @@ __device__ __forceinline__ uint32_t max_pairs(uint32_t a, uint32_t b) { uint32_t
 // The rows of a warp's share, each brought to one size by its own largest element; returns what that of the lane's row was raised by. A call of its own: in line, it
 // takes registers from the softmax around it (a prompt of 3001 tokens, windows of 1000, 259 us in place of 247).
 template <int D, int TYPE, bool KEYS> __device__ __noinline__ int rescale_queries(const AttentionParams& p, int64_t mine, uint8_t* to, int first) {
-    using F = Form<D, TYPE, KEYS>;
+    using F = Form<D, TYPE, KEYS, false>;
     constexpr int SHARE = 128 / D, ROWS = KEYS ? 16 : 32, BATCH = 4;
     const int lane = threadIdx.x & 31, e = 4 * (lane % (D / 4));
     int raise = 0;
@@ -206,7 +215,7 @@ template <int D, int TYPE, bool KEYS> __device__ __noinline__ int rescale_querie
 // to be 2 or more, and finite, as an f16 number. Where it is not, the warp's rows are taken once more. (Every row by its own largest element at once made a block's
 // take-up 1.7 us longer: 32 prompts of 128 tokens 71 us in place of 68. Queries a thousandth of the usual size: 88 us, and the four prompts 402 in place of 356.)
 template <int D, int TYPE, bool KEYS> __device__ __forceinline__ float load_queries(const AttentionParams& p, const Item& it, uint8_t* to, int block_row, int first, int group) {
-    using F = Form<D, TYPE, KEYS>;
+    using F = Form<D, TYPE, KEYS, false>;
     constexpr int SHARE = 128 / D, ROWS = KEYS ? 16 : 32, BATCH = ROWS / SHARE < 8 ? ROWS / SHARE : 8;  // rows an access; rows a warp; accesses at a time
     const int lane = threadIdx.x & 31, own = block_row + first + (lane & (ROWS - 1)), at = it.row0 + own, e = 4 * (lane % (D / 4));
     const int64_t mine = own < it.rows ? (int64_t)(it.start + at / group) * p.q_stride + (int64_t)(it.kv * group + at % group) * D : -1;
@@ -266,9 +275,9 @@ template <int D, int TYPE, bool KEYS> __device__ __forceinline__ float load_quer
     return factor_of(p.scale, raise);
 }
 
-template <int D, int TYPE, bool KEYS>
+template <int D, int TYPE, bool KEYS, bool CODES>
 __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
-    using F = Form<D, TYPE, KEYS>;
+    using F = Form<D, TYPE, KEYS, CODES>;
     constexpr int PARTS = F::PARTS, KT = F::KT, STAGES = F::STAGES;
     extern __shared__ __align__(1024) unsigned char dynamic[];
     uint8_t* const smem = dynamic;  // (there is no other shared memory in front of it)
@@ -279,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
     const int group = p.q_heads / p.kv_heads;
 
     if (tid == 0) {
-        for (int i = 0; i < STAGES; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); mbar_init(&sh.landed[i], 1); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&sh.full[i], CODES ? 2 : 1); mbar_init(&sh.empty[i], 1); mbar_init(&sh.landed[i], 1); }
         for (int i = 0; i < kItems; ++i) { mbar_init(&sh.item_full[i], 1); mbar_init(&sh.item_empty[i], kSoftmaxWarps + 3); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], KEYS ? 8 : 4);
@@ -370,6 +379,80 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
         return key0 < every_low || key0 + KT > every_high;
     };
 
+    auto prefetch = [&](const Item& of) {
+        for (int row = lane; row < of.rows; row += 32) {
+            const int at = of.row0 + row;
+            const char* q = (const char*)(p.q + (int64_t)(of.start + at / group) * p.q_stride + (int64_t)(of.kv * group + at % group) * D);
+#pragma unroll
+            for (int line = 0; line < D * 4; line += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + line));
+        }
+    };
+    // Codes: two warps bring each tile from where it landed to what the tensor core reads, half its pieces each, and the scales of its keys (half 0) and values (1) beside it.
+    // Sixteen lines of 64 codes, 1024 bytes, landed in the upper half of the 2048 bytes that their f16 numbers take (pages of eight: eight lines, 512 in 1024): a warp has read them
+    // all before it writes. 16 codes a lane are one load, a permute and a subtraction for two codes, and two stores, none of which meets a bank twice.
+    auto widen = [&](int half) {
+        Ring at(STAGES);
+        uint32_t key_tiles = 0;
+        while (const Item* it = next_item()) {
+            const int tiles = it->take * (KEYS ? 2 : 1);
+            const int32_t* table = p.block_table + (int64_t)it->r * p.table_stride;
+            for (int n = 0; n < 2 * tiles; ++n, at.next()) {
+                const bool values = is_values(n, tiles);
+                const int key0 = it->first_key + tile_of(n, tiles) * KT, slot = at.slot;
+                float scale[KT / 32];
+                if (!values) {  // (on their way while the tile is)
+#pragma unroll
+                    for (int i = 0; i < KT / 32; ++i) {
+                        const int key = key0 + 32 * i + lane;
+                        const int64_t page = key >= it->low && key < it->high ? __ldcg(table + (key >> p.page_shift)) : -1;
+                        scale[i] = page >= 0 && page < p.pages ? __ldcg((half ? p.v_scale : p.k_scale) + page * p.scale_page + it->kv * p.scale_head + (key & ((1 << p.page_shift) - 1)) * p.scale_line) : 0.0f;
+                    }
+                }
+                if (!mbar_wait_warp(&sh.landed[slot], at.phase, p.wait_ns, dead)) atomicExch(p.error_flag, 54);
+                if (dead) break;  // (the tile may be on its way: it is not touched, and not handed on)
+                uint8_t* const tile = ring + slot * F::TILE_BYTES;
+                constexpr int BLOCKS = KT / 16 * (D / 64);
+#pragma unroll 2
+                for (int b = half; b < BLOCKS; b += 2) {
+                    uint8_t* const to = tile + b * 2048;
+                    uint4 raw[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        raw[i] = *(const uint4*)(to + (p.page_shift == 3 ? 512 * (2 * i + 1) : 1024 + 512 * i) + 16 * lane);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int line = 8 * i + (lane >> 2);
+                        const uint32_t x = turn_codes(raw[i].x), y = turn_codes(raw[i].y), z = turn_codes(raw[i].z), w = turn_codes(raw[i].w);
+                        *(uint4*)(to + swizzled(line, 2 * (lane & 3))) = make_uint4(widen_codes<0, 1>(x), widen_codes<2, 3>(x), widen_codes<0, 1>(y), widen_codes<2, 3>(y));
+                        *(uint4*)(to + swizzled(line, 2 * (lane & 3) + 1)) = make_uint4(widen_codes<0, 1>(z), widen_codes<2, 3>(z), widen_codes<0, 1>(w), widen_codes<2, 3>(w));
+                    }
+                }
+                if (!values) {
+                    const int place = key_tiles++ % F::SCALE_TILES;
+                    int most = 0, least = 254;
+#pragma unroll
+                    for (int i = 0; i < KT / 32; ++i) {
+                        sh.scales[place][half][32 * i + lane] = scale[i];
+                        const int e = (int)(__float_as_uint(scale[i]) >> 23 & 0xff);
+                        most = max(most, e);
+                        least = min(least, scale[i] == 0.0f ? 254 : e);  // (a value of zero takes no weight's bits)
+                    }
+                    most = __reduce_max_sync(0xffffffffu, most);
+                    least = __reduce_min_sync(0xffffffffu, least);
+                    if (half && lane == 0) sh.level[place] = most == 255 || most - least > kEven ? kUneven : min(max(most, 127 - 80), 127 + 90) - 127;
+                }
+                fence_to_tensor_core();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.full[slot]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.item_empty[item_at.slot]);
+            item_at.next();
+        }
+    };
+
     if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------ softmax: a thread a row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -450,21 +533,24 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     fence_before();
                     __syncwarp();
                     // (the loading warp took what is not finite out of the tile)
-                    if (*(volatile uint32_t*)&sh.odd[(keys_before + (KEYS ? 2 * (j - 1) + pipe : j - 1)) % kWords]) add_odd(key0 - kStep);
+                    if (!CODES && *(volatile uint32_t*)&sh.odd[(keys_before + (KEYS ? 2 * (j - 1) + pipe : j - 1)) % kWords]) add_odd(key0 - kStep);
                     if (j == tiles) break;
                     if (lane == 0) mbar_arrive(&sh.t_empty[pipe]);
                 }
                 if (!mbar_wait_warp(&sh.s_full[pipe], tiles_done & 1, p.wait_ns, dead)) atomicExch(p.error_flag, 42);
                 fence_after();
                 const uint32_t there = *(volatile uint32_t*)&sh.pages_there[(keys_before + (KEYS ? 2 * j + pipe : j)) % kWords];
-                const bool all = key0 >= low && key0 + KT <= high && there == 0xffffffffu;
+                const int place = (keys_before + (KEYS ? 2 * j + pipe : j)) % F::SCALE_TILES;
+                const float *of_keys = sh.scales[place][0], *of_values = sh.scales[place][1];
+                const int level = CODES ? *(volatile int*)&sh.level[place] : 0;
+                const bool all = key0 >= low && key0 + KT <= high && there == 0xffffffffu && level != kUneven;
                 // the columns of 32 keys that this row sees
                 auto shown = [&](int c) -> uint32_t {
                     const int from = key0 + 32 * c, a = min(max(high - from, 0), 32), b = min(max(low - from, 0), 32);
                     uint32_t on = (a == 32 ? 0xffffffffu : (1u << a) - 1) & ~(b == 32 ? 0xffffffffu : (1u << b) - 1);
                     if (there != 0xffffffffu)
                         for (int i = 0; i < 32; ++i)
-                            if (!(there >> ((from - key0 + i) >> p.page_shift) & 1)) on &= ~(1u << i);
+                            if (!(there >> ((from - key0 + i) >> (CODES ? min(p.page_shift, kCodesShift) : p.page_shift)) & 1)) on &= ~(1u << i);
                     return on;
                 };
                 float f;
@@ -483,10 +569,21 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                         uint32_t s[32];
                         tmem_ld32(scores + 32 * c, s);
                         tmem_ld_wait(s);
+                        if (CODES) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 k = *(const float4*)(of_keys + 32 * c + i);
+                                const Pair a = pair_mul(pair_of(s[i], s[i + 1]), pair_of(k.x, k.y)), b = pair_mul(pair_of(s[i + 2], s[i + 3]), pair_of(k.z, k.w));
+                                s[i] = __float_as_uint(pair_at(a, 0)); s[i + 1] = __float_as_uint(pair_at(a, 1)); s[i + 2] = __float_as_uint(pair_at(b, 0)); s[i + 3] = __float_as_uint(pair_at(b, 1));
+                            }
+                        }
                         if (kMasked) {
                             const uint32_t on = shown(c);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[i] = on >> i & 1 ? s[i] : 0xff800000u;
+                            for (int i = 0; i < 32; ++i) {
+                                s[i] = on >> i & 1 ? s[i] : 0xff800000u;
+                                if (CODES) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), factor, exponent_of(of_values[32 * c + i])));  // (the scale's exponent counts)
+                            }
                         }
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
@@ -494,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                             top2 = fmaxf(fmaxf(top2, __uint_as_float(s[i + 2])), __uint_as_float(s[i + 3]));
                         }
                     }
-                    top = fmaxf(base, fmaf(fmaxf(top, top2), factor, -kRaise<TYPE>));
+                    top = CODES && kMasked ? fmaxf(base, fmaxf(top, top2) - kRaise<TYPE>) : fmaxf(base, fmaf(fmaxf(top, top2), factor, (float)level - kRaise<TYPE>));
                     const float from = top == -INFINITY ? 0.0f : top;
                     f = exp2_fast(base - from);
                     base = top;
@@ -509,14 +606,31 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                         uint32_t hi[16], mid[16], lo[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
+                            if (CODES) {
+                                const float2 k = *(const float2*)(of_keys + 32 * c + 2 * i);
+                                const Pair scaled = pair_mul(pair_of(s[2 * i], s[2 * i + 1]), pair_of(k.x, k.y));
+                                s[2 * i] = __float_as_uint(pair_at(scaled, 0));
+                                s[2 * i + 1] = __float_as_uint(pair_at(scaled, 1));
+                            }
                             if (kMasked) {
                                 s[2 * i] = on >> (2 * i) & 1 ? s[2 * i] : 0xff800000u;
                                 s[2 * i + 1] = on >> (2 * i + 1) & 1 ? s[2 * i + 1] : 0xff800000u;
                             }
                             const Pair x = pair_fma(pair_of(s[2 * i], s[2 * i + 1]), factors, down);
-                            const float a = exp2_fast(pair_at(x, 0)), b = exp2_fast(pair_at(x, 1));
+                            float a = exp2_fast(pair_at(x, 0)), b = exp2_fast(pair_at(x, 1));
                             Pair v = pair_of(a, b);
                             add[i & 1] = pair_add(add[i & 1], v);
+                            if (CODES) {
+                                const float2 scale = *(const float2*)(of_values + 32 * c + 2 * i);
+                                v = pair_mul(v, pair_of(scale.x, scale.y));
+                                a = pair_at(v, 0);
+                                b = pair_at(v, 1);
+                                if (kMasked) {  // (a scale that the row does not see may be infinite, and 0 * inf is no 0)
+                                    a = on >> (2 * i) & 1 ? a : 0.0f;
+                                    b = on >> (2 * i + 1) & 1 ? b : 0.0f;
+                                    v = pair_of(a, b);
+                                }
+                            }
                             hi[i] = rqattn::pair_of<TYPE>(a, b);
                             v = pair_fma(pair_of(to_float<TYPE>((uint16_t)hi[i]), to_float<TYPE>((uint16_t)(hi[i] >> 16))), minus, v);
                             mid[i] = rqattn::pair_of<TYPE>(pair_at(v, 0), pair_at(v, 1));
@@ -654,7 +768,10 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     }
-    if (warp == kIssuer) {
+    if (CODES && (warp == kFetcher || warp == kMender)) {
+        // ------------------------------------------------------------ the widening warps
+        widen(warp == kMender);
+    } else if (warp == kIssuer) {
         // ------------------------------------------------------------ the issuing warp
         Ring at(STAGES);
         uint32_t sums[2] = {0, 0}, item_count = 0;
@@ -756,14 +873,9 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
         release(&sh.ended);
         if (!arrived(&sh.ended, 0)) atomicExch(p.error_flag, 49);
     } else if (warp == kFetcher) {
-        // ------------------------------------------------------------ the items' queries, into L2 ahead of their use
+        // ------------------------------------------------------------ the items' queries, into L2 ahead of their use (codes: by the loading warp)
         while (const Item* it = next_item()) {
-            for (int row = lane; row < it->rows; row += 32) {
-                const int at = it->row0 + row;
-                const char* q = (const char*)(p.q + (int64_t)(it->start + at / group) * p.q_stride + (int64_t)(it->kv * group + at % group) * D);
-#pragma unroll
-                for (int line = 0; line < D * 4; line += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + line));
-            }
+            prefetch(*it);
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.item_empty[item_at.slot]);
             item_at.next();
@@ -848,7 +960,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
             item_at.next();
             return i;
         };
-        const int box_shift = min(p.page_shift, KT == 128 ? 7 : 6), boxes = KT >> box_shift;  // a copy brings 64 elements of a page, or of a tile
+        const int box_shift = min(p.page_shift, CODES ? kCodesShift : (KT == 128 ? 7 : 6)), boxes = KT >> box_shift;  // a copy brings 64 elements of a page, or of a tile
         const int box = lane & (boxes - 1), column = lane / boxes;                               // this lane's copy
         Ring at(STAGES);
         uint32_t key_tiles = 0, value_tiles = 0;
@@ -887,19 +999,22 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     ++value_tiles;
                 }
                 uint64_t* bar = &sh.full[slot];
-                if (values && is_edge(i, key0)) {  // (to the mending warp first, which hands it on)
+                if (CODES || (values && is_edge(i, key0))) {  // (to the mending or the widening warps first, which hand it on)
                     bar = &sh.landed[slot];
                     landings ^= 1u << slot;
                 }
-                if (lane == 0) mbar_expect_tx(bar, F::TILE_BYTES);
+                if (lane == 0) mbar_expect_tx(bar, F::LANDED_BYTES);
                 __syncwarp();
                 if (column < D / 64) {
-                    const uint32_t to = smem_u32(ring) + slot * F::TILE_BYTES + column * (KT * 128) + box * (128 << box_shift);
+                    const uint32_t to = smem_u32(ring) + slot * F::TILE_BYTES + column * (KT * 128) + box * (128 << box_shift) + (CODES ? 64 << box_shift : 0);
                     tma_load_4d(to, values ? &v_map : &k_map, column * 64, (key0 + (box << box_shift)) & ((1 << p.page_shift) - 1), i.kv, now, bar);
                 }
                 __syncwarp();
                 at.next();
-                if (n == 1) following = deal();  // ahead of its use: its queries are fetched while this one's tiles are
+                if (n == 1) {
+                    following = deal();  // ahead of its use: its queries are fetched while this one's tiles are
+                    if (CODES) prefetch(following);
+                }
             }
         }
         // Every copy has landed before the CTA ends, whoever gave up: the last ones to the mending warp, and the last ones of each slot (a barrier that nothing was
@@ -917,10 +1032,10 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
     if (warp == kIssuer) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-template <int D, int TYPE, bool KEYS>
+template <int D, int TYPE, bool KEYS, bool CODES = false>
 int launch_form(rq_ctx* ctx, const AttentionParams& p, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
-    using F = Form<D, TYPE, KEYS>;
-    auto kernel = rq_attention_tc_kernel<D, TYPE, KEYS>;
+    using F = Form<D, TYPE, KEYS, CODES>;
+    auto kernel = rq_attention_tc_kernel<D, TYPE, KEYS, CODES>;
     constexpr size_t smem = F::Q_BYTES + F::STAGES * F::TILE_BYTES + sizeof(Shared<F>);
     static_assert(smem <= 227 * 1024, "shared memory");
     static bool configured[64] = {};  // by device: the opt-in to large shared memory
@@ -932,15 +1047,18 @@ int launch_form(rq_ctx* ctx, const AttentionParams& p, const CUtensorMap& k, con
     return launch(kernel, dim3((unsigned)ctas), kThreads, smem, s, p, k, v);
 }
 
-// The cache as a TMA reads it: elements, lines, heads, pages; a copy is 64 elements of `lines` lines, swizzled as the tensor core reads them
+// The cache as a TMA reads it: elements, lines, heads, pages; a copy is 64 elements of `lines` lines, swizzled as the tensor core reads them (codes: as they are)
 int make_map(CUtensorMap* map, const void* base, const rq_kv_cache& c, int lines) {
     rq_encode_tiled encode = nullptr;
     const int rc = rq_tensor_map_encoder(&encode);
     if (rc) return rc;
     const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.heads, (cuuint64_t)c.pages};
-    const cuuint64_t strides[3] = {2 * (cuuint64_t)c.line_stride, 2 * (cuuint64_t)(c.heads > 1 ? c.head_stride : 8), 2 * (cuuint64_t)(c.pages > 1 ? c.page_stride : 8)};
+    const bool codes = c.type == RQ_KV_INT8;
+    const cuuint64_t bytes = codes ? 1 : 2;
+    const cuuint64_t strides[3] = {bytes * (cuuint64_t)c.line_stride, c.heads > 1 ? bytes * (cuuint64_t)c.head_stride : 16, c.pages > 1 ? bytes * (cuuint64_t)c.page_stride : 16};
     const cuuint32_t box[4] = {64, (cuuint32_t)lines, 1, 1}, step[4] = {1, 1, 1, 1};
-    const CUresult e = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, (void*)base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const CUresult e = encode(map, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, (void*)base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (e != CUDA_SUCCESS) return rq_fail(RQ_ERR_CUDA, "rq_attention: cuTensorMapEncodeTiled failed with %d", (int)e);
     return RQ_OK;
@@ -949,14 +1067,17 @@ int make_map(CUtensorMap* map, const void* base, const rq_kv_cache& c, int lines
 }  // namespace
 
 int rqattn::launch_tensor(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& c, bool one_tile, cudaStream_t s) {
-    if (c.type == RQ_KV_INT8) return RQ_ERR_UNSUPPORTED;
     // pages of whole groups of eight lines (the swizzle's), and strides that a tensor map can hold
     if (c.head_dim > 128 || c.page_size < 8 || c.line_stride <= 0 || (c.heads > 1 && c.head_stride <= 0) || (c.pages > 1 && c.page_stride <= 0) || c.head_stride >= (int64_t)1 << 38) return RQ_ERR_UNSUPPORTED;
-    const int tile = c.type == RQ_KV_F16 || c.head_dim == 64 ? 128 : 64, lines = c.page_size < tile ? c.page_size : tile;
+    const int tile = c.type == RQ_KV_INT8 ? 1 << kCodesShift : (c.type == RQ_KV_F16 || c.head_dim == 64 ? 128 : 64), lines = c.page_size < tile ? c.page_size : tile;
     alignas(64) CUtensorMap k, v;
     int rc = make_map(&k, c.k, c, lines);
     if (!rc) rc = make_map(&v, c.v, c, lines);
     if (rc) return rc;
+    if (c.type == RQ_KV_INT8) {
+        if (c.head_dim == 64) return one_tile ? launch_form<64, RQ_KV_F16, true, true>(ctx, p, k, v, s) : launch_form<64, RQ_KV_F16, false, true>(ctx, p, k, v, s);
+        return one_tile ? launch_form<128, RQ_KV_F16, true, true>(ctx, p, k, v, s) : launch_form<128, RQ_KV_F16, false, true>(ctx, p, k, v, s);
+    }
     if (c.type == RQ_KV_BF16) return c.head_dim == 64 ? launch_form<64, RQ_KV_BF16, true>(ctx, p, k, v, s) : launch_form<128, RQ_KV_BF16, true>(ctx, p, k, v, s);
     if (c.head_dim == 64) return one_tile ? launch_form<64, RQ_KV_F16, true>(ctx, p, k, v, s) : launch_form<64, RQ_KV_F16, false>(ctx, p, k, v, s);
     return one_tile ? launch_form<128, RQ_KV_F16, true>(ctx, p, k, v, s) : launch_form<128, RQ_KV_F16, false>(ctx, p, k, v, s);
