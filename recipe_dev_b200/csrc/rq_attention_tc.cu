@@ -41,15 +41,16 @@ using namespace rqmma;
 
 namespace {
 
-constexpr int kSoftmaxWarps = 8, kIssuer = 8, kLoader = 9, kFetcher = 10, kMender = 11, kThreads = 12 * 32;
-constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;                              // 2 * 224 + 56 = 3 * 168, what the block is launched with
+constexpr int kSoftmaxWarps = 8, kIssuer = 8, kLoader = 9, kFetcher = 10, kMender = 11, kWidener = 12;
 constexpr int kCodesShift = 4;  // a copy of codes brings at most sixteen lines
-constexpr int kUneven = 1 << 20, kEven = 12;  // exponents of a tile's scales of values: further apart than kEven, or of one that is no number
+constexpr int kEven = 12;       // exponents of a tile's scales of values that lie no further apart need no look at each
 constexpr int kItems = 4, kWords = 16;  // rings in shared memory: items, words on tiles of keys
 
 // CODES: the cache holds 8-bit codes, TYPE is what they become
 template <int D, int TYPE, bool KEYS_, bool CODES_> struct Form {
     static constexpr bool KEYS = KEYS_, CODES = CODES_;
+    // what the block is launched with is dealt out anew: 2 * 224 + 56 = 3 * 168; 2 * 208 + 2 * 48 = 4 * 128
+    static constexpr int WIDENERS = CODES ? 4 : 0, THREADS = (12 + WIDENERS) * 32, SOFTMAX_REGS = CODES ? 208 : 224, OTHER_REGS = CODES ? 48 : 56;
     static constexpr int PARTS = TYPE == RQ_KV_F16 ? 2 : 3;
     static constexpr int KT = TYPE == RQ_KV_F16 || D == 64 ? 128 : 64;  // keys a tile (bf16, 128 elements: 2 KT + 2 D + KT columns are what tensor memory holds with 64)
     static constexpr int TILE_BYTES = KT * D * 2, Q_PART = 128 * D * 2, Q_BYTES = (KEYS ? 1 : 2) * PARTS * Q_PART;
@@ -149,7 +150,7 @@ __device__ __forceinline__ void fence_to_tensor_core() { asm volatile("fence.pro
 
 template <typename F> struct Shared {
     uint64_t full[F::STAGES], empty[F::STAGES], item_full[kItems], item_empty[kItems], q_full[2], s_full[2], p_full[2][2], t_full[2], t_empty[2], q_empty, landed[F::STAGES], joined[4], ended;
-    int64_t warp_sums[kThreads / 32], range[2];
+    int64_t warp_sums[F::THREADS / 32], range[2];
     int where[4];
     Item items[kItems];
     uint32_t pages_there[kWords];  // a tile's pages that the cache has, a bit each; all ones: all of them
@@ -158,7 +159,7 @@ template <typename F> struct Shared {
     float factors[2][F::KEYS && F::PARTS == 2 ? 128 : 1];  // keys form over f16: of the rows' scores, the items in turn
     float joint[2][F::KEYS ? 128 : 1];  // keys form: the second pipe's base and sum of each row
     alignas(16) float scales[F::SCALE_TILES][2][F::CODES ? F::KT : 1];  // codes: of a tile's keys, of its values
-    int level[F::SCALE_TILES];                                            // codes: the largest exponent of its values' scales, or kUneven
+    int levels[F::SCALE_TILES][2][2];                                     // codes: the largest and the least exponent of the scales of either half of its values
 };
 
 __device__ __forceinline__ bool finite16(uint32_t v, int type) { const uint32_t e = type == RQ_KV_F16 ? 0x7c00u : 0x7f80u; return (v & e) != e; }
@@ -276,7 +277,7 @@ template <int D, int TYPE, bool KEYS> __device__ __forceinline__ float load_quer
 }
 
 template <int D, int TYPE, bool KEYS, bool CODES>
-__global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+__global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_attention_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using F = Form<D, TYPE, KEYS, CODES>;
     constexpr int PARTS = F::PARTS, KT = F::KT, STAGES = F::STAGES;
     extern __shared__ __align__(1024) unsigned char dynamic[];
@@ -288,8 +289,8 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
     const int group = p.q_heads / p.kv_heads;
 
     if (tid == 0) {
-        for (int i = 0; i < STAGES; ++i) { mbar_init(&sh.full[i], CODES ? 2 : 1); mbar_init(&sh.empty[i], 1); mbar_init(&sh.landed[i], 1); }
-        for (int i = 0; i < kItems; ++i) { mbar_init(&sh.item_full[i], 1); mbar_init(&sh.item_empty[i], kSoftmaxWarps + 3); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&sh.full[i], CODES ? F::WIDENERS : 1); mbar_init(&sh.empty[i], 1); mbar_init(&sh.landed[i], 1); }
+        for (int i = 0; i < kItems; ++i) { mbar_init(&sh.item_full[i], 1); mbar_init(&sh.item_empty[i], kSoftmaxWarps + (CODES ? 2 + F::WIDENERS : 3)); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], KEYS ? 8 : 4);
             mbar_init(&sh.s_full[i], 1);
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
         int64_t* const before = (int64_t*)smem;  // (the queries' place and, at most, the ring's first bytes)
         int64_t total = 0;
         if (tid == 0) before[0] = 0;
-        for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
+        for (int r0 = 0; r0 < p.requests; r0 += F::THREADS) {
             const int r = r0 + tid;
             int64_t units = 0;
             if (r < p.requests)
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
             if (lane == 31) sh.warp_sums[warp] = scan;
             __syncthreads();
             scan += total;
-            for (int w = 0; w < kThreads / 32; ++w) { if (w < warp) scan += sh.warp_sums[w]; total += sh.warp_sums[w]; }
+            for (int w = 0; w < F::THREADS / 32; ++w) { if (w < warp) scan += sh.warp_sums[w]; total += sh.warp_sums[w]; }
             if (r < p.requests) before[r + 1] = scan;
         }
         __syncthreads();
@@ -379,51 +380,59 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
         return key0 < every_low || key0 + KT > every_high;
     };
 
-    auto prefetch = [&](const Item& of) {
-        for (int row = lane; row < of.rows; row += 32) {
-            const int at = of.row0 + row;
-            const char* q = (const char*)(p.q + (int64_t)(of.start + at / group) * p.q_stride + (int64_t)(of.kv * group + at % group) * D);
-#pragma unroll
-            for (int line = 0; line < D * 4; line += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + line));
-        }
-    };
-    // Codes: two warps bring each tile from where it landed to what the tensor core reads, half its pieces each, and the scales of its keys (half 0) and values (1) beside it.
-    // Sixteen lines of 64 codes, 1024 bytes, landed in the upper half of the 2048 bytes that their f16 numbers take (pages of eight: eight lines, 512 in 1024): a warp has read them
-    // all before it writes. 16 codes a lane are one load, a permute and a subtraction for two codes, and two stores, none of which meets a bank twice.
-    auto widen = [&](int half) {
+    // Codes: four warps bring each tile from where it landed to what the tensor core reads, every fourth sixteen lines each, and a half each of the scales of its keys (0, 1) and
+    // of its values (2, 3) beside it. Sixteen lines landed in a part of the place that their f16 numbers take (128 elements: where the second 64 go; 64: in the upper half, pages
+    // of eight lines in that of their own): a warp has read them before it writes there. A lane's pieces are 16 codes, one load, two stores, so that no eight lanes meet a
+    // bank twice.
+    auto widen = [&](int which) {
+        constexpr int SHARE = KT / 64, PIECES = D / 32;  // scales, pieces of sixteen lines, of a lane
         Ring at(STAGES);
         uint32_t key_tiles = 0;
         while (const Item* it = next_item()) {
             const int tiles = it->take * (KEYS ? 2 : 1);
-            const int32_t* table = p.block_table + (int64_t)it->r * p.table_stride;
-            for (int n = 0; n < 2 * tiles; ++n, at.next()) {
-                const bool values = is_values(n, tiles);
-                const int key0 = it->first_key + tile_of(n, tiles) * KT, slot = at.slot;
-                float scale[KT / 32];
-                if (!values) {  // (on their way while the tile is)
+            const int32_t* table = p.block_table + (int64_t)it->r * p.table_stride + (it->first_key >> p.page_shift);
+            const float* scales = (which < 2 ? p.k_scale : p.v_scale) + it->kv * p.scale_head;
+            const int first = (which & 1) * (KT / 2) + lane, line0 = it->first_key & ((1 << p.page_shift) - 1), low = it->low - it->first_key, high = it->high - it->first_key;  // keys from the item's first
+            // Scales are on their way while the tile before is widened, and their pages' entries while the one before that is
+            int page[SHARE];
+            float scale[SHARE];
+            auto find = [&](int tile) {
 #pragma unroll
-                    for (int i = 0; i < KT / 32; ++i) {
-                        const int key = key0 + 32 * i + lane;
-                        const int64_t page = key >= it->low && key < it->high ? __ldcg(table + (key >> p.page_shift)) : -1;
-                        scale[i] = page >= 0 && page < p.pages ? __ldcg((half ? p.v_scale : p.k_scale) + page * p.scale_page + it->kv * p.scale_head + (key & ((1 << p.page_shift) - 1)) * p.scale_line) : 0.0f;
-                    }
+                for (int i = 0; i < SHARE; ++i) {
+                    const int key = tile * KT + first + 32 * i;
+                    page[i] = key >= low && key < high ? __ldcg(table + ((line0 + key) >> p.page_shift)) : -1;
                 }
+            };
+            auto load = [&](int tile) {
+#pragma unroll
+                for (int i = 0; i < SHARE; ++i) {
+                    const int line = (line0 + tile * KT + first + 32 * i) & ((1 << p.page_shift) - 1);
+                    scale[i] = page[i] >= 0 && page[i] < p.pages ? __ldcg(scales + page[i] * p.scale_page + line * p.scale_line) : 0.0f;
+                }
+            };
+            find(0);
+            load(0);
+            find(1);
+            for (int n = 0, tile = 0; n < 2 * tiles; ++n, at.next()) {
+                const bool values = is_values(n, tiles);
+                const int slot = at.slot;
                 if (!mbar_wait_warp(&sh.landed[slot], at.phase, p.wait_ns, dead)) atomicExch(p.error_flag, 54);
                 if (dead) break;  // (the tile may be on its way: it is not touched, and not handed on)
-                uint8_t* const tile = ring + slot * F::TILE_BYTES;
-                constexpr int BLOCKS = KT / 16 * (D / 64);
-#pragma unroll 2
-                for (int b = half; b < BLOCKS; b += 2) {
-                    uint8_t* const to = tile + b * 2048;
-                    uint4 raw[2];
+                // (short loops: laid out in a line they cost the softmax its place in the instruction caches, 236 -> 259 us)
+#pragma unroll 1
+                for (int block = which; block < KT / 16; block += F::WIDENERS) {
+                    uint8_t* const out = ring + slot * F::TILE_BYTES + block * 2048;
+                    uint4 raw[PIECES];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        raw[i] = *(const uint4*)(to + (p.page_shift == 3 ? 512 * (2 * i + 1) : 1024 + 512 * i) + 16 * lane);
+                    for (int i = 0; i < PIECES; ++i) {
+                        if (D == 64) raw[i] = *(const uint4*)(out + (p.page_shift == 3 ? 512 * (2 * i + 1) : 1024 + 512 * i) + 16 * lane);
+                        else raw[i] = *(const uint4*)(out + KT * 128 + (8 * (i >> 1) + (lane >> 2)) * 128 + ((i & 1) ^ (lane >> 2 & 1)) * 64 + (lane & 3) * 16);
                     }
                     __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int line = 8 * i + (lane >> 2);
+                    for (int i = 0; i < PIECES; ++i) {
+                        const int line = 8 * (D == 64 ? i : i >> 1) + (lane >> 2);
+                        uint8_t* const to = out + (D == 64 ? 0 : (i & 1) ^ (lane >> 2 & 1)) * (KT * 128);
                         const uint32_t x = turn_codes(raw[i].x), y = turn_codes(raw[i].y), z = turn_codes(raw[i].z), w = turn_codes(raw[i].w);
                         *(uint4*)(to + swizzled(line, 2 * (lane & 3))) = make_uint4(widen_codes<0, 1>(x), widen_codes<2, 3>(x), widen_codes<0, 1>(y), widen_codes<2, 3>(y));
                         *(uint4*)(to + swizzled(line, 2 * (lane & 3) + 1)) = make_uint4(widen_codes<0, 1>(z), widen_codes<2, 3>(z), widen_codes<0, 1>(w), widen_codes<2, 3>(w));
@@ -433,19 +442,23 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     const int place = key_tiles++ % F::SCALE_TILES;
                     int most = 0, least = 254;
 #pragma unroll
-                    for (int i = 0; i < KT / 32; ++i) {
-                        sh.scales[place][half][32 * i + lane] = scale[i];
+                    for (int i = 0; i < SHARE; ++i) {
+                        sh.scales[place][which >> 1][first + 32 * i] = scale[i];
                         const int e = (int)(__float_as_uint(scale[i]) >> 23 & 0xff);
                         most = max(most, e);
                         least = min(least, scale[i] == 0.0f ? 254 : e);  // (a value of zero takes no weight's bits)
                     }
                     most = __reduce_max_sync(0xffffffffu, most);
                     least = __reduce_min_sync(0xffffffffu, least);
-                    if (half && lane == 0) sh.level[place] = most == 255 || most - least > kEven ? kUneven : min(max(most, 127 - 80), 127 + 90) - 127;
+                    if (which >= 2 && lane == 0) { sh.levels[place][which & 1][0] = most; sh.levels[place][which & 1][1] = least; }
                 }
                 fence_to_tensor_core();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.full[slot]);
+                if (!values) {
+                    load(++tile);
+                    find(tile + 1);
+                }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.item_empty[item_at.slot]);
@@ -455,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
 
     if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------ softmax: a thread a row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::SOFTMAX_REGS));
         const int pipe = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t rows_at = tmem + ((uint32_t)(quarter * 32) << 16), scores = rows_at + pipe * KT, sums_at = rows_at + F::T_COL + pipe * D, lo_at = rows_at + F::LO_COL + pipe * (KT / 2);
         const int in_block = KEYS ? row : pipe * 128 + row;
@@ -542,8 +555,17 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                 const uint32_t there = *(volatile uint32_t*)&sh.pages_there[(keys_before + (KEYS ? 2 * j + pipe : j)) % kWords];
                 const int place = (keys_before + (KEYS ? 2 * j + pipe : j)) % F::SCALE_TILES;
                 const float *of_keys = sh.scales[place][0], *of_values = sh.scales[place][1];
-                const int level = CODES ? *(volatile int*)&sh.level[place] : 0;
-                const bool all = key0 >= low && key0 + KT <= high && there == 0xffffffffu && level != kUneven;
+                // (the exponent that counts for the tile: the largest, where they lie close together)
+                int level = 0;
+                bool even = true;
+                if (CODES) {
+                    const volatile int* l = &sh.levels[place][0][0];
+                    const int most = max(l[0], l[2]);
+                    even = most < 255 && most - min(l[1], l[3]) <= kEven;
+                    level = min(max(most, 127 - 80), 127 + 90) - 127;
+                }
+                // (codes: rows past the block's last, whose results nobody reads, hide nothing)
+                const bool all = (key0 >= low && key0 + KT <= high && there == 0xffffffffu) || (CODES && in_block >= it->rows);
                 // the columns of 32 keys that this row sees
                 auto shown = [&](int c) -> uint32_t {
                     const int from = key0 + 32 * c, a = min(max(high - from, 0), 32), b = min(max(low - from, 0), 32);
@@ -561,8 +583,8 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     if (lane == 0) mbar_arrive(&sh.p_full[pipe][half]);
                 };
                 // The loops over columns are loops: laid out in a line, with the masks, they were longer than the instruction caches are.
-                auto tile = [&](auto masked) {
-                    constexpr bool kMasked = decltype(masked)::value;
+                auto tile = [&](auto masked, auto uneven) {
+                    constexpr bool kMasked = decltype(masked)::value, kUneven = decltype(uneven)::value;
                     float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll 1
                     for (int c = 0; c < KT / 32; ++c) {
@@ -582,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
                                 s[i] = on >> i & 1 ? s[i] : 0xff800000u;
-                                if (CODES) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), factor, exponent_of(of_values[32 * c + i])));  // (the scale's exponent counts)
+                                if (kUneven) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), factor, exponent_of(of_values[32 * c + i])));  // (each scale's exponent counts)
                             }
                         }
 #pragma unroll
@@ -591,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                             top2 = fmaxf(fmaxf(top2, __uint_as_float(s[i + 2])), __uint_as_float(s[i + 3]));
                         }
                     }
-                    top = CODES && kMasked ? fmaxf(base, fmaxf(top, top2) - kRaise<TYPE>) : fmaxf(base, fmaf(fmaxf(top, top2), factor, (float)level - kRaise<TYPE>));
+                    top = kUneven ? fmaxf(base, fmaxf(top, top2) - kRaise<TYPE>) : fmaxf(base, fmaf(fmaxf(top, top2), factor, (float)level - kRaise<TYPE>));
                     const float from = top == -INFINITY ? 0.0f : top;
                     f = exp2_fast(base - from);
                     base = top;
@@ -604,11 +626,15 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                         tmem_ld_wait(s);
                         const uint32_t on = kMasked ? shown(c) : 0;
                         uint32_t hi[16], mid[16], lo[16];
+                        float4 two_keys, two_values;  // the scales of two pairs
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             if (CODES) {
-                                const float2 k = *(const float2*)(of_keys + 32 * c + 2 * i);
-                                const Pair scaled = pair_mul(pair_of(s[2 * i], s[2 * i + 1]), pair_of(k.x, k.y));
+                                if (!(i & 1)) {
+                                    two_keys = *(const float4*)(of_keys + 32 * c + 2 * i);
+                                    two_values = *(const float4*)(of_values + 32 * c + 2 * i);
+                                }
+                                const Pair scaled = pair_mul(pair_of(s[2 * i], s[2 * i + 1]), i & 1 ? pair_of(two_keys.z, two_keys.w) : pair_of(two_keys.x, two_keys.y));
                                 s[2 * i] = __float_as_uint(pair_at(scaled, 0));
                                 s[2 * i + 1] = __float_as_uint(pair_at(scaled, 1));
                             }
@@ -621,11 +647,10 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                             Pair v = pair_of(a, b);
                             add[i & 1] = pair_add(add[i & 1], v);
                             if (CODES) {
-                                const float2 scale = *(const float2*)(of_values + 32 * c + 2 * i);
-                                v = pair_mul(v, pair_of(scale.x, scale.y));
+                                v = pair_mul(v, i & 1 ? pair_of(two_values.z, two_values.w) : pair_of(two_values.x, two_values.y));
                                 a = pair_at(v, 0);
                                 b = pair_at(v, 1);
-                                if (kMasked) {  // (a scale that the row does not see may be infinite, and 0 * inf is no 0)
+                                if (kUneven) {  // (a scale that the row does not see may be infinite, and 0 * inf is no 0)
                                     a = on >> (2 * i) & 1 ? a : 0.0f;
                                     b = on >> (2 * i + 1) & 1 ? b : 0.0f;
                                     v = pair_of(a, b);
@@ -647,8 +672,9 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                     add[0] = pair_add(add[0], add[1]);
                     sum = fmaf(sum, f, pair_at(add[0], 0) + pair_at(add[0], 1));
                 };
-                if (__all_sync(0xffffffffu, all)) tile(std::false_type());
-                else tile(std::true_type());
+                if (CODES && !even) tile(std::true_type(), std::bool_constant<CODES>());
+                else if (__all_sync(0xffffffffu, all)) tile(std::false_type(), std::false_type());
+                else tile(std::true_type(), std::false_type());
                 weights_there(1);
                 // behind the last scores the queries' place is free: the next item's, before this one's sums are finished
                 if (j + 1 == tiles) {
@@ -766,11 +792,11 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
             ++items_done;
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::OTHER_REGS));
     }
-    if (CODES && (warp == kFetcher || warp == kMender)) {
-        // ------------------------------------------------------------ the widening warps
-        widen(warp == kMender);
+    if (CODES && warp >= kMender) {
+        // ------------------------------------------------------------ the widening warps (nothing is mended: a code is a number)
+        if (warp >= kWidener) widen(warp - kWidener);
     } else if (warp == kIssuer) {
         // ------------------------------------------------------------ the issuing warp
         Ring at(STAGES);
@@ -873,9 +899,14 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
         release(&sh.ended);
         if (!arrived(&sh.ended, 0)) atomicExch(p.error_flag, 49);
     } else if (warp == kFetcher) {
-        // ------------------------------------------------------------ the items' queries, into L2 ahead of their use (codes: by the loading warp)
+        // ------------------------------------------------------------ the items' queries, into L2 ahead of their use
         while (const Item* it = next_item()) {
-            prefetch(*it);
+            for (int row = lane; row < it->rows; row += 32) {
+                const int at = it->row0 + row;
+                const char* q = (const char*)(p.q + (int64_t)(it->start + at / group) * p.q_stride + (int64_t)(it->kv * group + at % group) * D);
+#pragma unroll
+                for (int line = 0; line < D * 4; line += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + line));
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.item_empty[item_at.slot]);
             item_at.next();
@@ -1005,16 +1036,23 @@ __global__ void __launch_bounds__(kThreads, 1) rq_attention_tc_kernel(const __gr
                 }
                 if (lane == 0) mbar_expect_tx(bar, F::LANDED_BYTES);
                 __syncwarp();
-                if (column < D / 64) {
-                    const uint32_t to = smem_u32(ring) + slot * F::TILE_BYTES + column * (KT * 128) + box * (128 << box_shift) + (CODES ? 64 << box_shift : 0);
-                    tma_load_4d(to, values ? &v_map : &k_map, column * 64, (key0 + (box << box_shift)) & ((1 << p.page_shift) - 1), i.kv, now, bar);
+                auto copy = [&](int column, int box, int page_at) {
+                    const uint32_t to = smem_u32(ring) + slot * F::TILE_BYTES + column * (KT * 128) + box * (128 << box_shift) + (CODES && D == 64 ? 64 << box_shift : 0);
+                    tma_load_4d(to, values ? &v_map : &k_map, CODES ? 0 : column * 64, (key0 + (box << box_shift)) & ((1 << p.page_shift) - 1), i.kv, page_at, bar);
+                };
+                if (CODES) {  // one lane after another costs 170 cycles a copy, one lane for all 40
+#pragma unroll 1
+                    for (int b = 0; b < boxes; ++b) {
+                        const int page_at = __shfl_sync(0xffffffffu, now, b);
+                        if (elect_one()) copy(D / 64 - 1, b, page_at);
+                        __syncwarp();
+                    }
+                } else if (column < D / 64) {
+                    copy(column, box, now);
                 }
                 __syncwarp();
                 at.next();
-                if (n == 1) {
-                    following = deal();  // ahead of its use: its queries are fetched while this one's tiles are
-                    if (CODES) prefetch(following);
-                }
+                if (n == 1) following = deal();  // ahead of its use: its queries are fetched while this one's tiles are
             }
         }
         // Every copy has landed before the CTA ends, whoever gave up: the last ones to the mending warp, and the last ones of each slot (a barrier that nothing was
@@ -1044,10 +1082,10 @@ int launch_form(rq_ctx* ctx, const AttentionParams& p, const CUtensorMap& k, con
         if (ctx->device < 64) configured[ctx->device] = true;
     }
     const int ctas = ctx->sm_count < kTensorCtas ? ctx->sm_count : kTensorCtas;
-    return launch(kernel, dim3((unsigned)ctas), kThreads, smem, s, p, k, v);
+    return launch(kernel, dim3((unsigned)ctas), F::THREADS, smem, s, p, k, v);
 }
 
-// The cache as a TMA reads it: elements, lines, heads, pages; a copy is 64 elements of `lines` lines, swizzled as the tensor core reads them (codes: as they are)
+// The cache as a TMA reads it: elements, lines, heads, pages; a copy is 64 elements of `lines` lines, swizzled as the tensor core reads them (codes: whole lines, as they are)
 int make_map(CUtensorMap* map, const void* base, const rq_kv_cache& c, int lines) {
     rq_encode_tiled encode = nullptr;
     const int rc = rq_tensor_map_encoder(&encode);
@@ -1056,7 +1094,7 @@ int make_map(CUtensorMap* map, const void* base, const rq_kv_cache& c, int lines
     const bool codes = c.type == RQ_KV_INT8;
     const cuuint64_t bytes = codes ? 1 : 2;
     const cuuint64_t strides[3] = {bytes * (cuuint64_t)c.line_stride, c.heads > 1 ? bytes * (cuuint64_t)c.head_stride : 16, c.pages > 1 ? bytes * (cuuint64_t)c.page_stride : 16};
-    const cuuint32_t box[4] = {64, (cuuint32_t)lines, 1, 1}, step[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {codes ? (cuuint32_t)c.head_dim : 64, (cuuint32_t)lines, 1, 1}, step[4] = {1, 1, 1, 1};
     const CUresult e = encode(map, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, (void*)base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
