@@ -1036,19 +1036,9 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
                 }
                 if (lane == 0) mbar_expect_tx(bar, F::LANDED_BYTES);
                 __syncwarp();
-                auto copy = [&](int column, int box, int page_at) {
-                    const uint32_t to = smem_u32(ring) + slot * F::TILE_BYTES + column * (KT * 128) + box * (128 << box_shift) + (CODES && D == 64 ? 64 << box_shift : 0);
-                    tma_load_4d(to, values ? &v_map : &k_map, CODES ? 0 : column * 64, (key0 + (box << box_shift)) & ((1 << p.page_shift) - 1), i.kv, page_at, bar);
-                };
-                if (CODES) {  // one lane after another costs 170 cycles a copy, one lane for all 40
-#pragma unroll 1
-                    for (int b = 0; b < boxes; ++b) {
-                        const int page_at = __shfl_sync(0xffffffffu, now, b);
-                        if (elect_one()) copy(D / 64 - 1, b, page_at);
-                        __syncwarp();
-                    }
-                } else if (column < D / 64) {
-                    copy(column, box, now);
+                if (column < (CODES ? 1 : D / 64)) {
+                    const uint32_t to = smem_u32(ring) + slot * F::TILE_BYTES + (CODES ? D / 64 - 1 : column) * (KT * 128) + box * (128 << box_shift) + (CODES && D == 64 ? 64 << box_shift : 0);
+                    tma_load_4d(to, values ? &v_map : &k_map, column * 64, (key0 + (box << box_shift)) & ((1 << p.page_shift) - 1), i.kv, now, bar);
                 }
                 __syncwarp();
                 at.next();
