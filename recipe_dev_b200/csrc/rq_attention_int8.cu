@@ -2,14 +2,17 @@
 //
 //   y = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q . k_j - m),  k_j = sk_j ck_j,  v_j = sv_j cv_j
 //
-// The form of rq_attention.cu's kernel: a warp takes its keys through a ring of its own in shared memory, queries and weights are taken apart into hi + lo f16 parts, one
-// mma.sync does both, sums are added up in fp32. What differs, since a tile is half the bytes and the codes are no operands yet:
-//   * Codes become f16 numbers on their way from shared memory into operand registers, exactly (a byte permute and a subtraction a pair). Scores are multiplied by sk, weights
-//     by sv before they are taken apart, both in fp32: nothing is rounded that the 16-bit caches' kernel would not round.
-//   * The elements of a product's sixteen may be any, if the queries' are the same: a thread's operands of four steps are sixteen neighbouring codes of a key, one 16-byte load.
-//     For the values a transposing matrix load moves pairs of neighbouring elements: the even ones make one column of the product, the odd ones the next.
+// The form of rq_attention.cu's kernel: a warp takes its keys through a ring of its own in shared memory, queries and weights are taken apart into parts that mma.sync takes,
+// sums are added up in fp32. What differs, since a tile is half the bytes:
+//   * Scores are products of bytes: a query is a whole number of 32 bits (of its row's step, a power of two), four digits of eight bits; the sixteen rows of an operand are eight
+//     rows' first digits above their second ones, or third above fourth. Sums are exact, and joined and multiplied by factor and key's scale in fp32.
+//   * The elements of a product's thirty-two may be any, if the queries' are the same: a thread's operands of two steps are sixteen neighbouring codes of a key, one 16-byte load.
+//   * Values become f16 numbers on their way into operand registers, exactly (a byte permute and a subtraction a pair), weights times their scales hi + lo f16 parts. A transposing
+//     matrix load moves pairs of neighbouring elements: the even ones make one column of the product, the odd ones the next.
 //   * A warp's tile is 32 keys (16 for heads of 256): the same bytes on their way as there, and half the work on sums for each key.
 //   * A row's base is the largest score plus its value's scale's exponent, less 12: hi parts of weight * sv lie below 2^13 whatever the scales are.
+#include <type_traits>
+
 #include "rq_attention_rows.cuh"
 
 using namespace rqserve;
@@ -24,10 +27,24 @@ __device__ __forceinline__ void mma(float (&c)[4], bool first, uint32_t a0, uint
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-// four bytes, or zeros
-__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+// the same over bytes: thirty-two products each, exact
+__device__ __forceinline__ void mma(int (&c)[4], bool first, uint4 a, uint32_t b0, uint32_t b1) {
+    const int c0 = first ? 0 : c[0], c1 = first ? 0 : c[1], c2 = first ? 0 : c[2], c3 = first ? 0 : c[3];
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
+// Queries as whole numbers of 32 bits, n = 2^24 d0 + 2^16 d1 + 2^8 d2 + d3 with digits of -128 .. 127: |n| < 2^30, a row's largest element at least 2^29 (a power of two
+// brings it there; one below 2^-97 stays below)
+__device__ __forceinline__ int digits_raise(uint32_t largest) { return max(min(156 - (int)(largest >> 23), 126), -99); }
+// byte i of a word: digit of x[i]
+__device__ __forceinline__ void take_digits(const int (&n)[4], uint32_t (&digit)[4]) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = ((uint32_t)n[i] + 0x00808080u) ^ 0x00808080u;  // (carries go up, a byte of 128 and more is the digit less 256)
+    const uint32_t x = __byte_perm(b[0], b[1], 0x5140), y = __byte_perm(b[2], b[3], 0x5140), z = __byte_perm(b[0], b[1], 0x7362), w = __byte_perm(b[2], b[3], 0x7362);
+    digit[3] = __byte_perm(x, y, 0x5410); digit[2] = __byte_perm(x, y, 0x7632); digit[1] = __byte_perm(z, w, 0x5410); digit[0] = __byte_perm(z, w, 0x7632);
+}
+constexpr float kLess = 1.0f / 32768;  // what keys' scales are multiplied by, so that a sum of 2^44 times a scale has room
 
 template <int D> struct Form {
     static constexpr int TILE = D == 256 ? 16 : 32, STAGES = 2;  // keys a warp takes at a time; tiles of its ring
@@ -41,17 +58,17 @@ template <int D, int RT> struct Tiles {
     union {
         struct {
             uint8_t codes[kWarps][Form<D>::STAGES][2][Form<D>::TILE][D];
-            float scales[kWarps][Form<D>::STAGES][2][Form<D>::TILE];
         };
         float out[kWarps][8 * RT][D + 8];  // the warps' sums
     };
-    uint4 q[RT][D / 16][32];  // operand registers of the queries: hi above lo
+    uint4 q[RT][D / 32][2][32];                // operand registers of the queries: first digits above second, third above fourth
+    float scales[kWarps][3][Form<D>::TILE];   // of a warp's tile: of the keys, of the values, and these's exponents
 };
 
 template <int D, int RT>
 __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionParams p) {
     using F = Form<D>;
-    constexpr int ROWS = 8 * RT, STEPS = D / 16, TILE = F::TILE, UNIT = kWarps * TILE, NT = TILE / 8, LINES = F::LINES;
+    constexpr int ROWS = 8 * RT, STEPS = D / 32, TILE = F::TILE, UNIT = kWarps * TILE, NT = TILE / 8, LINES = F::LINES;
     constexpr uint32_t ALL = TILE == 32 ? 0xffffffffu : 0xffffu;
     extern __shared__ __align__(128) unsigned char dynamic[];
     Tiles<D, RT>& sh = *(Tiles<D, RT>*)dynamic;
@@ -96,7 +113,10 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
         const char* k_lane = (const char*)p.k + kv * p.head_stride + 16 * lane_chunk;
         const int64_t k_to_v = (const char*)p.v - (const char*)p.k;
         const float *k_scale = p.k_scale + kv * p.scale_head, *v_scale = p.v_scale + kv * p.scale_head;
-        const uint32_t ring = smem_u32(&sh.codes[warp][0][0][0][0]), scales_at = smem_u32(&sh.scales[warp][0][0][lane_key]);
+        const uint32_t ring = smem_u32(&sh.codes[warp][0][0][0][0]);
+        // the keys that every row sees
+        const int every_high = min(key_stop, position0 + row0 / group + 1);
+        const int every_low = p.window > 0 ? position0 + (row0 + max(rows, 1) - 1) / group - p.window + 1 : 0;
         // where a tile's keys lie: lane l finds key l's page, -1 for a key that no row sees
         auto page_of = [&](int key0) -> int {
             const int key = key0 + lane_key;
@@ -132,41 +152,53 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
                     }
                 }
             }
-            // a lane its key's scales (sixteen keys: one half of the lanes the keys', the other the values')
-            const int64_t scale_at = (int64_t)max(page, 0) * p.scale_page + (int64_t)((key0 + lane_key) & line_mask) * p.scale_line;
-            const uint32_t scale_to = scales_at + stage * (2 * TILE * 4);
-            if (TILE == 32 || lane < 16) copy4(scale_to, k_scale + scale_at, page >= 0);
-            if (TILE == 32 || lane >= 16) copy4(scale_to + TILE * 4, v_scale + scale_at, page >= 0);
+        };
+        // a lane's key's scales
+        float key_scale = 0.0f, value_scale = 0.0f;
+        auto load_scales = [&](int key0, int page) {
+            const int64_t at = (int64_t)page * p.scale_page + (int64_t)((key0 + lane_key) & line_mask) * p.scale_line;
+            key_scale = page >= 0 ? __ldcg(k_scale + at) : 0.0f;
+            value_scale = page >= 0 ? __ldcg(v_scale + at) : 0.0f;
         };
         int key0 = key_first + warp * TILE, ahead = key0, stage = 0;
         int page = page_of(ahead);
         uint32_t seen = __ballot_sync(0xffffffffu, page >= 0) & ALL, seen_next = 0;  // the tile's keys that some row sees
         if (ahead < key_stop) fetch(ahead, page, seen, 0);
         copies_commit();
+        load_scales(ahead, page);
         ahead += UNIT;
         page = page_of(ahead);
 
-        // queries: brought to one size and taken apart, as the tensor core's operand registers (a thread's of step 4 j + i: elements 64 j + 16 t4 + 4 i + 0 .. 3); a warp
+        // queries: brought to one size and taken apart, as the tensor core's operand registers (a thread's of step 2 j + i: elements 64 j + 16 t4 + 8 i + 0 .. 7); a warp
         // has every fourth step of all rows
         float factor[RT];  // of the scores of row g
         {
-            constexpr int MINE = RT * STEPS / kWarps;
-            float4 x[MINE];
+            constexpr int MINE = (RT * STEPS + kWarps - 1) / kWarps;
+            float x[MINE][8];
             uint32_t largest[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) largest[rt] = 0;
 #pragma unroll
             for (int n = 0; n < MINE; ++n) {
-                const int rt = n * kWarps / STEPS, step = n * kWarps % STEPS + warp, row = rt * 8 + g;
-                x[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (row < rows) {
+                const int item = n * kWarps + warp, rt = item / STEPS, step = item % STEPS, row = rt * 8 + g;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[n][e] = 0.0f;
+                if (item < RT * STEPS && row < rows) {
                     const int at = row0 + row;
-                    const float* from = p.q + (int64_t)(p.starts[r] + at / group) * p.q_stride + (int64_t)(kv * group + at % group) * D + 64 * (step >> 2) + 16 * t4 + 4 * (step & 3);
-                    if (p.wide) x[n] = __ldcg((const float4*)from);
-                    else x[n] = make_float4(__ldcg(from), __ldcg(from + 1), __ldcg(from + 2), __ldcg(from + 3));
+                    const float* from = p.q + (int64_t)(p.starts[r] + at / group) * p.q_stride + (int64_t)(kv * group + at % group) * D + 64 * (step >> 1) + 16 * t4 + 8 * (step & 1);
+                    if (p.wide) {
+                        const float4 v = __ldcg((const float4*)from), w = __ldcg((const float4*)from + 1);
+                        x[n][0] = v.x; x[n][1] = v.y; x[n][2] = v.z; x[n][3] = v.w; x[n][4] = w.x; x[n][5] = w.y; x[n][6] = w.z; x[n][7] = w.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[n][e] = __ldcg(from + e);
+                    }
                 }
-                largest[rt] = max(max(largest[rt], __float_as_uint(x[n].x) & 0x7fffffffu), __float_as_uint(x[n].y) & 0x7fffffffu);
-                largest[rt] = max(max(largest[rt], __float_as_uint(x[n].z) & 0x7fffffffu), __float_as_uint(x[n].w) & 0x7fffffffu);
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    if (t == rt)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) largest[t] = max(largest[t], __float_as_uint(x[n][e]) & 0x7fffffffu);
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
@@ -180,20 +212,25 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
             for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) largest[rt] = max(largest[rt], row_largest[w][rt * 8 + g]);
-                const int raise = raise_of(largest[rt]);
+                const int raise = digits_raise(largest[rt]);
                 raised[rt] = power_of_two(raise);
-                factor[rt] = factor_of(p.scale, raise);
+                factor[rt] = factor_of(p.scale / kLess, raise);
             }
 #pragma unroll
             for (int n = 0; n < MINE; ++n) {
-                const int rt = n * kWarps / STEPS, step = n * kWarps % STEPS + warp;
-                x[n].x *= raised[rt]; x[n].y *= raised[rt]; x[n].z *= raised[rt]; x[n].w *= raised[rt];
-                uint4 a;
-                a.x = take_pair<RQ_KV_F16>(x[n].x, x[n].y);
-                a.z = take_pair<RQ_KV_F16>(x[n].z, x[n].w);
-                a.y = rqattn::pair_of<RQ_KV_F16>(x[n].x, x[n].y);
-                a.w = rqattn::pair_of<RQ_KV_F16>(x[n].z, x[n].w);
-                sh.q[rt][step][lane] = a;
+                const int item = n * kWarps + warp, rt = item / STEPS, step = item % STEPS;
+                if (item >= RT * STEPS) break;
+                const float f = RT == 2 && rt ? raised[RT - 1] : raised[0];
+                uint32_t d[2][4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    int whole[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) whole[i] = __float2int_rn(x[n][4 * e + i] * f);
+                    take_digits(whole, d[e]);
+                }
+                sh.q[rt][step][0][lane] = make_uint4(d[0][0], d[0][1], d[1][0], d[1][1]);
+                sh.q[rt][step][1][lane] = make_uint4(d[0][2], d[0][3], d[1][2], d[1][3]);
             }
         }
         __syncthreads();
@@ -209,76 +246,103 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
         }
         for (; key0 < key_stop; key0 += UNIT, stage = stage + 1 == F::STAGES ? 0 : stage + 1, seen = seen_next) {
             const uint32_t keys = ring + stage * F::STAGE, values = keys + TILE * D;
-            __syncwarp();  // the other stage has been read
+            __syncwarp();  // the other stage, and the scales, have been read
+            if (TILE == 32 || lane < TILE) {
+                sh.scales[warp][0][lane_key] = key_scale * kLess;
+                sh.scales[warp][1][lane_key] = value_scale;
+                sh.scales[warp][2][lane_key] = exponent_of(value_scale);
+            }
             seen_next = __ballot_sync(0xffffffffu, page >= 0) & ALL;
             if (ahead < key_stop) fetch(ahead, page, seen_next, stage ^ 1);
             copies_commit();
+            load_scales(ahead, page);
             ahead += UNIT;
             page = page_of(ahead);
             copies_wait<1>();
             __syncwarp();
             // scores: of keys 8 i + 2 t4 + {0, 1} and row g
-            float c[RT][NT][4];
+            float s[RT][NT][2];
+            {
+                int c[RT][NT][2][4];
 #pragma unroll
-            for (int j = 0; j < D / 64; ++j) {
-                uint4 w[NT];
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const uint32_t from = keys + (8 * i + g) * D + (placed<D>(8 * i + g, 4 * j + t4) << 4);
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w) : "r"(from) : "memory");
-                }
-#pragma unroll
-                for (int step = 0; step < 4; ++step) {
-                    uint4 a[RT];
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) a[rt] = sh.q[rt][4 * j + step][lane];
+                for (int j = 0; j < D / 64; ++j) {
+                    uint4 w[NT];
 #pragma unroll
                     for (int i = 0; i < NT; ++i) {
-                        const uint32_t word = turn_codes(step == 0 ? w[i].x : step == 1 ? w[i].y : step == 2 ? w[i].z : w[i].w);
-                        const uint32_t b0 = widen_codes<0, 1>(word), b1 = widen_codes<2, 3>(word);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) mma(c[rt][i], j == 0 && step == 0, a[rt].x, a[rt].y, a[rt].z, a[rt].w, b0, b1);
+                        const uint32_t from = keys + (8 * i + g) * D + (placed<D>(8 * i + g, 4 * j + t4) << 4);
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w) : "r"(from) : "memory");
                     }
+#pragma unroll
+                    for (int step = 0; step < 2; ++step)
+#pragma unroll
+                        for (int part = 0; part < 2; ++part)
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) {
+                                const uint4 a = sh.q[rt][2 * j + step][part][lane];
+#pragma unroll
+                                for (int i = 0; i < NT; ++i) mma(c[rt][i][part], j == 0 && step == 0, a, step ? w[i].z : w[i].x, step ? w[i].w : w[i].y);
+                            }
                 }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int i = 0; i < NT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) s[rt][i][e] = fmaf((float)(c[rt][i][0][e] * 256 + c[rt][i][0][2 + e]), 65536.0f, (float)(c[rt][i][1][e] * 256 + c[rt][i][1][2 + e]));
             }
             // weights
             uint32_t w_hi[RT][NT], w_lo[RT][NT];
             float old[RT];
-            {
-                float2 ks[NT], vs[NT];
+            auto weigh = [&](auto masked) {
+                constexpr bool kMasked = decltype(masked)::value;
+                float top[RT];
 #pragma unroll
-                for (int i = 0; i < NT; ++i) { ks[i] = *(const float2*)&sh.scales[warp][stage][0][8 * i + 2 * t4]; vs[i] = *(const float2*)&sh.scales[warp][stage][1][8 * i + 2 * t4]; }
+                for (int rt = 0; rt < RT; ++rt) top[rt] = -INFINITY;
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    float s[NT][2], top = -INFINITY;
+                for (int i = 0; i < NT; ++i) {
+                    const float2 ks = *(const float2*)&sh.scales[warp][0][8 * i + 2 * t4], level = *(const float2*)&sh.scales[warp][2][8 * i + 2 * t4];
 #pragma unroll
-                    for (int i = 0; i < NT; ++i)
+                    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const int at = 8 * i + 2 * t4 + e, key = key0 + at;
-                            s[i][e] = (c[rt][i][e] + c[rt][i][2 + e]) * (e ? ks[i].y : ks[i].x);
-                            if (key < low[rt] || key >= high[rt] || !(seen >> at & 1)) s[i][e] = -INFINITY;
-                            top = fmaxf(top, fmaf(s[i][e], factor[rt], exponent_of(e ? vs[i].y : vs[i].x)));
+                            s[rt][i][e] *= e ? ks.y : ks.x;
+                            if (kMasked && (key < low[rt] || key >= high[rt] || !(seen >> at & 1))) s[rt][i][e] = -INFINITY;
+                            top[rt] = fmaxf(top[rt], fmaf(s[rt][i][e], factor[rt], e ? level.y : level.x));
                         }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    top = fmaxf(base[rt], top - kRaise<RQ_KV_F16>);
-                    const float from = top == -INFINITY ? 0.0f : top;
-                    old[rt] = exp2_fast(base[rt] - from);
-                    base[rt] = top;
-                    float add = 0.0f;
+                }
+                float from[RT], add[RT];
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        const float a = exp2_fast(fmaf(s[i][0], factor[rt], -from)), b = exp2_fast(fmaf(s[i][1], factor[rt], -from));
-                        add += a + b;
-                        // (a scale that the row must not see may be infinite, and 0 * inf is no 0)
-                        float x = s[i][0] == -INFINITY ? 0.0f : a * vs[i].x, y = s[i][1] == -INFINITY ? 0.0f : b * vs[i].y;
+                for (int rt = 0; rt < RT; ++rt) {
+                    top[rt] = fmaxf(top[rt], __shfl_xor_sync(0xffffffffu, top[rt], 1));
+                    top[rt] = fmaxf(top[rt], __shfl_xor_sync(0xffffffffu, top[rt], 2));
+                    top[rt] = fmaxf(base[rt], top[rt] - kRaise<RQ_KV_F16>);
+                    from[rt] = top[rt] == -INFINITY ? 0.0f : top[rt];
+                    old[rt] = exp2_fast(base[rt] - from[rt]);
+                    base[rt] = top[rt];
+                    add[rt] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const float2 vs = *(const float2*)&sh.scales[warp][1][8 * i + 2 * t4];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const float a = exp2_fast(fmaf(s[rt][i][0], factor[rt], -from[rt])), b = exp2_fast(fmaf(s[rt][i][1], factor[rt], -from[rt]));
+                        add[rt] += a + b;
+                        float x = a * vs.x, y = b * vs.y;
+                        if (kMasked) {  // (a scale that the row must not see may be infinite, and 0 * inf is no 0)
+                            x = s[rt][i][0] == -INFINITY ? 0.0f : x;
+                            y = s[rt][i][1] == -INFINITY ? 0.0f : y;
+                        }
                         w_hi[rt][i] = take_pair<RQ_KV_F16>(x, y);
                         w_lo[rt][i] = rqattn::pair_of<RQ_KV_F16>(x, y);
                     }
-                    sum[rt] = fmaf(sum[rt], old[rt], add);
                 }
-            }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) sum[rt] = fmaf(sum[rt], old[rt], add[rt]);
+            };
+            if (key0 >= every_low && key0 + TILE <= every_high && seen == ALL) weigh(std::false_type());
+            else weigh(std::true_type());
             const int value_line = lane & 15, value_half = lane >> 4;
 #pragma unroll
             for (int n2 = 0; n2 < D / 32; ++n2) {
