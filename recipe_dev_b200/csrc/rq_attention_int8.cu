@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "rq_attention_rows.cuh"
+#include "rq_pairs.cuh"
 
 using namespace rqserve;
 using namespace rqattn;
@@ -46,6 +47,9 @@ __device__ __forceinline__ void take_digits(const int (&n)[4], uint32_t (&digit)
 }
 constexpr float kLess = 1.0f / 32768;  // what keys' scales are multiplied by, so that a sum of 2^44 times a scale has room
 
+// Taking up the rows of a request and head (their queries, the first tile, the sums at the end) costs a CTA as much as some units: so many lead each one's own in the dealing
+constexpr int kLead = 2;
+
 template <int D> struct Form {
     static constexpr int TILE = D == 256 ? 16 : 32, STAGES = 2;  // keys a warp takes at a time; tiles of its ring
     static constexpr int CHUNKS = D / 16, LINES = 32 / CHUNKS;   // 16-byte pieces of a line; lines that a warp copies an instruction
@@ -53,6 +57,9 @@ template <int D> struct Form {
 };
 // Where a line's pieces lie, so that neither eight lines' same piece (matrix loads) nor four pieces each of two lines meet a bank twice
 template <int D> __device__ __forceinline__ int placed(int line, int chunk) { return chunk ^ (D == 64 ? line >> 1 & 3 : (line & 1) << 2 | (line >> 1 & 3)); }
+
+// a / b, neither negative: mostly small ones
+__device__ __forceinline__ int64_t divided(int64_t a, int64_t b) { return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }
 
 template <int D, int RT> struct Tiles {
     union {
@@ -65,8 +72,11 @@ template <int D, int RT> struct Tiles {
     float scales[kWarps][3][Form<D>::TILE];   // of a warp's tile: of the keys, of the values, and these's exponents
 };
 
+// CTAs that an SM holds, by what their shared memory and their sums in registers leave room for
+template <int D, int RT> constexpr int kResident = D == 256 || (D == 128 && RT == 2) ? 2 : (D == 64 && RT == 1 ? 4 : 3);
+
 template <int D, int RT>
-__global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionParams p) {
+__global__ void __launch_bounds__(kThreads, kResident<D, RT>) rq_attention_int8_kernel(AttentionParams p) {
     using F = Form<D>;
     constexpr int ROWS = 8 * RT, STEPS = D / 32, TILE = F::TILE, UNIT = kWarps * TILE, NT = TILE / 8, LINES = F::LINES;
     constexpr uint32_t ALL = TILE == 32 ? 0xffffffffu : 0xffffu;
@@ -82,7 +92,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
     const int group = p.q_heads / p.kv_heads;
     wait_for_previous();
 
-    const Deal deal = deal_units<ROWS, TILE>(p, before, sums);
+    const Deal deal = deal_units<ROWS, TILE, kLead>(p, before, sums);
     if (blockIdx.x >= deal.ctas) return;
     int64_t u = deal.begin;
 
@@ -91,11 +101,34 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
         int r = 0;
         for (int hi = p.requests - 1; r < hi;) { const int mid = (r + hi + 1) >> 1; if (before[mid] <= u) r = mid; else hi = mid - 1; }
         const Request rq = request_of<ROWS, TILE>(p, r);
-        const int64_t in_request = u - before[r], item = in_request / rq.units, first_unit = in_request % rq.units;
-        const int kv = (int)(item % p.kv_heads), row0 = (int)(item / p.kv_heads) * ROWS, rows = min(ROWS, rq.here * group - row0);
-        const int64_t item_begin = u - first_unit, item_end = item_begin + rq.units, stop = min(item_end, deal.end);
-        const int key_first = rq.begin + (int)first_unit * UNIT, key_stop = min(rq.end, rq.begin + (int)(stop - item_begin) * UNIT);
+        const int64_t in_request = u - before[r], item_units = kLead + rq.units, item = divided(in_request, item_units), item_begin = before[r] + item * item_units, item_end = item_begin + item_units;
+        const int64_t tile = divided(item, p.kv_heads), stop = min(item_end, deal.end);
+        const int kv = (int)(item - tile * p.kv_heads), row0 = (int)tile * ROWS, rows = min(ROWS, rq.here * group - row0), offset = (int)(u - item_begin), first_unit = max(offset - kLead, 0);
+        const int units = (int)(stop - item_begin) - kLead - first_unit;
         u = stop;
+        if (units <= 0) continue;  // (a range that ends in the lead: the next CTA has it all)
+        const int key_first = rq.begin + first_unit * UNIT, key_stop = min(rq.end, key_first + units * UNIT), start = p.starts[r];
+
+        // the queries, on their way while the first keys are found
+        constexpr int MINE = (RT * STEPS + kWarps - 1) / kWarps;
+        float x[MINE][8];
+#pragma unroll
+        for (int n = 0; n < MINE; ++n) {
+            const int of = n * kWarps + warp, step = of % STEPS, row = of / STEPS * 8 + g;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[n][e] = 0.0f;
+            if (of < RT * STEPS && row < rows) {
+                const int at = row0 + row;
+                const float* from = p.q + (int64_t)(start + at / group) * p.q_stride + (int64_t)(kv * group + at % group) * D + 64 * (step >> 1) + 16 * t4 + 8 * (step & 1);
+                if (p.wide) {
+                    const float4 v = __ldcg((const float4*)from), w = __ldcg((const float4*)from + 1);
+                    x[n][0] = v.x; x[n][1] = v.y; x[n][2] = v.z; x[n][3] = v.w; x[n][4] = w.x; x[n][5] = w.y; x[n][6] = w.z; x[n][7] = w.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[n][e] = __ldcg(from + e);
+                }
+            }
+        }
 
         // the keys that some row sees and that this thread's rows see: [low, high)
         int low[RT], high[RT];
@@ -124,8 +157,24 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
             return entry < p.pages ? max(entry, -1) : -1;
         };
         // A warp copies LINES lines an instruction, this lane one piece of one of them
+        const bool plain = p.page_shift >= 4 && p.line_bytes == D;
         auto fetch = [&](int key0, int page, uint32_t seen, int stage) {
             const uint32_t to = ring + stage * F::STAGE + lane_line * D;
+            if (plain && seen == ALL) {  // nothing but the pages' addresses changes from tile to tile
+#pragma unroll
+                for (int half = 0; half < TILE / 16; ++half) {
+                    const int at = __shfl_sync(0xffffffffu, page, 16 * half);
+                    const char* from = k_lane + (uint64_t)(uint32_t)at * p.page_bytes + (uint32_t)((((key0 + 16 * half) & line_mask) + lane_line) * D);
+                    const char* values_from = from + k_to_v;
+#pragma unroll
+                    for (int i = 0; i < 16 / LINES; ++i) {
+                        const uint32_t place = to + (16 * half + i * LINES) * D + (placed<D>(i * LINES + lane_line, lane_chunk) << 4);
+                        copy16(place, from + i * LINES * D, true);
+                        copy16(place + TILE * D, values_from + i * LINES * D, true);
+                    }
+                }
+                return;
+            }
 #pragma unroll
             for (int half = 0; half < TILE / 16; ++half) {
                 if (p.page_shift >= 4) {  // sixteen keys of a multiple of sixteen share a page
@@ -173,33 +222,16 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
         // has every fourth step of all rows
         float factor[RT];  // of the scores of row g
         {
-            constexpr int MINE = (RT * STEPS + kWarps - 1) / kWarps;
-            float x[MINE][8];
             uint32_t largest[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) largest[rt] = 0;
 #pragma unroll
-            for (int n = 0; n < MINE; ++n) {
-                const int item = n * kWarps + warp, rt = item / STEPS, step = item % STEPS, row = rt * 8 + g;
+            for (int n = 0; n < MINE; ++n)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[n][e] = 0.0f;
-                if (item < RT * STEPS && row < rows) {
-                    const int at = row0 + row;
-                    const float* from = p.q + (int64_t)(p.starts[r] + at / group) * p.q_stride + (int64_t)(kv * group + at % group) * D + 64 * (step >> 1) + 16 * t4 + 8 * (step & 1);
-                    if (p.wide) {
-                        const float4 v = __ldcg((const float4*)from), w = __ldcg((const float4*)from + 1);
-                        x[n][0] = v.x; x[n][1] = v.y; x[n][2] = v.z; x[n][3] = v.w; x[n][4] = w.x; x[n][5] = w.y; x[n][6] = w.z; x[n][7] = w.w;
-                    } else {
+                for (int rt = 0; rt < RT; ++rt)
+                    if ((n * kWarps + warp) / STEPS == rt)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[n][e] = __ldcg(from + e);
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-                    if (t == rt)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) largest[t] = max(largest[t], __float_as_uint(x[n][e]) & 0x7fffffffu);
-            }
+                        for (int e = 0; e < 8; ++e) largest[rt] = max(largest[rt], __float_as_uint(x[n][e]) & 0x7fffffffu);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 largest[rt] = max(largest[rt], __shfl_xor_sync(0xffffffffu, largest[rt], 1));
@@ -236,13 +268,13 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
         __syncthreads();
 
         float base[RT], sum[RT];  // base: -inf while the row has seen no key
-        float2 acc[RT][D / 8];    // elements 16 c + 4 t4 + {0, 2} (2 c), + {1, 3} (2 c + 1)
+        Pair acc[RT][D / 8];      // elements 16 c + 4 t4 + {0, 2} (2 c), + {1, 3} (2 c + 1)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             base[rt] = -INFINITY;
             sum[rt] = 0.0f;
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) acc[rt][n] = make_float2(0.0f, 0.0f);
+            for (int n = 0; n < D / 8; ++n) acc[rt][n] = ::pair_of(0.0f, 0.0f);
         }
         for (; key0 < key_stop; key0 += UNIT, stage = stage + 1 == F::STAGES ? 0 : stage + 1, seen = seen_next) {
             const uint32_t keys = ring + stage * F::STAGE, values = keys + TILE * D;
@@ -369,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
 #pragma unroll
                         for (int half = 0; half < TILE / 16; ++half)
                             mma(d, half == 0, w_hi[rt][2 * half], w_lo[rt][2 * half], w_hi[rt][2 * half + 1], w_lo[rt][2 * half + 1], b0[half], b1[half]);
-                        acc[rt][4 * n2 + i] = fma2(acc[rt][4 * n2 + i], make_float2(old[rt], old[rt]), make_float2(d[0] + d[2], d[1] + d[3]));
+                        acc[rt][4 * n2 + i] = pair_fma(acc[rt][4 * n2 + i], ::pair_of(old[rt], old[rt]), pair_add(::pair_of(d[0], d[1]), ::pair_of(d[2], d[3])));
                     }
                 }
             }
@@ -385,10 +417,10 @@ __global__ void __launch_bounds__(kThreads) rq_attention_int8_kernel(AttentionPa
             if (t4 == 0) { warp_base[warp][rt * 8 + g] = base[rt]; warp_sum[warp][rt * 8 + g] = sum[rt]; }
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
-                *(float4*)&sh.out[warp][rt * 8 + g][16 * n + 4 * t4] = make_float4(acc[rt][2 * n].x, acc[rt][2 * n + 1].x, acc[rt][2 * n].y, acc[rt][2 * n + 1].y);
+                *(float4*)&sh.out[warp][rt * 8 + g][16 * n + 4 * t4] = make_float4(pair_at(acc[rt][2 * n], 0), pair_at(acc[rt][2 * n + 1], 0), pair_at(acc[rt][2 * n], 1), pair_at(acc[rt][2 * n + 1], 1));
         }
         __syncthreads();
-        join_rows<D, ROWS>(p, &sh.out[0][0][0], warp_base, warp_sum, item_begin, item_end, deal, p.starts[r], row0, rows, kv, last_arrival);
+        join_rows<D, ROWS, kLead>(p, &sh.out[0][0][0], warp_base, warp_sum, item_begin, item_end, deal, start, row0, rows, kv, last_arrival);
         __syncthreads();  // the shared sums are free again
     }
 }

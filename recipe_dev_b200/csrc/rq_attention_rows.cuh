@@ -55,14 +55,14 @@ template <int ROWS, int TILE> __device__ __forceinline__ Request request_of(cons
 struct Deal {
     int64_t total, ctas, begin, end;
 };
-// before: the units before each request, left behind; sums: a number a warp
-template <int ROWS, int TILE> __device__ __forceinline__ Deal deal_units(const AttentionParams& p, int64_t* before, int64_t* sums) {
+// before: the units before each request, left behind; sums: a number a warp. LEAD: units that each row tile and head counts for in the dealing beside its own
+template <int ROWS, int TILE, int LEAD = 0> __device__ __forceinline__ Deal deal_units(const AttentionParams& p, int64_t* before, int64_t* sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = p.q_heads / p.kv_heads;
     int64_t total = 0;
     if (tid == 0) before[0] = 0;
     for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
         int64_t units = 0;
-        if (r0 + tid < p.requests) { const Request q = request_of<ROWS, TILE>(p, r0 + tid); units = (int64_t)q.here * group > p.few ? 0 : q.units * q.tiles * p.kv_heads; }
+        if (r0 + tid < p.requests) { const Request q = request_of<ROWS, TILE>(p, r0 + tid); units = (int64_t)q.here * group > p.few ? 0 : (LEAD + q.units) * q.tiles * p.kv_heads; }
         int64_t scan = units;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) { const int64_t o = __shfl_up_sync(0xffffffffu, scan, off); if (lane >= off) scan += o; }
@@ -79,23 +79,78 @@ template <int ROWS, int TILE> __device__ __forceinline__ Deal deal_units(const A
     return d;
 }
 
-// The warps' sums of rows (out: [warp][row][D + 8]; their bases and sums of weights) to y, or, where other CTAs have parts of the rows' units [item_begin, item_end), to the
-// work area; the last of those CTAs joins the parts in CTA order. start: the request's first token. Begins behind a barrier that all have written before.
+// A row's results: sums over the sum of weights
+template <int D> __device__ __forceinline__ void put_row(const AttentionParams& p, int start, int at, int kv, int e, float4 v, float total_weight) {
+    const int group = p.q_heads / p.kv_heads;
+    float* y = p.y + (int64_t)(start + at / group) * p.y_stride + (int64_t)(kv * group + at % group) * D;
+    const float inverse = total_weight == 0.0f ? 0.0f : 1.0f / total_weight;
+    v.x *= inverse; v.y *= inverse; v.z *= inverse; v.w *= inverse;
+    if (p.wide) *(float4*)(y + e) = v;
+    else { y[e] = v.x; y[e + 1] = v.y; y[e + 2] = v.z; y[e + 3] = v.w; }
+}
+
+// The parts that CTAs first_cta .. last_cta have left of some rows, joined.
 template <int D, int ROWS>
-__device__ __forceinline__ void join_rows(const AttentionParams& p, const float* out, const float (&warp_base)[kWarps][ROWS], const float (&warp_sum)[kWarps][ROWS], int64_t item_begin,
+__device__ __forceinline__ void join_parts(const AttentionParams& p, float* out, int64_t first_cta, int64_t last_cta, int start, int row0, int rows, int kv) {
+    const int tid = threadIdx.x;
+    const int64_t stride = ROWS * (D + 2);
+    // The parts' bases and sums of weights are brought by all threads side by side, some parts at a time, and their sums many at once; they are added up in CTA order. (Each thread
+    // for itself, one load behind another, took the last CTA of 55 ten microseconds.)
+    constexpr int ITEMS = (ROWS * (D / 4) + kThreads - 1) / kThreads, kParts = 64;
+    static_assert(kThreads % ROWS == 0 && 2 * kParts * ROWS <= kWarps * ROWS * (D + 8) && kThreads <= kWarps * ROWS * (D + 8), "the place of the warps' sums");
+    const int parts = (int)(last_cta - first_cta) + 1, my_row = tid % ROWS;
+    auto part = [&](int c) { return p.partial + ((first_cta + c) * 2 + (c == 0)) * stride; };
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int c = tid / ROWS; c < parts; c += kThreads / ROWS) top = fmaxf(top, __ldcg(part(c) + ROWS * D + my_row));
+    out[tid] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = my_row; i < kThreads; i += ROWS) top = fmaxf(top, out[i]);
+    const float to = top == -INFINITY ? 0.0f : top;
+    float4 v[ITEMS];
+    float weight[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) { v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); weight[i] = 0.0f; }
+    for (int c0 = 0; c0 < parts; c0 += kParts) {
+        const int here = min(kParts, parts - c0);
+        __syncthreads();
+#pragma unroll 4
+        for (int c = tid / ROWS; c < here; c += kThreads / ROWS) {
+            const float* from = part(c0 + c) + ROWS * D + my_row;
+            *(float2*)(out + 2 * (c * ROWS + my_row)) = make_float2(exp2_fast(__ldcg(from) - to), __ldcg(from + ROWS));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int item = tid + i * kThreads, row = item / (D / 4), e = 4 * (item % (D / 4));
+            if (row >= rows) break;
+#pragma unroll 16
+            for (int c = 0; c < here; ++c) {
+                const float4 o = __ldcg((const float4*)(part(c0 + c) + row * D + e));
+                const float2 f = *(const float2*)(out + 2 * (c * ROWS + row));
+                v[i].x = fmaf(o.x, f.x, v[i].x); v[i].y = fmaf(o.y, f.x, v[i].y); v[i].z = fmaf(o.z, f.x, v[i].z); v[i].w = fmaf(o.w, f.x, v[i].w);
+                weight[i] = fmaf(f.y, f.x, weight[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int item = tid + i * kThreads, row = item / (D / 4), e = 4 * (item % (D / 4));
+        if (row < rows) put_row<D>(p, start, row0 + row, kv, e, v[i], weight[i]);
+    }
+}
+
+// The warps' sums of rows (out: [warp][row][D + 8]; their bases and sums of weights) to y, or, where other CTAs have parts of the rows' units [item_begin, item_end), to the
+// work area; the last of those CTAs joins the parts in CTA order (LEAD: as dealt, the first units of an item are nobody's work). start: the request's first token. Begins behind a barrier that all have written before.
+template <int D, int ROWS, int LEAD = 0>
+__device__ __forceinline__ void join_rows(const AttentionParams& p, float* out, const float (&warp_base)[kWarps][ROWS], const float (&warp_sum)[kWarps][ROWS], int64_t item_begin,
                                           int64_t item_end, const Deal& deal, int start, int row0, int rows, int kv, uint32_t& last_arrival) {
-    const int tid = threadIdx.x, group = p.q_heads / p.kv_heads;
-    const int64_t first_cta = ((item_begin + 1) * deal.ctas - 1) / deal.total, last_cta = (item_end * deal.ctas - 1) / deal.total;
+    const int tid = threadIdx.x;
+    const int64_t first_cta = ((item_begin + LEAD + 1) * deal.ctas - 1) / deal.total, last_cta = (item_end * deal.ctas - 1) / deal.total;
     const bool whole = first_cta == last_cta;
     const int64_t stride = ROWS * (D + 2);
     float* mine = p.partial + ((int64_t)blockIdx.x * 2 + (blockIdx.x == first_cta)) * stride;
-    auto row_of = [&](int row) { const int at = row0 + row; return p.y + (int64_t)(start + at / group) * p.y_stride + (int64_t)(kv * group + at % group) * D; };
-    auto put = [&](float* y, int e, float4 v, float total_weight) {
-        const float inverse = total_weight == 0.0f ? 0.0f : 1.0f / total_weight;
-        v.x *= inverse; v.y *= inverse; v.z *= inverse; v.w *= inverse;
-        if (p.wide) *(float4*)(y + e) = v;
-        else { y[e] = v.x; y[e + 1] = v.y; y[e + 2] = v.z; y[e + 3] = v.w; }
-    };
     for (int i = tid; i < ROWS * (D / 4); i += kThreads) {
         const int row = i / (D / 4), e = 4 * (i % (D / 4));
         if (row >= rows) break;
@@ -113,7 +168,7 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, const float*
             weight = fmaf(warp_sum[w][row], f, weight);
         }
         if (whole) {
-            put(row_of(row), e, v, weight);
+            put_row<D>(p, start, row0 + row, kv, e, v, weight);
         } else {
             __stcg((float4*)(mine + row * D + e), v);
             if (e == 0) { __stcg(mine + ROWS * D + row, top); __stcg(mine + ROWS * D + ROWS + row, weight); }
@@ -127,24 +182,7 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, const float*
         if (last_arrival == (uint32_t)(last_cta - first_cta)) {
             if (tid == 0) p.arrived[first_cta] = 0;
             __threadfence();
-            for (int i = tid; i < ROWS * (D / 4); i += kThreads) {
-                const int row = i / (D / 4), e = 4 * (i % (D / 4));
-                if (row >= rows) break;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                float weight = 0.0f, top = -INFINITY;
-#pragma unroll 8
-                for (int64_t c = first_cta; c <= last_cta; ++c) top = fmaxf(top, __ldcg(p.partial + (c * 2 + (c == first_cta)) * stride + ROWS * D + row));
-                const float to = top == -INFINITY ? 0.0f : top;
-#pragma unroll 8
-                for (int64_t c = first_cta; c <= last_cta; ++c) {
-                    const float* from = p.partial + (c * 2 + (c == first_cta)) * stride;
-                    const float f = exp2_fast(__ldcg(from + ROWS * D + row) - to);
-                    const float4 o = __ldcg((const float4*)(from + row * D + e));
-                    v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
-                    weight = fmaf(__ldcg(from + ROWS * D + ROWS + row), f, weight);
-                }
-                put(row_of(row), e, v, weight);
-            }
+            join_parts<D, ROWS>(p, out, first_cta, last_cta, start, row0, rows, kv);
         }
     }
 }
