@@ -125,7 +125,7 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, float* out,
         for (int i = 0; i < ITEMS; ++i) {
             const int item = tid + i * kThreads, row = item / (D / 4), e = 4 * (item % (D / 4));
             if (row >= rows) break;
-#pragma unroll 16
+#pragma unroll 28
             for (int c = 0; c < here; ++c) {
                 const float4 o = __ldcg((const float4*)(part(c0 + c) + row * D + e));
                 const float2 f = *(const float2*)(out + 2 * (c * ROWS + row));

@@ -2,16 +2,16 @@
 //
 //   log p_t = (x_t - m) - log Z,  Z = sum_i e^(x_i - m);  H = log Z - sum_i e^(x_i - m) (x_i - m) / Z: two terms that are not negative, nothing cancels
 //
-// A row is dealt out over a cluster of up to sixteen CTAs, a contiguous share each, which go through it in rounds of sixteen logits a thread, the next round's on their way.
-// A thread keeps a running maximum, the sum and the first moment against it, and how many of its logits lie ahead of the given token's (whose logit is read first).
-// Alternatives: a CTA keeps a list of logits above a bound that at least `top` of those that it has seen reach. The first bound comes from the warps: the least of their
-// k-th largest threads' largest logits, k = ceil(top / warps), which is reached by at least `top` logits and, where logits are in no order, by a few times as many. A list of
-// more than twice `top` is cut down to the first `top` of it by comparison of all with all, and the bound is then the last of these: later logits have to be larger (equal ones
-// come behind by their index). A round that would overflow the list is gone through again with the bound that 64 votes over the threads' largest find exactly, at most
-// sixteen a thread over it. At the end the first CTA of the cluster joins the CTAs' sums in their order and their lists through distributed shared memory: the same bits on
-// every run.
+// A row is dealt out over a cluster of up to eight CTAs, a contiguous share each, which stream through it: a thread keeps a running maximum, the sum and the first moment against it,
+// and how many of its logits lie ahead of the given token's (whose logit is read beside the first ones). There is no barrier before the end of a share.
+// Alternatives: each thread also leaves the largest logit of each of up to sixteen segments of its logits in shared memory. The `top`-th largest of the threads' largest logits (its
+// upper sixteen bits, found by as many votes) is a bound that at least `top` logits of the share reach; the largest of the CTAs' bounds holds for the row. Segments that
+// reach it, a few times `top` of them, are read again (from L2), and their logits that reach it go to the first CTA's list through distributed shared memory, which puts them in
+// order by comparison of all with all. Where equal or ordered logits overflow the list, the exact key of the `top`-th logit is found bit by bit, in 64 rounds over the row.
+// Sums are joined in the order of warps and CTAs: the same bits on every run.
 #include <cooperative_groups.h>
 
+#include "rq_pairs.cuh"
 #include "rq_serve.cuh"
 
 using namespace rqserve;
@@ -20,8 +20,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kQuads = 4, kEach = 4 * kQuads, kRound = kThreads * kEach;
-constexpr int kList = 2048, kMostCtas = 16;
-static_assert(kMostCtas * RQ_MAX_ALTERNATIVES <= kList && 2 * kEach * RQ_MAX_ALTERNATIVES <= kList, "lists");
+constexpr int kList = 2048, kMostCtas = 8, kSegments = 16;
 
 typedef unsigned long long u64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -46,12 +45,6 @@ __device__ __forceinline__ float above(float x) {
     return __uint_as_float((u << 1) == 0 ? 1u : (u >> 31 ? u - 1 : u + 1));
 }
 
-// the largest number below x (x >= -inf); below -inf: none, it is -inf
-__device__ __forceinline__ float below(float x) {
-    const uint32_t u = __float_as_uint(x);
-    return x != x || x == -INFINITY ? -INFINITY : __uint_as_float((u << 1) == 0 ? 0x80000001u : (u >> 31 ? u + 1 : u - 1));
-}
-
 // A maximum, the sum of 2^d and of d 2^d over logits, d = (x - maximum) log2(e)
 struct Sums {
     float top, sum, moment;
@@ -71,28 +64,22 @@ struct Sums {
 };
 
 struct Shared {
-    u64 list[kList], best[RQ_MAX_ALTERNATIVES];
     Sums warp_sums[kWarps], sums;
     int warp_ahead[kWarps], ahead;
-    uint32_t warp_bound[kWarps];
-    int listed, found;  // entries of list; of best
 };
-
-// The first `top` of the n entries of the list, in order, to best; their number
-__device__ __forceinline__ int keep_best(Shared& sh, int n, int top) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const u64 key = sh.list[i];
-        int before = 0;
-#pragma unroll 8
-        for (int j = 0; j < n; ++j) before += sh.list[j] > key;
-        if (before < top) sh.best[before] = key;
-    }
-    return min(n, top);
-}
+struct Lists {
+    float largest[kSegments][kThreads];  // of a thread's segments
+    u64 list[kList], best[RQ_MAX_ALTERNATIVES];
+    float bound;  // at least `top` logits of the share reach it
+    int listed;
+    u64 warp_count[kWarps], count;
+};
 
 template <bool ALTERNATIVES>
 __global__ void __launch_bounds__(kThreads) rq_logprobs_kernel(LogprobParams p) {
     __shared__ Shared sh;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    Lists& lists = *(Lists*)dynamic;  // (with alternatives)
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     launch_dependents();
@@ -100,134 +87,106 @@ __global__ void __launch_bounds__(kThreads) rq_logprobs_kernel(LogprobParams p) 
     // quads are counted from the 16-byte boundary at or before the row
     const int skew = (int)((uintptr_t)x >> 2 & 3), end = p.vocabulary + skew, quads = (end + 3) / 4;
     const int first = rank * p.share, last = min(first + p.share, quads);
-    if (tid == 0) { sh.listed = 0; sh.found = 0; }
     wait_for_previous();
+
+    // sixteen logits of the round that begins at `quad0`: four quads, neighbours by thread; past the share's ends -inf
+    const float* const row_at = x - skew;
+    const int whole = min(last, end / 4);  // quads below lie inside, from the second one on (the first one too, where the row begins at a boundary)
+    auto load = [&](int quad0, float (&v)[kEach]) {
+        const float* from = row_at + 4 * (int64_t)(quad0 + tid);
+        if ((quad0 > 0 || skew == 0) && quad0 + kThreads * kQuads <= whole) {
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j) {
+                const float4 a = __ldcg((const float4*)from + j * kThreads);
+                v[4 * j] = a.x; v[4 * j + 1] = a.y; v[4 * j + 2] = a.z; v[4 * j + 3] = a.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int quad = quad0 + tid + i / 4 * kThreads, at = 4 * quad + i % 4;
+                v[i] = quad < last && at >= skew && at < end ? __ldcg(from + 4 * (i / 4) * kThreads + i % 4) : -INFINITY;
+            }
+        }
+    };
+    auto key_of = [&](float v, int quad0, int i) { return rank_key(v, 4 * (quad0 + tid + (i / 4) * kThreads) + i % 4 - skew); };
+
+    float v[kEach];
+    load(first, v);
     const int token = p.token ? p.token[row] : -1;
     const bool has_token = token >= 0 && token < p.vocabulary;
     // A logit is ahead of the given token's where it reaches `equal`, by a lower index, or `larger`. (A token at -inf has all of lower index ahead of it, the ones that count as -inf
     // among them: these are added at the end.)
     const float mine = has_token ? fmaxf(__ldcg(x + token), -INFINITY) : INFINITY, larger = above(mine), equal = mine == -INFINITY ? NAN : mine;
     const int token_at = has_token ? token + skew : -1;
-    if (ALTERNATIVES) __syncthreads();
 
-    auto load = [&](int quad, float (&v)[kEach]) {
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j) {
-            const int at = 4 * (quad + j * kThreads);
-            float4 a = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            if (quad + j * kThreads < last) {
-                const float* from = x - skew + at;
-                if (at >= skew && at + 4 <= end) {
-                    a = __ldcs((const float4*)from);
-                } else {
-                    if (at >= skew && at < end) a.x = __ldcs(from);
-                    if (at + 1 >= skew && at + 1 < end) a.y = __ldcs(from + 1);
-                    if (at + 2 >= skew && at + 2 < end) a.z = __ldcs(from + 2);
-                    if (at + 3 >= skew && at + 3 < end) a.w = __ldcs(from + 3);
-                }
-            }
-            v[4 * j] = a.x; v[4 * j + 1] = a.y; v[4 * j + 2] = a.z; v[4 * j + 3] = a.w;
-        }
-    };
-
+    // ---- the share -------------------------------------------------------------------------------------
+    const int rounds = (p.share + kThreads * kQuads - 1) / (kThreads * kQuads), segment_rounds = (rounds + kSegments - 1) / kSegments;
     Sums sums = {-INFINITY, 0.0f, 0.0f};
-    int ahead = 0;
-    float bound = -INFINITY;  // logits above it may be alternatives
-    bool bounded = !ALTERNATIVES;
-    float now[kEach], then[kEach];
-    load(first + tid, then);
-    for (int quad0 = first; quad0 < last; quad0 += kThreads * kQuads) {
-        const int quad = quad0 + tid;
+    float segment_top = -INFINITY;
+    int ahead = 0, left = segment_rounds, segment = 0;
+    Pair sum = pair_of(0.0f, 0.0f), moment = sum;  // of the even logits, of the odd ones
+    const Pair scale = pair_of(kLog2e, kLog2e);
+    const bool ranked = p.rank != nullptr && has_token;
+    for (int round = 0, quad0 = first; round < rounds; ++round, quad0 += kThreads * kQuads) {
+        if (round) load(quad0, v);
+        float top = v[0];
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) now[i] = fmaxf(then[i], -INFINITY);  // (NaN counts as -inf)
-        load(quad + kThreads * kQuads, then);
-        float top = now[0];
-#pragma unroll
-        for (int i = 1; i < kEach; ++i) top = fmaxf(top, now[i]);
-        if (top > sums.top) sums.move_to(top);
-        float sum = 0.0f, moment = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const float d = fmaxf((now[i] - sums.top) * kLog2e, -200.0f), e = exp2_fast(d);  // (-inf: 2^-200 is none)
-            sum += e;
-            moment = fmaf(e, d, moment);
+        for (int i = 1; i < kEach; ++i) top = fmaxf(top, v[i]);
+        if (top > sums.top) {
+            // the sums against the new maximum: (m + s d) f, s f
+            const float d = sums.top == -INFINITY ? 0.0f : fmaxf((sums.top - top) * kLog2e, -200.0f), f = exp2_fast(d);
+            moment = pair_mul(pair_fma(sum, pair_of(d, d), moment), pair_of(f, f));
+            sum = pair_mul(sum, pair_of(f, f));
+            sums.top = top;
         }
-        sums.sum += sum;
-        sums.moment += moment;
+        const Pair down = pair_of(-sums.top, -sums.top);
+        Pair here = pair_of(0.0f, 0.0f), here_moment = here;
 #pragma unroll
-        for (int j = 0; j < kQuads; ++j) {
-            const int at = 4 * (quad + j * kThreads);
-            if (at <= token_at && token_at <= at + 3) {
+        for (int i = 0; i < kEach; i += 2) {
+            Pair d = pair_mul(pair_add(pair_of(v[i], v[i + 1]), down), scale);
+            const float a = fmaxf(pair_at(d, 0), -200.0f), b = fmaxf(pair_at(d, 1), -200.0f);  // (-inf and NaN: 2^-200 is none)
+            const Pair e = pair_of(exp2_fast(a), exp2_fast(b));
+            here = pair_add(here, e);
+            here_moment = pair_fma(e, pair_of(a, b), here_moment);
+        }
+        sum = pair_add(sum, here);
+        moment = pair_add(moment, here_moment);
+        if (ranked && top >= mine) {  // (none of a round's is ahead otherwise, and of a token at -inf all above are)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ahead += now[4 * j + e] >= (at + e < token_at ? equal : larger);
-            } else {
-                const float from = at < token_at ? equal : larger;
+            for (int j = 0; j < kQuads; ++j) {
+                const int at = 4 * (quad0 + tid + j * kThreads);
+                if (at <= token_at && token_at <= at + 3) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ahead += now[4 * j + e] >= from;
+                    for (int e = 0; e < 4; ++e) ahead += v[4 * j + e] >= (at + e < token_at ? equal : larger);
+                } else {
+                    const float from = at < token_at ? equal : larger;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ahead += v[4 * j + e] >= from;
+                }
             }
         }
         if (ALTERNATIVES) {
-            if (!bounded) {
-                // the least of the warps' k-th largest of their threads' largest logits
-                uint32_t key = ascending(top), kth = 0;
-                for (int k = (p.top + kWarps - 1) / kWarps; k > 0; --k) {
-                    kth = __reduce_max_sync(0xffffffffu, key);
-                    const uint32_t who = __ballot_sync(0xffffffffu, key == kth);
-                    if (lane == __ffs(who) - 1) key = 0;
-                }
-                if (lane == 0) sh.warp_bound[warp] = kth;
-                __syncthreads();
-                kth = sh.warp_bound[0];
-#pragma unroll
-                for (int w = 1; w < kWarps; ++w) kth = min(kth, sh.warp_bound[w]);
-                bound = below(value_of((u64)kth << 32));  // (logits that reach it are listed)
-                bounded = true;
-            }
-            const int held = sh.listed;
-            __syncthreads();  // (everybody has read it)
-            auto list = [&](u64 least) {
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    if (now[i] > bound) {
-                        const u64 key = rank_key(now[i], 4 * (quad + (i / 4) * kThreads) + i % 4 - skew);
-                        if (key < least) continue;
-                        const int at = atomicAdd(&sh.listed, 1);
-                        if (at < kList) sh.list[at] = key;
-                    }
-                }
-            };
-            if (top > bound) list(0);
-            __syncthreads();
-            int n = sh.listed;
-            if (n > kList) {
-                // again, with a bound that at most `top` threads reach: the top-th of the threads' largest keys, bit by bit
-                __syncthreads();
-                if (tid == 0) sh.listed = held;
-                u64 largest = 0;
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    const u64 key = now[i] > bound ? rank_key(now[i], 4 * (quad + (i / 4) * kThreads) + i % 4 - skew) : 0;
-                    largest = key > largest ? key : largest;
-                }
-                u64 least = 0;
-                for (int bit = 63; bit >= 0; --bit)
-                    if (__syncthreads_count(largest >= (least | 1ull << bit)) >= p.top) least |= 1ull << bit;
-                list(least);
-                __syncthreads();
-                n = sh.listed;
-            }
-            if (n > 2 * p.top + 32) {
-                keep_best(sh, n, p.top);
-                __syncthreads();
-                for (int i = tid; i < p.top; i += kThreads) sh.list[i] = sh.best[i];
-                if (tid == 0) sh.listed = p.top;
-                bound = value_of(sh.best[p.top - 1]);
-                __syncthreads();
+            segment_top = fmaxf(segment_top, top);
+            if (--left == 0) {
+                lists.largest[segment++][tid] = segment_top;
+                segment_top = -INFINITY;
+                left = segment_rounds;
             }
         }
     }
-
-    // ---- the CTA's sums and list -----------------------------------------------------------------------
+    sums.sum = pair_at(sum, 0) + pair_at(sum, 1);
+    sums.moment = pair_at(moment, 0) + pair_at(moment, 1);
+    if (ALTERNATIVES) {
+        if (left != segment_rounds) lists.largest[segment++][tid] = segment_top;
+        if (tid == 0) lists.listed = 0;
+        // the top-th of the threads' largest logits, by the upper sixteen bits of its place in their order
+        const uint32_t key = ascending(sums.top + 0.0f);
+        uint32_t bound = 0;
+#pragma unroll 1
+        for (int bit = 31; bit >= 16; --bit)
+            if (__syncthreads_count(key >= (bound | 1u << bit)) >= p.top) bound |= 1u << bit;
+        if (tid == 0) lists.bound = bound <= ascending(-INFINITY) ? -INFINITY : value_of((u64)bound << 32);
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
         Sums o;
@@ -244,75 +203,116 @@ __global__ void __launch_bounds__(kThreads) rq_logprobs_kernel(LogprobParams p) 
         sh.sums = sums;
         sh.ahead = ahead;
     }
-    if (ALTERNATIVES) {
-        const int n = keep_best(sh, sh.listed, p.top);
-        if (tid == 0) sh.found = n;
+    auto meet = [&]() {
+        if (ctas > 1) cluster.sync();
+        else __syncthreads();
+    };
+    meet();
+
+    // ---- the row's ---------------------------------------------------------------------------------
+    Sums all = sh.sums;
+    if (rank == 0)
+        for (int c = 1; c < ctas; ++c) all.add(cluster.map_shared_rank(&sh, c)->sums);
+    const bool nothing = all.top == -INFINITY;  // (the first CTA's to say)
+    const float log_sum = logf(all.sum);
+    if (rank == 0 && tid == 0) {
+        int before = mine == -INFINITY ? token : 0;
+        for (int c = 0; c < ctas; ++c) before += cluster.map_shared_rank(&sh, c)->ahead;
+        if (p.token) {
+            if (p.logprob) p.logprob[row] = !has_token ? 0.0f : (nothing || mine == -INFINITY ? -INFINITY : (mine - all.top) - log_sum);
+            if (p.rank) p.rank[row] = has_token && !nothing ? before : -1;
+        }
+        if (p.entropy) p.entropy[row] = nothing ? 0.0f : log_sum - all.moment / all.sum * kLn2;
     }
-    if (ctas > 1) cluster.sync();
-    else __syncthreads();
-    if (rank == 0) {
-        // ---- the row's -------------------------------------------------------------------------------
-        sums = sh.sums;
-        ahead = sh.ahead;
-        for (int c = 1; c < ctas; ++c) {
-            const Shared* other = cluster.map_shared_rank(&sh, c);
-            sums.add(other->sums);
-            ahead += other->ahead;
-        }
-        const bool nothing = sums.top == -INFINITY;
-        const float log_sum = logf(sums.sum);
-        if (tid == 0) {
-            if (p.token) {
-                if (p.logprob) p.logprob[row] = !has_token ? 0.0f : (nothing || mine == -INFINITY ? -INFINITY : (mine - sums.top) - log_sum);
-                if (p.rank) p.rank[row] = has_token && !nothing ? ahead + (mine == -INFINITY ? token : 0) : -1;
-            }
-            if (p.entropy) p.entropy[row] = nothing ? 0.0f : log_sum - sums.moment / sums.sum * kLn2;
-        }
-        if (ALTERNATIVES) {
-            int found = sh.found;
-            if (ctas > 1) {
-                // of the CTAs' lists, what is not below the last of a full one
-                u64 least = 0;
-                for (int c = 0; c < ctas; ++c) {
-                    const Shared* other = cluster.map_shared_rank(&sh, c);
-                    const u64 key = other->found == p.top ? other->best[p.top - 1] : 0;
-                    least = key > least ? key : least;
+    if (ALTERNATIVES) {
+        float bound = -INFINITY;
+        for (int c = 0; c < ctas; ++c) bound = fmaxf(bound, cluster.map_shared_rank(&lists, c)->bound);
+        Lists* const leader = cluster.map_shared_rank(&lists, 0);
+        // logits that reach the bound, and the key, to the first CTA
+        auto send = [&](u64 least) {
+            for (int n = 0; n < segment; ++n) {
+                if (!(lists.largest[n][tid] >= bound)) continue;
+                for (int round = n * segment_rounds; round < min((n + 1) * segment_rounds, rounds); ++round) {
+                    const int quad0 = first + round * kThreads * kQuads;
+                    load(quad0, v);
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {
+                        if (v[i] >= bound && v[i] > -INFINITY) {
+                            const u64 key = key_of(v[i], quad0, i);
+                            if (key < least) continue;
+                            const int at = atomicAdd(&leader->listed, 1);
+                            if (at < kList) leader->list[at] = key;
+                        }
+                    }
                 }
-                __syncthreads();
-                if (tid == 0) sh.listed = 0;
-                __syncthreads();
-                for (int i = tid; i < ctas * p.top; i += kThreads) {
-                    const int c = i / p.top, at = i % p.top;
-                    const Shared* other = cluster.map_shared_rank(&sh, c);
-                    if (at >= other->found) continue;
-                    const u64 key = other->best[at];
-                    if (key >= least) sh.list[atomicAdd(&sh.listed, 1)] = key;
-                }
-                __syncthreads();
-                found = keep_best(sh, sh.listed, p.top);
-                __syncthreads();
             }
+        };
+        send(0);
+        meet();
+        if (leader->listed > kList) {
+            // too many that are equal to the bound or nearly: the key of the top-th logit, bit by bit, is one that exactly `top` reach
+            u64 least = 0;
+#pragma unroll 1
+            for (int bit = 63; bit >= 0; --bit) {
+                const u64 tried = least | 1ull << bit;
+                int count = 0;
+                for (int n = 0; n < segment; ++n) {
+                    if (!(lists.largest[n][tid] >= bound)) continue;
+                    for (int round = n * segment_rounds; round < min((n + 1) * segment_rounds, rounds); ++round) {
+                        const int quad0 = first + round * kThreads * kQuads;
+                        load(quad0, v);
+#pragma unroll
+                        for (int i = 0; i < kEach; ++i) count += v[i] > -INFINITY && key_of(v[i], quad0, i) >= tried;
+                    }
+                }
+                const int of_warp = __reduce_add_sync(0xffffffffu, count);
+                if (lane == 0) lists.warp_count[warp] = of_warp;
+                __syncthreads();
+                if (tid == 0) {
+                    u64 sum = 0;
+                    for (int w = 0; w < kWarps; ++w) sum += lists.warp_count[w];
+                    lists.count = sum;
+                }
+                meet();
+                u64 sum = 0;
+                for (int c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(&lists, c)->count;
+                if (sum >= (u64)p.top) least = tried;
+                meet();  // (counts have been read)
+            }
+            if (rank == 0 && tid == 0) lists.listed = 0;
+            meet();
+            send(least);
+            meet();
+        }
+        if (rank == 0) {
+            const int n = lists.listed, found = min(n, p.top);
+            for (int i = tid; i < n; i += kThreads) {
+                const u64 key = lists.list[i];
+                int before = 0;
+#pragma unroll 8
+                for (int j = 0; j < n; ++j) before += lists.list[j] > key;
+                if (before < p.top) lists.best[before] = key;
+            }
+            __syncthreads();
             for (int i = tid; i < p.top; i += kThreads) {
                 const bool there = i < found;
-                if (p.top_token) p.top_token[(int64_t)row * p.top + i] = there ? (int32_t)~(uint32_t)sh.best[i] : -1;
-                if (p.top_logprob) p.top_logprob[(int64_t)row * p.top + i] = there ? (value_of(sh.best[i]) - sums.top) - log_sum : -INFINITY;
+                if (p.top_token) p.top_token[(int64_t)row * p.top + i] = there ? (int32_t)~(uint32_t)lists.best[i] : -1;
+                if (p.top_logprob) p.top_logprob[(int64_t)row * p.top + i] = there ? (value_of(lists.best[i]) - all.top) - log_sum : -INFINITY;
             }
         }
     }
     if (ctas > 1) cluster.sync();  // nobody leaves while its shared memory may be read
 }
 
+static_assert(sizeof(Lists) + sizeof(Shared) <= 47 * 1024, "48 KB need no opt-in");
+
 template <bool ALTERNATIVES>
-int launch_logprobs(rq_ctx* ctx, const LogprobParams& p, int rows, int ctas, cudaStream_t s) {
+int launch_logprobs(const LogprobParams& p, int rows, int ctas, cudaStream_t s) {
     auto kernel = rq_logprobs_kernel<ALTERNATIVES>;
-    static bool configured[64] = {};  // by device: the opt-in to clusters of sixteen
-    if (ctx->device >= 64 || !configured[ctx->device]) {
-        RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        if (ctx->device < 64) configured[ctx->device] = true;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * ctas));
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = ALTERNATIVES ? sizeof(Lists) : 0;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -342,5 +342,5 @@ extern "C" int rq_logprobs(rq_ctx* ctx, const float* logits, int64_t row_stride,
     while (ctas < kMostCtas && (int64_t)rows * ctas * 2 <= 8 * ctx->sm_count && vocabulary > (int64_t)ctas * 2 * kRound) ctas *= 2;
     LogprobParams p = {logits, token, logprob, entropy, top_logprob, rank, top_token, row_stride, (int)vocabulary, top, 0};
     p.share = (int)(((vocabulary + 3 + 3) / 4 + ctas - 1) / ctas);  // (a row may begin three logits behind a boundary)
-    return top > 0 ? launch_logprobs<true>(ctx, p, rows, ctas, (cudaStream_t)stream) : launch_logprobs<false>(ctx, p, rows, ctas, (cudaStream_t)stream);
+    return top > 0 ? launch_logprobs<true>(p, rows, ctas, (cudaStream_t)stream) : launch_logprobs<false>(p, rows, ctas, (cudaStream_t)stream);
 }
