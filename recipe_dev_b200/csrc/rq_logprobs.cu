@@ -2,13 +2,14 @@
 //
 //   log p_t = (x_t - m) - log Z,  Z = sum_i e^(x_i - m);  H = log Z - sum_i e^(x_i - m) (x_i - m) / Z: two terms that are not negative, nothing cancels
 //
-// A row is dealt out over a cluster of up to eight CTAs, a contiguous share each, which stream through it: a thread keeps a running maximum, the sum and the first moment against it,
-// and how many of its logits lie ahead of the given token's (whose logit is read beside the first ones). There is no barrier before the end of a share.
+// A row is dealt out over a cluster of up to eight CTAs (few rows: sixteen), a contiguous share each, which stream through it: a thread keeps a running maximum, the sum and the
+// first moment against it, and how many of its logits lie ahead of the given token's (whose logit is read beside the first ones). There is no barrier before the end of a share.
 // Alternatives: each thread also leaves the largest logit of each of up to sixteen segments of its logits in shared memory. The `top`-th largest of the threads' largest logits (its
-// upper sixteen bits, found by as many votes) is a bound that at least `top` logits of the share reach; the largest of the CTAs' bounds holds for the row. Segments that
-// reach it, a few times `top` of them, are read again (from L2), and their logits that reach it go to the first CTA's list through distributed shared memory, which puts them in
-// order by comparison of all with all. Where equal or ordered logits overflow the list, the exact key of the `top`-th logit is found bit by bit, in 64 rounds over the row.
-// Sums are joined in the order of warps and CTAs: the same bits on every run.
+// upper sixteen bits, by a search of one warp) is a bound that at least `top` logits of the share reach, and the largest of the CTAs' bounds holds for the row. Segments that
+// reach it are read again (from L2), and their logits that reach it, a few times `top` of the row's, go to the CTA's part of the first CTA's list, which puts them in order by
+// comparison of all with all. Where equal or ordered logits overflow a part, the exact key of the `top`-th logit is found bit by bit, in 64 rounds over the row. What
+// others need is written into their shared memory; a cluster meets twice.
+// Sums are joined in a fixed order: the same bits on every run.
 #include <cooperative_groups.h>
 
 #include "rq_pairs.cuh"
@@ -20,7 +21,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kQuads = 4, kEach = 4 * kQuads, kRound = kThreads * kEach;
-constexpr int kList = 2048, kMostCtas = 8, kSegments = 16;
+constexpr int kList = 2048, kMostCtas = 16, kSegments = 16;
 
 typedef unsigned long long u64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -63,17 +64,44 @@ struct Sums {
     }
 };
 
+// Sums of a warp's lanes, over lanes 0 .. n - 1 (a power of two) in lane 0, in a fixed order
+__device__ __forceinline__ void add_lanes(Sums& sums, int& ahead, int n) {
+    for (int off = n / 2; off > 0; off >>= 1) {
+        Sums o;
+        o.top = __shfl_down_sync(0xffffffffu, sums.top, off);
+        o.sum = __shfl_down_sync(0xffffffffu, sums.sum, off);
+        o.moment = __shfl_down_sync(0xffffffffu, sums.moment, off);
+        sums.add(o);
+        ahead += __shfl_down_sync(0xffffffffu, ahead, off);
+    }
+}
+
 struct Shared {
-    Sums warp_sums[kWarps], sums;
-    int warp_ahead[kWarps], ahead;
+    Sums warp_sums[kWarps];
+    int warp_ahead[kWarps];
+    // the first CTA's: of the CTAs
+    Sums sums[kMostCtas];
+    int ahead[kMostCtas];
+    float row_top, log_sum;
 };
 struct Lists {
-    float largest[kSegments][kThreads];  // of a thread's segments
-    u64 list[kList], best[RQ_MAX_ALTERNATIVES];
-    float bound;  // at least `top` logits of the share reach it
+    union {
+        float largest[kSegments][kThreads];  // of a thread's segments
+        u64 kept[kList];                     // the first CTA's, at the end: all logits that reach the row's bound (of small shared memory, loads have the L1 cache to be on their way in)
+    };
+    uint32_t keys[kThreads];             // of the threads' largest logits
     int listed;
+    // every CTA's: the CTAs' bounds, each reached by at least `top` logits of a share, and how many logits they have sent
+    float bounds[kMostCtas];
+    int sent[kMostCtas];
+    // the first CTA's: the CTAs' logits that reach the row's bound, a part each, and the first of them
+    u64 list[kList], best[RQ_MAX_ALTERNATIVES];
+    int held;
     u64 warp_count[kWarps], count;
 };
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 template <bool ALTERNATIVES>
 __global__ void __launch_bounds__(kThreads) rq_logprobs_kernel(LogprobParams p) {
@@ -83,6 +111,7 @@ __global__ void __launch_bounds__(kThreads) rq_logprobs_kernel(LogprobParams p) 
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     launch_dependents();
+    if (ctas > 1) cluster_arrive();  // (nobody writes to a CTA that has not begun)
     const float* x = p.logits + row * p.stride;
     // quads are counted from the 16-byte boundary at or before the row
     const int skew = (int)((uintptr_t)x >> 2 & 3), end = p.vocabulary + skew, quads = (end + 3) / 4;
@@ -178,57 +207,73 @@ __global__ void __launch_bounds__(kThreads) rq_logprobs_kernel(LogprobParams p) 
     sums.moment = pair_at(moment, 0) + pair_at(moment, 1);
     if (ALTERNATIVES) {
         if (left != segment_rounds) lists.largest[segment++][tid] = segment_top;
-        if (tid == 0) lists.listed = 0;
-        // the top-th of the threads' largest logits, by the upper sixteen bits of its place in their order
-        const uint32_t key = ascending(sums.top + 0.0f);
-        uint32_t bound = 0;
-#pragma unroll 1
-        for (int bit = 31; bit >= 16; --bit)
-            if (__syncthreads_count(key >= (bound | 1u << bit)) >= p.top) bound |= 1u << bit;
-        if (tid == 0) lists.bound = bound <= ascending(-INFINITY) ? -INFINITY : value_of((u64)bound << 32);
+        lists.keys[tid] = ascending(sums.top + 0.0f);
+        if (tid == 0) { lists.listed = 0; lists.held = 0; }
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        Sums o;
-        o.top = __shfl_xor_sync(0xffffffffu, sums.top, off);
-        o.sum = __shfl_xor_sync(0xffffffffu, sums.sum, off);
-        o.moment = __shfl_xor_sync(0xffffffffu, sums.moment, off);
-        sums.add(o);
-        ahead += __shfl_xor_sync(0xffffffffu, ahead, off);
-    }
+    add_lanes(sums, ahead, 32);
     if (lane == 0) { sh.warp_sums[warp] = sums; sh.warp_ahead[warp] = ahead; }
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kWarps; ++w) { sums.add(sh.warp_sums[w]); ahead += sh.warp_ahead[w]; }
-        sh.sums = sums;
-        sh.ahead = ahead;
+    if (ctas > 1) cluster_wait();
+    Shared* const first_sh = ctas > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
+    Lists* const first_lists = !ALTERNATIVES ? nullptr : (ctas > 1 ? cluster.map_shared_rank(&lists, 0) : &lists);
+    if (warp == kWarps - 1) {
+        sums = sh.warp_sums[lane % kWarps];
+        ahead = sh.warp_ahead[lane % kWarps];
+        add_lanes(sums, ahead, kWarps);
+        if (lane == 0) { first_sh->sums[rank] = sums; first_sh->ahead[rank] = ahead; }
     }
     auto meet = [&]() {
-        if (ctas > 1) cluster.sync();
+        if (ctas > 1) { cluster_arrive(); cluster_wait(); }
         else __syncthreads();
     };
+    const int part = kList / ctas;
+    if (ALTERNATIVES) {
+        if (warp == 0) {
+            // the top-th of the threads' largest logits, by the upper sixteen bits of its place in their order
+            uint32_t key[kThreads / 32], bound = 0;
+#pragma unroll
+            for (int i = 0; i < kThreads / 32; ++i) key[i] = lists.keys[32 * i + lane];
+#pragma unroll 1
+            for (int bit = 30; bit >= 16; bit -= 2) {  // two bits a step: how many reach each of three, ten bits a count
+                const uint32_t step = 1u << bit;
+                uint32_t count = 0;
+#pragma unroll
+                for (int i = 0; i < kThreads / 32; ++i) count += (key[i] >= bound + step ? 1u : 0u) + (key[i] >= bound + 2 * step ? 1u << 10 : 0u) + (key[i] >= bound + 3 * step ? 1u << 20 : 0u);
+                count = __reduce_add_sync(0xffffffffu, count);
+                if ((int)(count >> 20) >= p.top) bound += 3 * step;
+                else if ((int)(count >> 10 & 1023) >= p.top) bound += 2 * step;
+                else if ((int)(count & 1023) >= p.top) bound += step;
+            }
+            const float at = bound <= ascending(-INFINITY) ? -INFINITY : value_of((u64)bound << 32);
+            if (lane < ctas) (ctas > 1 ? cluster.map_shared_rank(&lists, lane) : &lists)->bounds[rank] = at;
+        }
+    }
     meet();
 
-    // ---- the row's ---------------------------------------------------------------------------------
-    Sums all = sh.sums;
-    if (rank == 0)
-        for (int c = 1; c < ctas; ++c) all.add(cluster.map_shared_rank(&sh, c)->sums);
-    const bool nothing = all.top == -INFINITY;  // (the first CTA's to say)
-    const float log_sum = logf(all.sum);
-    if (rank == 0 && tid == 0) {
-        int before = mine == -INFINITY ? token : 0;
-        for (int c = 0; c < ctas; ++c) before += cluster.map_shared_rank(&sh, c)->ahead;
-        if (p.token) {
-            if (p.logprob) p.logprob[row] = !has_token ? 0.0f : (nothing || mine == -INFINITY ? -INFINITY : (mine - all.top) - log_sum);
-            if (p.rank) p.rank[row] = has_token && !nothing ? before : -1;
+    // ---- the row's -----------------------------------------------------------------------------------
+    if (rank == 0 && warp == kWarps - 1) {
+        if (ctas > 1) {
+            sums = sh.sums[lane % ctas];
+            ahead = sh.ahead[lane % ctas];
+            add_lanes(sums, ahead, ctas);
         }
-        if (p.entropy) p.entropy[row] = nothing ? 0.0f : log_sum - all.moment / all.sum * kLn2;
+        if (lane == 0) {
+            const bool nothing = sums.top == -INFINITY;
+            const float log_sum = logf(sums.sum);
+            if (p.token) {
+                if (p.logprob) p.logprob[row] = !has_token ? 0.0f : (nothing || mine == -INFINITY ? -INFINITY : (mine - sums.top) - log_sum);
+                if (p.rank) p.rank[row] = has_token && !nothing ? ahead + (mine == -INFINITY ? token : 0) : -1;
+            }
+            if (p.entropy) p.entropy[row] = nothing ? 0.0f : log_sum - sums.moment / sums.sum * kLn2;
+            sh.row_top = sums.top;
+            sh.log_sum = log_sum;
+        }
+        __syncwarp();
     }
     if (ALTERNATIVES) {
-        float bound = -INFINITY;
-        for (int c = 0; c < ctas; ++c) bound = fmaxf(bound, cluster.map_shared_rank(&lists, c)->bound);
-        Lists* const leader = cluster.map_shared_rank(&lists, 0);
-        // logits that reach the bound, and the key, to the first CTA
+        // logits that reach the bound, and the key, to this CTA's part of the first one's list
+        float bound = lists.bounds[0];
+        for (int c = 1; c < ctas; ++c) bound = fmaxf(bound, lists.bounds[c]);
         auto send = [&](u64 least) {
             for (int n = 0; n < segment; ++n) {
                 if (!(lists.largest[n][tid] >= bound)) continue;
@@ -240,17 +285,21 @@ __global__ void __launch_bounds__(kThreads) rq_logprobs_kernel(LogprobParams p) 
                         if (v[i] >= bound && v[i] > -INFINITY) {
                             const u64 key = key_of(v[i], quad0, i);
                             if (key < least) continue;
-                            const int at = atomicAdd(&leader->listed, 1);
-                            if (at < kList) leader->list[at] = key;
+                            const int at = atomicAdd(&lists.listed, 1);
+                            if (at < part) first_lists->list[rank * part + at] = key;
                         }
                     }
                 }
             }
+            __syncthreads();
+            if (tid < ctas) (ctas > 1 ? cluster.map_shared_rank(&lists, tid) : &lists)->sent[rank] = lists.listed;
         };
         send(0);
         meet();
-        if (leader->listed > kList) {
-            // too many that are equal to the bound or nearly: the key of the top-th logit, bit by bit, is one that exactly `top` reach
+        bool overflow = false;
+        for (int c = 0; c < ctas; ++c) overflow = overflow || lists.sent[c] > part;
+        if (overflow) {
+            // too many that are equal to a bound or nearly: the key of the top-th logit, bit by bit, is one that exactly `top` reach
             u64 least = 0;
 #pragma unroll 1
             for (int bit = 63; bit >= 0; --bit) {
@@ -262,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) rq_logprobs_kernel(LogprobParams p) 
                         const int quad0 = first + round * kThreads * kQuads;
                         load(quad0, v);
 #pragma unroll
-                        for (int i = 0; i < kEach; ++i) count += v[i] > -INFINITY && key_of(v[i], quad0, i) >= tried;
+                        for (int i = 0; i < kEach; ++i) count += v[i] >= bound && v[i] > -INFINITY && key_of(v[i], quad0, i) >= tried;
                     }
                 }
                 const int of_warp = __reduce_add_sync(0xffffffffu, count);
@@ -275,40 +324,46 @@ __global__ void __launch_bounds__(kThreads) rq_logprobs_kernel(LogprobParams p) 
                 }
                 meet();
                 u64 sum = 0;
-                for (int c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(&lists, c)->count;
+                for (int c = 0; c < ctas; ++c) sum += (ctas > 1 ? cluster.map_shared_rank(&lists, c) : &lists)->count;
                 if (sum >= (u64)p.top) least = tried;
                 meet();  // (counts have been read)
             }
-            if (rank == 0 && tid == 0) lists.listed = 0;
-            meet();
+            if (tid == 0) lists.listed = 0;
+            __syncthreads();
             send(least);
             meet();
         }
-        if (rank == 0) {
-            const int n = lists.listed, found = min(n, p.top);
-            for (int i = tid; i < n; i += kThreads) {
-                const u64 key = lists.list[i];
-                int before = 0;
+        if (rank != 0) return;
+        // all that is needed lies in the first CTA
+        for (int c = warp; c < ctas; c += kWarps)
+            for (int i = lane; i < lists.sent[c]; i += 32) lists.kept[atomicAdd(&lists.held, 1)] = lists.list[c * part + i];
+        __syncthreads();
+        const int n = lists.held, found = min(n, p.top);
+        for (int i = tid; i < n; i += kThreads) {
+            const u64 key = lists.kept[i];
+            int before = 0;
 #pragma unroll 8
-                for (int j = 0; j < n; ++j) before += lists.list[j] > key;
-                if (before < p.top) lists.best[before] = key;
-            }
-            __syncthreads();
-            for (int i = tid; i < p.top; i += kThreads) {
-                const bool there = i < found;
-                if (p.top_token) p.top_token[(int64_t)row * p.top + i] = there ? (int32_t)~(uint32_t)lists.best[i] : -1;
-                if (p.top_logprob) p.top_logprob[(int64_t)row * p.top + i] = there ? (value_of(lists.best[i]) - all.top) - log_sum : -INFINITY;
-            }
+            for (int j = 0; j < n; ++j) before += lists.kept[j] > key;
+            if (before < p.top) lists.best[before] = key;
+        }
+        __syncthreads();
+        for (int i = tid; i < p.top; i += kThreads) {
+            const bool there = i < found;
+            if (p.top_token) p.top_token[(int64_t)row * p.top + i] = there ? (int32_t)~(uint32_t)lists.best[i] : -1;
+            if (p.top_logprob) p.top_logprob[(int64_t)row * p.top + i] = there ? (value_of(lists.best[i]) - sh.row_top) - sh.log_sum : -INFINITY;
         }
     }
-    if (ctas > 1) cluster.sync();  // nobody leaves while its shared memory may be read
 }
 
-static_assert(sizeof(Lists) + sizeof(Shared) <= 47 * 1024, "48 KB need no opt-in");
-
 template <bool ALTERNATIVES>
-int launch_logprobs(const LogprobParams& p, int rows, int ctas, cudaStream_t s) {
+int launch_logprobs(rq_ctx* ctx, const LogprobParams& p, int rows, int ctas, cudaStream_t s) {
     auto kernel = rq_logprobs_kernel<ALTERNATIVES>;
+    static bool configured[64] = {};  // by device: the opt-ins to clusters of sixteen and to large shared memory
+    if (ctx->device >= 64 || !configured[ctx->device]) {
+        RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        if (ALTERNATIVES) RQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Lists)));
+        if (ctx->device < 64) configured[ctx->device] = true;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * ctas));
     cfg.blockDim = dim3(kThreads);
@@ -338,9 +393,10 @@ extern "C" int rq_logprobs(rq_ctx* ctx, const float* logits, int64_t row_stride,
     if (top > 0 && !top_token && !top_logprob) return rq_fail(RQ_ERR_INVALID, "rq_logprobs: alternatives without a place for them");
     if (((uintptr_t)logits & 3) != 0) return rq_fail(RQ_ERR_INVALID, "rq_logprobs: logits must be 4-byte aligned");
     DeviceGuard guard(ctx->device);
+    // CTAs a row: as many as the GPU holds at once (four an SM), of shares of two rounds and more; sixteen where every CTA has an SM to itself
     int ctas = 1;
-    while (ctas < kMostCtas && (int64_t)rows * ctas * 2 <= 8 * ctx->sm_count && vocabulary > (int64_t)ctas * 2 * kRound) ctas *= 2;
+    while (ctas < kMostCtas && (int64_t)rows * ctas * 2 <= (ctas == 8 ? 1 : 4) * ctx->sm_count && vocabulary > (int64_t)ctas * 2 * kRound) ctas *= 2;
     LogprobParams p = {logits, token, logprob, entropy, top_logprob, rank, top_token, row_stride, (int)vocabulary, top, 0};
     p.share = (int)(((vocabulary + 3 + 3) / 4 + ctas - 1) / ctas);  // (a row may begin three logits behind a boundary)
-    return top > 0 ? launch_logprobs<true>(p, rows, ctas, (cudaStream_t)stream) : launch_logprobs<false>(p, rows, ctas, (cudaStream_t)stream);
+    return top > 0 ? launch_logprobs<true>(ctx, p, rows, ctas, (cudaStream_t)stream) : launch_logprobs<false>(ctx, p, rows, ctas, (cudaStream_t)stream);
 }
