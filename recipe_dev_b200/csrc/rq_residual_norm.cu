@@ -68,32 +68,25 @@ __global__ void __launch_bounds__(1024) rq_residual_norm_kernel(JoinParams p) {
     wait_for_previous();
     const float one_gate = p.gate && !p.gate_elements ? __ldcg(gate) : 1.0f;
     float of_delta = 1.0f;
+    // what is read of a gain or gate: ones where there is none
+    auto ones_or = [&](const float* from, int64_t at) { return from ? load4<WIDE, true>(from, at, p.n) : make_float4(1.0f, 1.0f, 1.0f, 1.0f); };
+    auto gate_of = [&](int64_t at) { return p.gate && p.gate_elements ? load4<WIDE>(gate, at, p.n) : make_float4(one_gate, one_gate, one_gate, one_gate); };
     // x' of four elements
-    auto join = [&](float4 a, float4 d, int64_t at) {
-        if (p.delta_gain) {
-            const float4 g = load4<WIDE, true>(p.delta_gain, at, p.n);
-            d.x = d.x * of_delta * g.x; d.y = d.y * of_delta * g.y; d.z = d.z * of_delta * g.z; d.w = d.w * of_delta * g.w;
-        }
-        if (p.gate) {
-            const float4 g = p.gate_elements ? load4<WIDE, true>(gate, at, p.n) : make_float4(one_gate, one_gate, one_gate, one_gate);
-            d.x *= g.x; d.y *= g.y; d.z *= g.z; d.w *= g.w;
-        }
-        return make_float4(fmaf(p.scale, d.x, a.x), fmaf(p.scale, d.y, a.y), fmaf(p.scale, d.z, a.z), fmaf(p.scale, d.w, a.w));
+    auto join = [&](float4 a, float4 d, float4 of_block, float4 g) {
+        if (p.delta_gain) { d.x = d.x * of_delta * of_block.x; d.y = d.y * of_delta * of_block.y; d.z = d.z * of_delta * of_block.z; d.w = d.w * of_delta * of_block.w; }
+        return make_float4(fmaf(p.scale, d.x * g.x, a.x), fmaf(p.scale, d.y * g.y, a.y), fmaf(p.scale, d.z * g.z, a.z), fmaf(p.scale, d.w * g.w, a.w));
     };
-    auto normed = [&](float4 v, float f, int64_t at) {
-        v.x *= f; v.y *= f; v.z *= f; v.w *= f;
-        if (p.gain) {
-            const float4 g = load4<WIDE, true>(p.gain, at, p.n);
-            v.x *= g.x; v.y *= g.y; v.z *= g.z; v.w *= g.w;
-        }
-        return v;
-    };
+    auto normed = [&](float4 v, float f, float4 g) { return make_float4(v.x * f * g.x, v.y * f * g.y, v.z * f * g.z, v.w * f * g.w); };
     auto factor = [&](float sum) { return 1.0f / sqrtf(sum / (float)p.n + p.epsilon); };
     if (HELD) {
         constexpr int N = HELD ? HELD : 1;
-        float4 a[N], d[N];
+        constexpr bool kAhead = N <= 2;  // gains and gates on their way with the rest (of four, registers do not hold them)
+        float4 a[N], d[N], g[N], block_gain[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) { d[i] = load4<WIDE>(delta, first + i * step, p.n); a[i] = load4<WIDE>(x, first + i * step, p.n); }
+        if (kAhead)
+#pragma unroll
+            for (int i = 0; i < N; ++i) { g[i] = gate_of(first + i * step); block_gain[i] = ones_or(p.delta_gain, first + i * step); }
         if (p.delta_gain) {
             float sum = 0.0f;
 #pragma unroll
@@ -103,13 +96,16 @@ __global__ void __launch_bounds__(1024) rq_residual_norm_kernel(JoinParams p) {
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            a[i] = join(a[i], d[i], first + i * step);
+            a[i] = kAhead ? join(a[i], d[i], block_gain[i], g[i]) : join(a[i], d[i], ones_or(p.delta_gain, first + i * step), gate_of(first + i * step));
             store4<WIDE>(out, first + i * step, p.n, a[i]);
             sum = squares(a[i], sum);
         }
+        if (kAhead)
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] = ones_or(p.gain, first + i * step);
         const float f = factor(block_sum(sum, ahead));
 #pragma unroll
-        for (int i = 0; i < N; ++i) store4<WIDE>(y, first + i * step, p.n, normed(a[i], f, first + i * step));
+        for (int i = 0; i < N; ++i) store4<WIDE>(y, first + i * step, p.n, normed(a[i], f, kAhead ? g[i] : ones_or(p.gain, first + i * step)));
     } else {
         if (p.delta_gain) {
             float sum = 0.0f;
@@ -120,14 +116,14 @@ __global__ void __launch_bounds__(1024) rq_residual_norm_kernel(JoinParams p) {
         float sum = 0.0f;
 #pragma unroll 2
         for (int64_t at = first; at < p.n; at += step) {
-            const float4 v = join(load4<WIDE>(x, at, p.n), load4<WIDE>(delta, at, p.n), at);
+            const float4 v = join(load4<WIDE>(x, at, p.n), load4<WIDE>(delta, at, p.n), ones_or(p.delta_gain, at), gate_of(at));
             store4<WIDE>(out, at, p.n, v);
             sum = squares(v, sum);
         }
         const float f = factor(block_sum(sum, ahead));
         // (a thread reads again what it wrote itself)
 #pragma unroll 4
-        for (int64_t at = first; at < p.n; at += step) store4<WIDE>(y, at, p.n, normed(load4<WIDE>(out, at, p.n), f, at));
+        for (int64_t at = first; at < p.n; at += step) store4<WIDE>(y, at, p.n, normed(load4<WIDE>(out, at, p.n), f, ones_or(p.gain, at)));
     }
 }
 
