@@ -1,10 +1,12 @@
 """What the serving step's newer calls refuse, they refuse before anything of the device is touched (no GPU: the context is a stand-in that nothing looks into)."""
 import ctypes as C
+from types import SimpleNamespace
 
 import pytest
 
 import recipe_dev_b200 as rq
 from recipe_dev_b200 import capi
+
 
 @pytest.fixture(scope="module")
 def lib():
@@ -73,3 +75,15 @@ def test_tensors_of_the_wrong_place():
         ctx.logprobs(plane, ints)
     with pytest.raises(ValueError, match="device"):
         ctx.residual_norm(plane, plane)
+
+
+def test_the_small_decoder():
+    pytest.importorskip("torch")
+    from recipe_dev_b200 import serve
+
+    for how in (dict(norms="behind"), dict(residual_scale=0.5)):
+        with pytest.raises(ValueError, match="norms"):
+            serve.Decoder(None, 1, 64, 1, 1, 64, 64, 10, 4, **how)
+    for n in (-1, 65):
+        with pytest.raises(ValueError, match="alternatives"):
+            serve.Batch(SimpleNamespace(positions=32, vocabulary=100), [[1]], 1, logprobs=n)
