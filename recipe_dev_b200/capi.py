@@ -785,37 +785,42 @@ class Context:
         Planes are fp32 [tokens, n] with contiguous tokens; without delta_gain delta is taken as it is, without gain the norm has none; gate: [n], [tokens, 1] or [tokens, n]."""
         if _F32 is None:
             _with_torch()
+        shape, device = x.shape, self.device
+        tokens, n = shape
         if x_out is None:
             x_out = x
         if y is None:
             import torch
 
-            y = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-        tokens, n = x.shape
-        planes = []
-        for a in (x, delta, x_out, y):
-            if a.dtype is not _F32 or a.get_device() != self.device or a.shape != x.shape or a.stride(1) != 1:
-                raise ValueError("residual_norm: x, delta, x_out and y must be CUDA fp32 planes [tokens, n] with contiguous tokens, on the context's device")
-            planes.append((a.data_ptr(), a.stride(0)))
-        gains = []
-        for g in (delta_gain, gain):
-            if g is not None and (g.dtype is not _F32 or g.get_device() != self.device or g.shape != (n,) or not g.is_contiguous()):
-                raise ValueError("residual_norm: a gain holds n contiguous fp32 values")
-            gains.append(0 if g is None else g.data_ptr())
-        at = by_element = by_token = 0
+            y = torch.empty(shape, dtype=torch.float32, device=x.device)
+        (x_stride, xe), (d_stride, de), (o_stride, oe), (y_stride, ye) = x.stride(), delta.stride(), x_out.stride(), y.stride()
+        # (in one condition: a loop over the planes takes a short call a third longer)
+        if not (x.dtype is delta.dtype is x_out.dtype is y.dtype is _F32 and xe == de == oe == ye == 1 and delta.shape == shape and (x_out is x or x_out.shape == shape) and y.shape == shape
+                and x.get_device() == delta.get_device() == x_out.get_device() == y.get_device() == device):
+            raise ValueError("residual_norm: x, delta, x_out and y must be CUDA fp32 planes [tokens, n] with contiguous tokens, on the context's device")
+        gain_at = delta_gain_at = gate_at = by_element = by_token = 0
+        if gain is not None:
+            gain_at = self._gain(gain, n)
+        if delta_gain is not None:
+            delta_gain_at = self._gain(delta_gain, n)
         if gate is not None:
             shape, stride = gate.shape, gate.stride()
-            if gate.dtype is not _F32 or gate.get_device() != self.device or shape not in ((n,), (tokens, 1), (tokens, n)):
-                raise ValueError("residual_norm: a gate is CUDA fp32 [n], [tokens, 1] or [tokens, n]")
-            at, by_element, by_token = gate.data_ptr(), int(shape[-1] == n and n > 1), stride[0] if len(shape) == 2 else 0
+            if gate.dtype is not _F32 or gate.get_device() != device or shape not in ((n,), (tokens, 1), (tokens, n)):
+                raise ValueError("residual_norm: a gate is CUDA fp32 [n], [tokens, 1] or [tokens, n], on the context's device")
+            gate_at, by_element, by_token = gate.data_ptr(), int(shape[-1] == n and n > 1), stride[0] if len(shape) == 2 else 0
             if by_element and stride[-1] != 1:
                 raise ValueError("residual_norm: a gate's values of a token must be contiguous")
-        (x_at, x_stride), (d_at, d_stride), (o_at, o_stride), (y_at, y_stride) = planes
-        rc = self.lib.rq_residual_norm(self.handle, x_at, x_stride, d_at, d_stride, n, tokens, gains[0], at, by_element, by_token, residual_scale, gains[1], epsilon, o_at, o_stride,
-                                       y_at, y_stride, self._on(stream))
+        rc = self.lib.rq_residual_norm(self.handle, x.data_ptr(), x_stride, delta.data_ptr(), d_stride, n, tokens, delta_gain_at, gate_at, by_element, by_token, residual_scale, gain_at, epsilon,
+                                       x_out.data_ptr(), o_stride, y.data_ptr(), y_stride, self._on(stream))
         if rc:
             _check(rc)
         return y
+
+    def _gain(self, gain, n: int) -> int:
+        """The address of a gain of n values."""
+        if gain.dtype is not _F32 or gain.get_device() != self.device or gain.shape != (n,) or not gain.is_contiguous():
+            raise ValueError("residual_norm: a gain holds n contiguous fp32 values on the context's device")
+        return gain.data_ptr()
 
     def activation_records(self, x, step: int, stream=None):
         """The 36-byte int8 records of x ([cols] or [tokens, cols]) as a uint8 CUDA tensor."""
