@@ -58,11 +58,8 @@ template <int D, int TYPE, int RT> struct Tiles {
     uint2 q_lo[TYPE == RQ_KV_BF16 ? RT : 1][D / 16][32];  // the third parts
 };
 
-// CTAs that an SM holds, by what their shared memory and their sums in registers leave room for
-template <int D, int TYPE, int RT> constexpr int kResident = D == 256 || (RT == 2 && (D == 128 || TYPE == RQ_KV_BF16)) ? 2 : (D == 64 && TYPE == RQ_KV_F16 && RT == 1 ? 4 : 3);
-
 template <int D, int TYPE, int RT>
-__global__ void __launch_bounds__(kThreads, kResident<D, TYPE, RT>) rq_attention_rows_kernel(AttentionParams p) {
+__global__ void __launch_bounds__(kThreads) rq_attention_rows_kernel(AttentionParams p) {
     constexpr int ROWS = 8 * RT, STEPS = D / 16, PARTS = TYPE == RQ_KV_F16 ? 2 : 3, CHUNKS = D / 8, LINES = 32 / CHUNKS > 0 ? 32 / CHUNKS : 1;
     extern __shared__ __align__(128) unsigned char dynamic[];
     Tiles<D, TYPE, RT>& sh = *(Tiles<D, TYPE, RT>*)dynamic;

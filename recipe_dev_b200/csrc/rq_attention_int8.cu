@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D, RT>) rq_attention_int8_
                 *(float4*)&sh.out[warp][rt * 8 + g][16 * n + 4 * t4] = make_float4(pair_at(acc[rt][2 * n], 0), pair_at(acc[rt][2 * n + 1], 0), pair_at(acc[rt][2 * n], 1), pair_at(acc[rt][2 * n + 1], 1));
         }
         __syncthreads();
-        join_rows<D, ROWS, kLead>(p, &sh.out[0][0][0], warp_base, warp_sum, item_begin, item_end, deal, start, row0, rows, kv, last_arrival);
+        join_rows<D, ROWS, kLead, true>(p, &sh.out[0][0][0], warp_base, warp_sum, item_begin, item_end, deal, start, row0, rows, kv, last_arrival);
         __syncthreads();  // the shared sums are free again
     }
 }

@@ -89,13 +89,14 @@ template <int D> __device__ __forceinline__ void put_row(const AttentionParams& 
     else { y[e] = v.x; y[e + 1] = v.y; y[e + 2] = v.z; y[e + 3] = v.w; }
 }
 
-// The parts that CTAs first_cta .. last_cta have left of some rows, joined.
+// The parts that CTAs first_cta .. last_cta have left of some rows, joined: many of them. (Of few, each thread is done by itself sooner than through shared memory: a token over 1001 keys
+// 9.1 us, 10.4 so.)
 template <int D, int ROWS>
 __device__ __forceinline__ void join_parts(const AttentionParams& p, float* out, int64_t first_cta, int64_t last_cta, int start, int row0, int rows, int kv) {
     const int tid = threadIdx.x;
     const int64_t stride = ROWS * (D + 2);
     // The parts' bases and sums of weights are brought by all threads side by side, some parts at a time, and their sums many at once; they are added up in CTA order. (Each thread
-    // for itself, one load behind another, took the last CTA of 55 ten microseconds.)
+    // for itself, a few loads at a time, took the last CTA of 55 ten microseconds.)
     constexpr int ITEMS = (ROWS * (D / 4) + kThreads - 1) / kThreads, kParts = 64;
     static_assert(kThreads % ROWS == 0 && 2 * kParts * ROWS <= kWarps * ROWS * (D + 8) && kThreads <= kWarps * ROWS * (D + 8), "the place of the warps' sums");
     const int parts = (int)(last_cta - first_cta) + 1, my_row = tid % ROWS;
@@ -142,8 +143,10 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, float* out,
 }
 
 // The warps' sums of rows (out: [warp][row][D + 8]; their bases and sums of weights) to y, or, where other CTAs have parts of the rows' units [item_begin, item_end), to the
-// work area; the last of those CTAs joins the parts in CTA order (LEAD: as dealt, the first units of an item are nobody's work). start: the request's first token. Begins behind a barrier that all have written before.
-template <int D, int ROWS, int LEAD = 0>
+// work area; the last of those CTAs joins the parts in CTA order (LEAD: as dealt, the first units of an item are nobody's work; MANY: of more than kFewParts by join_parts). start: the
+// request's first token. Begins behind a barrier that all have written before.
+constexpr int kFewParts = 16;
+template <int D, int ROWS, int LEAD = 0, bool MANY = false>
 __device__ __forceinline__ void join_rows(const AttentionParams& p, float* out, const float (&warp_base)[kWarps][ROWS], const float (&warp_sum)[kWarps][ROWS], int64_t item_begin,
                                           int64_t item_end, const Deal& deal, int start, int row0, int rows, int kv, uint32_t& last_arrival) {
     const int tid = threadIdx.x;
@@ -182,7 +185,28 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, float* out, 
         if (last_arrival == (uint32_t)(last_cta - first_cta)) {
             if (tid == 0) p.arrived[first_cta] = 0;
             __threadfence();
-            join_parts<D, ROWS>(p, out, first_cta, last_cta, start, row0, rows, kv);
+            if (MANY && last_cta - first_cta >= kFewParts) {
+                join_parts<D, ROWS>(p, out, first_cta, last_cta, start, row0, rows, kv);
+                return;
+            }
+            for (int i = tid; i < ROWS * (D / 4); i += kThreads) {
+                const int row = i / (D / 4), e = 4 * (i % (D / 4));
+                if (row >= rows) break;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float weight = 0.0f, top = -INFINITY;
+#pragma unroll 8
+                for (int64_t c = first_cta; c <= last_cta; ++c) top = fmaxf(top, __ldcg(p.partial + (c * 2 + (c == first_cta)) * stride + ROWS * D + row));
+                const float to = top == -INFINITY ? 0.0f : top;
+#pragma unroll 8
+                for (int64_t c = first_cta; c <= last_cta; ++c) {
+                    const float* from = p.partial + (c * 2 + (c == first_cta)) * stride;
+                    const float f = exp2_fast(__ldcg(from + ROWS * D + row) - to);
+                    const float4 o = __ldcg((const float4*)(from + row * D + e));
+                    v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
+                    weight = fmaf(__ldcg(from + ROWS * D + ROWS + row), f, weight);
+                }
+                put_row<D>(p, start, row0 + row, kv, e, v, weight);
+            }
         }
     }
 }
