@@ -403,7 +403,7 @@ int launch_rows(rq_ctx* ctx, const AttentionParams& p, int type, bool two, cudaS
     if (type == RQ_KV_F16) return two ? launch_rows<D, RQ_KV_F16, MOST>(ctx, p, s) : launch_rows<D, RQ_KV_F16, 1>(ctx, p, s);
     return two ? launch_rows<D, RQ_KV_BF16, MOST>(ctx, p, s) : launch_rows<D, RQ_KV_BF16, 1>(ctx, p, s);
 }
-int launch_rows_of(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s) {
+int launch_rows_of(rq_ctx* ctx, const CodesParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s) {
     if (cache.type == RQ_KV_INT8) return launch_rows_int8(ctx, p, cache, two, s);
     if (cache.head_dim == 64) return launch_rows<64>(ctx, p, cache.type, two, s);
     if (cache.head_dim == 128) return launch_rows<128>(ctx, p, cache.type, two, s);
@@ -444,7 +444,7 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
     if (rc) return rc;
     rc = rq_order_work_areas(ctx, s);
     if (rc) return rc;
-    AttentionParams p = {};
+    CodesParams p = {};
     p.q = q; p.y = y; p.k = (const uint16_t*)cache->k; p.v = (const uint16_t*)cache->v; p.block_table = block_table; p.starts = starts; p.lengths = lengths;
     p.partial = (float*)ctx->attn_scratch; p.arrived = (uint32_t*)(ctx->attn_scratch + kPartialBytes);
     p.q_stride = q_t_stride; p.y_stride = y_t_stride; p.table_stride = table_stride; p.head_stride = cache->head_stride; p.pages = cache->pages; p.tokens = tokens; p.requests = requests; p.q_heads = q_heads; p.kv_heads = cache->heads;

@@ -19,7 +19,10 @@ struct AttentionParams {
     int wide;  // q and y allow accesses of 16 bytes (1), of 32 (2)
     int* error_flag;
     unsigned long long wait_ns;
-    const float *k_scale, *v_scale;  // a cache of codes: of each position's head
+};
+// A cache of codes: the scales of each position's head
+struct CodesParams : AttentionParams {
+    const float *k_scale, *v_scale;
     int64_t scale_page, scale_head, scale_line;
 };
 
@@ -32,10 +35,10 @@ constexpr size_t kPartialBytes = sizeof(float) * (kTensorPartial > kRowPartial ?
 
 // Rows by the hundred (rq_attention_tc.cu); one_tile: at most 128 rows a request and key head. RQ_ERR_UNSUPPORTED (no error text) = a cache that it does not
 // serve: 256 elements a head, pages of fewer than eight positions, strides of zero.
-int launch_tensor(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool one_tile, cudaStream_t s);
+int launch_tensor(rq_ctx* ctx, const CodesParams& p, const rq_kv_cache& cache, bool one_tile, cudaStream_t s);
 
 // Rows by the few over a cache of codes (rq_attention_int8.cu); two: sixteen rows at a time
-int launch_rows_int8(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s);
+int launch_rows_int8(rq_ctx* ctx, const CodesParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s);
 
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are 2^(s - max + kRaise): an f16 part below 2^-14 loses bits, raised by 2^12 that is a weight of 2^-26 of the row's largest. bf16 has fp32's exponents: its

@@ -76,7 +76,7 @@ template <int D, int RT> struct Tiles {
 template <int D, int RT> constexpr int kResident = D == 256 || (D == 128 && RT == 2) ? 2 : (D == 64 && RT == 1 ? 4 : 3);
 
 template <int D, int RT>
-__global__ void __launch_bounds__(kThreads, kResident<D, RT>) rq_attention_int8_kernel(AttentionParams p) {
+__global__ void __launch_bounds__(kThreads, kResident<D, RT>) rq_attention_int8_kernel(CodesParams p) {
     using F = Form<D>;
     constexpr int ROWS = 8 * RT, STEPS = D / 32, TILE = F::TILE, UNIT = kWarps * TILE, NT = TILE / 8, LINES = F::LINES;
     constexpr uint32_t ALL = TILE == 32 ? 0xffffffffu : 0xffffu;
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D, RT>) rq_attention_int8_
 }
 
 template <int D, int RT>
-int launch_rows(rq_ctx* ctx, const AttentionParams& p, cudaStream_t s) {
+int launch_rows(rq_ctx* ctx, const CodesParams& p, cudaStream_t s) {
     auto kernel = rq_attention_int8_kernel<D, RT>;
     // The grid decides where rows are cut, and with it the last bits: it follows from the call alone. Shared memory holds eight bytes a request, by steps of 128 of them.
     const int step = (p.requests + kRequestStep - 1) / kRequestStep, dev = ctx->device;
@@ -446,7 +446,7 @@ int launch_rows(rq_ctx* ctx, const AttentionParams& p, cudaStream_t s) {
 
 }  // namespace
 
-int rqattn::launch_rows_int8(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s) {
+int rqattn::launch_rows_int8(rq_ctx* ctx, const CodesParams& p, const rq_kv_cache& cache, bool two, cudaStream_t s) {
     if (cache.head_dim == 64) return two ? launch_rows<64, 2>(ctx, p, s) : launch_rows<64, 1>(ctx, p, s);
     if (cache.head_dim == 128) return two ? launch_rows<128, 2>(ctx, p, s) : launch_rows<128, 1>(ctx, p, s);
     return launch_rows<256, 1>(ctx, p, s);

@@ -80,8 +80,7 @@ template <int ROWS, int TILE, int LEAD = 0> __device__ __forceinline__ Deal deal
 }
 
 // A row's results: sums over the sum of weights
-template <int D> __device__ __forceinline__ void put_row(const AttentionParams& p, int start, int at, int kv, int e, float4 v, float total_weight) {
-    const int group = p.q_heads / p.kv_heads;
+template <int D> __device__ __forceinline__ void put_row(const AttentionParams& p, int group, int start, int at, int kv, int e, float4 v, float total_weight) {
     float* y = p.y + (int64_t)(start + at / group) * p.y_stride + (int64_t)(kv * group + at % group) * D;
     const float inverse = total_weight == 0.0f ? 0.0f : 1.0f / total_weight;
     v.x *= inverse; v.y *= inverse; v.z *= inverse; v.w *= inverse;
@@ -138,7 +137,7 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, float* out,
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int item = tid + i * kThreads, row = item / (D / 4), e = 4 * (item % (D / 4));
-        if (row < rows) put_row<D>(p, start, row0 + row, kv, e, v[i], weight[i]);
+        if (row < rows) put_row<D>(p, p.q_heads / p.kv_heads, start, row0 + row, kv, e, v[i], weight[i]);
     }
 }
 
@@ -149,7 +148,7 @@ constexpr int kFewParts = 16;
 template <int D, int ROWS, int LEAD = 0, bool MANY = false>
 __device__ __forceinline__ void join_rows(const AttentionParams& p, float* out, const float (&warp_base)[kWarps][ROWS], const float (&warp_sum)[kWarps][ROWS], int64_t item_begin,
                                           int64_t item_end, const Deal& deal, int start, int row0, int rows, int kv, uint32_t& last_arrival) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, group = p.q_heads / p.kv_heads;
     const int64_t first_cta = ((item_begin + LEAD + 1) * deal.ctas - 1) / deal.total, last_cta = (item_end * deal.ctas - 1) / deal.total;
     const bool whole = first_cta == last_cta;
     const int64_t stride = ROWS * (D + 2);
@@ -166,12 +165,12 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, float* out, 
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float f = exp2_fast(warp_base[w][row] - to);
-            const float4 o = *(const float4*)&out[((int64_t)w * ROWS + row) * (D + 8) + e];
+            const float4 o = *(const float4*)&out[(w * ROWS + row) * (D + 8) + e];
             v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
             weight = fmaf(warp_sum[w][row], f, weight);
         }
         if (whole) {
-            put_row<D>(p, start, row0 + row, kv, e, v, weight);
+            put_row<D>(p, group, start, row0 + row, kv, e, v, weight);
         } else {
             __stcg((float4*)(mine + row * D + e), v);
             if (e == 0) { __stcg(mine + ROWS * D + row, top); __stcg(mine + ROWS * D + ROWS + row, weight); }
@@ -205,7 +204,7 @@ __device__ __forceinline__ void join_rows(const AttentionParams& p, float* out, 
                     v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
                     weight = fmaf(__ldcg(from + ROWS * D + ROWS + row), f, weight);
                 }
-                put_row<D>(p, start, row0 + row, kv, e, v, weight);
+                put_row<D>(p, group, start, row0 + row, kv, e, v, weight);
             }
         }
     }

@@ -49,6 +49,7 @@ constexpr int kItems = 4, kWords = 16;  // rings in shared memory: items, words 
 // CODES: the cache holds 8-bit codes, TYPE is what they become
 template <int D, int TYPE, bool KEYS_, bool CODES_> struct Form {
     static constexpr bool KEYS = KEYS_, CODES = CODES_;
+    using Params = std::conditional_t<CODES, CodesParams, AttentionParams>;
     // what the block is launched with is dealt out anew: 2 * 224 + 56 = 3 * 168; 2 * 208 + 2 * 48 = 4 * 128
     static constexpr int WIDENERS = CODES ? 4 : 0, THREADS = (12 + WIDENERS) * 32, SOFTMAX_REGS = CODES ? 208 : 224, OTHER_REGS = CODES ? 48 : 56;
     static constexpr int PARTS = TYPE == RQ_KV_F16 ? 2 : 3;
@@ -277,7 +278,7 @@ template <int D, int TYPE, bool KEYS> __device__ __forceinline__ float load_quer
 }
 
 template <int D, int TYPE, bool KEYS, bool CODES>
-__global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_attention_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+__global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_attention_tc_kernel(const __grid_constant__ typename Form<D, TYPE, KEYS, CODES>::Params p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using F = Form<D, TYPE, KEYS, CODES>;
     constexpr int PARTS = F::PARTS, KT = F::KT, STAGES = F::STAGES;
     extern __shared__ __align__(1024) unsigned char dynamic[];
@@ -385,84 +386,86 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
     // of eight lines in that of their own): a warp has read them before it writes there. A lane's pieces are 16 codes, one load, two stores, so that no eight lanes meet a
     // bank twice.
     auto widen = [&](int which) {
-        constexpr int SHARE = KT / 64, PIECES = D / 32;  // scales, pieces of sixteen lines, of a lane
-        Ring at(STAGES);
-        uint32_t key_tiles = 0;
-        while (const Item* it = next_item()) {
-            const int tiles = it->take * (KEYS ? 2 : 1);
-            const int32_t* table = p.block_table + (int64_t)it->r * p.table_stride + (it->first_key >> p.page_shift);
-            const float* scales = (which < 2 ? p.k_scale : p.v_scale) + it->kv * p.scale_head;
-            const int first = (which & 1) * (KT / 2) + lane, line0 = it->first_key & ((1 << p.page_shift) - 1), low = it->low - it->first_key, high = it->high - it->first_key;  // keys from the item's first
-            // Scales are on their way while the tile before is widened, and their pages' entries while the one before that is
-            int page[SHARE];
-            float scale[SHARE];
-            auto find = [&](int tile) {
-#pragma unroll
-                for (int i = 0; i < SHARE; ++i) {
-                    const int key = tile * KT + first + 32 * i;
-                    page[i] = key >= low && key < high ? __ldcg(table + ((line0 + key) >> p.page_shift)) : -1;
-                }
-            };
-            auto load = [&](int tile) {
-#pragma unroll
-                for (int i = 0; i < SHARE; ++i) {
-                    const int line = (line0 + tile * KT + first + 32 * i) & ((1 << p.page_shift) - 1);
-                    scale[i] = page[i] >= 0 && page[i] < p.pages ? __ldcg(scales + page[i] * p.scale_page + line * p.scale_line) : 0.0f;
-                }
-            };
-            find(0);
-            load(0);
-            find(1);
-            for (int n = 0, tile = 0; n < 2 * tiles; ++n, at.next()) {
-                const bool values = is_values(n, tiles);
-                const int slot = at.slot;
-                if (!mbar_wait_warp(&sh.landed[slot], at.phase, p.wait_ns, dead)) atomicExch(p.error_flag, 54);
-                if (dead) break;  // (the tile may be on its way: it is not touched, and not handed on)
-                // (short loops: laid out in a line they cost the softmax its place in the instruction caches, 236 -> 259 us)
-#pragma unroll 1
-                for (int block = which; block < KT / 16; block += F::WIDENERS) {
-                    uint8_t* const out = ring + slot * F::TILE_BYTES + block * 2048;
-                    uint4 raw[PIECES];
-#pragma unroll
-                    for (int i = 0; i < PIECES; ++i) {
-                        if (D == 64) raw[i] = *(const uint4*)(out + (p.page_shift == 3 ? 512 * (2 * i + 1) : 1024 + 512 * i) + 16 * lane);
-                        else raw[i] = *(const uint4*)(out + KT * 128 + (8 * (i >> 1) + (lane >> 2)) * 128 + ((i & 1) ^ (lane >> 2 & 1)) * 64 + (lane & 3) * 16);
-                    }
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < PIECES; ++i) {
-                        const int line = 8 * (D == 64 ? i : i >> 1) + (lane >> 2);
-                        uint8_t* const to = out + (D == 64 ? 0 : (i & 1) ^ (lane >> 2 & 1)) * (KT * 128);
-                        const uint32_t x = turn_codes(raw[i].x), y = turn_codes(raw[i].y), z = turn_codes(raw[i].z), w = turn_codes(raw[i].w);
-                        *(uint4*)(to + swizzled(line, 2 * (lane & 3))) = make_uint4(widen_codes<0, 1>(x), widen_codes<2, 3>(x), widen_codes<0, 1>(y), widen_codes<2, 3>(y));
-                        *(uint4*)(to + swizzled(line, 2 * (lane & 3) + 1)) = make_uint4(widen_codes<0, 1>(z), widen_codes<2, 3>(z), widen_codes<0, 1>(w), widen_codes<2, 3>(w));
-                    }
-                }
-                if (!values) {
-                    const int place = key_tiles++ % F::SCALE_TILES;
-                    int most = 0, least = 254;
+        if constexpr (CODES) {
+            constexpr int SHARE = KT / 64, PIECES = D / 32;  // scales, pieces of sixteen lines, of a lane
+            Ring at(STAGES);
+            uint32_t key_tiles = 0;
+            while (const Item* it = next_item()) {
+                const int tiles = it->take * (KEYS ? 2 : 1);
+                const int32_t* table = p.block_table + (int64_t)it->r * p.table_stride + (it->first_key >> p.page_shift);
+                const float* scales = (which < 2 ? p.k_scale : p.v_scale) + it->kv * p.scale_head;
+                const int first = (which & 1) * (KT / 2) + lane, line0 = it->first_key & ((1 << p.page_shift) - 1), low = it->low - it->first_key, high = it->high - it->first_key;  // keys from the item's first
+                // Scales are on their way while the tile before is widened, and their pages' entries while the one before that is
+                int page[SHARE];
+                float scale[SHARE];
+                auto find = [&](int tile) {
 #pragma unroll
                     for (int i = 0; i < SHARE; ++i) {
-                        sh.scales[place][which >> 1][first + 32 * i] = scale[i];
-                        const int e = (int)(__float_as_uint(scale[i]) >> 23 & 0xff);
-                        most = max(most, e);
-                        least = min(least, scale[i] == 0.0f ? 254 : e);  // (a value of zero takes no weight's bits)
+                        const int key = tile * KT + first + 32 * i;
+                        page[i] = key >= low && key < high ? __ldcg(table + ((line0 + key) >> p.page_shift)) : -1;
                     }
-                    most = __reduce_max_sync(0xffffffffu, most);
-                    least = __reduce_min_sync(0xffffffffu, least);
-                    if (which >= 2 && lane == 0) { sh.levels[place][which & 1][0] = most; sh.levels[place][which & 1][1] = least; }
+                };
+                auto load = [&](int tile) {
+#pragma unroll
+                    for (int i = 0; i < SHARE; ++i) {
+                        const int line = (line0 + tile * KT + first + 32 * i) & ((1 << p.page_shift) - 1);
+                        scale[i] = page[i] >= 0 && page[i] < p.pages ? __ldcg(scales + page[i] * p.scale_page + line * p.scale_line) : 0.0f;
+                    }
+                };
+                find(0);
+                load(0);
+                find(1);
+                for (int n = 0, tile = 0; n < 2 * tiles; ++n, at.next()) {
+                    const bool values = is_values(n, tiles);
+                    const int slot = at.slot;
+                    if (!mbar_wait_warp(&sh.landed[slot], at.phase, p.wait_ns, dead)) atomicExch(p.error_flag, 54);
+                    if (dead) break;  // (the tile may be on its way: it is not touched, and not handed on)
+                    // (short loops: laid out in a line they cost the softmax its place in the instruction caches, 236 -> 259 us)
+#pragma unroll 1
+                    for (int block = which; block < KT / 16; block += F::WIDENERS) {
+                        uint8_t* const out = ring + slot * F::TILE_BYTES + block * 2048;
+                        uint4 raw[PIECES];
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i) {
+                            if (D == 64) raw[i] = *(const uint4*)(out + (p.page_shift == 3 ? 512 * (2 * i + 1) : 1024 + 512 * i) + 16 * lane);
+                            else raw[i] = *(const uint4*)(out + KT * 128 + (8 * (i >> 1) + (lane >> 2)) * 128 + ((i & 1) ^ (lane >> 2 & 1)) * 64 + (lane & 3) * 16);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i) {
+                            const int line = 8 * (D == 64 ? i : i >> 1) + (lane >> 2);
+                            uint8_t* const to = out + (D == 64 ? 0 : (i & 1) ^ (lane >> 2 & 1)) * (KT * 128);
+                            const uint32_t x = turn_codes(raw[i].x), y = turn_codes(raw[i].y), z = turn_codes(raw[i].z), w = turn_codes(raw[i].w);
+                            *(uint4*)(to + swizzled(line, 2 * (lane & 3))) = make_uint4(widen_codes<0, 1>(x), widen_codes<2, 3>(x), widen_codes<0, 1>(y), widen_codes<2, 3>(y));
+                            *(uint4*)(to + swizzled(line, 2 * (lane & 3) + 1)) = make_uint4(widen_codes<0, 1>(z), widen_codes<2, 3>(z), widen_codes<0, 1>(w), widen_codes<2, 3>(w));
+                        }
+                    }
+                    if (!values) {
+                        const int place = key_tiles++ % F::SCALE_TILES;
+                        int most = 0, least = 254;
+#pragma unroll
+                        for (int i = 0; i < SHARE; ++i) {
+                            sh.scales[place][which >> 1][first + 32 * i] = scale[i];
+                            const int e = (int)(__float_as_uint(scale[i]) >> 23 & 0xff);
+                            most = max(most, e);
+                            least = min(least, scale[i] == 0.0f ? 254 : e);  // (a value of zero takes no weight's bits)
+                        }
+                        most = __reduce_max_sync(0xffffffffu, most);
+                        least = __reduce_min_sync(0xffffffffu, least);
+                        if (which >= 2 && lane == 0) { sh.levels[place][which & 1][0] = most; sh.levels[place][which & 1][1] = least; }
+                    }
+                    fence_to_tensor_core();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.full[slot]);
+                    if (!values) {
+                        load(++tile);
+                        find(tile + 1);
+                    }
                 }
-                fence_to_tensor_core();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.full[slot]);
-                if (!values) {
-                    load(++tile);
-                    find(tile + 1);
-                }
+                if (lane == 0) mbar_arrive(&sh.item_empty[item_at.slot]);
+                item_at.next();
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.item_empty[item_at.slot]);
-            item_at.next();
         }
     };
 
@@ -1061,7 +1064,7 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
 }
 
 template <int D, int TYPE, bool KEYS, bool CODES = false>
-int launch_form(rq_ctx* ctx, const AttentionParams& p, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
+int launch_form(rq_ctx* ctx, const CodesParams& p, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s) {
     using F = Form<D, TYPE, KEYS, CODES>;
     auto kernel = rq_attention_tc_kernel<D, TYPE, KEYS, CODES>;
     constexpr size_t smem = F::Q_BYTES + F::STAGES * F::TILE_BYTES + sizeof(Shared<F>);
@@ -1072,7 +1075,7 @@ int launch_form(rq_ctx* ctx, const AttentionParams& p, const CUtensorMap& k, con
         if (ctx->device < 64) configured[ctx->device] = true;
     }
     const int ctas = ctx->sm_count < kTensorCtas ? ctx->sm_count : kTensorCtas;
-    return launch(kernel, dim3((unsigned)ctas), F::THREADS, smem, s, p, k, v);
+    return launch(kernel, dim3((unsigned)ctas), F::THREADS, smem, s, (const typename F::Params&)p, k, v);
 }
 
 // The cache as a TMA reads it: elements, lines, heads, pages; a copy is 64 elements of `lines` lines, swizzled as the tensor core reads them (codes: whole lines, as they are)
@@ -1094,7 +1097,7 @@ int make_map(CUtensorMap* map, const void* base, const rq_kv_cache& c, int lines
 
 }  // namespace
 
-int rqattn::launch_tensor(rq_ctx* ctx, const AttentionParams& p, const rq_kv_cache& c, bool one_tile, cudaStream_t s) {
+int rqattn::launch_tensor(rq_ctx* ctx, const CodesParams& p, const rq_kv_cache& c, bool one_tile, cudaStream_t s) {
     // pages of whole groups of eight lines (the swizzle's), and strides that a tensor map can hold
     if (c.head_dim > 128 || c.page_size < 8 || c.line_stride <= 0 || (c.heads > 1 && c.head_stride <= 0) || (c.pages > 1 && c.page_stride <= 0) || c.head_stride >= (int64_t)1 << 38) return RQ_ERR_UNSUPPORTED;
     const int tile = c.type == RQ_KV_INT8 ? 1 << kCodesShift : (c.type == RQ_KV_F16 || c.head_dim == 64 ? 128 : 64), lines = c.page_size < tile ? c.page_size : tile;
