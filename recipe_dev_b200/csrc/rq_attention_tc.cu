@@ -46,12 +46,18 @@ constexpr int kCodesShift = 4;  // a copy of codes brings at most sixteen lines
 constexpr int kEven = 12;       // exponents of a tile's scales of values that lie no further apart need no look at each
 constexpr int kItems = 4, kWords = 16;  // rings in shared memory: items, words on tiles of keys
 
+// Taking a block up (its queries, the first scores, the sums at the end: 21 us) costs as much as some units (3.9 us): so many lead each block's own in the dealing.
+// Without it the CTAs that got a prompt's first blocks, short ones, were the last to end. 32 + 2 x 8 heads of 128, f16, without | with, over the same batches again and
+// again: four prompts of 1021 to 3001 tokens 620 | 350 us, one of 12001 2816 | 1883, eight of 512 138 | 120, two of 3001 with windows of 1000 425 | 244, 509 tokens over 7680 125 |
+// 123; 32 of 128, all blocks of one unit, 67 | 68; 16 requests of 48 rows over 8192 keys 205 | 219.
+// Over codes a unit takes longer: by three 509 tokens over 7680 keys 164 us, the four prompts 452, by four 164 and 461, by two 164 and 467.
+
 // CODES: the cache holds 8-bit codes, TYPE is what they become
 template <int D, int TYPE, bool KEYS_, bool CODES_> struct Form {
     static constexpr bool KEYS = KEYS_, CODES = CODES_;
     using Params = std::conditional_t<CODES, CodesParams, AttentionParams>;
-    // what the block is launched with is dealt out anew: 2 * 224 + 56 = 3 * 168; 2 * 208 + 2 * 48 = 4 * 128
-    static constexpr int WIDENERS = CODES ? 4 : 0, THREADS = (12 + WIDENERS) * 32, SOFTMAX_REGS = CODES ? 208 : 224, OTHER_REGS = CODES ? 48 : 56;
+    // registers that the block is launched with are dealt out anew: 2 * 224 + 56 = 3 * 168; 2 * 200 + 2 * 56 = 4 * 128 (208 and 48: the four prompts 469 us in place of 461)
+    static constexpr int WIDENERS = CODES ? 4 : 0, THREADS = (12 + WIDENERS) * 32, SOFTMAX_REGS = CODES ? 200 : 224, OTHER_REGS = 56, LEAD = CODES ? 3 : 4;
     static constexpr int PARTS = TYPE == RQ_KV_F16 ? 2 : 3;
     static constexpr int KT = TYPE == RQ_KV_F16 || D == 64 ? 128 : 64;  // keys a tile (bf16, 128 elements: 2 KT + 2 D + KT columns are what tensor memory holds with 64)
     static constexpr int TILE_BYTES = KT * D * 2, Q_PART = 128 * D * 2, Q_BYTES = (KEYS ? 1 : 2) * PARTS * Q_PART;
@@ -92,12 +98,6 @@ template <typename F> __device__ __forceinline__ Block block_of(const AttentionP
     k.units = max(1, (k.high - k.begin + F::UNIT - 1) / F::UNIT);
     return k;
 }
-
-// Taking a block up (its queries, the first scores, the sums at the end: 21 us) costs as much as some units (3.9 us): so many lead each block's own in the dealing.
-// Without it the CTAs that got a prompt's first blocks, short ones, were the last to end. 32 + 2 x 8 heads of 128, f16, without | with, over the same batches again and
-// again: four prompts of 1021 to 3001 tokens 620 | 350 us, one of 12001 2816 | 1883, eight of 512 138 | 120, two of 3001 with windows of 1000 425 | 244, 509 tokens over 7680 125 |
-// 123; 32 of 128, all blocks of one unit, 67 | 68; 16 requests of 48 rows over 8192 keys 205 | 219.
-constexpr int kLead = 4;
 
 // One block's part of a CTA's range of units, as the roles need it; take = 0: there are no more
 struct Item {
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
             const int r = r0 + tid;
             int64_t units = 0;
             if (r < p.requests)
-                for (int b = blocks_of<F>(p, r, group) - 1; b >= 0; --b) units += kLead + block_of<F>(p, r, b, group).units;
+                for (int b = blocks_of<F>(p, r, group) - 1; b >= 0; --b) units += F::LEAD + block_of<F>(p, r, b, group).units;
             units *= p.kv_heads;
             int64_t scan = units;
 #pragma unroll
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
             int units = 1;
             if (total)
                 while (true) {
-                    units = kLead + block_of<F>(p, r, b, group).units;
+                    units = F::LEAD + block_of<F>(p, r, b, group).units;
                     if (left < (int64_t)units * p.kv_heads) break;
                     left -= (int64_t)units * p.kv_heads;
                     ++b;
@@ -969,14 +969,14 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
             Item i = {};
             if (u < end && !dead) {
                 const Block k = block_of<F>(p, r, b, group);
-                const int64_t item_begin = u - offset, item_end = item_begin + kLead + k.units;
-                const int first_unit = max(offset - kLead, 0);
+                const int64_t item_begin = u - offset, item_end = item_begin + F::LEAD + k.units;
+                const int first_unit = max(offset - F::LEAD, 0);
                 u = min(item_end, end);
-                i.take = max((int)(u - item_begin) - kLead - first_unit, 0);  // (none where a range ends in a block's lead: the next CTA has it all)
+                i.take = max((int)(u - item_begin) - F::LEAD - first_unit, 0);  // (none where a range ends in a block's lead: the next CTA has it all)
                 i.first_key = k.begin + first_unit * F::UNIT;
                 i.low = k.low; i.high = k.high; i.end = k.end; i.start = k.start; i.row0 = k.row0; i.rows = k.rows; i.position0 = k.position0; i.kv = kv; i.r = r;
-                const bool all = offset <= kLead && u == item_end;  // nobody else's
-                i.first_cta = all ? blockIdx.x : (int)(((item_begin + kLead + 1) * ctas - 1) / total);
+                const bool all = offset <= F::LEAD && u == item_end;  // nobody else's
+                i.first_cta = all ? blockIdx.x : (int)(((item_begin + F::LEAD + 1) * ctas - 1) / total);
                 i.last_cta = all ? blockIdx.x : (int)((item_end * ctas - 1) / total);
                 offset = 0;
                 if (++kv == p.kv_heads) {
