@@ -355,7 +355,8 @@ int rq_rope_table(rq_ctx* ctx, double base, double frequency_scale, int rotary, 
  * (x / sqrt(mean(x^2) + epsilon) * gain; gain null: no norm), then the rotation of its first `rotary` elements by the row
  * positions[t] of the table (a position outside it is clamped into it),
  *   (a, b) -> (a cos - b sin, a sin + b cos), pairs (a, b) = (x[i], x[i + rotary / 2]) for RQ_ROPE_HALVES, (x[2 i], x[2 i + 1]) for RQ_ROPE_PAIRS,
- * queries to q_out (which may be q), keys and, as they are, values to the cache at slots[t] (a slot outside it is passed over),
+ * queries to q_out (which may be q), keys and, as they are, values to the cache at slots[t] (a slot outside it is passed over; what a slot holds that several tokens of
+ * the call name is not defined),
  * rounded to the cache's type once. RQ_KV_INT8: a head's scale is its largest magnitude over 127 (fp32), its codes are x / scale rounded to the nearest whole
  * number, ties to even; a head of zeros (or one whose scale would be less than 2^-126) has scale 0 and codes 0, one with an infinity or a NaN has that as its scale. Heads of a token lie head_dim apart; tokens *_t_stride apart, any alignment. rotary: a
  * multiple of 16 up to head_dim, or 0 (no rotation, no table). */

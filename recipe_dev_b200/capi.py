@@ -274,6 +274,8 @@ class KvCache:
                 raise ValueError("KvCache: an int8 cache needs k_scale and v_scale")
             if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or not k_scale.is_cuda or not v_scale.is_cuda or k_scale.shape != k.shape[:3] or v_scale.shape != k.shape[:3] or k_scale.stride() != v_scale.stride():
                 raise ValueError("KvCache: k_scale and v_scale must be CUDA float32 tensors [pages, heads, page_size] of one layout")
+            if not k.device == v.device == k_scale.device == v_scale.device:
+                raise ValueError("KvCache: codes and scales must lie on one device")
             scales = (k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride())
         elif k_scale is not None or v_scale is not None:
             raise ValueError("KvCache: only an int8 cache has scales")

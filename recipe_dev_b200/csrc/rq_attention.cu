@@ -462,7 +462,9 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
     // The rows kernel reads a request's keys once for every sixteen rows (from L2, from the second time on), the tensor-core kernel makes scores of 128 whatever
     // there is. 8192 cached keys, 32 + 2 x 8 heads of 128, f16, rows kernel | tensor cores: 16 requests of 16 rows 102 | 217 us, 32 rows 180 | 219, 48 rows 259 | 219,
     // 128 rows 656 | 209; one request of 32 rows 35 | 44, 48 rows 39 | 44, 128 rows 71 | 45. bf16: 16 requests of 32 rows 265 | 371, 48 rows 407 | 373.
-    if (rows > 32) {
+    // Over codes, whose widening the tensor-core kernel repeats for every 128 or 256 rows: 16 requests of 32 rows 143 | 206, 48 rows 213 | 206, 64 rows 285 | 207; one request of 48 rows 34 | 49, 64
+    // rows 33 | 49, 128 rows 52 | 50; 64 elements a head, 16 requests of 48 rows 123 | 177, 64 rows 157 | 177.
+    if (rows > (cache->type == RQ_KV_INT8 ? 48 : 32)) {
         // Where a request may be a decode step among prompts, the rows kernel takes those and the tensor-core kernel the rest: 63 decode steps over 4096 keys and
         // a chunk of 512 are 267 us in two launches, 509 by the tensor cores alone, 531 by the rows kernel alone; 7 over 300 keys and a prompt of 100: 33, 27, 22.
         const int few = requests > 1 && tokens < requests * (rows / group) ? (group <= 8 ? 8 : 32) : 0;
