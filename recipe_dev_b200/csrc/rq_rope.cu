@@ -7,7 +7,7 @@
 // contiguous access and the other element of a pair half a head apart one shuffle; the four sums of squares are added up together. Everything is held in fp32 and a
 // key or value is rounded once, to the cache's type. (In place: a warp has read what it writes.) 2039 tokens of 32 + 2 x 8 heads of 128: 22.0 us, 4.2 TB/s; with five
 // shuffles and a square root a head 23.8, and of that form with two heads a warp 24.4, eight 27.7, CTAs of eight warps 24.9; one head a warp 30.3. 64 tokens 10.1 us, one
-// 9.4, which is what a call from Python takes.
+// 9.4, which is what a call from Python takes. Into a cache of codes, whose heads' largest magnitudes are one reduction of a warp each: 2039 tokens 23.7 us, 3.8 TB/s.
 #include "rq_serve.cuh"
 
 using namespace rqserve;
