@@ -186,6 +186,7 @@ static const char* wait_code_text(int code) {
         case 51: return "attention, mending warp: a tile of values never arrived";
         case 52: return "attention, softmax warps: the other pipe's sums never came";
         case 53: return "attention, softmax warps: a row's factor never came";
+        case 54: return "attention, widening warps: a tile of codes never arrived";
         default: return "unknown wait";
     }
 }
