@@ -196,3 +196,38 @@ def test_recorded_and_on_another_stream(rq_ctx):
         torch.cuda.synchronize()
         assert torch.equal(out["logprob"], want["logprob"]) and torch.equal(out["top_token"], want["top_token"])
     sequence.free()
+
+
+def test_refusals(rq_ctx):
+    import torch
+
+    x, t = torch.zeros((3, 50), device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    f = torch.zeros(3, device="cuda")
+    tops = torch.zeros((3, 4), dtype=torch.int32, device="cuda")
+    for wrong in (dict(logits=x.double()), dict(logits=x.T), dict(logits=x.cpu()), dict(token=t.long()), dict(token=t[:2]), dict(logprob=f.double()), dict(rank=f), dict(entropy=f[:2]),
+                  dict(top_token=tops, top_logprob=torch.zeros((3, 5), device="cuda")), dict(top_token=tops[:2]), dict(top_token=tops[:, :0]), dict(token=None, rank=t), dict(token=None, logprob=f)):
+        with pytest.raises(ValueError):
+            rq_ctx.logprobs(**dict(logits=x, token=t) | wrong)
+    import recipe_dev_b200 as rq
+
+    with pytest.raises(rq.RqError, match="0 to 64"):
+        rq_ctx.logprobs(x, top_token=torch.zeros((3, 65), dtype=torch.int32, device="cuda"))
+    rq_ctx.check()
+
+
+@pytest.mark.parametrize("rows,vocabulary", [(1, 262144), (3, 131072), (37, 65537), (40, 262144), (148, 33000)])
+@pytest.mark.parametrize("top", [1, 64])
+def test_every_number_of_ctas_a_row(rq_ctx, rows, vocabulary, top):
+    compare(rq_ctx, *some(rows, vocabulary, rows), top)
+
+
+def test_all_alternatives_in_one_share(rq_ctx):
+    """The likeliest tokens are neighbours: one CTA has them all, and few of its threads."""
+    import torch
+
+    x, token = some(5, 200001, 3)
+    x[0, 150000:150064] += 50.0
+    x[1, -70:] += 50.0
+    x[2, :64] = torch.linspace(40.0, 41.0, 64, device="cuda")
+    x[3, 77777:77787] = 60.0
+    compare(rq_ctx, x, token, 64)

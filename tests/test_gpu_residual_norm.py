@@ -136,3 +136,26 @@ def test_recorded(rq_ctx):
         want_x = torch.empty_like(x)
         assert torch.equal(rq_ctx.residual_norm(x, delta, gain, x_out=want_x), y) and torch.equal(want_x, out)
     sequence.free()
+
+
+def test_refusals(rq_ctx):
+    import torch
+
+    x, n = torch.zeros((4, 64), device="cuda"), torch.zeros(64, device="cuda")
+    for wrong in (dict(delta=x[:, :32]), dict(delta=x.double()), dict(delta=x.cpu()), dict(delta=x.T.contiguous().T), dict(gain=n[:32]), dict(delta_gain=n.double()), dict(gate=torch.zeros(4, device="cuda")),
+                  dict(gate=torch.zeros((4, 32), device="cuda")), dict(gate=torch.zeros((64, 4), device="cuda").T), dict(y=x[:2]), dict(x_out=x[:, :32])):
+        with pytest.raises(ValueError):
+            rq_ctx.residual_norm(**dict(x=x, delta=x, gain=n) | wrong)
+    rq_ctx.check()
+
+
+def test_gates_by_broadcast_and_by_stride(rq_ctx):
+    import torch
+
+    x, delta = torch.randn((5, 96), device="cuda"), torch.randn((5, 96), device="cuda")
+    gate = torch.randn((5, 200), device="cuda")
+    for g in (gate[:, 3:99], gate[:, 7:8], gate[:1, :96].expand(5, 96)):
+        out = torch.empty_like(x)
+        rq_ctx.residual_norm(x, delta, gate=g, x_out=out)
+        want = x.double() + g.double() * delta.double()
+        assert ((out.double() - want).abs() <= STEP * (2 * (g.double() * delta.double()).abs() + want.abs())).all()
