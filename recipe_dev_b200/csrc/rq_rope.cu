@@ -7,7 +7,7 @@
 // contiguous access and the other element of a pair half a head apart one shuffle; the four sums of squares are added up together. Everything is held in fp32 and a
 // key or value is rounded once, to the cache's type. (In place: a warp has read what it writes.) 2039 tokens of 32 + 2 x 8 heads of 128: 22.0 us, 4.2 TB/s; with five
 // shuffles and a square root a head 23.8, and of that form with two heads a warp 24.4, eight 27.7, CTAs of eight warps 24.9; one head a warp 30.3. 64 tokens 10.1 us, one
-// 9.4, which is what a call from Python takes. Into a cache of codes, whose heads' largest magnitudes are one reduction of a warp each: 2039 tokens 23.7 us, 3.8 TB/s.
+// 9.4, which is what a call from Python takes. Into a cache of codes, whose heads' largest magnitudes are one reduction of a warp each: 2039 tokens 21.5 us, 4.1 TB/s (f16 21.5 among its own calls too; of that with an address for each head 22.6).
 #include "rq_serve.cuh"
 
 using namespace rqserve;
@@ -65,15 +65,21 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
     const int head0 = (int)(item % (uint32_t)groups) * kHeads;
     wait_for_previous();
     if (t >= (uint32_t)p.tokens) return;
-    // every head's elements on their way at once, with the token's place and position
+    // every head's elements on their way at once, with the token's place and position; heads of one plane lie side by side
     float x[kHeads][E];
+    auto plane_of = [&](int head) {
+        return (head < p.q_heads ? p.q + t * p.q_stride + (int64_t)head * D
+                                 : (head < p.q_heads + p.kv_heads ? p.k + t * p.k_stride + (int64_t)(head - p.q_heads) * D : p.v + t * p.v_stride + (int64_t)(head - p.q_heads - p.kv_heads) * D)) + first;
+    };
+    const int end_of_plane = head0 < p.q_heads ? p.q_heads : (head0 < p.q_heads + p.kv_heads ? p.q_heads + p.kv_heads : heads);
+    const bool one_plane = head0 + kHeads <= end_of_plane;
+    if (one_plane) {
+        const float* from = plane_of(head0);
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        const int head = min(head0 + i, heads - 1);  // (one past the last is loaded for nothing)
-        const bool is_q = head < p.q_heads, is_k = head < p.q_heads + p.kv_heads;
-        const float* from = is_q ? p.q + t * p.q_stride + (int64_t)head * D
-                                 : (is_k ? p.k + t * p.k_stride + (int64_t)(head - p.q_heads) * D : p.v + t * p.v_stride + (int64_t)(head - p.q_heads - p.kv_heads) * D);
-        load<E, WIDE>(from + first, x[i]);
+        for (int i = 0; i < kHeads; ++i) load<E, WIDE>(from + i * D, x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) load<E, WIDE>(plane_of(min(head0 + i, heads - 1)), x[i]);  // (one past the last is loaded for nothing)
     }
     const int slot = __ldcg(p.slots + t);
     const bool turns = first < p.rotary && head0 < p.q_heads + p.kv_heads, low = first < half;
