@@ -17,6 +17,8 @@
 //   * The keys of all requests and heads, in units of 64, are dealt out evenly: every CTA takes an equal range of units, wherever it begins and ends.
 //     Rows whose units fall to several CTAs are joined, in CTA order, by whichever of these is the last to leave its sums: the same bits on every run.
 // One token over 131071 keys, 32 + 2 x 8 heads of 128, f16: 94.5 us, 0.87 of the measured copy's bandwidth (another GPU 96.5); 64 requests of up to 8191 keys, bf16: 176 us, 0.93 (184).
+#include <cmath>
+
 #include "rq_attention_rows.cuh"
 
 using namespace rqserve;
@@ -457,6 +459,8 @@ extern "C" int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int
         p.page_bytes = (uint32_t)cache->page_stride; p.line_bytes = (uint32_t)cache->line_stride;
         p.k_scale = cache->k_scale; p.v_scale = cache->v_scale;
         p.scale_page = cache->scale_page_stride; p.scale_head = cache->scale_head_stride; p.scale_line = cache->scale_line_stride;
+        p.scale_size = (float)(2.0 * frexp((double)scale * (double)kLog2e, &p.scale_exponent));
+        --p.scale_exponent;
     }
     const int64_t rows = (int64_t)(max_fresh > 0 ? (max_fresh < tokens ? max_fresh : tokens) : tokens) * group;
     // The rows kernel reads a request's keys once for every sixteen rows (from L2, from the second time on), the tensor-core kernel makes scores of 128 whatever

@@ -24,6 +24,8 @@ struct AttentionParams {
 struct CodesParams : AttentionParams {
     const float *k_scale, *v_scale;
     int64_t scale_page, scale_head, scale_line;
+    float scale_size;  // scale * log2(e) = scale_size * 2^scale_exponent, 1 <= scale_size <= 2
+    int scale_exponent;
 };
 
 // What the work area holds: sums of rows for each CTA's first and last item (the tensor-core kernel: two tiles of 128 rows of 128 elements and their
@@ -87,6 +89,16 @@ template <int TYPE> __device__ __forceinline__ uint32_t take_pair(float& a, floa
 // of that element without its sign; rows of zeros and below 2^-112 stay below, those that are not finite are none afterwards either.
 __device__ __forceinline__ int raise_of(uint32_t largest) { return min(141 - (int)(largest >> 23), 126); }  // from -114
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// Over codes: a row's scores are sums of codes times its queries, raised, times a key's scale and scale_size * 2^exponent. So that no product in between is past fp32's range where
+// the score is not, the power of two is taken in two parts, 2^first with the sum (a number of 1 to 2^45) before it meets the key's scale, the rest with scale_size after that: with
+// 2^80 at most 2^125 meets a scale, and what the rest would raise stays below the score itself; from 2^-126 the sum stays a normal number.
+struct PowerParts {
+    float first, rest;
+};
+__device__ __forceinline__ PowerParts power_parts(float size, int exponent) {
+    const int first = min(max(exponent, -126), 80);
+    return {power_of_two(first), size * power_of_two(min(max(exponent - first, -126), 126))};
+}
 constexpr int kUsualRaise = 7;  // right for rows whose largest element is 2^-6 .. 2^9
 // What scores are multiplied by to be exponents of two: positive and finite, so that masked scores stay -inf and scores of zero stay zero
 __device__ __forceinline__ float factor_of(float scale, int raise) { return fminf(fmaxf(scale * power_of_two(-raise) * kLog2e, 1.2e-38f), 3e38f); }

@@ -38,8 +38,8 @@ __device__ __forceinline__ void mma(int (&c)[4], bool first, uint4 a, uint32_t b
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 // Queries as whole numbers of 32 bits, n = 2^24 d0 + 2^16 d1 + 2^8 d2 + d3 with digits of -128 .. 127: |n| < 2^30, a row's largest element at least 2^29 (a power of two
-// brings it there; one below 2^-97 stays below)
-__device__ __forceinline__ int digits_raise(uint32_t largest) { return max(min(156 - (int)(largest >> 23), 126), -99); }
+// brings it there; one below 2^-126 stays below, exactly)
+__device__ __forceinline__ int digits_raise(uint32_t largest) { return 156 - (int)(largest >> 23); }  // from -99 to 156: in two steps
 // byte i of a word: digit of x[i]
 __device__ __forceinline__ void take_digits(const int (&n)[4], uint32_t (&digit)[4]) {
     uint32_t b[4];
@@ -48,7 +48,6 @@ __device__ __forceinline__ void take_digits(const int (&n)[4], uint32_t (&digit)
     const uint32_t x = __byte_perm(b[0], b[1], 0x5140), y = __byte_perm(b[2], b[3], 0x5140), z = __byte_perm(b[0], b[1], 0x7362), w = __byte_perm(b[2], b[3], 0x7362);
     digit[3] = __byte_perm(x, y, 0x5410); digit[2] = __byte_perm(x, y, 0x7632); digit[1] = __byte_perm(z, w, 0x5410); digit[0] = __byte_perm(z, w, 0x7632);
 }
-constexpr float kLess = 1.0f / 32768;  // what keys' scales are multiplied by, so that a sum of 2^44 times a scale has room
 
 // Taking up the rows of a request and head (their queries, the first tile, the sums at the end) costs a CTA as much as some units: so many lead each one's own in the dealing
 // (64 requests of up to 8191 keys: none 119 us, one 115, two 112, four 113).
@@ -224,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D, RT>) rq_attention_int8_
 
         // queries: brought to one size and taken apart, as the tensor core's operand registers (a thread's of step 2 j + i: elements 64 j + 16 t4 + 8 i + 0 .. 7); a warp
         // has every fourth step of all rows
-        float factor[RT];  // of the scores of row g
+        float lift[RT], factor[RT];  // of the sums of row g, and of their products with keys' scales
         {
             uint32_t largest[RT];
 #pragma unroll
@@ -243,26 +242,29 @@ __global__ void __launch_bounds__(kThreads, kResident<D, RT>) rq_attention_int8_
                 if (t4 == 0) row_largest[warp][rt * 8 + g] = largest[rt];
             }
             __syncthreads();
-            float raised[RT];
+            float raised[RT], more[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) largest[rt] = max(largest[rt], row_largest[w][rt * 8 + g]);
                 const int raise = digits_raise(largest[rt]);
-                raised[rt] = power_of_two(raise);
-                factor[rt] = factor_of(p.scale / kLess, raise);
+                raised[rt] = power_of_two(min(raise, 126));
+                more[rt] = power_of_two(max(raise - 126, 0));
+                const PowerParts parts = power_parts(p.scale_size, p.scale_exponent - raise);
+                lift[rt] = parts.first;
+                factor[rt] = parts.rest;
             }
 #pragma unroll
             for (int n = 0; n < MINE; ++n) {
                 const int item = n * kWarps + warp, rt = item / STEPS, step = item % STEPS;
                 if (item >= RT * STEPS) break;
-                const float f = RT == 2 && rt ? raised[RT - 1] : raised[0];
+                const float f = RT == 2 && rt ? raised[RT - 1] : raised[0], f2 = RT == 2 && rt ? more[RT - 1] : more[0];
                 uint32_t d[2][4];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     int whole[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) whole[i] = __float2int_rn(x[n][4 * e + i] * f);
+                    for (int i = 0; i < 4; ++i) whole[i] = __float2int_rn(x[n][4 * e + i] * f * f2);
                     take_digits(whole, d[e]);
                 }
                 sh.q[rt][step][0][lane] = make_uint4(d[0][0], d[0][1], d[1][0], d[1][1]);
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D, RT>) rq_attention_int8_
             const uint32_t keys = ring + stage * F::STAGE, values = keys + TILE * D;
             __syncwarp();  // the other stage, and the scales, have been read
             if (TILE == 32 || lane < TILE) {
-                sh.scales[warp][0][lane_key] = key_scale * kLess;
+                sh.scales[warp][0][lane_key] = key_scale;
                 sh.scales[warp][1][lane_key] = value_scale;
                 sh.scales[warp][2][lane_key] = exponent_of(value_scale);
             }
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D, RT>) rq_attention_int8_
 #pragma unroll
                     for (int i = 0; i < NT; ++i)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) s[rt][i][e] = fmaf((float)(c[rt][i][0][e] * 256 + c[rt][i][0][2 + e]), 65536.0f, (float)(c[rt][i][1][e] * 256 + c[rt][i][1][2 + e]));
+                        for (int e = 0; e < 2; ++e) s[rt][i][e] = fmaf((float)(c[rt][i][0][e] * 256 + c[rt][i][0][2 + e]), 65536.0f * lift[rt], (float)(c[rt][i][1][e] * 256 + c[rt][i][1][2 + e]) * lift[rt]);
             }
             // weights
             uint32_t w_hi[RT][NT], w_lo[RT][NT];
