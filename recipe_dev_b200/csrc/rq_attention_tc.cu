@@ -51,6 +51,9 @@ namespace {
 constexpr int kSoftmaxWarps = 8, kIssuer = 8, kLoader = 9, kFetcher = 10, kMender = 11, kWidener = 12;
 constexpr int kCodesShift = 4;  // a copy of codes brings at most sixteen lines
 constexpr int kEven = 12;       // exponents of a tile's scales of values that lie no further apart need no look at each
+// Keys' scales of 2^-60 to 2^61 meet a row's sum (at most 2^30) before its power of two does: neither is past fp32's range, and a score that the power's lower end, 2^-126, is
+// too large for is less than 2^-34. Other tiles, and rows of powers above 2^126, take it in two parts.
+constexpr int kUsual = 60;
 constexpr int kItems = 4, kWords = 16;  // rings in shared memory: items, words on tiles of keys
 
 // Taking a block up (its queries, the first scores, the sums at the end: 21 us) costs as much as some units (3.9 us): so many lead each block's own in the dealing.
@@ -164,10 +167,10 @@ template <typename F> struct Shared {
     uint32_t pages_there[kWords];  // a tile's pages that the cache has, a bit each; all ones: all of them
     uint32_t odd[kWords];          // whether something was taken out of a tile's values
     uint32_t tmem_slot;
-    float factors[2][F::KEYS && F::PARTS == 2 ? 128 : 1];  // keys form over f16: of the rows' scores, the items in turn
+    float factors[2][F::KEYS && F::PARTS == 2 ? 128 : 1];  // keys form over f16: of the rows' scores (codes: their powers of two, as bits), the items in turn
     float joint[2][F::KEYS ? 128 : 1];  // keys form: the second pipe's base and sum of each row
     alignas(16) float scales[F::SCALE_TILES][2][F::CODES ? F::KT : 1];  // codes: of a tile's keys, of its values
-    int levels[F::SCALE_TILES][2][2];                                     // codes: the largest and the least exponent of the scales of either half of its values
+    int levels[F::SCALE_TILES][4][2];                                     // codes: the largest and the least exponent of the scales of either half of its keys, and of its values
 };
 
 __device__ __forceinline__ bool finite16(uint32_t v, int type) { const uint32_t e = type == RQ_KV_F16 ? 0x7c00u : 0x7f80u; return (v & e) != e; }
@@ -179,10 +182,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
 
 __device__ __forceinline__ uint32_t max_pairs(uint32_t a, uint32_t b) { uint32_t r; asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
 
-// The rows of a warp's share, each brought to one size by its own largest element; returns what that of the lane's row was raised by. A call of its own: in line, it
-// takes registers from the softmax around it (a prompt of 3001 tokens, windows of 1000, 259 us in place of 247).
-template <int D, int TYPE, bool KEYS> __device__ __noinline__ int rescale_queries(const AttentionParams& p, int64_t mine, uint8_t* to, int first) {
-    using F = Form<D, TYPE, KEYS, false>;
+// The rows of a warp's share, each brought to one size by its own largest element; returns what that of the lane's row was raised by. (Over codes rows below 2^-112 too, in two
+// steps: keys may be as large as they are small. f16 keys may not.) A call of its own: in line, it takes registers from the softmax around it (a prompt of 3001 tokens,
+// windows of 1000, 259 us in place of 247).
+template <int D, int TYPE, bool KEYS, bool CODES> __device__ __noinline__ int rescale_queries(const AttentionParams& p, int64_t mine, uint8_t* to, int first) {
+    using F = Form<D, TYPE, KEYS, CODES>;
     constexpr int SHARE = 128 / D, ROWS = KEYS ? 16 : 32, BATCH = 4;
     const int lane = threadIdx.x & 31, e = 4 * (lane % (D / 4));
     int raise = 0;
@@ -205,12 +209,16 @@ template <int D, int TYPE, bool KEYS> __device__ __noinline__ int rescale_querie
             float top = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
 #pragma unroll
             for (int off = D / 8; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            const int here = raise_of(__float_as_uint(top)), told = __shfl_sync(0xffffffffu, here, (lane % SHARE) * (D / 4));
+            const int here = CODES ? 141 - (int)(__float_as_uint(top) >> 23) : raise_of(__float_as_uint(top)), told = __shfl_sync(0xffffffffu, here, (lane % SHARE) * (D / 4));
             if ((lane & (ROWS - SHARE)) == r) raise = told;
-            const float raised = power_of_two(here);
+            const float raised = power_of_two(CODES ? min(here, 126) : here);
             const int row = first + r + lane / (D / 4);
             uint8_t* place = to + (e >> 6) * (128 * 128) + swizzled(row, (e & 63) >> 3) + 2 * (e & 7);
             x[i].x *= raised; x[i].y *= raised; x[i].z *= raised; x[i].w *= raised;
+            if (CODES) {
+                const float more = power_of_two(max(here - 126, 0));
+                x[i].x *= more; x[i].y *= more; x[i].z *= more; x[i].w *= more;
+            }
 #pragma unroll
             for (int part = 0; part < F::PARTS; ++part) *(uint2*)(place + part * F::Q_PART) = make_uint2(take_pair<TYPE>(x[i].x, x[i].y), take_pair<TYPE>(x[i].z, x[i].w));
         }
@@ -219,12 +227,12 @@ template <int D, int TYPE, bool KEYS> __device__ __noinline__ int rescale_querie
 }
 
 // Queries of a warp's share of the block's rows, brought to one size (f16) and taken apart, as the tensor core reads them: a row is one contiguous access, eight
-// accesses on their way at a time. (A thread that reads a row of its own meets 32 lines an instruction.) Returns the factor of the scores of the lane's row.
+// accesses on their way at a time. (A thread that reads a row of its own meets 32 lines an instruction.) Returns what the lane's row was raised by.
 // Over f16 all rows are multiplied by the same power of two first, and the parts themselves say whether that was the right one for each: a row's largest element has
 // to be 2 or more, and finite, as an f16 number. Where it is not, the warp's rows are taken once more. (Every row by its own largest element at once made a block's
 // take-up 1.7 us longer: 32 prompts of 128 tokens 71 us in place of 68. Queries a thousandth of the usual size: 88 us, and the four prompts 402 in place of 356.)
-template <int D, int TYPE, bool KEYS> __device__ __forceinline__ float load_queries(const AttentionParams& p, const Item& it, uint8_t* to, int block_row, int first, int group) {
-    using F = Form<D, TYPE, KEYS, false>;
+template <int D, int TYPE, bool KEYS, bool CODES> __device__ __forceinline__ int load_queries(const AttentionParams& p, const Item& it, uint8_t* to, int block_row, int first, int group) {
+    using F = Form<D, TYPE, KEYS, CODES>;
     constexpr int SHARE = 128 / D, ROWS = KEYS ? 16 : 32, BATCH = ROWS / SHARE < 8 ? ROWS / SHARE : 8;  // rows an access; rows a warp; accesses at a time
     const int lane = threadIdx.x & 31, own = block_row + first + (lane & (ROWS - 1)), at = it.row0 + own, e = 4 * (lane % (D / 4));
     const int64_t mine = own < it.rows ? (int64_t)(it.start + at / group) * p.q_stride + (int64_t)(it.kv * group + at % group) * D : -1;
@@ -277,11 +285,11 @@ template <int D, int TYPE, bool KEYS> __device__ __forceinline__ float load_quer
             lacking = __ballot_sync(0xffffffffu, !(all >> ((row >> 1) + (row & 1) * 16) & 1)) & rows_there;
         }
         if (__any_sync(0xffffffffu, too_large) || lacking) {
-            raise = rescale_queries<D, TYPE, KEYS>(p, mine, to, first);
+            raise = rescale_queries<D, TYPE, KEYS, CODES>(p, mine, to, first);
         }
     }
     fence_to_tensor_core();
-    return factor_of(p.scale, raise);
+    return raise;
 }
 
 template <int D, int TYPE, bool KEYS, bool CODES>
@@ -455,11 +463,11 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
                             sh.scales[place][which >> 1][first + 32 * i] = scale[i];
                             const int e = (int)(__float_as_uint(scale[i]) >> 23 & 0xff);
                             most = max(most, e);
-                            least = min(least, scale[i] == 0.0f ? 254 : e);  // (a value of zero takes no weight's bits)
+                            least = min(least, scale[i] == 0.0f ? 254 : e);  // (a value of zero takes no weight's bits, a key of zero is none of an extreme size)
                         }
                         most = __reduce_max_sync(0xffffffffu, most);
                         least = __reduce_min_sync(0xffffffffu, least);
-                        if (which >= 2 && lane == 0) { sh.levels[place][which & 1][0] = most; sh.levels[place][which & 1][1] = least; }
+                        if (lane == 0) { sh.levels[place][which][0] = most; sh.levels[place][which][1] = least; }
                     }
                     fence_to_tensor_core();
                     __syncwarp();
@@ -484,10 +492,13 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
         const int in_block = KEYS ? row : pipe * 128 + row;
         uint32_t tiles_done = 0, keys_before = 0, items_done = 0;  // this pipe's tiles; the items' tiles of keys; items
         float factor = 1.0f;  // of this row's scores
+        int exponent = 0;     // codes: their power of two
         auto queries = [&](const Item& of, uint32_t n) {  // of the n-th item
             const int first = quarter * 32 + (KEYS ? pipe * 16 : 0);
-            factor = load_queries<D, TYPE, KEYS>(p, of, smem + (KEYS ? 0 : pipe * PARTS * F::Q_PART), KEYS ? 0 : pipe * 128, first, group);
-            if (KEYS && PARTS == 2 && lane < 16) sh.factors[n & 1][first + lane] = factor;
+            const int raise = load_queries<D, TYPE, KEYS, CODES>(p, of, smem + (KEYS ? 0 : pipe * PARTS * F::Q_PART), KEYS ? 0 : pipe * 128, first, group);
+            if constexpr (CODES) exponent = p.scale_exponent - raise;
+            else factor = factor_of(p.scale, raise);
+            if (KEYS && PARTS == 2 && lane < 16) sh.factors[n & 1][first + lane] = CODES ? __int_as_float(exponent) : factor;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.q_full[KEYS ? 0 : pipe]);
         };
@@ -507,7 +518,8 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
             // (keys form: the rows' queries are brought by the warps of both pipes)
             if (KEYS && PARTS == 2) {
                 if (!mbar_wait_warp(&sh.q_full[0], items_done & 1, p.wait_ns, dead)) atomicExch(p.error_flag, 53);
-                factor = sh.factors[items_done & 1][row];
+                if (CODES) exponent = __float_as_int(sh.factors[items_done & 1][row]);
+                else factor = sh.factors[items_done & 1][row];
             }
             float base = -INFINITY, sum = 0.0f, old = 1.0f;  // base: -inf while the row has seen no key
 #pragma unroll
@@ -570,8 +582,8 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
                 bool even = true;
                 if (CODES) {
                     const volatile int* l = &sh.levels[place][0][0];
-                    const int most = max(l[0], l[2]);
-                    even = most < 255 && most - min(l[1], l[3]) <= kEven;
+                    const int most = max(l[4], l[6]);
+                    even = most < 255 && most - min(l[5], l[7]) <= kEven && max(l[0], l[2]) <= 127 + kUsual && min(l[1], l[3]) >= 127 - kUsual && exponent <= 126;
                     level = min(max(most, 127 - 80), 127 + 90) - 127;
                 }
                 // (codes: rows past the block's last, whose results nobody reads, hide nothing)
@@ -595,7 +607,13 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
                 // The loops over columns are loops: laid out in a line, with the masks, they were longer than the instruction caches are.
                 auto tile = [&](auto masked, auto uneven) {
                     constexpr bool kMasked = decltype(masked)::value, kUneven = decltype(uneven)::value;
-                    float top = -INFINITY, top2 = -INFINITY;
+                    float top = -INFINITY, top2 = -INFINITY, lift = 1.0f;
+                    // (keys of usual sizes: the power of two may wait)
+                    if constexpr (CODES) {
+                        const PowerParts parts = power_parts(p.scale_size, exponent);
+                        lift = parts.first;
+                        factor = kUneven ? parts.rest : p.scale_size * power_of_two(max(exponent, -126));
+                    }
 #pragma unroll 1
                     for (int c = 0; c < KT / 32; ++c) {
                         uint32_t s[32];
@@ -604,6 +622,9 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
                         if (CODES) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4) {
+                                if (kUneven)
+#pragma unroll
+                                    for (int n = 0; n < 4; ++n) s[i + n] = __float_as_uint(__uint_as_float(s[i + n]) * lift);
                                 const float4 k = *(const float4*)(of_keys + 32 * c + i);
                                 const Pair a = pair_mul(pair_of(s[i], s[i + 1]), pair_of(k.x, k.y)), b = pair_mul(pair_of(s[i + 2], s[i + 3]), pair_of(k.z, k.w));
                                 s[i] = __float_as_uint(pair_at(a, 0)); s[i + 1] = __float_as_uint(pair_at(a, 1)); s[i + 2] = __float_as_uint(pair_at(b, 0)); s[i + 3] = __float_as_uint(pair_at(b, 1));
@@ -644,6 +665,10 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
                                     two_keys = *(const float4*)(of_keys + 32 * c + 2 * i);
                                     two_values = *(const float4*)(of_values + 32 * c + 2 * i);
                                 }
+                                if (kUneven) {
+                                    s[2 * i] = __float_as_uint(__uint_as_float(s[2 * i]) * lift);
+                                    s[2 * i + 1] = __float_as_uint(__uint_as_float(s[2 * i + 1]) * lift);
+                                }
                                 const Pair scaled = pair_mul(pair_of(s[2 * i], s[2 * i + 1]), i & 1 ? pair_of(two_keys.z, two_keys.w) : pair_of(two_keys.x, two_keys.y));
                                 s[2 * i] = __float_as_uint(pair_at(scaled, 0));
                                 s[2 * i + 1] = __float_as_uint(pair_at(scaled, 1));
@@ -682,7 +707,7 @@ __global__ void __launch_bounds__(Form<D, TYPE, KEYS, CODES>::THREADS, 1) rq_att
                     add[0] = pair_add(add[0], add[1]);
                     sum = fmaf(sum, f, pair_at(add[0], 0) + pair_at(add[0], 1));
                 };
-                if (CODES && !even) tile(std::true_type(), std::bool_constant<CODES>());
+                if (CODES && !__all_sync(0xffffffffu, even)) tile(std::true_type(), std::bool_constant<CODES>());
                 else if (__all_sync(0xffffffffu, all)) tile(std::false_type(), std::false_type());
                 else tile(std::true_type(), std::false_type());
                 weights_there(1);
