@@ -373,8 +373,9 @@ int rq_rope_store(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, 
  * alignment. max_fresh is the most new tokens that a request has, as far as the host knows: the choice of kernel, and with
  * it the last bits, rests on it; every kernel serves every batch.
  * Activations stay fp32: queries and weights meet the 16-bit keys and values as two (f16) or three (bf16) 16-bit parts, products
- * are added in 32 bits. (RQ_KV_INT8: codes are f16 numbers, scales are applied in fp32; values up to 2^90 in size.) Queries and keys may be of any size as long as scale times their products stays within fp32; a row of queries that is not finite, or that sees
- * keys or values that are not, has no defined outputs (the other rows are as ever). The same bits on every run of the same call.
+ * are added in 32 bits. (RQ_KV_INT8: codes are f16 numbers, scales are applied in fp32; heads of values from 2^-86 to
+ * 2^90 in size, smaller ones lose bits.) Queries and keys may be of any size as long as scale times their products stays below 2^24 (fp32 scores of that size tell keys apart by whole
+ * numbers); a row of queries that is not finite or passes that, or that sees keys or values that are not finite, has no defined outputs (the other rows are as ever). The same bits on every run of the same call.
  * The context keeps a work area for rows whose keys are dealt out over several CTAs; the first call, or rq_attention_reserve ahead of a recording, allocates it. */
 int rq_attention_reserve(rq_ctx* ctx);
 int rq_attention(rq_ctx* ctx, const float* q, int64_t q_t_stride, int q_heads, const rq_kv_cache* cache, const int32_t* block_table, int64_t table_stride,
