@@ -7,7 +7,9 @@
 // contiguous access and the other element of a pair half a head apart one shuffle; the four sums of squares are added up together. Everything is held in fp32 and a
 // key or value is rounded once, to the cache's type. (In place: a warp has read what it writes.) 2039 tokens of 32 + 2 x 8 heads of 128: 22.0 us, 4.2 TB/s; with five
 // shuffles and a square root a head 23.8, and of that form with two heads a warp 24.4, eight 27.7, CTAs of eight warps 24.9; one head a warp 30.3. 64 tokens 10.1 us, one
-// 9.4, which is what a call from Python takes. Into a cache of codes, whose heads' largest magnitudes are one reduction of a warp each: 2039 tokens 21.5 us, 4.1 TB/s (f16 21.5 among its own calls too; of that with an address for each head 22.6).
+// 9.4, which is what a call from Python takes. Into a cache of codes, whose heads' largest magnitudes are one reduction of a warp each: 2039 tokens
+// 21.7 us, 4.1 TB/s (f16 21.0 among its own calls too; with an address for each head one more).
+#include "rq_pairs.cuh"
 #include "rq_serve.cuh"
 
 using namespace rqserve;
@@ -168,8 +170,10 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
         }
     }
     if (TYPE == RQ_KV_INT8 && stored && head0 + kHeads > p.q_heads) {
-        // A head's largest magnitude (as bits without the sign: infinities and NaN lie above the numbers), its scale, and its codes: x / scale + 1.5 * 2^23 rounded once,
-        // to a whole number, whose low byte is the code. A lane makes one head's scale (the four heads' one after another, by all lanes: 2039 tokens 23.7 us, so 22.6)
+        // A head's largest magnitude (as bits without the sign: infinities and NaN lie above the numbers), its scale, and its codes, the whole numbers nearest to x / scale, ties to even:
+        // x times the scale's reciprocal + 1.5 * 2^23 is rounded once, to a whole number, whose low byte is the code. The reciprocal is rounded too, so that next to a border that
+        // may be the other code (a few of ten million): what is left, x - code * scale, is exact, and more than half a scale, or half a scale from an odd code, is the next code's.
+        // (2039 tokens 21.7 us, without a look at what is left 21.3.) A lane makes one head's scale (the four heads' one after another, by all lanes: 2039 tokens 23.7 us, so 22.6)
         const int64_t place = page * p.scale_page + (slot & ((1 << p.page_shift) - 1)) * p.scale_line;
         float scale_here, inverse_here;
         {
@@ -194,10 +198,25 @@ __global__ void __launch_bounds__(kWarps * 32) rq_rope_kernel(RopeParams p) {
         for (int n = 0; n < kHeads; ++n) {
             const int at = head0 + n - p.q_heads;  // among the keys' heads and then the values'
             if (at < 0 || at >= 2 * p.kv_heads) continue;
-            const float inverse = __shfl_sync(0xffffffffu, inverse_here, n);
+            const float inverse = __shfl_sync(0xffffffffu, inverse_here, n), step = __shfl_sync(0xffffffffu, scale_here, n);
             uint32_t codes[E];
+            float most_left = 0.0f;
+            auto left = [&](int i) { return fmaf(__uint_as_float(codes[i]) - 12582912.0f, -step, x[n][i]); };
 #pragma unroll
-            for (int i = 0; i < E; ++i) codes[i] = __float_as_uint(fmaf(x[n][i], inverse, 12582912.0f));
+            for (int i = 0; i < E; i += 2) {
+                const Pair of = pair_of(x[n][i], x[n][i + 1]), raised = pair_fma(of, pair_of(inverse, inverse), pair_of(12582912.0f, 12582912.0f));
+                const Pair rest = pair_fma(pair_add(raised, pair_of(-12582912.0f, -12582912.0f)), pair_of(-step, -step), of);
+                codes[i] = __float_as_uint(pair_at(raised, 0));
+                codes[i + 1] = __float_as_uint(pair_at(raised, 1));
+                most_left = fmaxf(fmaxf(most_left, fabsf(pair_at(rest, 0))), fabsf(pair_at(rest, 1)));
+            }
+            if (__any_sync(0xffffffffu, step > 0.0f && 2.0f * most_left >= step)) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const float rest = left(i), twice = 2.0f * fabsf(rest);
+                    if (step > 0.0f && (twice > step || (twice == step && (codes[i] & 1)))) codes[i] += rest > 0.0f ? 1 : -1;
+                }
+            }
             const int kv = at < p.kv_heads ? at : at - p.kv_heads;
             int8_t* to = (int8_t*)(at < p.kv_heads ? p.k_cache : p.v_cache) + kv * p.head_stride + line;
             uint32_t w[E / 4 > 0 ? E / 4 : 1];
