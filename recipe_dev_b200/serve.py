@@ -66,7 +66,8 @@ class Decoder:
         return self.ctx.matvec(w, x, y, stream=stream) if x.shape[0] <= 8 else self.ctx.matmul(w, x, y, stream=stream)
 
     def hidden_states(self, ids, batch, max_fresh: int, at, stream=None):
-        """ids: int32 [tokens]; batch: the plan's table, starts, lengths, slots and positions; at: planes. The last layer's outputs [tokens, hidden]."""
+        """ids: int32 [tokens]; batch: the plan's table, starts, lengths, slots and positions; at: planes. The last layer's outputs [tokens, hidden]; with norms on both
+        sides they have had the last norm, which is made with the sum in front of it."""
         import torch
 
         ctx, x, h, parts = self.ctx, at["x"], at["h"], at["parts"]
@@ -97,16 +98,18 @@ class Decoder:
                 with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream, self.device)):
                     torch.nn.functional.silu(at["gated"], inplace=True).mul_(at["up"])
             delta = self._product(layer["down"], at["gated"], at["delta"], stream)
-            if both:  # (with the norm in front of the next layer; the last one's is the head's)
+            if both:  # (with the norm in front of the next layer, or of the head)
                 following = self.layers[n + 1]["gains"][0] if n + 1 < len(self.layers) else self.last_gain
                 ctx.residual_norm(x, delta, following, layer["behind"][1], residual_scale=self.residual_scale, y=h, stream=stream)
             else:
                 ctx.add(x, delta, x, stream=stream)
-        return x
+        return h if both and self.layers else x
 
     def logits(self, x, at, stream=None):
-        self.ctx.rmsnorm(x, self.last_gain, y=at["last"], stream=stream)
-        return self._product(self.embedding, at["last"], at["logits"], stream)
+        """Of hidden_states' rows, or some of them."""
+        if self.norms == "before" or not self.layers:
+            x = self.ctx.rmsnorm(x, self.last_gain, y=at["last"], stream=stream)
+        return self._product(self.embedding, x, at["logits"], stream)
 
 
 class Batch:
