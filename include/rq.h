@@ -402,7 +402,8 @@ int rq_sample(rq_ctx* ctx, const float* logits, int64_t row_stride, int rows, in
  *   top_token[r][n], top_logprob[r][n], n < top: the likeliest tokens in that order, with their log probabilities.
  * token null: logprob and rank are not written; a null output is not wanted (top = 0: no alternatives). A token outside the vocabulary (a padding row's)
  * gets logprob 0 and rank -1. NaN counts as -inf; tokens at -inf are no alternatives: where fewer than `top` are left the rest is -1 and -inf. A row without any value
- * above -inf has logprob -inf, rank -1, entropy 0; one with +inf has no defined outputs. fp32 arithmetic, sums in a fixed order. At most RQ_MAX_VOCABULARY
+ * above -inf has logprob -inf, rank -1, entropy 0; one with +inf has no defined outputs. fp32 arithmetic; the order of additions follows from rows, vocabulary and where the row
+ * begins (the same bits for the same call; in another batch a row's last bits may be others). At most RQ_MAX_VOCABULARY
  * tokens and RQ_MAX_ALTERNATIVES alternatives. */
 #define RQ_MAX_ALTERNATIVES 64
 int rq_logprobs(rq_ctx* ctx, const float* logits, int64_t row_stride, int rows, int64_t vocabulary, const int32_t* token, float* logprob, float* entropy, int32_t* rank,
