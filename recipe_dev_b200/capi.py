@@ -279,7 +279,7 @@ class KvCache:
             scales = (k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride())
         elif k_scale is not None or v_scale is not None:
             raise ValueError("KvCache: only an int8 cache has scales")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.get_device()
         self.pages, self.heads, self.page_size, self.head_dim = k.shape
         sp, sh, sl, _ = k.stride()
         self._struct = _KvCacheStruct(k.data_ptr(), v.data_ptr(), kinds[k.dtype], self.heads, self.head_dim, self.page_size, self.pages, sp, sh, sl, *scales)
@@ -668,6 +668,8 @@ class Context:
         if _F32 is None:
             _with_torch()
         tokens = q.shape[0]
+        if cache.device != self.device:
+            raise ValueError("rope_store: the cache must lie on the context's device")
         if q_out is None:
             import torch
 
@@ -706,6 +708,8 @@ class Context:
         if _F32 is None:
             _with_torch()
         tokens, n, d = q.shape[0], lengths.shape[0], cache.head_dim
+        if cache.device != self.device:
+            raise ValueError("attention: the cache must lie on the context's device")
         if y is None:
             import torch
 
