@@ -12,8 +12,8 @@
 //   * A warp's tile is 32 keys (16 for heads of 256): the same bytes on their way as there, and half the work on sums for each key. A lane brings its key's scales through registers.
 //   * A row's base is the largest score plus its value's scale's exponent, less 12: hi parts of weight * sv lie below 2^13 whatever the scales are.
 // Bound by the bytes of the cache while the loop runs (at 7 TB/s of reading), and by both ends of a launch: the first tiles 4 to 5 us after its beginning, CTAs that are done 4 us apart, and
-// 3 to 8 us for the parts of rows. One token over 131071 keys, 32 + 2 x 8 heads of 128: 57.6 us, 0.73 of the measured copy's bandwidth (f16: 94); 64 requests of up to 8191 keys: 111 us, 0.76
-// (bf16: 185); one token over 1001 keys 9.4. With scores of f16 numbers too (as values are taken), 1130 instructions a tile in place of 750, 80 and 143 us.
+// 3 to 8 us for the parts of rows. One token over 131071 keys, 32 + 2 x 8 heads of 128: 57.4 us, 0.74 of the measured copy's bandwidth (f16: 94); 64 requests of up to 8191 keys: 111 us, 0.76
+// (bf16: 185); one token over 1001 keys 9.4 (in a recorded sequence 9.0). With scores of f16 numbers too (as values are taken), 1130 instructions a tile in place of 750, 80 and 143 us.
 #include <type_traits>
 
 #include "rq_attention_rows.cuh"

@@ -34,8 +34,8 @@
 // the others' waits run out too and all meet at the end. The loading warp leaves when every copy has landed.
 //
 // 509 tokens over 7680 keys, 32 + 2 x 8 heads of 128, f16: 137 us, 66 GFLOP of them useful (0.29 of the measured peak, 0.59 with both parts), products under way
-// 56 % of the time; four prompts of 1021 to 3001 tokens 378 us, 150 GFLOP (both called among other cases; over the same two batches again and again 123 and 350). Over codes 163 and 449 us,
-// products under way 41 % of the time.
+// 56 % of the time; four prompts of 1021 to 3001 tokens 378 us, 150 GFLOP (both called among other cases; over the same two batches again and again 123 and 350). Over codes 160 and 440 us,
+// products under way 41 % of the time; that form spills 746 bytes of stores a thread and 964 of loads (over f16 606 and 800), half of them in the issuing warp.
 #include <type_traits>
 
 #include "rq_attention.cuh"

@@ -13,7 +13,8 @@
 //
 // Bound by bytes for many rows: 2039 x 32000 without alternatives 50 us, 5.2 TB/s, 0.79 of the measured copy (23 instructions a logit, one at a time, in place of nine: 55). For rows that a cluster
 // each takes, by what comes behind the stream: 64 x 262144 with twenty alternatives 27.6 us, 13 to 16 of them the stream (CTAs of SMs that hold four, or three), then 1 for the sums, 1.5 for
-// the bound, 1.5 for each meeting, 3 for the segments, 2 for the order. A list kept up to date in every round, with barriers: 60 us by sixteen CTAs a row, 34 by eight.
+// the bound, 1.5 for each meeting, 3 for the segments, 2 for the order; 2039 x 32000 with twenty 77. One row in a recorded sequence: of 32000 3.7 us, with twenty alternatives 8.4, of 262144
+// with twenty 12.7. A list kept up to date in every round, with barriers: 60 us by sixteen CTAs a row, 34 by eight.
 #include <cooperative_groups.h>
 
 #include "rq_pairs.cuh"

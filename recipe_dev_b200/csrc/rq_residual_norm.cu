@@ -5,8 +5,9 @@
 // A CTA takes a token and holds it in registers from its one reading to its last writing: two sums over the CTA, one barrier each, lie between them. Bound by bytes
 // for a prompt, by the launch and the chain of a load and two sums for a few tokens. Sums of squares are held in fp32: of a thread's elements, of a warp by shuffles, of
 // the warps by shuffles again, in every warp for itself; the order follows from the width alone, so that a token has the same bits in every call.
-// 2039 tokens of 4096 with a gate for each element 30.8 us, 5.4 TB/s, 0.83 of the measured copy (one element in four a thread 34.5, sixteen elements a thread 35.4, eight with gates and
-// gains loaded where they are used 32.5); 64 of 2560 7.7 us and one of 4096 7.3, which is what a call from Python takes.
+// 2039 tokens of 4096 with a gate for each element 30.5 us, 5.4 TB/s, 0.83 of the measured copy (one element in four a thread 34.5, sixteen elements a thread 35.4, eight with gates and
+// gains loaded where they are used 32.5); 64 of 2560 7.9 us and one of 4096 7.6, which is what a call from Python takes (in a
+// recorded sequence 3.0 and 2.1).
 #include "rq_serve.cuh"
 
 using namespace rqserve;

@@ -5,10 +5,10 @@
 // Bound by bytes for a prompt (everything is read once and written once) and by the launch for a few tokens: a warp takes four heads of one token, all of them on
 // their way at once and with one reading of the token's row of the table; its lanes hold head_dim / 32 neighbouring elements of each, so that a head is one
 // contiguous access and the other element of a pair half a head apart one shuffle; the four sums of squares are added up together. Everything is held in fp32 and a
-// key or value is rounded once, to the cache's type. (In place: a warp has read what it writes.) 2039 tokens of 32 + 2 x 8 heads of 128: 22.0 us, 4.2 TB/s; with five
-// shuffles and a square root a head 23.8, and of that form with two heads a warp 24.4, eight 27.7, CTAs of eight warps 24.9; one head a warp 30.3. 64 tokens 10.1 us, one
-// 9.4, which is what a call from Python takes. Into a cache of codes, whose heads' largest magnitudes are one reduction of a warp each: 2039 tokens
-// 21.7 us, 4.1 TB/s (f16 21.0 among its own calls too; with an address for each head one more).
+// key or value is rounded once, to the cache's type. (In place: a warp has read what it writes.) 2039 tokens of 32 + 2 x 8 heads of 128, calls one after
+// another: 21.0 us, 4.4 TB/s. (When it took 22.0: with five shuffles and a square root a head 23.8, and of that form with two heads a warp 24.4, eight 27.7, CTAs of eight warps 24.9; one
+// head a warp 30.3.) One token and 64 take 9.4 and 10.1 us from Python, which is the host's, and 2.5 and 3.2 in a recorded sequence. Into a cache of codes, whose heads' largest magnitudes are one reduction of a warp each: 2039 tokens
+// 21.7 us, 4.1 TB/s (with an address for each head of one plane a microsecond more). Neither bytes nor issue (64 %) is at its limit: a warp has no loads on their way while it reduces.
 #include "rq_pairs.cuh"
 #include "rq_serve.cuh"
 
